@@ -25,6 +25,7 @@ Q8_SLOTS, Q8_SLOT_ELEMS = 5, 4096
 # layer-0 fingerprint tags (engine.h G4E_FP_*), as dump_kv_fingerprint names them
 FP_TAGS = ("attn_norm", "K_pre_norm", "K_pre_rope", "K_store", "K_read0", "K_readN", "q_out")
 F32, F16, Q4_K, Q5_K, Q6_K, BF16 = 0, 1, 12, 13, 14, 30
+KV_Q8 = 1024   # paged KV caches: int8 codes, one fp32 scale a token and kv head
 
 VP, I, SZ, F = C.c_void_p, C.c_int, C.c_size_t, C.c_float
 
@@ -107,6 +108,13 @@ _SIGS = {
     "g4_attn_decode_ring": (I, [VP, VP, VP, I, I, I, I, I, I, I, F, VP]),
     "g4_attn_decode_noalloc": (I, [VP, VP, VP, I, I, I, I, I, I, F, VP]),
     "g4_softmax": (I, [VP, I]),
+    "g4_kv_pool_bytes": (SZ, [I, I, I, I, I]),
+    "g4_kv_page_store": (I, [VP, VP, I, I, I, I, I, VP, I, VP, VP, I, VP, VP, I, I]),
+    "g4_kv_page_load": (I, [VP, VP, I, I, I, I, I, VP, I, VP, VP, I, VP, VP, I, I]),
+    "g4_attn_decode_paged_part_bytes": (SZ, [I, I, I]),
+    "g4_attn_decode_paged": (I, [VP, I, VP, VP, I, I, I, I, I, VP, I, VP, I, I, I, F, VP, VP, I]),
+    "g4_attn_prompt_packed_work_bytes": (SZ, [I, I, I, I, I]),
+    "g4_attn_prompt_packed": (I, [VP, I, VP, VP, I, VP, I, I, VP, I, I, I, I, I, I, F, VP]),
     "g4_emb_lookup": (I, [VP, VP, I, I, I, I]),
     "g4_argmax_part_bytes": (SZ, [I]),
     "g4_argmax": (I, [VP, I, VP, VP, VP, VP]),

@@ -42,6 +42,9 @@ enum {
 
 /* ggml tensor type ids, main.c:85-92 */
 enum { G4_F32 = 0, G4_F16 = 1, G4_Q4_K = 12, G4_Q5_K = 13, G4_Q6_K = 14, G4_BF16 = 30 };
+/* the library's own: int8 codes with one fp32 scale for each token and kv
+ * head (paged KV caches only) */
+enum { G4_KV_Q8 = 1024 };
 
 /* ---------------------------------------------------------------------------
  * Lifecycle and memory.  No reference counterpart (main.c keeps everything in
@@ -390,6 +393,76 @@ int g4_attn_decode_noalloc(const float *q, const float *kc, const float *vc, int
                            int n_heads, int n_kv, int hd, float attn_scale, float *out);
 /* softmax(float *x, int n), main.c:1478 */
 int g4_softmax(float *x, int n);
+
+/* ---------------------------------------------------------------------------
+ * Many sequences at once (the reference runs one, main.c:2324-2448): a KV
+ * cache in pages that sequences take as they grow, the attention of one new
+ * token of every sequence over it, and the attention of whole prompts packed
+ * one after the other.  head_dim 64, 128, 256 or 512 throughout; any number of
+ * q heads per kv head; 1 to 4096 sequences.  Lengths, tables and row starts
+ * are read on the device, so that a captured graph follows them; nothing is
+ * allocated, cleared or waited for.
+ *
+ * Pools: K and V of a layer are two pools of g4_kv_pool_bytes() bytes
+ * (16-byte aligned; the layout is the library's own) of n_pages pages of
+ * `page` tokens (a power of two from 16 to 4096), n_kv heads of hd, of type
+ *   G4_F32; G4_F16, G4_BF16: rounded to nearest even;
+ *   G4_KV_Q8: d = max|x| / 127 over a token's head (an fp32 division), codes
+ *     rint(x / d) (codes 0 if d is 0), read back as code * d; a head that holds
+ *     an infinity or NaN reads back as NaN.
+ * table (device): table[s * table_stride + i] is the page of positions
+ * i * page .. of sequence s.  Entries that no position in use needs are not
+ * read.  Pages are never looked at past a sequence's length, so what is left
+ * there by others (infinities, NaN) does not matter.
+ * Packed rows: sequence s has rows cu[s] .. cu[s+1]-1 (cu: n_seqs + 1
+ * ascending device ints, cu[n_seqs] <= m); m is the number of rows the
+ * buffers hold.  Rows of no sequence are neither read nor written.
+ * ------------------------------------------------------------------------- */
+/* bytes of one pool; 0 if a size or the type is not one of the above */
+size_t g4_kv_pool_bytes(int type, int n_pages, int page, int n_kv, int hd);
+/* The KV append (main.c:1901-1904) for the packed rows of k and v (n_kv * hd
+ * floats, kv_stride floats apart; finished as g4_qkv_post_rows leaves them):
+ * row i of sequence s goes to position lens[s] - n + i, n = cu[s+1] - cu[s],
+ * i.e. lens[s] counts the new rows.  The sequences' pages must be distinct
+ * where they are written.  A sequence whose cu or lens do not fit (n > lens,
+ * rows past m, positions past the table) is skipped, rows of pages outside the
+ * pool are dropped.  k, v 16-byte aligned, kv_stride a multiple of 4. */
+int g4_kv_page_store(void *kp, void *vp, int type, int n_pages, int page, int n_kv, int hd, const int *table,
+                     int table_stride, const float *k, const float *v, int kv_stride, const int *cu, const int *lens,
+                     int n_seqs, int m);
+/* The way back: positions lens[s] - n .. lens[s] - 1 of sequence s, rounded
+ * values as fp32, into its packed rows (n = lens[s]: all of them).  Rows of
+ * pages outside the pool become NaN; a sequence whose cu or lens do not fit is
+ * skipped. */
+int g4_kv_page_load(const void *kp, const void *vp, int type, int n_pages, int page, int n_kv, int hd, const int *table,
+                    int table_stride, float *k, float *v, int kv_stride, const int *cu, const int *lens, int n_seqs,
+                    int m);
+/* The attention block (main.c:1909-1950) of one token of every sequence: q
+ * row s (n_heads * hd floats, q_stride apart) over positions
+ * max(0, lens[s] - window) .. lens[s] - 1 (window 0: all), the token's own K/V
+ * being stored already, into out row s (out_stride apart).  fp32 results
+ * whatever the cache's type: the products of q and of the weights with what
+ * the cache holds are exact, their sums fp32.  lens[s] = 0 gives zeros; a page
+ * outside the pool or a length past the table gives NaN in that sequence's row.
+ * Where what a head sees holds infinities or NaN, its output is what the
+ * formula gives or NaN.  part: g4_attn_decode_paged_part_bytes() bytes that no
+ * call running at the same time uses (its contents need not be kept).  q, out,
+ * part 16-byte aligned, strides multiples of 4. */
+size_t g4_attn_decode_paged_part_bytes(int n_heads, int n_kv, int hd);
+int g4_attn_decode_paged(const float *q, int q_stride, const void *kp, const void *vp, int type, int n_pages, int page,
+                         int n_kv, int hd, const int *table, int table_stride, const int *lens, int n_seqs, int window,
+                         int n_heads, float attn_scale, float *part, float *out, int out_stride);
+/* The attention block (main.c:1909-1950) of every row of whole prompts: row i
+ * of a sequence sees that sequence's rows max(0, i + 1 - window) .. i (window
+ * 0: 0 .. i).  q, k, v, out rows of one type, G4_F32, G4_F16 or G4_BF16, their
+ * strides in elements (16-byte aligned rows).  Rows of out past cu[n_seqs] and
+ * those of sequences whose cu does not fit are left as they are.  work:
+ * g4_attn_prompt_packed_work_bytes() bytes that no call running at the same
+ * time uses (its contents need not be kept); out may not overlap the inputs. */
+size_t g4_attn_prompt_packed_work_bytes(int type, int n_seqs, int m, int n_kv, int hd);
+int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void *v, int kv_stride, void *out,
+                          int out_stride, int type, const int *cu, int n_seqs, int m, int window, int n_heads, int n_kv,
+                          int hd, float attn_scale, void *work);
 
 /* ---------------------------------------------------------------------------
  * Step glue (main.c:1696-1778, 1988-1993, 2045-2049)

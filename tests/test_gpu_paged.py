@@ -1,0 +1,524 @@
+"""GPU parity of the paged KV cache (stored, read back), of the attention of one
+new token of every sequence over it, and of the attention of packed prompts,
+against plain forms in 64 bits (tests/paged_np.py holds them and derives the
+bounds).
+
+The cache append is main.c:1901-1904 and the attention block main.c:1909-1950
+of the reference, which runs one sequence.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import paged_np as pn
+
+pytestmark = pytest.mark.gpu
+
+F = C.c_float
+NAN = np.float32(np.nan)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from g4 import Lib
+    L = Lib.get()
+    L.init(0)
+    L.L.g4_set_stream(None)
+    return L
+
+
+def dbuf(lib, a):
+    from g4 import DBuf
+    return DBuf.from_array(lib, np.ascontiguousarray(a))
+
+
+def filled(lib, nbytes, byte=0xFF):
+    """device bytes all set: NaN in every type, codes -1"""
+    from g4 import DBuf
+    b = DBuf(lib, nbytes)
+    lib.g4_memset(b.ptr, byte, nbytes)
+    return b
+
+
+class Cache:
+    """two pools and the pages of a batch of sequences"""
+
+    def __init__(self, lib, rng, kind, hd, n_kv, page, lens, table=None, pages=None):
+        self.lib, self.kind, self.hd, self.n_kv, self.page = lib, kind, hd, n_kv, page
+        if table is None:
+            table, pages = pn.page_table(rng, lens, page)
+        self.table, self.pages = np.ascontiguousarray(table, np.int32), pages
+        size = lib.L.g4_kv_pool_bytes(kind, pages, page, n_kv, hd)
+        self.k, self.v = filled(lib, size), filled(lib, size)
+        self.dtable = dbuf(lib, self.table)
+
+    def args(self):
+        return (self.k.ptr, self.v.ptr, self.kind, self.pages, self.page, self.n_kv, self.hd, self.dtable.ptr,
+                self.table.shape[1])
+
+    def store(self, k, v, n, lens, m=None, stride=None):
+        """rows k, v [m, stride floats] of n[s] rows a sequence"""
+        dk, dv, cu, dl = (dbuf(self.lib, a) for a in (k, v, pn.starts(n), np.asarray(lens, np.int32)))
+        self.lib.g4_kv_page_store(*self.args(), dk.ptr, dv.ptr, stride or k.shape[1], cu.ptr, dl.ptr, len(n),
+                                  m or k.shape[0])
+        self.lib.g4_sync()
+
+    def load(self, n, lens, pad=0, stride=None):
+        w = stride or self.n_kv * self.hd
+        rows = sum(n) + pad
+        dk, dv = filled(self.lib, rows * w * 4, 0x3F), filled(self.lib, rows * w * 4, 0x3F)
+        cu, dl = dbuf(self.lib, pn.starts(n)), dbuf(self.lib, np.asarray(lens, np.int32))
+        self.lib.g4_kv_page_load(*self.args(), dk.ptr, dv.ptr, w, cu.ptr, dl.ptr, len(n), rows)
+        return tuple(d.to_array(np.float32).reshape(rows, w) for d in (dk, dv))
+
+
+def rows(rng, m, heads, hd):
+    return rng.standard_normal((m, heads * hd)).astype(np.float32)
+
+
+def same(a, b):
+    """equal values (signed zeros alike), NaN where NaN"""
+    return np.array_equal(a, b, equal_nan=True)
+
+
+UNTOUCHED = np.full(1, 0x3F3F3F3F, np.uint32).view(np.float32)[0]
+
+
+@pytest.mark.parametrize("kind", pn.TYPES)
+@pytest.mark.parametrize("hd,n_kv,page", [(64, 3, 16), (128, 1, 32), (256, 2, 64), (512, 2, 16), (256, 1, 4096)])
+def test_store_load(lib, kind, hd, n_kv, page):
+    """Ragged turns appended one after the other, read back whole: lengths of 0
+    and 1, pages and blocks that end inside a turn, rows past the last sequence
+    and strides wider than the rows."""
+    rng = np.random.default_rng(hd + page)
+    turns = [[5, 0, 1, 33, 16, 64, 2], [1, 1, 1, 1, 1, 1, 1], [0, 40, 15, 0, 31, 17, 14]]
+    total = np.sum(turns, 0)
+    c = Cache(lib, rng, kind, hd, n_kv, page, total)
+    had = np.zeros(7, int)
+    w = n_kv * hd
+    all_k, all_v = [[[] for _ in range(7)] for _ in range(2)]
+    for n in turns:
+        m, stride = sum(n) + 3, w + 8
+        k, v = rows(rng, m, 1, stride), rows(rng, m, 1, stride)
+        k[-3:] = v[-3:] = NAN
+        had = had + n
+        c.store(k, v, n, had, m=m)
+        at = 0
+        for s, t in enumerate(n):
+            all_k[s].append(k[at:at + t, :w])
+            all_v[s].append(v[at:at + t, :w])
+            at += t
+    wk, wv = (np.concatenate([r for s in a for r in s]) for a in (all_k, all_v))
+    for pad, stride in ((0, None), (4, w + 12)):
+        gk, gv = c.load(list(total), total, pad=pad, stride=stride)
+        n = sum(total)
+        for got, want in ((gk, wk), (gv, wv)):
+            assert same(got[:n, :w], pn.held(want, kind, hd))
+            assert (got[n:] == UNTOUCHED).all() and (got[:, w:] == UNTOUCHED).all()
+    # the last rows of each sequence only
+    last = [min(int(t), 9) for t in total]
+    gk, gv = c.load(last, total)
+    pick = np.concatenate([np.arange(e - t, e) for t, e in zip(last, np.cumsum(total))])
+    assert same(gk, pn.held(wk[pick], kind, hd)) and same(gv, pn.held(wv[pick], kind, hd))
+
+
+@pytest.mark.parametrize("kind", pn.TYPES)
+def test_store_leaves_others(lib, kind):
+    """A store changes the new positions only: every byte of the pools that
+    belongs to another position stays."""
+    rng = np.random.default_rng(3)
+    hd, n_kv, page = 128, 2, 32
+    lens = [70, 41]
+    c = Cache(lib, rng, kind, hd, n_kv, page, [96, 96])
+    full = rows(rng, 192, n_kv, hd)
+    c.store(full, full[::-1].copy(), [96, 96], [96, 96])
+    before = [np.split(a, 2) for a in c.load([96, 96], [96, 96])]
+    new = rows(rng, 12, n_kv, hd)
+    c.store(new, -new, [7, 5], lens)
+    after = [np.split(a, 2) for a in c.load([96, 96], [96, 96])]
+    for i, sign in ((0, 1), (1, -1)):
+        for s, n in ((0, 7), (1, 5)):
+            rows_new = new[:7] if s == 0 else new[7:]
+            want = before[i][s].copy()
+            want[lens[s] - n:lens[s]] = pn.held(sign * rows_new, kind, hd)
+            assert same(after[i][s], want)
+
+
+def test_q8_rows(lib):
+    """Quantisation's edges: zero rows, subnormal and huge rows, ties, one large
+    element, an infinity or NaN (the whole head reads NaN, its neighbours not)."""
+    rng = np.random.default_rng(4)
+    hd, n_kv = 256, 2
+    x = rows(rng, 16, n_kv, hd)
+    x[0] = 0
+    x[1] *= np.float32(1e-44)
+    x[2] *= np.float32(7e37)
+    x[3, :hd] = np.float32(0.5) * (np.arange(hd) % 255 - 127)     # d = 0.5: codes exact
+    x[4, :hd] = np.arange(hd) - 127.5                                # nothing exact
+    x[5, 7] = 1e6
+    x[6, 3] = np.inf
+    x[7, hd + 4] = -np.inf
+    x[8, hd - 1] = np.nan
+    x[9] = -0.0
+    x[10, :hd] = np.where(np.arange(hd) == 0, 127, 0.5 + np.arange(hd) % 100)   # d = 1: ties
+    c = Cache(lib, rng, pn.Q8, hd, n_kv, 16, [16])
+    c.store(x, x[::-1].copy(), [16], [16])
+    gk, gv = c.load([16], [16])
+    assert same(gk, pn.held(x, pn.Q8, hd)) and same(gv, pn.held(x[::-1], pn.Q8, hd))
+    assert np.isnan(gk[6, :hd]).all() and np.isfinite(gk[6, hd:]).all()
+
+
+def test_half_rows(lib):
+    """16-bit caches keep infinities and NaN, round to even and, fp16, overflow to infinity"""
+    rng = np.random.default_rng(5)
+    x = rows(rng, 16, 1, 64)
+    x[0, :6] = [np.inf, -np.inf, np.nan, 65519.9, 65520.0, 1e-8]
+    x[1, :4] = [1 + 2.0 ** -11, 1 + 3 * 2.0 ** -11, 1 + 2.0 ** -8, 1 + 3 * 2.0 ** -8]
+    for kind in (pn.F16, pn.BF16, pn.F32):
+        c = Cache(lib, rng, kind, 64, 1, 16, [16])
+        c.store(x, -x, [16], [16])
+        gk, gv = c.load([16], [16])
+        assert same(gk, pn.held(x, kind, 64)) and same(gv, pn.held(-x, kind, 64))
+
+
+def test_rows_that_do_not_fit(lib):
+    """Sequences whose lengths do not fit and pages outside the pool: skipped,
+    dropped, read as NaN; their neighbours are not touched."""
+    rng = np.random.default_rng(6)
+    hd, n_kv, page = 64, 1, 16
+    table = np.array([[0, 1], [2, 99], [3, 4], [-7, 5], [6, 7]], np.int32)
+    c = Cache(lib, rng, pn.F32, hd, n_kv, page, None, table=table, pages=8)
+    n = [20, 32, 33, 32, 10]
+    lens = np.array([20, 32, 33, 32, 9], np.int32)      # 2: past the table; 4: fewer than its rows
+    x = rows(rng, sum(n), n_kv, hd)
+    c.store(x, x, n, lens)
+    gk, _ = c.load(n, lens)
+    at = pn.starts(n)
+    part = [gk[at[s]:at[s + 1]] for s in range(5)]
+    want = [x[at[s]:at[s + 1]] for s in range(5)]
+    assert same(part[0], want[0])
+    assert same(part[1][:16], want[1][:16]) and np.isnan(part[1][16:]).all()
+    assert (part[2] == UNTOUCHED).all() and (part[4] == UNTOUCHED).all()
+    assert np.isnan(part[3][:16]).all() and same(part[3][16:], want[3][16:])
+    # row starts that are not ascending or run past m: those sequences are skipped
+    good = rows(rng, 8, n_kv, hd)
+    c2 = Cache(lib, rng, pn.F32, hd, n_kv, page, [16] * 4)
+    dk, dl = dbuf(lib, good), dbuf(lib, np.array([16, 16, 16, 16], np.int32))
+    old = rows(rng, 64, n_kv, hd)
+    c2.store(old, old, [16] * 4, [16] * 4)
+    before, _ = c2.load([16] * 4, [16] * 4)
+    cu = dbuf(lib, np.array([0, 4, 3, -2, 200], np.int32))
+    lib.g4_kv_page_store(*c2.args(), dk.ptr, dk.ptr, hd, cu.ptr, dl.ptr, 4, 8)
+    after, _ = c2.load([16] * 4, [16] * 4)
+    assert same(after[16:], before[16:])
+
+
+def run_decode(lib, c, q, lens, n_heads, window, scale, q_stride=None, out_stride=None):
+    n, hd = len(lens), c.hd
+    dq, dl = dbuf(lib, q), dbuf(lib, np.asarray(lens, np.int32))
+    os = out_stride or n_heads * hd
+    out = filled(lib, n * os * 4, 0x3F)
+    part = filled(lib, lib.L.g4_attn_decode_paged_part_bytes(n_heads, c.n_kv, hd))
+    lib.g4_attn_decode_paged(dq.ptr, q.shape[1], *c.args(), dl.ptr, n, window, n_heads, F(scale), part.ptr, out.ptr, os)
+    return out.to_array(np.float32).reshape(n, os)
+
+
+def check_decode(lib, seed, kind, hd, n_heads, n_kv, page, lens, window=0, scale=None, gain=3.0, extra=0):
+    rng = np.random.default_rng(seed)
+    scale = hd ** -0.5 if scale is None else scale
+    c = Cache(lib, rng, kind, hd, n_kv, page, lens)
+    k, v = rows(rng, sum(lens), n_kv, hd), rows(rng, sum(lens), n_kv, hd)
+    if sum(lens):
+        c.store(k, v, list(lens), lens)
+    q = rows(rng, len(lens), 1, n_heads * hd + extra) * np.float32(gain)
+    got = run_decode(lib, c, q, lens, n_heads, window, scale, out_stride=n_heads * hd + extra)
+    at = pn.starts(lens)
+    hk, hv = pn.held(k, kind, hd), pn.held(v, kind, hd)
+    for s, t in enumerate(lens):
+        o = got[s, :n_heads * hd].reshape(n_heads, hd)
+        if t == 0:
+            assert (o == 0).all(), s
+            continue
+        first = max(0, t - window) if window else 0
+        want, bound = pn.attention(q[s:s + 1, :n_heads * hd].reshape(1, n_heads, hd),
+                                   hk[at[s]:at[s + 1]].reshape(t, n_kv, hd), hv[at[s]:at[s + 1]].reshape(t, n_kv, hd),
+                                   [first], scale)
+        err = np.abs(o - want[0])
+        assert (err <= bound[0]).all(), (s, t, float((err / bound[0]).max()))
+    if extra:
+        assert (got[:, n_heads * hd:] == UNTOUCHED).all()
+
+
+@pytest.mark.parametrize("kind", pn.TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_decode_types(lib, kind, hd):
+    """every cache type and head_dim, ragged lengths with 0 and 1 among them"""
+    check_decode(lib, 10 + hd, kind, hd, 8, 2, 16, [1, 0, 15, 16, 17, 31, 33, 64, 65, 100, 257, 0, 700])
+
+
+@pytest.mark.parametrize("n_heads,n_kv", [(1, 1), (3, 3), (8, 1), (10, 2), (12, 1), (16, 1), (24, 8), (17, 1), (40, 2)])
+def test_decode_heads(lib, n_heads, n_kv):
+    """one head to twenty heads on a kv head"""
+    for kind, hd in ((pn.BF16, 128), (pn.Q8, 256)):
+        check_decode(lib, 30 + n_heads, kind, hd, n_heads, n_kv, 32, [5, 130, 64, 1])
+
+
+@pytest.mark.parametrize("window", [1, 7, 64, 100, 512, 5000])
+def test_decode_window(lib, window):
+    """windows that end inside a block, at one and past the length; pages before the window have been given away"""
+    lens = [1, 6, 63, 64, 65, 400, 1025]
+    for kind, hd, page in ((pn.F32, 256, 16), (pn.Q8, 64, 64)):
+        check_decode(lib, 50 + window, kind, hd, 4, 2, page, lens, window=window)
+
+
+def test_decode_window_pages_gone(lib):
+    """entries of pages that lie wholly before the window are never read"""
+    rng = np.random.default_rng(60)
+    hd, n_kv, page, t, w = 128, 1, 16, 200, 50
+    c = Cache(lib, rng, pn.BF16, hd, n_kv, page, [t])
+    k, v = rows(rng, t, n_kv, hd), rows(rng, t, n_kv, hd)
+    c.store(k, v, [t], [t])
+    q = rows(rng, 1, 2, hd)
+    a = run_decode(lib, c, q, [t], 2, w, 0.1)
+    c.table[0, :(t - w) // page] = -1
+    c.dtable = dbuf(lib, c.table)
+    b = run_decode(lib, c, q, [t], 2, w, 0.1)
+    assert np.isfinite(a).all() and same(a, b)
+
+
+@pytest.mark.parametrize("kind,hd", [(pn.BF16, 256), (pn.Q8, 512), (pn.F32, 64)])
+def test_decode_long(lib, kind, hd):
+    """one long sequence, split over many workgroups, beside short ones"""
+    check_decode(lib, 70, kind, hd, 4, 1, 64, [3, 20011, 0, 129])
+
+
+def test_decode_many(lib):
+    """more sequences than workgroups"""
+    rng = np.random.default_rng(71)
+    check_decode(lib, 71, pn.BF16, 64, 2, 2, 16, [int(x) for x in rng.integers(0, 40, 700)])
+
+
+def test_decode_strides(lib):
+    """q and out rows wider than their heads"""
+    check_decode(lib, 72, pn.F16, 256, 8, 2, 32, [40, 3, 77], extra=12)
+
+
+def test_decode_pages_outside(lib):
+    """a page outside the pool or a length past the table: NaN in that sequence's row and nowhere else"""
+    rng = np.random.default_rng(73)
+    hd, page = 64, 16
+    for kind in pn.TYPES:
+        c = Cache(lib, rng, kind, hd, 1, page, [40, 40, 40, 40])
+        x = rows(rng, 160, 1, hd)
+        c.store(x, x, [40] * 4, [40] * 4)
+        q = rows(rng, 4, 2, hd)
+        a = run_decode(lib, c, q, [40, 40, 40, 40], 2, 0, 0.2)
+        c.table[1, 1] = c.pages
+        c.table[2, 2] = -1
+        c.dtable = dbuf(lib, c.table)
+        b = run_decode(lib, c, q, [40, 40, 40, c.table.shape[1] * page + 1], 2, 0, 0.2)
+        assert same(a[0], b[0]) and np.isnan(b[1:]).all()
+        d = run_decode(lib, c, q, [40, 16, -3, 40], 2, 0, 0.2)
+        assert same(d[0], a[0]) and np.isfinite(d[1]).all() and np.isnan(d[2]).all() and same(d[3], a[3])
+
+
+@pytest.mark.parametrize("kind", [pn.F32, pn.F16, pn.BF16])
+def test_decode_not_finite(lib, kind):
+    """infinities and NaN at positions that are not seen change nothing; seen, they make their heads NaN or
+    infinite and no others"""
+    rng = np.random.default_rng(74)
+    hd, n_kv, page, t = 128, 2, 32, 90
+    c = Cache(lib, rng, kind, hd, n_kv, page, [128, 128])
+    k, v = rows(rng, 256, n_kv, hd), rows(rng, 256, n_kv, hd)
+    k2, v2 = k.copy(), v.copy()
+    for a in (k2, v2):      # past the length, before the window
+        a[t:128] = NAN
+        a[t + 1] = np.inf
+        a[:10] = -np.inf
+    q = rows(rng, 2, 4, hd)
+    c.store(k, v, [128, 128], [128, 128])
+    want = run_decode(lib, c, q, [t, 128], 4, 80, 0.1)
+    c.store(k2, v2, [128, 128], [128, 128])
+    assert same(run_decode(lib, c, q, [t, 128], 4, 80, 0.1), want)
+    k2[50, :5] = NAN        # seen by the heads of kv head 0 in sequence 0
+    c.store(k2, v2, [128, 128], [128, 128])
+    got = run_decode(lib, c, q, [t, 128], 4, 80, 0.1).reshape(2, 4, hd)
+    want = want.reshape(2, 4, hd)
+    assert np.isnan(got[0, :2]).all() and same(got[0, 2:], want[0, 2:]) and same(got[1], want[1])
+
+
+def test_decode_extremes(lib):
+    """scores far apart (one key takes all), all equal, large magnitudes of K and V, a negative scale"""
+    for kind in (pn.F32, pn.BF16, pn.Q8):
+        check_decode(lib, 75, kind, 128, 4, 2, 16, [50, 300], gain=60.0, scale=1.0)
+        check_decode(lib, 76, kind, 128, 4, 2, 16, [50, 300], gain=0.0, scale=1.0)
+        check_decode(lib, 77, kind, 128, 4, 2, 16, [50, 300], scale=-0.09)
+    check_decode(lib, 78, pn.BF16, 256, 4, 2, 16, [50, 300], gain=1e-18, scale=1e17)
+
+
+NPT = {pn.F32: np.float32, pn.F16: np.float16, pn.BF16: np.uint16}
+
+
+def cast(x, kind):
+    """(array of the type's bits, its values in float32)"""
+    if kind == pn.BF16:
+        b = pn.bf16_bits(x)
+        return b, pn.bf16_back(b)
+    y = x.astype(NPT[kind])
+    return y, y.astype(np.float32)
+
+
+def run_prompt(lib, q, k, v, kind, cu, m, window, n_heads, n_kv, hd, scale, out_stride=None):
+    """rows of the type's bits -> (out bits, out as float32); out starts as 0x3F3F..."""
+    es = q.dtype.itemsize
+    os = out_stride or n_heads * hd
+    out = filled(lib, m * os * es, 0x3F)
+    dq, dk, dv, dcu = (dbuf(lib, a) for a in (q, k, v, np.asarray(cu, np.int32)))
+    n = len(cu) - 1
+    work = filled(lib, lib.L.g4_attn_prompt_packed_work_bytes(kind, n, m, n_kv, hd))
+    lib.g4_attn_prompt_packed(dq.ptr, q.shape[1], dk.ptr, dv.ptr, k.shape[1], out.ptr, os, kind, dcu.ptr, n, m, window,
+                              n_heads, n_kv, hd, F(scale), work.ptr)
+    bits = out.to_array(NPT[kind]).reshape(m, os)
+    return bits, (pn.bf16_back(bits) if kind == pn.BF16 else bits.astype(np.float32))
+
+
+def check_prompt(lib, seed, kind, hd, n_heads, n_kv, n, window=0, scale=None, gain=2.0, pad=0, extra=0, some=None):
+    rng = np.random.default_rng(seed)
+    scale = hd ** -0.5 if scale is None else scale
+    m, cu = sum(n) + pad, pn.starts(n)
+    q, qf = cast(rows(rng, m, 1, n_heads * hd + extra) * np.float32(gain), kind)
+    k, kf = cast(rows(rng, m, 1, n_kv * hd + extra), kind)
+    v, vf = cast(rows(rng, m, 1, n_kv * hd + extra), kind)
+    bits, got = run_prompt(lib, q, k, v, kind, cu, m, window, n_heads, n_kv, hd, scale, out_stride=n_heads * hd + extra)
+    for s, t in enumerate(n):
+        for lo in range(0, t, 128):
+            hi = min(t, lo + 128)
+            if some is not None and lo and hi < t and lo // 128 % some:
+                continue
+            first = [max(0, i + 1 - window) if window else 0 for i in range(lo, hi)]
+            r = slice(cu[s] + lo, cu[s] + hi)
+            kk = slice(cu[s], cu[s] + hi)
+            want, bound = pn.attention(qf[r, :n_heads * hd].reshape(hi - lo, n_heads, hd),
+                                       kf[kk, :n_kv * hd].reshape(hi, n_kv, hd), vf[kk, :n_kv * hd].reshape(hi, n_kv, hd),
+                                       first, scale)
+            if kind != pn.F32:
+                # weights rounded to the type once (each off by HALF of itself: of sum p |v|, which is at most
+                # max |v|, and by the smallest subnormal's half at a maximum of 1) and the result rounded to it
+                big = np.abs(vf[kk, :n_kv * hd]).max()
+                bound = bound + pn.HALF[kind] * (np.abs(want) + 1.01 * big) + 2.0 ** -25 * hi * big
+            err = np.abs(got[r, :n_heads * hd].reshape(hi - lo, n_heads, hd) - want)
+            assert (err <= bound).all(), (s, lo, float((err / bound).max()))
+    untouched = np.full(1, 0x3F3F3F3F, np.uint32).view(bits.dtype)[0]
+    assert (bits[sum(n):] == untouched).all() and (bits[:, n_heads * hd:] == untouched).all()
+
+
+@pytest.mark.parametrize("kind", [pn.F32, pn.F16, pn.BF16])
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_prompt_types(lib, kind, hd):
+    """every type and head_dim; sequences of 0, 1 and odd lengths, rows past the last one"""
+    check_prompt(lib, 100 + hd, kind, hd, 8, 2, [1, 0, 31, 32, 33, 0, 70, 129, 2], pad=5)
+
+
+@pytest.mark.parametrize("n_heads,n_kv", [(1, 1), (3, 3), (5, 1), (8, 1), (10, 2), (12, 1), (24, 8), (20, 1)])
+def test_prompt_heads(lib, n_heads, n_kv):
+    for kind, hd in ((pn.F32, 128), (pn.BF16, 64)):
+        check_prompt(lib, 120 + n_heads, kind, hd, n_heads, n_kv, [40, 1, 65, 100])
+
+
+@pytest.mark.parametrize("window", [1, 5, 32, 64, 100, 512])
+def test_prompt_window(lib, window):
+    for kind, hd in ((pn.F32, 256), (pn.F16, 128), (pn.BF16, 512)):
+        check_prompt(lib, 140 + window, kind, hd, 4, 2, [3, 96, 150, 33], window=window)
+
+
+@pytest.mark.parametrize("kind,hd,window", [(pn.F32, 256, 512), (pn.F32, 512, 0), (pn.BF16, 256, 0), (pn.F16, 128, 300)])
+def test_prompt_long(lib, kind, hd, window):
+    """thousands of rows, the first, the last and some between them checked"""
+    check_prompt(lib, 150, kind, hd, 2, 1, [1500, 2777], window=window, some=8)
+
+
+def test_prompt_strides(lib):
+    for kind in (pn.F32, pn.F16, pn.BF16):
+        check_prompt(lib, 160, kind, 128, 4, 2, [50, 7], extra=8, pad=2)
+
+
+def test_prompt_many(lib):
+    """hundreds of short sequences"""
+    rng = np.random.default_rng(161)
+    check_prompt(lib, 161, pn.BF16, 64, 2, 1, [int(x) for x in rng.integers(0, 9, 600)])
+
+
+def test_prompt_extremes(lib):
+    """weights on one key, equal weights, a negative scale, magnitudes far from 1"""
+    for kind in (pn.F32, pn.BF16):
+        check_prompt(lib, 162, kind, 128, 4, 2, [150], gain=60.0, scale=1.0)
+        check_prompt(lib, 163, kind, 128, 4, 2, [150], gain=0.0, scale=1.0)
+        check_prompt(lib, 164, kind, 128, 4, 2, [150], scale=-0.09)
+        check_prompt(lib, 165, kind, 128, 4, 2, [150], gain=1e-18, scale=1e17)
+
+
+@pytest.mark.parametrize("kind", [pn.F32, pn.F16, pn.BF16])
+def test_prompt_not_finite(lib, kind):
+    """infinities and NaN in rows of other sequences, in rows past the last sequence and in later rows of the same
+    sequence change no row that does not see them; a row that sees them has NaN in the heads that do"""
+    rng = np.random.default_rng(166)
+    hd, n_heads, n_kv, n = 128, 4, 2, [50, 45, 20]
+    m, cu = sum(n) + 6, pn.starts(n)
+    q, k, v = (rows(rng, m, h, hd) for h in (n_heads, n_kv, n_kv))
+    a = run_prompt(lib, *(cast(x, kind)[0] for x in (q, k, v)), kind, cu, m, 0, n_heads, n_kv, hd, 0.1)[1]
+    k[cu[3]:] = v[cu[3]:] = q[cu[3]:] = NAN
+    v[50 + 37, hd + 3] = np.inf         # row 37 of sequence 1, kv head 1
+    k[50 + 40, 5] = NAN                 # row 40, kv head 0
+    b = run_prompt(lib, *(cast(x, kind)[0] for x in (q, k, v)), kind, cu, m, 0, n_heads, n_kv, hd, 0.1)[1]
+    a, b = (x.reshape(m, n_heads, hd) for x in (a, b))
+    assert same(a[:87, 2:], b[:87, 2:]) and same(a[:90, :2], b[:90, :2])
+    assert same(a[95:115], b[95:115])
+    assert not np.isfinite(b[87:95, 2:, 3]).any() and np.isnan(b[90:95, :2]).all()
+
+
+def test_prompt_starts_that_do_not_fit(lib):
+    """row starts that are not ascending or run past m: those sequences' rows are left as they are"""
+    rng = np.random.default_rng(167)
+    hd, m = 64, 40
+    q, k, v = (rows(rng, m, 2, hd) for _ in range(3))
+    bits, got = run_prompt(lib, q, k, v, pn.F32, [0, 10, 300, 290, -5], m, 0, 2, 2, hd, 0.1)
+    assert (got[10:] == UNTOUCHED).all()
+    want, bound = pn.attention(q[:10].reshape(10, 2, hd), k[:10].reshape(10, 2, hd), v[:10].reshape(10, 2, hd), [0] * 10, 0.1)
+    assert (np.abs(got[:10].reshape(10, 2, hd) - want) <= bound).all() or (got[:10] == UNTOUCHED).all()
+
+
+def test_serving(lib):
+    """The operators as a server uses them: prompts of a ragged batch (attention, cache written), then steps of
+    one token each; every output equals a plain forward over the whole sequences."""
+    rng = np.random.default_rng(200)
+    hd, n_heads, n_kv, page, window, scale = 256, 8, 2, 16, 100, 1 / 16
+    n, steps = [37, 1, 130, 64], 20
+    lens = np.array(n)
+    total = [t + steps for t in n]
+    seqs = [tuple(rows(rng, t, h, hd) for h in (n_heads, n_kv, n_kv)) for t in total]
+    for kind in pn.TYPES:
+        c = Cache(lib, rng, kind, hd, n_kv, page, total)
+        q, k, v = (np.concatenate([s[i][:t] for s, t in zip(seqs, n)]) for i in range(3))
+        got = [[x] for x in np.split(run_prompt(lib, q, k, v, pn.F32, pn.starts(n), len(q), window, n_heads, n_kv, hd,
+                                                scale)[1], pn.starts(n)[1:-1])]
+        c.store(k, v, n, n)
+        for i in range(steps):
+            q, k, v = (np.stack([s[j][t + i] for s, t in zip(seqs, n)]) for j in range(3))
+            c.store(k, v, [1] * 4, lens + i + 1)
+            o = run_decode(lib, c, q, lens + i + 1, n_heads, window, scale)
+            for s in range(4):
+                got[s].append(o[s:s + 1])
+        gk, _ = c.load(total, total)
+        assert same(gk, pn.held(np.concatenate([s[1] for s in seqs]), kind, hd))
+        for s, t in enumerate(n):
+            qs, ks, vs = seqs[s]
+            o = np.concatenate(got[s]).reshape(total[s], n_heads, hd)
+            hk, hv = pn.held(ks, kind, hd), pn.held(vs, kind, hd)
+            first = [max(0, i + 1 - window) for i in range(total[s])]
+            want, bound = pn.attention(qs[:t].reshape(t, n_heads, hd), ks[:t].reshape(t, n_kv, hd),
+                                       vs[:t].reshape(t, n_kv, hd), first[:t], scale)
+            assert (np.abs(o[:t] - want) <= bound).all()
+            want, bound = pn.attention(qs[t:].reshape(steps, n_heads, hd), hk.reshape(-1, n_kv, hd),
+                                       hv.reshape(-1, n_kv, hd), first[t:], scale)
+            assert (np.abs(o[t:] - want) <= bound).all()
