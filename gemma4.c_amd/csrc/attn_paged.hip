@@ -8,6 +8,14 @@
 namespace g4 {
 namespace {
 
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+
+// workgroups that share the work: one a CU at head_dim 512, whose sums take half the registers, else two
+constexpr int kPagedMaxWG = 512;
+constexpr int paged_lg_wg(int hd) { return hd == 512 ? 8 : 9; }
+constexpr int kHeadsWG = 16;                                // q heads of a workgroup: the columns of a product
+constexpr float kLog2e = 1.4426950408889634f;
+
 struct PagedArgs {
     KvPool p;
     const float* q;
@@ -15,73 +23,571 @@ struct PagedArgs {
     const int* lens;
     float* part;
     int q_stride, out_stride, n_seqs, window, n_heads;
+    int group, ngrp;   // q heads a kv head, workgroup columns' groups of them
     float scale;
 };
 
-template <int TYPE>
-__device__ __forceinline__ float elem(const uint8_t* p) {
-    if (TYPE == G4_F32) return *reinterpret_cast<const float*>(p);
-    if (TYPE == G4_F16) return (float)*reinterpret_cast<const _Float16*>(p);
-    if (TYPE == G4_BF16) return bf16_to_f32(*reinterpret_cast<const uint16_t*>(p));
-    return (float)*reinterpret_cast<const int8_t*>(p);
+// ---- shares of the work ------------------------------------------------------
+// An item is a sequence, a kv head and up to 16 of its q heads; it consists of
+// the 32-key tiles its window touches.  All items' tiles form one line,
+// sequences in order, and workgroup w takes the tiles N w / 512 .. N (w + 1) /
+// 512 - 1 of it, whatever the lengths are: a long sequence is spread over many
+// workgroups, many short ones share one.
+
+// tiles of a sequence and its first one; 0 tiles: an empty sequence or a
+// length that does not fit
+__device__ __forceinline__ int seq_tiles(const PagedArgs& a, int len, int& first) {
+    first = 0;
+    if (len <= 0 || !a.p.fits(len)) return 0;
+    if (a.window > 0 && len > a.window) first = (len - a.window) >> 5;
+    return ((len - 1) >> 5) - first + 1;
 }
 
-// One workgroup a head and sequence, a key a wave at a time:
-// s_t = scale q . K_t, o = sum_t softmax(s)_t V_t with a running maximum.
-template <int TYPE, int HD>
-__global__ __launch_bounds__(256) void attn_paged_simple_kernel(PagedArgs a) {
-    constexpr int ES = TYPE == G4_F32 ? 4 : TYPE == G4_KV_Q8 ? 1 : 2, N = HD / 64;
-    const int h = blockIdx.x, s = blockIdx.y, kvh = h / (a.n_heads / a.p.n_kv);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __shared__ float red[4][HD + 2];
-    const int len = a.lens[s];
-    bool bad = !a.p.fits(len);
-    const int last = bad ? 0 : len, first = a.window > 0 && last > a.window ? last - a.window : 0;
-    float q[N], o[N] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; i++) q[i] = a.q[(size_t)s * a.q_stride + h * HD + i * 64 + lane] * a.scale;
-    for (int t = first + wave; t < last; t += 4) {
-        const int page = a.p.page_of(s, t);
-        if (page < 0) { bad = true; break; }
-        const size_t block = a.p.block_of(page, kvh, t);
-        const uint8_t* kb = a.p.kp + block * (16 * HD * ES);
-        const uint8_t* vb = a.p.vp + block * (16 * HD * ES);
-        float x = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; i++) x = fmaf(q[i], elem<TYPE>(kb + kv_k_byte<ES>(t & 15, i * 64 + lane)), x);
-        x = wave_sum(x);
-        float dv = 1.0f;
-        if (TYPE == G4_KV_Q8) {
-            x *= reinterpret_cast<const float*>(a.p.kp + a.p.scale_off)[block * 16 + (t & 15)];
-            dv = reinterpret_cast<const float*>(a.p.vp + a.p.scale_off)[block * 16 + (t & 15)];
-        }
-        const float mn = fmaxf(m, x), f = m == mn ? 1.0f : expf(m - mn), w = expf(x - mn);
-        l = l * f + w;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < N; i++) o[i] = fmaf(w * dv, elem<TYPE>(vb + kv_v_byte<ES>(t & 15, i * 64 + lane)), o[i] * f);
+struct Line {
+    unsigned long long total;   // N, all tiles
+    unsigned long long before;  // tiles of one (kv head, heads) before sequence s
+    int s;
+};
+
+// N and the sequence that tile u = at(N) lies in (of_seq >= 0: that sequence
+// instead), by the whole workgroup of 256 threads: a prefix sum over the
+// lengths, which is cheaper than a launch that would leave it in memory
+template <typename At>
+__device__ __forceinline__ Line find_line(const PagedArgs& a, At at, int of_seq, unsigned long long* red) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = (a.n_seqs + 255) >> 8, s0 = tid * per;
+    const int rep = a.p.n_kv * a.ngrp;
+    unsigned long long sum = 0;
+    for (int i = 0; i < per; i++) {
+        int f;
+        if (s0 + i < a.n_seqs) sum += seq_tiles(a, a.lens[s0 + i], f);
     }
-    if (bad) l = __uint_as_float(0x7fc00000u);
+    unsigned long long x = sum;
 #pragma unroll
-    for (int i = 0; i < N; i++) red[wave][i * 64 + lane] = o[i];
-    if (lane == 0) { red[wave][HD] = m; red[wave][HD + 1] = l; }
-    __syncthreads();
-    float top = -INFINITY;
-    for (int w = 0; w < 4; w++) top = fmaxf(top, red[w][HD]);
-    for (int d = threadIdx.x; d < HD; d += 256) {
-        float num = 0.0f, den = 0.0f;
-        for (int w = 0; w < 4; w++) {
-            const float f = red[w][HD] == top ? 1.0f : expf(red[w][HD] - top);
-            num += f * red[w][d];
-            den += f * red[w][HD + 1];
+    for (int d = 1; d < 64; d <<= 1) {
+        const unsigned long long o = __shfl_up(x, d, 64);
+        if (lane >= d) x += o;
+    }
+    if (lane == 63) red[wave] = x;
+    lds_sync();
+    unsigned long long base = 0, all = 0;
+    for (int w = 0; w < 4; w++) {
+        if (w < wave) base += red[w];
+        all += red[w];
+    }
+    unsigned long long before = base + x - sum;
+    Line r;
+    r.total = all * rep;
+    const unsigned long long u = at(r.total);
+    if (of_seq >= 0 ? s0 <= of_seq && of_seq < s0 + per : u >= before * rep && u < (before + sum) * rep) {
+        int s = s0;
+        for (;; s++) {
+            int f;
+            const int t = seq_tiles(a, a.lens[s], f);
+            if (of_seq >= 0 ? s == of_seq : u < (before + t) * rep) break;
+            before += t;
         }
-        a.out[(size_t)s * a.out_stride + h * HD + d] = den == 0.0f ? 0.0f : num / den;
+        red[4] = before;
+        red[5] = (unsigned)s;
+    }
+    lds_sync();
+    r.before = red[4];
+    r.s = (int)red[5];
+    return r;
+}
+
+// floats of a partial result: [head][hd] sums, then each head's maximum and weight sum
+__host__ __device__ inline size_t part_floats(int group, int hd) {
+    return (size_t)(group < kHeadsWG ? group : kHeadsWG) * (hd + 2);
+}
+
+// ---- operands ------------------------------------------------------------------
+// A float is the sum of three bf16: its leading 8, middle 8 and last 8 bits.
+// Every product of two such terms is exact, so that matrix instructions on 16
+// bits give the fp32 product.
+__device__ __forceinline__ uint32_t hi_halves(uint32_t x0, uint32_t x1) { return __builtin_amdgcn_perm(x1, x0, 0x07060302u); }
+__device__ __forceinline__ float rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+template <int NT>
+__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&t)[NT]) {
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        t[i] = hi_halves(__float_as_uint(x0), __float_as_uint(x1));
+        if (i + 1 < NT) {
+            x0 = rest(x0);
+            x1 = rest(x1);
+        }
+    }
+}
+__device__ __forceinline__ b8_t as_b8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_bit_cast(b8_t, make_uint4(a, b, c, d));
+}
+
+template <int TYPE>
+struct CacheType;
+template <>
+struct CacheType<G4_F32> { static constexpr int ES = 4, NT = 3; };
+template <>
+struct CacheType<G4_F16> { static constexpr int ES = 2, NT = 2; };   // 11 bits: two terms
+template <>
+struct CacheType<G4_BF16> { static constexpr int ES = 2, NT = 1; };
+template <>
+struct CacheType<G4_KV_Q8> { static constexpr int ES = 1, NT = 1; };
+
+// two cached elements of a word pair as bf16 terms; codes (|c| <= 128) are exact in one
+template <int TYPE>
+__device__ __forceinline__ void pair_terms(const uint32_t* w, int i, uint32_t (&t)[CacheType<TYPE>::NT]) {
+    if constexpr (TYPE == G4_F32) {
+        split_pair<3>(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]), t);
+    } else if constexpr (TYPE == G4_F16) {
+        const h2_t h = bits_h2(w[i]);
+        split_pair<2>((float)h[0], (float)h[1], t);
+    } else if constexpr (TYPE == G4_BF16) {
+        t[0] = w[i];
+    } else {
+        const int c0 = (int8_t)(w[i >> 1] >> (i & 1 ? 16 : 0)), c1 = (int8_t)(w[i >> 1] >> (i & 1 ? 24 : 8));
+        t[0] = hi_halves(__float_as_uint((float)c0), __float_as_uint((float)c1));
+    }
+}
+// eight elements that start at element 2 * i0 of w
+template <int TYPE>
+__device__ __forceinline__ void oct_terms(const uint32_t* w, int i0, b8_t (&t)[CacheType<TYPE>::NT]) {
+    constexpr int NT = CacheType<TYPE>::NT;
+    uint32_t p[4][NT];
+#pragma unroll
+    for (int i = 0; i < 4; i++) pair_terms<TYPE>(w, i0 + i, p[i]);
+#pragma unroll
+    for (int k = 0; k < NT; k++) t[k] = as_b8(p[0][k], p[1][k], p[2][k], p[3][k]);
+}
+// c + small += a . b over terms; what is left out is below 2^-30 of the
+// product.  The leading terms' products have the sum c to themselves: a sum
+// of 16 products and not of 16 x 6 loses that much less to rounding, which
+// matters in scores (exponents), while the others are 2^-7 of it and less.
+template <int NT>
+__device__ __forceinline__ void mfma_terms(const b8_t (&a)[NT], const b8_t (&b)[3], f4_t& c, f4_t& small) {
+#pragma unroll
+    for (int i = NT - 1; i >= 0; i--)
+#pragma unroll
+        for (int j = 2; j >= 0; j--) {
+            if (i + j == 0) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[0], c, 0, 0, 0);
+            else if (i + j < 4) small = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], small, 0, 0, 0);
+        }
+}
+
+// One wave takes 32 keys at a time, S^T = K Q^T (rows keys, columns q heads):
+// a lane then holds the scores of one head at the eight keys 4 g + r and
+// 16 + 4 g + r, which are, as they stand, its operand of O^T += V^T P^T (rows
+// dims).  The cache's layout has each lane's K and V operands in 16
+// consecutive bytes, so keys and values go from memory to the products through
+// registers alone: no LDS, no barrier and no lane exchange but the one of the
+// running maximum, which moves only when a score passes it by 2^8.
+// Bound by the cache's bytes; DEPTH loads of 1 KB stay in flight a wave.
+template <int TYPE, int HD, int DEPTH>
+__global__ __launch_bounds__(256, HD == 512 ? 1 : 2) void attn_paged_kernel(PagedArgs a) {
+    constexpr int ES = CacheType<TYPE>::ES, NT = CacheType<TYPE>::NT, kLgWG = paged_lg_wg(HD);
+    constexpr int KC = HD * ES / 64;                      // 1 KB pieces of a 16-token block
+    constexpr int CPS = ES == 4 ? 2 : 1;                  // pieces of a product step of 32 dims (ES 1: half a piece)
+    constexpr int SPC = ES == 1 ? 2 : 1;                  // product steps of a piece
+    constexpr int NL = 4 * KC, STEPS = HD / 32, NTILE = HD / 16, TPC = 4 / ES;   // TPC: 16-dim tiles of a V piece
+    static_assert(NL % DEPTH == 0, "ring");
+    constexpr int kQBytes = STEPS * 3 * 1024, kSumBytes = 2 * NTILE * 1024;
+    __shared__ __align__(16) uint8_t buf[kQBytes > kSumBytes ? kQBytes : kSumBytes];
+    __shared__ unsigned long long red[8];
+    __shared__ float mls[2][4][kHeadsWG];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned w = blockIdx.x;
+    const Line ln = find_line(a, [&](unsigned long long n) { return (n * w) >> kLgWG; }, -1, red);
+    unsigned long long cur = (ln.total * w) >> kLgWG;
+    const unsigned long long end = (ln.total * (w + 1)) >> kLgWG;
+    if (cur >= end) return;
+    const int rep = a.p.n_kv * a.ngrp;
+    int s = __builtin_amdgcn_readfirstlane(ln.s);
+    unsigned off = (unsigned)(cur - ln.before * rep);     // tile within the sequence's items
+    int first_tile, len = __builtin_amdgcn_readfirstlane(a.lens[s]);
+    int tiles = seq_tiles(a, len, first_tile);
+    int item = __builtin_amdgcn_readfirstlane((int)(off / (unsigned)tiles));
+    int tile0 = __builtin_amdgcn_readfirstlane((int)(off - (unsigned)item * tiles));
+    while (true) {
+        const unsigned long long left = end - cur;
+        const int tile1 = left < (unsigned long long)(tiles - tile0) ? tile0 + (int)left : tiles;
+        const int kvh = item / a.ngrp, hg = item - kvh * a.ngrp;
+        const int nh = a.group - hg * kHeadsWG < kHeadsWG ? a.group - hg * kHeadsWG : kHeadsWG;
+        const int head0 = kvh * a.group + hg * kHeadsWG;
+        const int first = a.window > 0 && len > a.window ? len - a.window : 0;
+
+        // ---- q, times scale log2(e), as three terms in the products' order ----
+        const float qs = a.scale * kLog2e;
+        for (int x = tid; x < STEPS * 64; x += 256) {
+            const int st = x >> 6, l = x & 63, lg = l >> 4, lc = l & 15;
+            float4 q0 = make_float4(0, 0, 0, 0), q1 = q0;
+            if (lc < nh) {
+                const float* qr = a.q + (size_t)s * a.q_stride + (size_t)(head0 + lc) * HD;
+                const int d0 = ES == 4 ? st * 32 + lg * 4 : ES == 2 ? st * 32 + lg * 8 : (st >> 1) * 64 + lg * 16 + (st & 1) * 8;
+                q0 = *reinterpret_cast<const float4*>(qr + d0);
+                q1 = *reinterpret_cast<const float4*>(qr + d0 + (ES == 4 ? 16 : 4));
+            }
+            uint32_t t[4][3];
+            split_pair<3>(q0.x * qs, q0.y * qs, t[0]);
+            split_pair<3>(q0.z * qs, q0.w * qs, t[1]);
+            split_pair<3>(q1.x * qs, q1.y * qs, t[2]);
+            split_pair<3>(q1.z * qs, q1.w * qs, t[3]);
+#pragma unroll
+            for (int k = 0; k < 3; k++)
+                reinterpret_cast<uint4*>(buf)[(st * 3 + k) * 64 + l] = make_uint4(t[0][k], t[1][k], t[2][k], t[3][k]);
+        }
+        lds_sync();
+
+        // ---- the wave's tiles ----
+        f4_t o[NTILE] = {};
+        float m = -INFINITY, l = 0.0f;
+        bool bad = false;
+        // where a tile's two blocks are; blocks without a key in use take the other's place
+        size_t blk[2], nblk[2];
+        auto place = [&](int tile, size_t (&b)[2]) {
+            const int pos = (first_tile + tile) << 5;
+            const int pa = pos + 16 > first ? pos : pos + 16, pb = pos + 16 < len ? pos + 16 : pos;
+            const int ga = a.p.page_of(s, pa), gb = a.p.page_of(s, pb);
+            bad = bad || ga < 0 || gb < 0;
+            b[0] = a.p.block_of(ga < 0 ? 0 : ga, kvh, pa);
+            b[1] = a.p.block_of(gb < 0 ? 0 : gb, kvh, pb);
+        };
+        auto rsrc = [&](const uint8_t* pool, size_t b, bool on) {
+            return __builtin_amdgcn_make_buffer_rsrc((void*)(pool + b * (16 * HD * ES)), 0, on ? 16 * HD * ES : 0, kBufWord3);
+        };
+        // load i of a tile: K pieces in the order of the product steps, then V pieces, blocks in turn
+        auto load = [&](int i, const __amdgpu_buffer_rsrc_t (&k)[2], const __amdgpu_buffer_rsrc_t (&v)[2]) {
+            if (i < 2 * KC) {
+                const int b = i / CPS & 1, c = i / (2 * CPS) * CPS + i % CPS;
+                return buf_load16(k[b], lane * 16, c * 1024);
+            }
+            return buf_load16(v[i & 1], lane * 16, (i - 2 * KC) / 2 * 1024);
+        };
+        int tile = tile0 + wave;
+        if (tile < tile1) {
+            uint4 ring[DEPTH];
+            place(tile, blk);
+            __amdgpu_buffer_rsrc_t kr[2], vr[2], kn[2], vn[2];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                kr[b] = rsrc(a.p.kp, blk[b], true);
+                vr[b] = rsrc(a.p.vp, blk[b], true);
+            }
+#pragma unroll
+            for (int i = 0; i < DEPTH; i++) ring[i] = load(i, kr, vr);
+            for (; tile < tile1; tile += 4) {
+                const bool more = tile + 4 < tile1;
+                if (more) {
+                    place(tile + 4, nblk);
+                } else {
+                    nblk[0] = blk[0];
+                    nblk[1] = blk[1];
+                }
+                // past the last tile the loads have no bytes to read
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    kn[b] = rsrc(a.p.kp, nblk[b], more);
+                    vn[b] = rsrc(a.p.vp, nblk[b], more);
+                }
+                float ksc[8], vsc[8];
+                if (TYPE == G4_KV_Q8) {
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        const float4 x = reinterpret_cast<const float4*>(a.p.kp + a.p.scale_off)[blk[b] * 4 + g];
+                        const float4 y = reinterpret_cast<const float4*>(a.p.vp + a.p.scale_off)[blk[b] * 4 + g];
+                        ksc[4 * b] = x.x; ksc[4 * b + 1] = x.y; ksc[4 * b + 2] = x.z; ksc[4 * b + 3] = x.w;
+                        vsc[4 * b] = y.x; vsc[4 * b + 1] = y.y; vsc[4 * b + 2] = y.z; vsc[4 * b + 3] = y.w;
+                    }
+                }
+                auto take = [&](int i) {
+                    const uint4 x = ring[i % DEPTH];
+                    ring[i % DEPTH] = i + DEPTH < NL ? load(i + DEPTH, kr, vr) : load(i + DEPTH - NL, kn, vn);
+                    return x;
+                };
+                f4_t sc[2] = {}, ss[2] = {};
+#pragma unroll
+                for (int st = 0; st < STEPS / SPC; st++) {
+                    b8_t qt[SPC][3];
+#pragma unroll
+                    for (int h = 0; h < SPC; h++)
+#pragma unroll
+                        for (int k = 0; k < 3; k++)
+                            qt[h][k] = __builtin_bit_cast(b8_t, reinterpret_cast<const uint4*>(buf)[((st * SPC + h) * 3 + k) * 64 + lane]);
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        uint32_t x[4 * CPS];
+#pragma unroll
+                        for (int c = 0; c < CPS; c++) {
+                            const uint4 y = take((st * 2 + b) * CPS + c);
+                            x[4 * c] = y.x; x[4 * c + 1] = y.y; x[4 * c + 2] = y.z; x[4 * c + 3] = y.w;
+                        }
+#pragma unroll
+                        for (int h = 0; h < SPC; h++) {
+                            b8_t kt[NT];
+                            oct_terms<TYPE>(x, 4 * h, kt);
+                            mfma_terms<NT>(kt, qt[h], sc[b], ss[b]);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // ---- weights ----
+                const int pos = ((first_tile + tile) << 5) + 4 * g;
+                float x[8], top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int key = pos + 16 * (i >> 2) + (i & 3);
+                    float y = sc[i >> 2][i & 3] + ss[i >> 2][i & 3];
+                    if (TYPE == G4_KV_Q8) y *= ksc[i];
+                    x[i] = key >= first && key < len ? y : -INFINITY;
+                    top = fmaxf(top, x[i]);
+                }
+                if (__any(top > m + 8.0f)) {
+                    top = fmaxf(top, shfl_xor(top, 16));
+                    top = fmaxf(top, shfl_xor(top, 32));
+                    top = fmaxf(top, m);
+                    const float f = top == m ? 1.0f : exp2f(m - top);
+                    m = top;
+                    l *= f;
+#pragma unroll
+                    for (int i = 0; i < NTILE; i++) o[i] *= f;
+                }
+                uint32_t pw[4][3];
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    float p[2];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int key = pos + 16 * ((i + j) >> 2) + ((i + j) & 3);
+                        const bool in = key >= first && key < len;
+                        p[j] = in ? exp2f(x[i + j] - m) : 0.0f;
+                        l += p[j];
+                        if (TYPE == G4_KV_Q8) p[j] = in ? p[j] * vsc[i + j] : 0.0f;
+                    }
+                    split_pair<3>(p[0], p[1], pw[i / 2]);
+                }
+                b8_t pt[3];
+#pragma unroll
+                for (int k = 0; k < 3; k++) pt[k] = as_b8(pw[0][k], pw[1][k], pw[2][k], pw[3][k]);
+                // elements of keys not in use count as 0, whatever is left there
+                uint32_t keep[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int key = pos + 16 * (i >> 2) + (i & 3);
+                    keep[i] = key >= first && key < len ? 0xffffffffu : 0u;
+                }
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    uint4 y[2];
+                    y[0] = take(2 * KC + 2 * c);
+                    y[1] = take(2 * KC + 2 * c + 1);
+#pragma unroll
+                    for (int i = 0; i < TPC; i++) {
+                        // this lane's dim of tile c * TPC + i at its eight keys
+                        uint32_t v[2 * ES];
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {
+                            const uint32_t z[4] = {y[b].x, y[b].y, y[b].z, y[b].w};
+#pragma unroll
+                            for (int j = 0; j < ES; j++) {
+                                uint32_t k;
+                                if (ES == 4) k = keep[4 * b + j];
+                                else if (ES == 2) k = __builtin_amdgcn_perm(keep[4 * b + 2 * j + 1], keep[4 * b + 2 * j], 0x05040100u);
+                                else k = __builtin_amdgcn_perm(__builtin_amdgcn_perm(keep[4 * b + 3], keep[4 * b + 2], 0x0c0c0400u),
+                                                               __builtin_amdgcn_perm(keep[4 * b + 1], keep[4 * b], 0x0c0c0400u), 0x05040100u);
+                                v[b * ES + j] = z[i * ES + j] & k;
+                            }
+                        }
+                        b8_t vt[NT];
+                        oct_terms<TYPE>(v, 0, vt);
+                        mfma_terms<NT>(vt, pt, o[c * TPC + i], o[c * TPC + i]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                blk[0] = nblk[0];
+                blk[1] = nblk[1];
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    kr[b] = kn[b];
+                    vr[b] = vn[b];
+                }
+            }
+        }
+
+        // ---- the four waves' sums: 2, 3 -> 0, 1 -> 0 ----
+        l += shfl_xor(l, 16);
+        l += shfl_xor(l, 32);
+        if (bad) l = __uint_as_float(0x7fc00000u);
+        if (g == 0) {
+            mls[0][wave][col] = m;
+            mls[1][wave][col] = l;
+        }
+        lds_sync();   // q is no longer needed
+        float top = -INFINITY, sum = 0.0f, mine = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) top = fmaxf(top, mls[0][i][col]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float mi = mls[0][i][col], f = mi == top ? 1.0f : exp2f(mi - top);
+            sum += f * mls[1][i][col];
+            if (i == wave) mine = f;
+        }
+#pragma unroll
+        for (int i = 0; i < NTILE; i++) o[i] *= mine;
+        f4_t* box = reinterpret_cast<f4_t*>(buf) + (wave & 1) * NTILE * 64 + lane;
+        if (wave >= 2) {
+#pragma unroll
+            for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
+        }
+        lds_sync();
+        if (wave < 2) {
+#pragma unroll
+            for (int i = 0; i < NTILE; i++) o[i] += box[i * 64];
+            if (wave == 1) {
+#pragma unroll
+                for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
+            }
+        }
+        lds_sync();
+        if (wave == 0 && col < nh) {
+            const bool whole = tile0 == 0 && tile1 == tiles;
+            float* to;
+            float f = 1.0f;
+            if (whole) {
+                to = a.out + (size_t)s * a.out_stride + (size_t)(head0 + col) * HD;
+                f = 1.0f / sum;
+            } else {
+                float* slot = a.part + ((size_t)w * 2 + (tile0 == 0)) * part_floats(a.group, HD);
+                to = slot + col * HD;
+                if (g == 0) {
+                    slot += (a.group < kHeadsWG ? a.group : kHeadsWG) * HD;
+                    slot[2 * col] = top;
+                    slot[2 * col + 1] = sum;
+                }
+            }
+            box = reinterpret_cast<f4_t*>(buf) + NTILE * 64 + lane;
+#pragma unroll
+            for (int i = 0; i < NTILE; i++) {
+                const f4_t r = (o[i] + box[i * 64]) * f;
+                *reinterpret_cast<f4_t*>(to + i * 16 + g * 4) = r;
+            }
+        }
+        cur += (unsigned)(tile1 - tile0);
+        if (cur >= end) break;
+        lds_sync();   // the sums' place takes q again
+        if (tile1 < tiles || ++item == rep) {
+            item = 0;
+            do {
+                len = __builtin_amdgcn_readfirstlane(a.lens[++s]);
+                tiles = seq_tiles(a, len, first_tile);
+            } while (tiles == 0);
+        }
+        tile0 = 0;
+    }
+}
+
+// Joins the pieces of every sequence and head that more than one workgroup
+// took, with the weights 2^(m_i - max m); sequences without keys get zeros,
+// those whose length does not fit NaN.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
+    constexpr int LPR = HD / 4, GR = 256 / LPR, kLgWG = paged_lg_wg(HD);   // lanes a row of HD floats, pieces at a time
+    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    const int kvh = h / a.group, hg = (h - kvh * a.group) / kHeadsWG, col = h - kvh * a.group - hg * kHeadsWG;
+    __shared__ unsigned long long red[8];
+    __shared__ float fac[kPagedMaxWG], wred[4];
+    __shared__ __align__(16) float4 acc[256];
+    float* out = a.out + (size_t)s * a.out_stride + (size_t)h * HD;
+    const int len = a.lens[s];
+    int first;
+    const int tiles = seq_tiles(a, len, first);
+    if (tiles == 0) {
+        const float x = len == 0 ? 0.0f : __uint_as_float(0x7fc00000u);
+        if (tid < LPR) reinterpret_cast<float4*>(out)[tid] = make_float4(x, x, x, x);
+        return;
+    }
+    const Line ln = find_line(a, [](unsigned long long) { return 0ull; }, s, red);
+    const unsigned long long u0 = ln.before * (a.p.n_kv * a.ngrp) + (unsigned long long)(kvh * a.ngrp + hg) * tiles;
+    const unsigned long long n = ln.total;
+    const int w0 = (int)((((u0 + 1) << kLgWG) - 1) / n), w1 = (int)((((u0 + tiles) << kLgWG) - 1) / n);
+    if (w0 == w1) return;   // one workgroup had it all
+    // fewer tiles than workgroups: a tile each, some workgroups between them without one
+    const bool few = n < (1u << kLgWG);
+    const int np = few ? tiles : w1 - w0 + 1, gh = a.group < kHeadsWG ? a.group : kHeadsWG;
+    const size_t pf = part_floats(a.group, HD);
+    auto slot = [&](int i) {
+        const int w = few ? (int)(((((unsigned)u0 + i + 1) << kLgWG) - 1) / (unsigned)n) : w0 + i;
+        return a.part + ((size_t)w * 2 + (i == 0)) * pf;
+    };
+    // maxima, factors, weight sums: pieces tid and tid + 256
+    float m[2], l[2], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int i = tid + 256 * k;
+        m[k] = -INFINITY;
+        l[k] = 0.0f;
+        if (i < np) {
+            const float2 x = reinterpret_cast<const float2*>(slot(i) + gh * HD)[col];
+            m[k] = x.x;
+            l[k] = x.y;
+        }
+        top = fmaxf(top, m[k]);
+    }
+    top = wave_max(top);
+    if ((tid & 63) == 0) wred[tid >> 6] = top;
+    lds_sync();
+    top = fmaxf(fmaxf(wred[0], wred[1]), fmaxf(wred[2], wred[3]));
+    lds_sync();
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const float f = m[k] == top ? 1.0f : exp2f(m[k] - top);
+        fac[tid + 256 * k] = f;
+        sum += f * l[k];
+    }
+    sum = wave_sum(sum);
+    if ((tid & 63) == 0) wred[tid >> 6] = sum;
+    lds_sync();
+    sum = (wred[0] + wred[1]) + (wred[2] + wred[3]);
+    const int c = tid % LPR, gr = tid / LPR;
+    float4 x = make_float4(0, 0, 0, 0);
+    for (int i = gr; i < np; i += 8 * GR) {
+        float4 y[8];
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int j = i + k * GR < np ? i + k * GR : gr;
+            y[k] = reinterpret_cast<const float4*>(slot(j) + col * HD)[c];
+            f[k] = i + k * GR < np ? fac[j] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (i + k * GR >= np) continue;
+            x.x = fmaf(f[k], y[k].x, x.x);
+            x.y = fmaf(f[k], y[k].y, x.y);
+            x.z = fmaf(f[k], y[k].z, x.z);
+            x.w = fmaf(f[k], y[k].w, x.w);
+        }
+    }
+    acc[tid] = x;
+    lds_sync();
+    if (tid < LPR) {
+#pragma unroll
+        for (int k = 1; k < GR; k++) {
+            const float4 y = acc[k * LPR + tid];
+            x.x += y.x;
+            x.y += y.y;
+            x.z += y.z;
+            x.w += y.w;
+        }
+        const float r = 1.0f / sum;
+        reinterpret_cast<float4*>(out)[tid] = make_float4(x.x * r, x.y * r, x.z * r, x.w * r);
     }
 }
 
 template <int TYPE, int HD>
 void launch_paged(const PagedArgs& a) {
-    hipLaunchKernelGGL((attn_paged_simple_kernel<TYPE, HD>), dim3(a.n_heads, a.n_seqs), dim3(256), 0, g4_stream(), a);
+    constexpr int NL = HD * CacheType<TYPE>::ES / 16, R = HD == 512 ? 32 : 16, D = NL < R ? NL : R;
+    hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D>), dim3(1 << paged_lg_wg(HD)), dim3(256), 0, g4_stream(), a);
+    hipLaunchKernelGGL((attn_paged_join_kernel<HD>), dim3(a.n_heads, a.n_seqs), dim3(256), 0, g4_stream(), a);
 }
 template <int TYPE>
 void launch_paged(const PagedArgs& a, int hd) {
@@ -96,12 +602,9 @@ void launch_paged(const PagedArgs& a, int hd) {
 
 using namespace g4;
 
-constexpr int kPagedWG = 512;
-
 extern "C" size_t g4_attn_decode_paged_part_bytes(int n_heads, int n_kv, int hd) {
     if (n_heads < 1 || n_kv < 1 || n_heads % n_kv || (hd != 64 && hd != 128 && hd != 256 && hd != 512)) return 0;
-    const int g = n_heads / n_kv < 16 ? n_heads / n_kv : 16;
-    return (size_t)kPagedWG * 2 * g * (hd + 2) * 4;
+    return (size_t)kPagedMaxWG * 2 * part_floats(n_heads / n_kv, hd) * 4;
 }
 
 extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp, const void* vp, int type, int n_pages,
@@ -120,6 +623,8 @@ extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp
                  kKvMaxSeqs, window);
     a.q = q; a.out = out; a.lens = lens; a.part = part; a.q_stride = q_stride; a.out_stride = out_stride;
     a.n_seqs = n_seqs; a.window = window; a.n_heads = n_heads; a.scale = attn_scale;
+    a.group = n_heads / n_kv;
+    a.ngrp = (a.group + kHeadsWG - 1) / kHeadsWG;
     if (type == G4_F32) launch_paged<G4_F32>(a, hd);
     else if (type == G4_F16) launch_paged<G4_F16>(a, hd);
     else if (type == G4_BF16) launch_paged<G4_BF16>(a, hd);
