@@ -10,9 +10,7 @@ namespace {
 
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
-// workgroups that share the work: one a CU at head_dim 512, whose sums take half the registers, else two
-constexpr int kPagedMaxWG = 512;
-constexpr int paged_lg_wg(int hd) { return hd == 512 ? 8 : 9; }
+constexpr int kLgWG = 9, kPagedWG = 1 << kLgWG;   // workgroups that share the work, two a CU
 constexpr int kHeadsWG = 16;                                // q heads of a workgroup: the columns of a product
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -24,15 +22,17 @@ struct PagedArgs {
     float* part;
     int q_stride, out_stride, n_seqs, window, n_heads;
     int group, ngrp;   // q heads a kv head, workgroup columns' groups of them
+    int lead;          // units in front of an item's tiles
     float scale;
 };
 
 // ---- shares of the work ------------------------------------------------------
 // An item is a sequence, a kv head and up to 16 of its q heads; it consists of
-// the 32-key tiles its window touches.  All items' tiles form one line,
-// sequences in order, and workgroup w takes the tiles N w / 512 .. N (w + 1) /
+// the 32-key tiles its window touches, behind lead units that stand for what
+// it costs to begin and to end an item.  All items' units form one line,
+// sequences in order, and workgroup w takes the units N w / 512 .. N (w + 1) /
 // 512 - 1 of it, whatever the lengths are: a long sequence is spread over many
-// workgroups, many short ones share one.
+// workgroups, several short ones share one.
 
 // tiles of a sequence and its first one; 0 tiles: an empty sequence or a
 // length that does not fit
@@ -42,26 +42,48 @@ __device__ __forceinline__ int seq_tiles(const PagedArgs& a, int len, int& first
     if (a.window > 0 && len > a.window) first = (len - a.window) >> 5;
     return ((len - 1) >> 5) - first + 1;
 }
+__device__ __forceinline__ int seq_units(const PagedArgs& a, int len) {
+    int first;
+    const int t = seq_tiles(a, len, first);
+    return t ? t + a.lead : 0;
+}
 
 struct Line {
-    unsigned long long total;   // N, all tiles
-    unsigned long long before;  // tiles of one (kv head, heads) before sequence s
-    int s;
+    unsigned long long total;   // N, all units
+    unsigned long long before;  // units of one (kv head, heads) before sequence s
+    int s, len;
 };
 
-// N and the sequence that tile u = at(N) lies in (of_seq >= 0: that sequence
+// N and the sequence that unit u = at(N) lies in (of_seq >= 0: that sequence
 // instead), by the whole workgroup of 256 threads: a prefix sum over the
-// lengths, which is cheaper than a launch that would leave it in memory
+// lengths, which is cheaper than a launch that would leave it in memory.  Up
+// to 64 sequences each wave finds it by itself.
 template <typename At>
 __device__ __forceinline__ Line find_line(const PagedArgs& a, At at, int of_seq, unsigned long long* red) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (a.n_seqs + 255) >> 8, s0 = tid * per;
     const int rep = a.p.n_kv * a.ngrp;
-    unsigned long long sum = 0;
-    for (int i = 0; i < per; i++) {
-        int f;
-        if (s0 + i < a.n_seqs) sum += seq_tiles(a, a.lens[s0 + i], f);
+    if (a.n_seqs <= 64) {
+        const int len = lane < a.n_seqs ? a.lens[lane] : 0;
+        const unsigned t = seq_units(a, len);   // 64 times 2^26 and less
+        unsigned x = t;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const unsigned o = __shfl_up(x, d, 64);
+            if (lane >= d) x += o;
+        }
+        Line r;
+        r.total = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(x, 63) * rep;
+        const unsigned long long u = at(r.total);
+        const unsigned long long past = __ballot((unsigned long long)x * rep > u);
+        r.s = of_seq >= 0 ? of_seq : past ? __builtin_ctzll(past) : 0;
+        r.before = (unsigned)__builtin_amdgcn_readlane(x - t, r.s);
+        r.len = __builtin_amdgcn_readlane(len, r.s);
+        return r;
     }
+    const int per = (a.n_seqs + 255) >> 8, s0 = tid * per;
+    unsigned long long sum = 0;
+    for (int i = 0; i < per; i++)
+        if (s0 + i < a.n_seqs) sum += seq_units(a, a.lens[s0 + i]);
     unsigned long long x = sum;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -70,30 +92,40 @@ __device__ __forceinline__ Line find_line(const PagedArgs& a, At at, int of_seq,
     }
     if (lane == 63) red[wave] = x;
     lds_sync();
-    unsigned long long base = 0, all = 0;
+    unsigned long long before = x - sum, all = 0;
+#pragma unroll
     for (int w = 0; w < 4; w++) {
-        if (w < wave) base += red[w];
+        if (w < wave) before += red[w];
         all += red[w];
     }
-    unsigned long long before = base + x - sum;
     Line r;
     r.total = all * rep;
     const unsigned long long u = at(r.total);
     if (of_seq >= 0 ? s0 <= of_seq && of_seq < s0 + per : u >= before * rep && u < (before + sum) * rep) {
-        int s = s0;
+        int s = s0, len;
         for (;; s++) {
-            int f;
-            const int t = seq_tiles(a, a.lens[s], f);
+            len = a.lens[s];
+            const int t = seq_units(a, len);
             if (of_seq >= 0 ? s == of_seq : u < (before + t) * rep) break;
             before += t;
         }
         red[4] = before;
-        red[5] = (unsigned)s;
+        red[5] = (unsigned long long)(unsigned)s << 32 | (unsigned)len;
     }
     lds_sync();
     r.before = red[4];
-    r.s = (int)red[5];
+    r.s = (int)(red[5] >> 32);
+    r.len = (int)red[5];
     return r;
+}
+
+// the workgroup that has unit u of n: the quotient (u 512 + 511) / n, whose
+// double is off by one at most
+__device__ __forceinline__ int unit_wg(unsigned long long u, unsigned long long n) {
+    unsigned long long w = (unsigned long long)(((double)u * kPagedWG + (kPagedWG - 1)) / (double)n);
+    if ((n * w) >> kLgWG > u) w--;
+    else if ((n * (w + 1)) >> kLgWG <= u) w++;
+    return (int)w;
 }
 
 // floats of a partial result: [head][hd] sums, then each head's maximum and weight sum
@@ -182,16 +214,17 @@ __device__ __forceinline__ void mfma_terms(const b8_t (&a)[NT], const b8_t (&b)[
 // running maximum, which moves only when a score passes it by 2^8.
 // Bound by the cache's bytes; DEPTH loads of 1 KB stay in flight a wave.
 template <int TYPE, int HD, int DEPTH>
-__global__ __launch_bounds__(256, HD == 512 ? 1 : 2) void attn_paged_kernel(PagedArgs a) {
-    constexpr int ES = CacheType<TYPE>::ES, NT = CacheType<TYPE>::NT, kLgWG = paged_lg_wg(HD);
+__global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
+    constexpr int ES = CacheType<TYPE>::ES, NT = CacheType<TYPE>::NT;
     constexpr int KC = HD * ES / 64;                      // 1 KB pieces of a 16-token block
     constexpr int CPS = ES == 4 ? 2 : 1;                  // pieces of a product step of 32 dims (ES 1: half a piece)
     constexpr int SPC = ES == 1 ? 2 : 1;                  // product steps of a piece
     constexpr int NL = 4 * KC, STEPS = HD / 32, NTILE = HD / 16, TPC = 4 / ES;   // TPC: 16-dim tiles of a V piece
+    constexpr bool kKOnly = DEPTH <= 2 * KC;              // loads ahead of a tile's end are the next one's K
     static_assert(NL % DEPTH == 0, "ring");
     constexpr int kQBytes = STEPS * 3 * 1024, kSumBytes = 2 * NTILE * 1024;
     __shared__ __align__(16) uint8_t buf[kQBytes > kSumBytes ? kQBytes : kSumBytes];
-    __shared__ unsigned long long red[8];
+    __shared__ unsigned long long red[6];
     __shared__ float mls[2][4][kHeadsWG];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -202,18 +235,60 @@ __global__ __launch_bounds__(256, HD == 512 ? 1 : 2) void attn_paged_kernel(Page
     if (cur >= end) return;
     const int rep = a.p.n_kv * a.ngrp;
     int s = __builtin_amdgcn_readfirstlane(ln.s);
-    unsigned off = (unsigned)(cur - ln.before * rep);     // tile within the sequence's items
-    int first_tile, len = __builtin_amdgcn_readfirstlane(a.lens[s]);
+    int first_tile, len = __builtin_amdgcn_readfirstlane(ln.len);
     int tiles = seq_tiles(a, len, first_tile);
-    int item = __builtin_amdgcn_readfirstlane((int)(off / (unsigned)tiles));
-    int tile0 = __builtin_amdgcn_readfirstlane((int)(off - (unsigned)item * tiles));
+    const unsigned long long off = cur - ln.before * rep;   // unit within the sequence's items
+    int item = __builtin_amdgcn_readfirstlane((int)(off / (unsigned)(tiles + a.lead)));
+    int unit = __builtin_amdgcn_readfirstlane((int)(off - (unsigned long long)item * (tiles + a.lead)));
     while (true) {
         const unsigned long long left = end - cur;
-        const int tile1 = left < (unsigned long long)(tiles - tile0) ? tile0 + (int)left : tiles;
+        const int unit1 = left < (unsigned long long)(tiles + a.lead - unit) ? unit + (int)left : tiles + a.lead;
+        const int tile0 = unit > a.lead ? unit - a.lead : 0, tile1 = unit1 - a.lead;
+        if (tile1 > tile0) {
         const int kvh = item / a.ngrp, hg = item - kvh * a.ngrp;
         const int nh = a.group - hg * kHeadsWG < kHeadsWG ? a.group - hg * kHeadsWG : kHeadsWG;
         const int head0 = kvh * a.group + hg * kHeadsWG;
         const int first = a.window > 0 && len > a.window ? len - a.window : 0;
+
+        // ---- where a tile's two blocks are; one without a key in use is not read ----
+        bool bad = false;
+        auto pages = [&](int tile, bool on, int (&pg)[2]) {
+            const int pos = (first_tile + tile) << 5;
+            pg[0] = pg[1] = -1;
+            if (on && first - pos < 16) {
+                pg[0] = __builtin_amdgcn_readfirstlane(a.p.page_of(s, pos));
+                bad = bad || pg[0] < 0;
+            }
+            if (on && len - pos > 16) {
+                pg[1] = __builtin_amdgcn_readfirstlane(a.p.page_of(s, pos + 16));
+                bad = bad || pg[1] < 0;
+            }
+        };
+        auto block = [&](int tile, const int (&pg)[2], int i) {
+            return a.p.block_of(pg[i] < 0 ? 0 : pg[i], kvh, ((first_tile + tile) << 5) + 16 * i);
+        };
+        auto rsrc = [&](const uint8_t* pool, int tile, const int (&pg)[2], __amdgpu_buffer_rsrc_t (&r)[2]) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                r[i] = __builtin_amdgcn_make_buffer_rsrc((void*)(pool + block(tile, pg, i) * (16 * HD * ES)), 0,
+                                                         pg[i] < 0 ? 0 : 16 * HD * ES, kBufWord3);
+        };
+        // load i of a tile: K pieces in the order of the product steps, then V pieces, blocks in turn
+        auto load = [&](int i, const __amdgpu_buffer_rsrc_t (&k)[2], const __amdgpu_buffer_rsrc_t (&v)[2]) {
+            if (i < 2 * KC) {
+                const int b = i / CPS & 1, c = i / (2 * CPS) * CPS + i % CPS;
+                return buf_load16(k[b], lane * 16, c * 1024);
+            }
+            return buf_load16(v[i & 1], lane * 16, (i - 2 * KC) / 2 * 1024);
+        };
+        int tile = tile0 + wave, pg[2], npg[2];
+        uint4 ring[DEPTH];
+        __amdgpu_buffer_rsrc_t kr[2], vr[2], kn[2], vn[2];
+        pages(tile, tile < tile1, pg);
+        rsrc(a.p.kp, tile, pg, kr);
+        rsrc(a.p.vp, tile, pg, vr);
+#pragma unroll
+        for (int i = 0; i < DEPTH; i++) ring[i] = load(i, kr, vr);
 
         // ---- q, times scale log2(e), as three terms in the products' order ----
         const float qs = a.scale * kLog2e;
@@ -240,60 +315,19 @@ __global__ __launch_bounds__(256, HD == 512 ? 1 : 2) void attn_paged_kernel(Page
         // ---- the wave's tiles ----
         f4_t o[NTILE] = {};
         float m = -INFINITY, l = 0.0f;
-        bool bad = false;
-        // where a tile's two blocks are; blocks without a key in use take the other's place
-        size_t blk[2], nblk[2];
-        auto place = [&](int tile, size_t (&b)[2]) {
-            const int pos = (first_tile + tile) << 5;
-            const int pa = pos + 16 > first ? pos : pos + 16, pb = pos + 16 < len ? pos + 16 : pos;
-            const int ga = a.p.page_of(s, pa), gb = a.p.page_of(s, pb);
-            bad = bad || ga < 0 || gb < 0;
-            b[0] = a.p.block_of(ga < 0 ? 0 : ga, kvh, pa);
-            b[1] = a.p.block_of(gb < 0 ? 0 : gb, kvh, pb);
-        };
-        auto rsrc = [&](const uint8_t* pool, size_t b, bool on) {
-            return __builtin_amdgcn_make_buffer_rsrc((void*)(pool + b * (16 * HD * ES)), 0, on ? 16 * HD * ES : 0, kBufWord3);
-        };
-        // load i of a tile: K pieces in the order of the product steps, then V pieces, blocks in turn
-        auto load = [&](int i, const __amdgpu_buffer_rsrc_t (&k)[2], const __amdgpu_buffer_rsrc_t (&v)[2]) {
-            if (i < 2 * KC) {
-                const int b = i / CPS & 1, c = i / (2 * CPS) * CPS + i % CPS;
-                return buf_load16(k[b], lane * 16, c * 1024);
-            }
-            return buf_load16(v[i & 1], lane * 16, (i - 2 * KC) / 2 * 1024);
-        };
-        int tile = tile0 + wave;
-        if (tile < tile1) {
-            uint4 ring[DEPTH];
-            place(tile, blk);
-            __amdgpu_buffer_rsrc_t kr[2], vr[2], kn[2], vn[2];
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                kr[b] = rsrc(a.p.kp, blk[b], true);
-                vr[b] = rsrc(a.p.vp, blk[b], true);
-            }
-#pragma unroll
-            for (int i = 0; i < DEPTH; i++) ring[i] = load(i, kr, vr);
             for (; tile < tile1; tile += 4) {
-                const bool more = tile + 4 < tile1;
-                if (more) {
-                    place(tile + 4, nblk);
-                } else {
-                    nblk[0] = blk[0];
-                    nblk[1] = blk[1];
-                }
                 // past the last tile the loads have no bytes to read
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    kn[b] = rsrc(a.p.kp, nblk[b], more);
-                    vn[b] = rsrc(a.p.vp, nblk[b], more);
+                pages(tile + 4, tile + 4 < tile1, npg);
+                if (!kKOnly) {
+                    rsrc(a.p.kp, tile + 4, npg, kn);
+                    rsrc(a.p.vp, tile + 4, npg, vn);
                 }
                 float ksc[8], vsc[8];
                 if (TYPE == G4_KV_Q8) {
 #pragma unroll
                     for (int b = 0; b < 2; b++) {
-                        const float4 x = reinterpret_cast<const float4*>(a.p.kp + a.p.scale_off)[blk[b] * 4 + g];
-                        const float4 y = reinterpret_cast<const float4*>(a.p.vp + a.p.scale_off)[blk[b] * 4 + g];
+                        const float4 x = reinterpret_cast<const float4*>(a.p.kp + a.p.scale_off)[block(tile, pg, b) * 4 + g];
+                        const float4 y = reinterpret_cast<const float4*>(a.p.vp + a.p.scale_off)[block(tile, pg, b) * 4 + g];
                         ksc[4 * b] = x.x; ksc[4 * b + 1] = x.y; ksc[4 * b + 2] = x.z; ksc[4 * b + 3] = x.w;
                         vsc[4 * b] = y.x; vsc[4 * b + 1] = y.y; vsc[4 * b + 2] = y.z; vsc[4 * b + 3] = y.w;
                     }
@@ -304,14 +338,23 @@ __global__ __launch_bounds__(256, HD == 512 ? 1 : 2) void attn_paged_kernel(Page
                     return x;
                 };
                 f4_t sc[2] = {}, ss[2] = {};
+                // q of a step is read while the one before it is worked on
+                uint4 qn[SPC][3];
+                auto read_q = [&](int st) {
+#pragma unroll
+                    for (int h = 0; h < SPC; h++)
+#pragma unroll
+                        for (int k = 0; k < 3; k++) qn[h][k] = reinterpret_cast<const uint4*>(buf)[((st * SPC + h) * 3 + k) * 64 + lane];
+                };
+                read_q(0);
 #pragma unroll
                 for (int st = 0; st < STEPS / SPC; st++) {
                     b8_t qt[SPC][3];
 #pragma unroll
                     for (int h = 0; h < SPC; h++)
 #pragma unroll
-                        for (int k = 0; k < 3; k++)
-                            qt[h][k] = __builtin_bit_cast(b8_t, reinterpret_cast<const uint4*>(buf)[((st * SPC + h) * 3 + k) * 64 + lane]);
+                        for (int k = 0; k < 3; k++) qt[h][k] = __builtin_bit_cast(b8_t, qn[h][k]);
+                    if (st + 1 < STEPS / SPC) read_q(st + 1);
 #pragma unroll
                     for (int b = 0; b < 2; b++) {
                         uint32_t x[4 * CPS];
@@ -374,6 +417,7 @@ __global__ __launch_bounds__(256, HD == 512 ? 1 : 2) void attn_paged_kernel(Page
                     const int key = pos + 16 * (i >> 2) + (i & 3);
                     keep[i] = key >= first && key < len ? 0xffffffffu : 0u;
                 }
+                if (kKOnly) rsrc(a.p.kp, tile + 4, npg, kn);
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
                     uint4 y[2];
@@ -402,51 +446,60 @@ __global__ __launch_bounds__(256, HD == 512 ? 1 : 2) void attn_paged_kernel(Page
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                blk[0] = nblk[0];
-                blk[1] = nblk[1];
+                if (kKOnly) rsrc(a.p.vp, tile + 4, npg, vn);
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
                     kr[b] = kn[b];
                     vr[b] = vn[b];
+                    pg[b] = npg[b];
                 }
             }
-        }
 
         // ---- the four waves' sums: 2, 3 -> 0, 1 -> 0 ----
         l += shfl_xor(l, 16);
         l += shfl_xor(l, 32);
         if (bad) l = __uint_as_float(0x7fc00000u);
-        if (g == 0) {
-            mls[0][wave][col] = m;
-            mls[1][wave][col] = l;
-        }
-        lds_sync();   // q is no longer needed
-        float top = -INFINITY, sum = 0.0f, mine = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) top = fmaxf(top, mls[0][i][col]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float mi = mls[0][i][col], f = mi == top ? 1.0f : exp2f(mi - top);
-            sum += f * mls[1][i][col];
-            if (i == wave) mine = f;
-        }
-#pragma unroll
-        for (int i = 0; i < NTILE; i++) o[i] *= mine;
+        float top = m, sum = l;
+        const bool alone = tile1 - tile0 == 1;   // wave 0 had the only tile
         f4_t* box = reinterpret_cast<f4_t*>(buf) + (wave & 1) * NTILE * 64 + lane;
-        if (wave >= 2) {
+        if (!alone) {
+            if (g == 0) {
+                mls[0][wave][col] = m;
+                mls[1][wave][col] = l;
+            }
+            lds_sync();   // q is no longer needed
+            float mine = 0.0f;
+            top = -INFINITY;
+            sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
-        }
-        lds_sync();
-        if (wave < 2) {
+            for (int i = 0; i < 4; i++) top = fmaxf(top, mls[0][i][col]);
 #pragma unroll
-            for (int i = 0; i < NTILE; i++) o[i] += box[i * 64];
-            if (wave == 1) {
+            for (int i = 0; i < 4; i++) {
+                const float mi = mls[0][i][col], f = mi == top ? 1.0f : exp2f(mi - top);
+                sum += f * mls[1][i][col];
+                if (i == wave) mine = f;
+            }
+#pragma unroll
+            for (int i = 0; i < NTILE; i++) o[i] *= mine;
+            if (wave >= 2) {
 #pragma unroll
                 for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
             }
+            lds_sync();
+            if (wave < 2) {
+#pragma unroll
+                for (int i = 0; i < NTILE; i++) o[i] += box[i * 64];
+                if (wave == 1) {
+#pragma unroll
+                    for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
+                }
+            }
+            lds_sync();
+            if (wave == 0) {
+#pragma unroll
+                for (int i = 0; i < NTILE; i++) o[i] += box[(NTILE + i) * 64];
+            }
         }
-        lds_sync();
         if (wave == 0 && col < nh) {
             const bool whole = tile0 == 0 && tile1 == tiles;
             float* to;
@@ -463,39 +516,41 @@ __global__ __launch_bounds__(256, HD == 512 ? 1 : 2) void attn_paged_kernel(Page
                     slot[2 * col + 1] = sum;
                 }
             }
-            box = reinterpret_cast<f4_t*>(buf) + NTILE * 64 + lane;
 #pragma unroll
             for (int i = 0; i < NTILE; i++) {
-                const f4_t r = (o[i] + box[i * 64]) * f;
+                const f4_t r = o[i] * f;
                 *reinterpret_cast<f4_t*>(to + i * 16 + g * 4) = r;
             }
         }
-        cur += (unsigned)(tile1 - tile0);
+            lds_sync();   // the sums' place takes q again
+        }
+        cur += (unsigned)(unit1 - unit);
         if (cur >= end) break;
-        lds_sync();   // the sums' place takes q again
-        if (tile1 < tiles || ++item == rep) {
+        unit = 0;
+        if (++item == rep) {
             item = 0;
             do {
                 len = __builtin_amdgcn_readfirstlane(a.lens[++s]);
                 tiles = seq_tiles(a, len, first_tile);
             } while (tiles == 0);
         }
-        tile0 = 0;
     }
 }
 
 // Joins the pieces of every sequence and head that more than one workgroup
 // took, with the weights 2^(m_i - max m); sequences without keys get zeros,
 // those whose length does not fit NaN.
-template <int HD>
+// D of the HD dims a workgroup (blockIdx.z): 64 where there are few heads and
+// sequences, whose pieces then are as many.
+template <int HD, int D>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
-    constexpr int LPR = HD / 4, GR = 256 / LPR, kLgWG = paged_lg_wg(HD);   // lanes a row of HD floats, pieces at a time
+    constexpr int LPR = D / 4, GR = 256 / LPR;   // lanes a row of D floats, pieces at a time
     const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
     const int kvh = h / a.group, hg = (h - kvh * a.group) / kHeadsWG, col = h - kvh * a.group - hg * kHeadsWG;
-    __shared__ unsigned long long red[8];
-    __shared__ float fac[kPagedMaxWG], wred[4];
+    __shared__ unsigned long long red[6];
+    __shared__ float fac[kPagedWG], wred[4];
     __shared__ __align__(16) float4 acc[256];
-    float* out = a.out + (size_t)s * a.out_stride + (size_t)h * HD;
+    float* out = a.out + (size_t)s * a.out_stride + (size_t)h * HD + blockIdx.z * D;
     const int len = a.lens[s];
     int first;
     const int tiles = seq_tiles(a, len, first);
@@ -505,18 +560,16 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
         return;
     }
     const Line ln = find_line(a, [](unsigned long long) { return 0ull; }, s, red);
-    const unsigned long long u0 = ln.before * (a.p.n_kv * a.ngrp) + (unsigned long long)(kvh * a.ngrp + hg) * tiles;
     const unsigned long long n = ln.total;
-    const int w0 = (int)((((u0 + 1) << kLgWG) - 1) / n), w1 = (int)((((u0 + tiles) << kLgWG) - 1) / n);
+    const unsigned long long u0 =
+        ln.before * (a.p.n_kv * a.ngrp) + (unsigned long long)(kvh * a.ngrp + hg) * (tiles + a.lead) + a.lead;
+    const int w0 = unit_wg(u0, n), w1 = unit_wg(u0 + tiles - 1, n);
     if (w0 == w1) return;   // one workgroup had it all
-    // fewer tiles than workgroups: a tile each, some workgroups between them without one
-    const bool few = n < (1u << kLgWG);
+    // fewer units than workgroups: a unit each, some workgroups between them without one
+    const bool few = n < kPagedWG;
     const int np = few ? tiles : w1 - w0 + 1, gh = a.group < kHeadsWG ? a.group : kHeadsWG;
     const size_t pf = part_floats(a.group, HD);
-    auto slot = [&](int i) {
-        const int w = few ? (int)(((((unsigned)u0 + i + 1) << kLgWG) - 1) / (unsigned)n) : w0 + i;
-        return a.part + ((size_t)w * 2 + (i == 0)) * pf;
-    };
+    auto slot = [&](int i) { return a.part + ((size_t)(few ? unit_wg(u0 + i, n) : w0 + i) * 2 + (i == 0)) * pf; };
     // maxima, factors, weight sums: pieces tid and tid + 256
     float m[2], l[2], top = -INFINITY;
 #pragma unroll
@@ -555,7 +608,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const int j = i + k * GR < np ? i + k * GR : gr;
-            y[k] = reinterpret_cast<const float4*>(slot(j) + col * HD)[c];
+            y[k] = reinterpret_cast<const float4*>(slot(j) + col * HD + blockIdx.z * D)[c];
             f[k] = i + k * GR < np ? fac[j] : 0.0f;
         }
 #pragma unroll
@@ -585,9 +638,12 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
 
 template <int TYPE, int HD>
 void launch_paged(const PagedArgs& a) {
-    constexpr int NL = HD * CacheType<TYPE>::ES / 16, R = HD == 512 ? 32 : 16, D = NL < R ? NL : R;
-    hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D>), dim3(1 << paged_lg_wg(HD)), dim3(256), 0, g4_stream(), a);
-    hipLaunchKernelGGL((attn_paged_join_kernel<HD>), dim3(a.n_heads, a.n_seqs), dim3(256), 0, g4_stream(), a);
+    constexpr int NL = HD * CacheType<TYPE>::ES / 16, R = 4, D = NL < R ? NL : R;
+    hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D>), dim3(kPagedWG), dim3(256), 0, g4_stream(), a);
+    if (a.n_heads * a.n_seqs < 256)
+        hipLaunchKernelGGL((attn_paged_join_kernel<HD, 64>), dim3(a.n_heads, a.n_seqs, HD / 64), dim3(256), 0, g4_stream(), a);
+    else
+        hipLaunchKernelGGL((attn_paged_join_kernel<HD, HD>), dim3(a.n_heads, a.n_seqs, 1), dim3(256), 0, g4_stream(), a);
 }
 template <int TYPE>
 void launch_paged(const PagedArgs& a, int hd) {
@@ -604,7 +660,7 @@ using namespace g4;
 
 extern "C" size_t g4_attn_decode_paged_part_bytes(int n_heads, int n_kv, int hd) {
     if (n_heads < 1 || n_kv < 1 || n_heads % n_kv || (hd != 64 && hd != 128 && hd != 256 && hd != 512)) return 0;
-    return (size_t)kPagedMaxWG * 2 * part_floats(n_heads / n_kv, hd) * 4;
+    return (size_t)kPagedWG * 2 * part_floats(n_heads / n_kv, hd) * 4;
 }
 
 extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp, const void* vp, int type, int n_pages,
@@ -625,6 +681,7 @@ extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp
     a.n_seqs = n_seqs; a.window = window; a.n_heads = n_heads; a.scale = attn_scale;
     a.group = n_heads / n_kv;
     a.ngrp = (a.group + kHeadsWG - 1) / kHeadsWG;
+    a.lead = n_seqs * n_kv * a.ngrp > 64 ? 3 : 0;
     if (type == G4_F32) launch_paged<G4_F32>(a, hd);
     else if (type == G4_F16) launch_paged<G4_F16>(a, hd);
     else if (type == G4_BF16) launch_paged<G4_BF16>(a, hd);

@@ -82,6 +82,11 @@ def same(a, b):
     return np.array_equal(a, b, equal_nan=True)
 
 
+def within(err, bound, at):
+    worst = float(np.max(err / bound))
+    assert worst <= 1.0, (at, worst)
+
+
 UNTOUCHED = np.full(1, 0x3F3F3F3F, np.uint32).view(np.float32)[0]
 
 
@@ -245,7 +250,7 @@ def check_decode(lib, seed, kind, hd, n_heads, n_kv, page, lens, window=0, scale
                                    hk[at[s]:at[s + 1]].reshape(t, n_kv, hd), hv[at[s]:at[s + 1]].reshape(t, n_kv, hd),
                                    [first], scale)
         err = np.abs(o - want[0])
-        assert bool((err <= bound[0]).all()), (s, t, float((err / bound[0]).max()))
+        within(err, bound[0], (s, t))
     if extra:
         assert (got[:, n_heads * hd:] == UNTOUCHED).all()
 
@@ -408,7 +413,7 @@ def check_prompt(lib, seed, kind, hd, n_heads, n_kv, n, window=0, scale=None, ga
                 big = np.abs(vf[kk, :n_kv * hd]).max()
                 bound = bound + pn.HALF[kind] * (np.abs(want) + 1.01 * big) + 2.0 ** -25 * hi * big
             err = np.abs(got[r, :n_heads * hd].reshape(hi - lo, n_heads, hd) - want)
-            assert bool((err <= bound).all()), (s, lo, float((err / bound).max()))
+            within(err, bound, (s, lo))
     untouched = np.full(1, 0x3F3F3F3F, np.uint32).view(bits.dtype)[0]
     assert (bits[sum(n):] == untouched).all() and (bits[:, n_heads * hd:] == untouched).all()
 
