@@ -1,5 +1,22 @@
 // attn_packed.hip -- causal attention of whole prompts, packed one after the
 // other.
+//
+// Two launches.  The first puts K and V of every sequence into blocks of 32
+// keys in the order in which the matrix cores take them (32 x 32 x 16
+// products, whole kilobytes of 64 lanes x 16 bytes), a sequence's blocks
+// padded with zeros:
+//   K (operand rows = keys): lane 32 h + t of piece s holds key t's dims
+//     16 s + 8 h .. + 7;
+//   V (operand rows = dims): lane 32 h + n of piece 2 c + t holds dim 32 c + n
+//     of keys 16 t + 8 (j / 4) + 4 h + j % 4, j = 0 .. 7: the keys whose
+//     scores the lane half gets out of the first product.
+// The second launch then needs no transpose, no bank-conflict pattern and no
+// care for a neighbour's rows: tiles go from memory to LDS as they are
+// (buffer loads to LDS) and from there to the operands.
+//
+// A row of K or V that holds an infinity or NaN is stored as zeros and marked:
+// a query that sees it gets the score NaN there, others never meet it.
+#include <float.h>
 #include <math.h>
 
 #include "g4_kvpage.h"
@@ -8,72 +25,474 @@
 namespace g4 {
 namespace {
 
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+typedef float f16_t __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
 struct PackedArgs {
     const void* q;
     const void* k;
     const void* v;
     void* out;
-    void* work;
+    uint8_t* work;
     const int* cu;
-    int q_stride, kv_stride, out_stride, n_seqs, m, window, n_heads, n_kv;
+    int q_stride, kv_stride, out_stride, n_seqs, m, window, n_heads, n_kv, group;
+    int extra;      // units a sequence may need beyond its share
     float scale;
 };
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T x) { return (float)x; }
+// fp32 operands are products of three pairs of fp16 halves of a scaled row:
+// x = 2^e (hi + lo), the row's largest |hi| in [2^14, 2^15], so that x is met
+// within 2^-22 of itself or 2^-39 of the row's largest.
+template <int T>
+struct Kind;
+template <>
+struct Kind<G4_F32> {
+    static constexpr int ES = 4, NS = 2;
+    typedef float t;
+    typedef h8_t op;
+};
+template <>
+struct Kind<G4_F16> {
+    static constexpr int ES = 2, NS = 1;
+    typedef _Float16 t;
+    typedef h8_t op;
+};
+template <>
+struct Kind<G4_BF16> {
+    static constexpr int ES = 2, NS = 1;
+    typedef __bf16 t;
+    typedef b8_t op;
+};
+__device__ __forceinline__ f16_t mfma32(h8_t a, h8_t b, f16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f16_t mfma32(b8_t a, b8_t b, f16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-// One workgroup a row and head, a key a wave at a time.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void attn_packed_simple_kernel(PackedArgs a) {
-    constexpr int N = HD / 64;
-    const int row = blockIdx.x, h = blockIdx.y, kvh = h / (a.n_heads / a.n_kv);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __shared__ float red[4][HD + 2];
-    const int s = unit_seq(a.cu, a.n_seqs, 0, 0, (unsigned)row);
+// A block: K pieces (fp32: hi, then lo), V pieces (likewise), then 512 bytes:
+// fp32: each key's K scale 2^e, V exponent e, 2^-e; the mask of marked keys.
+constexpr int kMeta = 512, kMetaVExp = 128, kMetaVInv = 256, kMetaMask = 384;
+__host__ __device__ constexpr size_t block_bytes(int hd, int es) { return (size_t)64 * hd * es + kMeta; }
+
+// biased exponent of a row's largest magnitude -> the scale that brings it
+// to [2^14, 2^15) and its inverse; low: the smallest exponent told apart
+__device__ __forceinline__ float row_scale(int e) { return __uint_as_float((unsigned)(268 - e) << 23); }
+__device__ __forceinline__ float row_scale_inv(int e) { return __uint_as_float((unsigned)(e - 14) << 23); }
+constexpr int kLowK = 15;    // 2^-126 is a normal number
+constexpr int kLowV = 51;    // sums of 2^-e stay in range
+
+// ---- first launch: K and V into blocks -----------------------------------------
+// blockIdx: block, kv head, K or V.  Sequence s has the blocks (cu[s] >> 5) + s
+// and on.
+template <int T, int HD>
+__global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
+    typedef typename Kind<T>::t E;
+    constexpr int ES = Kind<T>::ES, NS = Kind<T>::NS;
+    constexpr int VW = 16 / ES;                            // elements of a 16-byte load
+    constexpr int LPR = HD / VW < 64 ? HD / VW : 64;       // lanes a row
+    constexpr int VPL = HD / VW / LPR, RPW = 64 / LPR, PASS = 8 / RPW;
+    __shared__ __align__(16) uint8_t img[64 * HD];         // one half (hi or lo) of K or V
+    __shared__ unsigned marks;
+    const unsigned id = blockIdx.x;
+    const int s = unit_seq(a.cu, a.n_seqs, 1, 5, 1, id);
     const int r0 = a.cu[s], r1 = a.cu[s + 1];
-    if (r0 < 0 || r1 > a.m || row < r0 || row >= r1) return;
-    const int first = a.window > 0 && row - r0 >= a.window ? row + 1 - a.window : r0;
-    const T* K = (const T*)a.k + (size_t)kvh * HD;
-    const T* V = (const T*)a.v + (size_t)kvh * HD;
-    float q[N], o[N] = {}, m = -INFINITY, l = 0.0f;
+    const unsigned b = id - unit_base(a.cu, s, 1, 5, 1);
+    if (r0 < 0 || r1 <= r0 || r1 > a.m || b >= (unsigned)((r1 - r0 + 31) >> 5)) return;
+    const int row0 = r0 + (int)b * 32, rows = r1 - row0 < 32 ? r1 - row0 : 32;
+    const bool is_v = blockIdx.z;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int sub = lane / LPR, col = lane % LPR;
+    const E* src = (const E*)(is_v ? a.v : a.k) + (size_t)blockIdx.y * HD;
+    if (tid == 0) marks = 0;
+    uint4 x[PASS][VPL];
 #pragma unroll
-    for (int i = 0; i < N; i++)
-        q[i] = to_f32(((const T*)a.q)[(size_t)row * a.q_stride + h * HD + i * 64 + lane]) * a.scale;
-    for (int t = first + wave; t <= row; t += 4) {
-        float x = 0.0f;
+    for (int i = 0; i < PASS; i++) {
+        const int t = (i * 4 + wave) * RPW + sub;
+        const size_t r = row0 + (t < rows ? t : 0);
 #pragma unroll
-        for (int i = 0; i < N; i++) x = fmaf(q[i], to_f32(K[(size_t)t * a.kv_stride + i * 64 + lane]), x);
-        x = wave_sum(x);
-        const float mn = fmaxf(m, x), f = m == mn ? 1.0f : expf(m - mn), w = expf(x - mn);
-        l = l * f + w;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < N; i++) o[i] = fmaf(w, to_f32(V[(size_t)t * a.kv_stride + i * 64 + lane]), o[i] * f);
+        for (int k = 0; k < VPL; k++)
+            x[i][k] = *reinterpret_cast<const uint4*>(src + r * a.kv_stride + (k * LPR + col) * VW);
     }
+    lds_sync();
+    uint8_t* rec = a.work + ((size_t)id * a.n_kv + blockIdx.y) * block_bytes(HD, ES);
+    uint8_t* out = rec + (is_v ? 32 * HD * ES : 0);
+    float* meta = reinterpret_cast<float*>(rec + 64 * HD * ES);
+    float sc[PASS];
 #pragma unroll
-    for (int i = 0; i < N; i++) red[wave][i * 64 + lane] = o[i];
-    if (lane == 0) { red[wave][HD] = m; red[wave][HD + 1] = l; }
-    __syncthreads();
-    float top = -INFINITY;
-    for (int w = 0; w < 4; w++) top = fmaxf(top, red[w][HD]);
-    for (int d = threadIdx.x; d < HD; d += 256) {
-        float num = 0.0f, den = 0.0f;
-        for (int w = 0; w < 4; w++) {
-            const float f = red[w][HD] == top ? 1.0f : expf(red[w][HD] - top);
-            num += f * red[w][d];
-            den += f * red[w][HD + 1];
+    for (int i = 0; i < PASS; i++) {
+        const int t = (i * 4 + wave) * RPW + sub;
+        // the row's largest magnitude, as integers: infinities and NaN come last
+        unsigned top = 0;
+#pragma unroll
+        for (int k = 0; k < VPL; k++) {
+            const unsigned w[4] = {x[i][k].x, x[i][k].y, x[i][k].z, x[i][k].w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                unsigned m;
+                if (ES == 4) m = w[j] & 0x7fffffffu;
+                else m = (w[j] & 0x7fffu) > (w[j] >> 16 & 0x7fffu) ? w[j] & 0x7fffu : w[j] >> 16 & 0x7fffu;
+                top = m > top ? m : top;
+            }
         }
-        ((T*)a.out)[(size_t)row * a.out_stride + h * HD + d] = (T)(num / den);
+#pragma unroll
+        for (int d = 1; d < LPR; d <<= 1) {
+            const unsigned o = __shfl_xor(top, d, 64);
+            top = o > top ? o : top;
+        }
+        const bool finite = top < (T == G4_F32 ? 0x7f800000u : T == G4_F16 ? 0x7c00u : 0x7f80u);
+        if (t >= rows || !finite) {
+#pragma unroll
+            for (int k = 0; k < VPL; k++) x[i][k] = make_uint4(0, 0, 0, 0);
+        }
+        if (t < rows && !finite && col == 0) atomicOr(&marks, 1u << t);
+        sc[i] = 1.0f;
+        if (T == G4_F32) {
+            const int low = is_v ? kLowV : kLowK;
+            const int e = t < rows && finite && (int)(top >> 23) > low ? (int)(top >> 23) : low;
+            sc[i] = row_scale(e);
+            if (col == 0) {
+                if (is_v) {
+                    meta[kMetaVExp / 4 + t] = (float)(e - 141);
+                    meta[kMetaVInv / 4 + t] = sc[i];
+                } else {
+                    meta[t] = row_scale_inv(e);
+                }
+            }
+        }
     }
+#pragma unroll
+    for (int half = 0; half < NS; half++) {
+        if (half) lds_sync();   // the first half has been read
+#pragma unroll
+        for (int i = 0; i < PASS; i++) {
+            const int t = (i * 4 + wave) * RPW + sub;
+#pragma unroll
+            for (int k = 0; k < VPL; k++) {
+                const int c = (k * LPR + col) * VW;
+                uint16_t e[VW];
+                const unsigned w[4] = {x[i][k].x, x[i][k].y, x[i][k].z, x[i][k].w};
+                if constexpr (T == G4_F32) {
+#pragma unroll
+                    for (int j = 0; j < VW; j += 2) {
+                        h2v_t hi, lo;
+                        split2(__uint_as_float(w[j]), __uint_as_float(w[j + 1]), sc[i], hi, lo);
+                        const unsigned y = __builtin_bit_cast(unsigned, half ? lo : hi);
+                        e[j] = (uint16_t)y;
+                        e[j + 1] = (uint16_t)(y >> 16);
+                    }
+                } else {
+                    __builtin_memcpy(e, w, 16);
+                }
+                if (is_v) {
+                    // key t = 16 u + 8 b + 4 h + i
+                    const int u = t >> 4, h = t >> 2 & 1, slot = (t >> 3 & 1) * 4 + (t & 3);
+#pragma unroll
+                    for (int j = 0; j < VW; j++) {
+                        const int d = c + j;
+                        *reinterpret_cast<uint16_t*>(img + ((d >> 5) * 2 + u) * 1024 + (h * 32 + (d & 31)) * 16 + slot * 2) = e[j];
+                    }
+                } else {
+                    __builtin_memcpy(__builtin_assume_aligned(img + (c >> 4) * 1024 + ((c >> 3 & 1) * 32 + t) * 16 + (c & 7) * 2, VW * 2),
+                                     e, VW * 2);
+                }
+            }
+        }
+        lds_sync();
+        for (int i = tid; i < 4 * HD; i += 256)
+            reinterpret_cast<uint4*>(out + half * 64 * HD)[i] = reinterpret_cast<const uint4*>(img)[i];
+    }
+    if (tid == 0) reinterpret_cast<unsigned*>(meta)[kMetaMask / 4 + is_v] = marks;
 }
 
-template <typename T>
-void launch_packed(const PackedArgs& a, int hd) {
-    const dim3 grid(a.m, a.n_heads);
-    if (hd == 64) hipLaunchKernelGGL((attn_packed_simple_kernel<T, 64>), grid, dim3(256), 0, g4_stream(), a);
-    else if (hd == 128) hipLaunchKernelGGL((attn_packed_simple_kernel<T, 128>), grid, dim3(256), 0, g4_stream(), a);
-    else if (hd == 256) hipLaunchKernelGGL((attn_packed_simple_kernel<T, 256>), grid, dim3(256), 0, g4_stream(), a);
-    else hipLaunchKernelGGL((attn_packed_simple_kernel<T, 512>), grid, dim3(256), 0, g4_stream(), a);
+// ---- second launch ------------------------------------------------------------------
+// A wave's job is 32 rows of one q head; a workgroup takes NJ consecutive jobs
+// of a kv head (the heads of 32 rows, then the next 32 rows), which share its
+// tiles of 32 keys in LDS.  S^T = K Q^T (rows keys, columns q rows): a lane
+// holds 16 of a row's 32 scores, which are, as they stand, its operand of
+// O^T += V^T P^T.  The running maximum moves only when a score passes it by
+// 2^8 (fp32: 2^4).  DS 2 (head_dim 512, whose q and o would not fit a wave's
+// registers): a job's dims are halved over two waves, whose partial scores
+// meet in LDS; K and V of a tile have one place each, and the next tile's K is
+// on its way while V is worked on, and the other way round.
+template <int T, int HD>
+struct Plan {
+    static constexpr int ES = Kind<T>::ES;
+    static constexpr int DS = HD == 512 ? 2 : 1;
+    static constexpr int NW = T == G4_F32 ? 4 : 8;                   // waves; 8: two a SIMD
+    static constexpr int NJ = NW / DS, LGROWS = NJ == 8 ? 8 : NJ == 4 ? 7 : 6;   // 32 NJ = 2^LGROWS rows
+    static constexpr int STAGE = 64 * HD * ES + 1024;                // bytes of a tile in LDS
+    static constexpr int STAGES = DS == 2 ? 1 : 2;
+    static constexpr int XCH = DS == 2 ? NW * 4096 : 0;
+    static constexpr int LDS = STAGE * STAGES + XCH;
+};
+
+template <int T, int HD>
+__global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void attn_packed_kernel(PackedArgs a) {
+    typedef Plan<T, HD> P;
+    typedef typename Kind<T>::t E;
+    typedef typename Kind<T>::op op;
+    constexpr int ES = P::ES, NS = Kind<T>::NS, NW = P::NW, DS = P::DS, NJ = P::NJ;
+    constexpr int KS = HD / 16 / DS, NT = HD / 32 / DS;   // a wave's product steps and 32-dim tiles
+    constexpr int kPieces = 4 * HD * ES / 64;             // KB of K and V of a tile (without the meta bytes)
+    constexpr int kPerWave = kPieces / NW;
+    constexpr float kSlack = T == G4_F32 ? 4.0f : 8.0f;
+    constexpr float kLift = T == G4_F32 ? 11.0f : 0.0f;   // fp16 weights: 2^11 above their fp32 size
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % DS;
+
+    // ---- whose rows ----
+    const unsigned id = blockIdx.x, kvh = id % (unsigned)a.n_kv, u = (gridDim.x - 1 - id) / (unsigned)a.n_kv;
+    const int s = unit_seq(a.cu, a.n_seqs, a.group, P::LGROWS, a.extra, u);
+    const int r0 = a.cu[s], r1 = a.cu[s + 1], n = r1 - r0;
+    if (r0 < 0 || n <= 0 || r1 > a.m) return;
+    const unsigned c = u - unit_base(a.cu, s, a.group, P::LGROWS, a.extra);
+    const long jobs = (long)((n + 31) >> 5) * a.group, job0 = (long)c * NJ;
+    if (job0 >= jobs) return;
+    const long jl = job0 + NJ < jobs ? job0 + NJ - 1 : jobs - 1;
+    const long job = job0 + wave / DS < jobs ? job0 + wave / DS : jl;
+    const bool mine = job0 + wave / DS < jobs;
+    const int jt = (int)(job / a.group), head = (int)kvh * a.group + (int)(job - (long)jt * a.group);
+    const int row = jt * 32 + col;                        // this lane's row of the sequence
+    auto first_key = [&](int r) { return a.window > 0 && r >= a.window ? r + 1 - a.window : 0; };
+    const int kt0 = first_key((int)(job0 / a.group) * 32) >> 5, kt1 = (int)(jl / a.group);
+    const int my0 = mine ? first_key(jt * 32) >> 5 : kt1 + 1, my1 = mine ? jt : kt0 - 1;
+    const int wfirst = first_key(row);
+    // tiles that every row of the job sees whole lie between these
+    const int full0 = (first_key(jt * 32 + 31) + 31) >> 5, full1 = jt - 1;
+
+    // ---- tiles on their way into LDS ----
+    const uint8_t* rec0 = a.work + ((size_t)unit_base(a.cu, s, 1, 5, 1) * a.n_kv + kvh) * block_bytes(HD, ES);
+    auto stage = [&](int kt, int from, int to) {   // this wave's share of the pieces from .. to - 1
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(rec0 + (size_t)kt * a.n_kv * block_bytes(HD, ES)), 0, (int)block_bytes(HD, ES), kBufWord3);
+        uint8_t* at = lds + (P::STAGES == 2 ? (kt & 1) * P::STAGE : 0);
+#pragma unroll
+        for (int i = 0; i < kPerWave; i++) {
+            const int piece = i * NW + wave;
+            if (i * NW >= from && i * NW < to) buf_load_lds16(r, at + piece * 1024, lane * 16, piece * 1024);
+        }
+        // the last half kilobyte (the other half: no such bytes)
+        if (to == kPieces && wave == 0) buf_load_lds16(r, at + kPieces * 1024, lane * 16, kPieces * 1024);
+    };
+    stage(kt0, 0, kPieces);
+
+    // ---- q ----
+    op q[NS][KS];
+    float fq = fabsf(a.scale) * kLog2e;
+    const E* qr = (const E*)a.q + (size_t)(r0 + (row < n ? row : n - 1)) * a.q_stride + (size_t)head * HD;
+    if constexpr (T == G4_F32) {
+        float4 x[DS][KS][2];
+        unsigned top = 0;
+#pragma unroll
+        for (int p = 0; p < DS; p++)
+#pragma unroll
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float4 y = reinterpret_cast<const float4*>(qr + (p == 0 ? part : 1 - part) * (HD / DS) + i * 16 + h * 8)[j];
+                    x[p][i][j] = y;
+                    const float e[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const unsigned m = __float_as_uint(e[k]) & 0x7fffffffu;
+                        top = m > top ? m : top;
+                    }
+                }
+        const unsigned o = __shfl_xor(top, 32, 64);
+        top = o > top ? o : top;
+        const int e = (int)(top >> 23) > kLowK ? (int)(top >> 23) : kLowK;
+        float sf = row_scale(e < 255 ? e : 254);
+        fq *= e < 255 ? row_scale_inv(e) : __uint_as_float(0x7fc00000u);
+        if (a.scale < 0.0f) sf = -sf;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            h2v_t hi[4], lo[4];
+            split2(x[0][i][0].x, x[0][i][0].y, sf, hi[0], lo[0]);
+            split2(x[0][i][0].z, x[0][i][0].w, sf, hi[1], lo[1]);
+            split2(x[0][i][1].x, x[0][i][1].y, sf, hi[2], lo[2]);
+            split2(x[0][i][1].z, x[0][i][1].w, sf, hi[3], lo[3]);
+            __builtin_memcpy(&q[0][i], hi, 16);
+            __builtin_memcpy(&q[1][i], lo, 16);
+        }
+    } else {
+        const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            uint4 x = *reinterpret_cast<const uint4*>(qr + part * (HD / DS) + i * 16 + h * 8);
+            if (a.scale == 0.0f) x = make_uint4(0, 0, 0, 0);
+            x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+            q[0][i] = __builtin_bit_cast(op, x);
+        }
+        if (a.scale == 0.0f) fq = 1.0f;
+    }
+
+    f16_t o[NT] = {};
+    float m = -FLT_MAX, l = 0.0f;
+    for (int kt = kt0; kt <= kt1; kt++) {
+        const uint8_t* at = lds + (P::STAGES == 2 ? (kt & 1) * P::STAGE : 0);
+        // this wave's copies have landed, then everyone's; and all are done with the tile before
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();
+        if (P::STAGES == 2 && kt < kt1) stage(kt + 1, 0, kPieces);
+        const bool work = kt >= my0 && kt <= my1;
+        f16_t sc = {}, sx = {};
+        if (work) {
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                const op k0 = *reinterpret_cast<const op*>(at + (part * KS + i) * 1024 + lane * 16);
+                sc = mfma32(k0, q[0][i], sc);
+                if constexpr (NS == 2) {
+                    const op k1 = *reinterpret_cast<const op*>(at + 64 * HD + (part * KS + i) * 1024 + lane * 16);
+                    sx = mfma32(k0, q[1][i], sx);
+                    sx = mfma32(k1, q[0][i], sx);
+                }
+            }
+            if constexpr (NS == 2) sc += sx;
+        }
+        if constexpr (DS == 2) {
+            f4_t* box = reinterpret_cast<f4_t*>(lds + P::STAGE * P::STAGES);
+            if (work) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    box[(wave * 4 + i) * 64 + lane] = f4_t{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+            }
+            lds_barrier();   // K is done with, too
+            if (kt < kt1) stage(kt + 1, 0, kPieces / 2);
+            if (work) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const f4_t y = box[((wave ^ 1) * 4 + i) * 64 + lane];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sc[4 * i + j] += y[j];
+                }
+            }
+        }
+        if (work) {
+            const float* meta = reinterpret_cast<const float*>(at + 64 * HD * ES);
+            const unsigned* mk = reinterpret_cast<const unsigned*>(meta) + kMetaMask / 4;
+            const unsigned marks = __builtin_amdgcn_readfirstlane(mk[0] | mk[1]);
+            float vinv[16];
+            if constexpr (T == G4_F32) {
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const float4 fk = *reinterpret_cast<const float4*>(meta + 8 * b + 4 * h);
+                    const float4 ve = *reinterpret_cast<const float4*>(meta + kMetaVExp / 4 + 8 * b + 4 * h);
+                    const float4 vi = *reinterpret_cast<const float4*>(meta + kMetaVInv / 4 + 8 * b + 4 * h);
+                    const float f[4] = {fk.x, fk.y, fk.z, fk.w}, e[4] = {ve.x, ve.y, ve.z, ve.w}, v[4] = {vi.x, vi.y, vi.z, vi.w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        sc[4 * b + i] = __builtin_fmaf(sc[4 * b + i], fq * f[i], e[i]);
+                        vinv[4 * b + i] = v[i];
+                    }
+                }
+            }
+            if (marks) {
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (marks >> (8 * (r >> 2) + 4 * h + (r & 3)) & 1) sc[r] = __uint_as_float(0x7fc00000u);
+            }
+            if (kt < full0 || kt > full1) {
+                const int hi = row - kt * 32 - 4 * h, lo = wfirst - kt * 32 - 4 * h;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int key = 8 * (r >> 2) + (r & 3);
+                    if (key > hi || key < lo) sc[r] = -INFINITY;
+                }
+            }
+            float top = sc[0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) top = fmaxf(top, sc[r]);
+            if constexpr (T != G4_F32) top *= fq;
+            if (__any(top > m + kSlack)) {
+                top = fmaxf(top, shfl_xor(top, 32));
+                top = fmaxf(top, m);
+                const float f = exp2f(m - top);
+                m = top;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < NT; i++) o[i] *= f;
+            }
+            const float base = m - kLift;
+            op p[NS][2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float x = sc[8 * t + j];
+                    w[j] = __builtin_amdgcn_exp2f(T == G4_F32 ? x - base : __builtin_fmaf(x, fq, -base));
+                    if constexpr (T == G4_F32) l = __builtin_fmaf(w[j], vinv[8 * t + j], l);
+                    else l += w[j];
+                }
+                if constexpr (T == G4_F32) {
+                    h2v_t hi[4], lo[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) split2(w[2 * j], w[2 * j + 1], 1.0f, hi[j], lo[j]);
+                    __builtin_memcpy(&p[0][t], hi, 16);
+                    __builtin_memcpy(&p[1][t], lo, 16);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) p[0][t][j] = (E)w[j];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const uint8_t* v = at + 32 * HD * ES + ((part * NT + i) * 2 + t) * 1024 + lane * 16;
+                    const op v0 = *reinterpret_cast<const op*>(v);
+                    o[i] = mfma32(v0, p[0][t], o[i]);
+                    if constexpr (NS == 2) {
+                        o[i] = mfma32(v0, p[1][t], o[i]);
+                        o[i] = mfma32(*reinterpret_cast<const op*>(v + 64 * HD), p[0][t], o[i]);
+                    }
+                }
+        }
+        if constexpr (P::STAGES == 1) {
+            lds_barrier();   // V is done with
+            if (kt < kt1) stage(kt + 1, kPieces / 2, kPieces);
+        }
+    }
+
+    if (!mine || row >= n) return;
+    l += shfl_xor(l, 32);
+    const float f = 1.0f / l;
+    E* out = (E*)a.out + (size_t)(r0 + row) * a.out_stride + (size_t)head * HD + part * (HD / DS);
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            E y[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = (E)(o[i][4 * b + j] * f);
+            __builtin_memcpy(__builtin_assume_aligned(out + i * 32 + 8 * b + 4 * h, 4 * ES), y, 4 * ES);
+        }
+}
+
+template <int T, int HD>
+int launch_packed(PackedArgs a) {
+    typedef Plan<T, HD> P;
+    static bool done = false;
+    if (!done) {
+        // more than 64 KB of LDS has to be asked for once
+        G4_HIP(hipFuncSetAttribute((const void*)attn_packed_kernel<T, HD>, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS));
+        done = true;
+    }
+    hipLaunchKernelGGL((packed_layout_kernel<T, HD>), dim3(a.m / 32 + a.n_seqs, a.n_kv, 2), dim3(256), 0, g4_stream(), a);
+    // a sequence of n rows has ceil(ceil(n / 32) group / NJ) units, at most
+    // n group / (32 NJ) + extra
+    a.extra = (31 * a.group + 32 * (P::NJ - 1) + 32 * P::NJ - 1) / (32 * P::NJ);
+    const size_t units = (((size_t)a.m * a.group) >> P::LGROWS) + (size_t)a.extra * a.n_seqs;
+    hipLaunchKernelGGL((attn_packed_kernel<T, HD>), dim3((unsigned)(units * a.n_kv)), dim3(64 * P::NW), P::LDS, g4_stream(), a);
+    return g4_check_launch("attn_packed_kernel");
+}
+template <int T>
+int launch_packed(const PackedArgs& a, int hd) {
+    if (hd == 64) return launch_packed<T, 64>(a);
+    if (hd == 128) return launch_packed<T, 128>(a);
+    if (hd == 256) return launch_packed<T, 256>(a);
+    return launch_packed<T, 512>(a);
 }
 
 int packed_size(int type) { return type == G4_F32 ? 4 : type == G4_F16 || type == G4_BF16 ? 2 : 0; }
@@ -87,8 +506,7 @@ extern "C" size_t g4_attn_prompt_packed_work_bytes(int type, int n_seqs, int m, 
     if (!packed_size(type) || n_seqs < 1 || n_seqs > kKvMaxSeqs || m < 1 || n_kv < 1 || n_kv > 65535 ||
         (hd != 64 && hd != 128 && hd != 256 && hd != 512))
         return 0;
-    const size_t blocks = (size_t)(m / 32 + n_seqs) * n_kv;
-    return blocks * (64 * hd * (type == G4_F32 ? 4 : 2) + 32 * 8 + 16);
+    return ((size_t)m / 32 + n_seqs) * n_kv * block_bytes(hd, packed_size(type));
 }
 
 extern "C" int g4_attn_prompt_packed(const void* q, int q_stride, const void* k, const void* v, int kv_stride, void* out,
@@ -108,11 +526,10 @@ extern "C" int g4_attn_prompt_packed(const void* q, int q_stride, const void* k,
                  kv_stride / hd >= n_kv && out_stride / hd >= n_heads,
                  "%s: strides %d, %d, %d (multiples of %d, heads * hd at least)", who, q_stride, kv_stride, out_stride, unit);
     PackedArgs a = {};
-    a.q = q; a.k = k; a.v = v; a.out = out; a.work = work; a.cu = cu; a.q_stride = q_stride; a.kv_stride = kv_stride;
-    a.out_stride = out_stride; a.n_seqs = n_seqs; a.m = m; a.window = window; a.n_heads = n_heads; a.n_kv = n_kv;
-    a.scale = attn_scale;
-    if (type == G4_F32) launch_packed<float>(a, hd);
-    else if (type == G4_F16) launch_packed<_Float16>(a, hd);
-    else launch_packed<__bf16>(a, hd);
-    return g4_check_launch("attn_packed_kernel");
+    a.q = q; a.k = k; a.v = v; a.out = out; a.work = (uint8_t*)work; a.cu = cu; a.q_stride = q_stride;
+    a.kv_stride = kv_stride; a.out_stride = out_stride; a.n_seqs = n_seqs; a.m = m; a.window = window;
+    a.n_heads = n_heads; a.n_kv = n_kv; a.group = n_heads / n_kv; a.scale = attn_scale;
+    if (type == G4_F32) return launch_packed<G4_F32>(a, hd);
+    if (type == G4_F16) return launch_packed<G4_F16>(a, hd);
+    return launch_packed<G4_BF16>(a, hd);
 }

@@ -64,18 +64,18 @@ struct KvPool {
 };
 
 // the sequence that work unit u belongs to: the largest s < n with
-// (cu[s] >> lg) + extra * s <= u (0 if there is none), found by a whole wave
-// in steps of 64 candidates.  Any contents of cu give an s in range.
-__device__ __forceinline__ int unit_seq(const int* __restrict__ cu, int n, int lg, int extra, unsigned u) {
+// (mul cu[s] >> lg) + extra * s <= u (0 if there is none), found by a whole
+// wave in steps of 64 candidates.  Any contents of cu give an s in range.
+__device__ __forceinline__ unsigned unit_base(const int* __restrict__ cu, int s, int mul, int lg, int extra) {
+    return (unsigned)(((unsigned long long)(unsigned)cu[s] * (unsigned)mul) >> lg) + (unsigned)extra * (unsigned)s;
+}
+__device__ __forceinline__ int unit_seq(const int* __restrict__ cu, int n, int mul, int lg, int extra, unsigned u) {
     const int lane = threadIdx.x & 63;
     int lo = 0;
     while (n > 1) {
         const int step = (n + 63) >> 6;
         bool in = (long)lane * step < n;
-        if (in) {
-            const int i = lo + lane * step;
-            in = ((unsigned)cu[i] >> lg) + (unsigned)extra * (unsigned)i <= u;
-        }
+        if (in) in = unit_base(cu, lo + lane * step, mul, lg, extra) <= u;
         const int c = __popcll(__ballot(in));
         const int adv = (c > 0 ? c - 1 : 0) * step;
         lo += adv;

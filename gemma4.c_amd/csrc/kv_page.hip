@@ -51,11 +51,11 @@ struct Unit {
 
 __device__ __forceinline__ bool find_unit(const RowArgs& a, Unit& u) {
     const unsigned id = blockIdx.x;
-    const int s = unit_seq(a.cu, a.n_seqs, 4, 2, id);
+    const int s = unit_seq(a.cu, a.n_seqs, 1, 4, 2, id);
     const int r0 = a.cu[s], r1 = a.cu[s + 1], len = a.lens[s];
     if (r0 < 0 || r1 <= r0 || r1 > a.m || r1 - r0 > len || !a.p.fits(len)) return false;
     const int pos0 = len - (r1 - r0);
-    const unsigned b = id - (((unsigned)r0 >> 4) + 2u * (unsigned)s);
+    const unsigned b = id - unit_base(a.cu, s, 1, 4, 2);
     const int first = pos0 >> 4, blocks = ((len - 1) >> 4) - first + 1;
     if (b >= (unsigned)blocks) return false;
     const int at = (first + (int)b) << 4;
