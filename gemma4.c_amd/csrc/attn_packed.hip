@@ -102,6 +102,12 @@ __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
     const bool is_v = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int sub = lane / LPR, col = lane % LPR;
+    // LDS slot of lane l's 16 bytes of a piece: the lanes of a row write to
+    // one slot of many pieces (K) or to every 4th or 8th slot (V), all on the
+    // same banks without the exchange
+    auto swz = [&](int piece, int l) {
+        return piece * 64 + (is_v ? l ^ (l >> 3 & 3) ^ (piece >> 1 & 1) << 2 : l ^ ((piece * 2 + (l >> 5)) & 7));
+    };
     const E* src = (const E*)(is_v ? a.v : a.k) + (size_t)blockIdx.y * HD;
     if (tid == 0) marks = 0;
     uint4 x[PASS][VPL];
@@ -189,17 +195,17 @@ __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
 #pragma unroll
                     for (int j = 0; j < VW; j++) {
                         const int d = c + j;
-                        *reinterpret_cast<uint16_t*>(img + ((d >> 5) * 2 + u) * 1024 + (h * 32 + (d & 31)) * 16 + slot * 2) = e[j];
+                        *reinterpret_cast<uint16_t*>(img + swz((d >> 5) * 2 + u, h * 32 + (d & 31)) * 16 + slot * 2) = e[j];
                     }
                 } else {
-                    __builtin_memcpy(__builtin_assume_aligned(img + (c >> 4) * 1024 + ((c >> 3 & 1) * 32 + t) * 16 + (c & 7) * 2, VW * 2),
-                                     e, VW * 2);
+                    __builtin_memcpy(__builtin_assume_aligned(img + swz(c >> 4, (c >> 3 & 1) * 32 + t) * 16 + (c & 7) * 2, VW * 2), e,
+                                     VW * 2);
                 }
             }
         }
         lds_sync();
         for (int i = tid; i < 4 * HD; i += 256)
-            reinterpret_cast<uint4*>(out + half * 64 * HD)[i] = reinterpret_cast<const uint4*>(img)[i];
+            reinterpret_cast<uint4*>(out + half * 64 * HD)[i] = reinterpret_cast<const uint4*>(img)[swz(i >> 6, i & 63)];
     }
     if (tid == 0) reinterpret_cast<unsigned*>(meta)[kMetaMask / 4 + is_v] = marks;
 }
@@ -214,32 +220,49 @@ __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
 // registers): a job's dims are halved over two waves, whose partial scores
 // meet in LDS; K and V of a tile have one place each, and the next tile's K is
 // on its way while V is worked on, and the other way round.
+// KSP 2 (16 bits): the two waves of a SIMD are given the same job and every
+// other tile, so that there are twice the workgroups, half as long, and the
+// one does its second product while the other is at its weights: waves 4 .. 7
+// put it off to the next tile.  Their sums meet at the end, in LDS.
 template <int T, int HD>
 struct Plan {
     static constexpr int ES = Kind<T>::ES;
     static constexpr int DS = HD == 512 ? 2 : 1;
     static constexpr int NW = T == G4_F32 ? 4 : 8;                   // waves; 8: two a SIMD
-    static constexpr int NJ = NW / DS, LGROWS = NJ == 8 ? 8 : NJ == 4 ? 7 : 6;   // 32 NJ = 2^LGROWS rows
-    static constexpr int STAGE = 64 * HD * ES + 1024;                // bytes of a tile in LDS
-    static constexpr int STAGES = DS == 2 ? 1 : 2;
-    static constexpr int XCH = DS == 2 ? NW * 4096 : 0;
-    static constexpr int LDS = STAGE * STAGES + XCH;
+    static constexpr int KSP = NW == 8 && DS == 1 ? 2 : 1;           // tiles at a time
+    static constexpr int NJ = NW / DS / KSP, LGROWS = NJ == 4 ? 7 : 6;   // 32 NJ = 2^LGROWS rows
+    // LDS: K and V of a tile are TB bytes each
+    static constexpr int TB = 32 * HD * ES;
+    static constexpr int NK = DS == 2 ? 1 : 2 * KSP, NV = DS == 2 ? 1 : KSP == 2 ? 5 : 2;
+    static constexpr int META = (NK + NV) * TB, XCH = META + 2 * KSP * 1024;
+    static constexpr int LDS = XCH + (DS == 2 ? NW * 4096 : 0);
+    static constexpr int JOIN = NJ * (HD * 128 + 256);               // sums of waves 4 .. 7
+    static_assert(LDS <= 160 * 1024 && NJ * DS * KSP == NW && (KSP == 1 || JOIN <= LDS), "LDS");
+    static __device__ __forceinline__ int k_at(int st, int kp) { return DS == 2 ? 0 : ((st & 1) * KSP + kp) * TB; }
+    static __device__ __forceinline__ int v_at(int st, int kp) {
+        return (NK + (DS == 2 ? 0 : kp == 0 ? st & 1 : 2 + st % 3)) * TB;
+    }
+    static __device__ __forceinline__ int meta_at(int st, int kp) { return META + ((st & 1) * KSP + kp) * 1024; }
 };
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 template <int T, int HD>
 __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void attn_packed_kernel(PackedArgs a) {
     typedef Plan<T, HD> P;
     typedef typename Kind<T>::t E;
     typedef typename Kind<T>::op op;
-    constexpr int ES = P::ES, NS = Kind<T>::NS, NW = P::NW, DS = P::DS, NJ = P::NJ;
+    constexpr int ES = P::ES, NS = Kind<T>::NS, NW = P::NW, DS = P::DS, NJ = P::NJ, KSP = P::KSP, TB = P::TB;
     constexpr int KS = HD / 16 / DS, NT = HD / 32 / DS;   // a wave's product steps and 32-dim tiles
-    constexpr int kPieces = 4 * HD * ES / 64;             // KB of K and V of a tile (without the meta bytes)
-    constexpr int kPerWave = kPieces / NW;
+    constexpr int kHalf = TB / 1024;                      // KB of a tile's K, of its V
     constexpr float kSlack = T == G4_F32 ? 4.0f : 8.0f;
     constexpr float kLift = T == G4_F32 ? 11.0f : 0.0f;   // fp16 weights: 2^11 above their fp32 size
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % DS;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % DS, kp = wave / (NJ * DS);
 
     // ---- whose rows ----
     const unsigned id = blockIdx.x, kvh = id % (unsigned)a.n_kv, u = (gridDim.x - 1 - id) / (unsigned)a.n_kv;
@@ -250,32 +273,48 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     const long jobs = (long)((n + 31) >> 5) * a.group, job0 = (long)c * NJ;
     if (job0 >= jobs) return;
     const long jl = job0 + NJ < jobs ? job0 + NJ - 1 : jobs - 1;
-    const long job = job0 + wave / DS < jobs ? job0 + wave / DS : jl;
-    const bool mine = job0 + wave / DS < jobs;
+    const int slot = wave / DS % NJ;
+    const bool mine = job0 + slot < jobs;
+    const long job = mine ? job0 + slot : jl;
     const int jt = (int)(job / a.group), head = (int)kvh * a.group + (int)(job - (long)jt * a.group);
     const int row = jt * 32 + col;                        // this lane's row of the sequence
     auto first_key = [&](int r) { return a.window > 0 && r >= a.window ? r + 1 - a.window : 0; };
     const int kt0 = first_key((int)(job0 / a.group) * 32) >> 5, kt1 = (int)(jl / a.group);
-    const int my0 = mine ? first_key(jt * 32) >> 5 : kt1 + 1, my1 = mine ? jt : kt0 - 1;
+    // the stages that have a tile for this wave: s0 .. s1 - 1
+    const int my0 = (first_key(jt * 32) >> 5) - kt0 - kp, my1 = jt - kt0 - kp;
+    const int s0 = mine && my0 > 0 ? (my0 + KSP - 1) / KSP : 0, s1 = mine && my1 >= 0 ? my1 / KSP + 1 : s0;
     const int wfirst = first_key(row);
     // tiles that every row of the job sees whole lie between these
     const int full0 = (first_key(jt * 32 + 31) + 31) >> 5, full1 = jt - 1;
 
-    // ---- tiles on their way into LDS ----
-    const uint8_t* rec0 = a.work + ((size_t)unit_base(a.cu, s, 1, 5, 1) * a.n_kv + kvh) * block_bytes(HD, ES);
-    auto stage = [&](int kt, int from, int to) {   // this wave's share of the pieces from .. to - 1
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(rec0 + (size_t)kt * a.n_kv * block_bytes(HD, ES)), 0, (int)block_bytes(HD, ES), kBufWord3);
-        uint8_t* at = lds + (P::STAGES == 2 ? (kt & 1) * P::STAGE : 0);
+    // ---- tiles on their way into LDS: stage st has the tiles kt0 + KSP st + (0 .. KSP - 1) ----
+    const int stages = (kt1 - kt0) / KSP + 1;
+    const uint8_t* rec0 = a.work + ((size_t)(unit_base(a.cu, s, 1, 5, 1) + kt0) * a.n_kv + kvh) * block_bytes(HD, ES);
+    const size_t rec_step = (size_t)a.n_kv * block_bytes(HD, ES);
+    constexpr int kShare = kHalf * KSP / NW;              // pieces a wave copies of a stage's K, of its V
+    constexpr int kWhole = kHalf / NW;                    // of one tile's (0: half the waves have a tile each)
+    static_assert(kHalf * KSP % NW == 0 && (kWhole || kShare == 1), "shares");
+    const int first_piece = kWhole ? wave : wave % kHalf;
+    auto stage = [&](int st, bool v) {
 #pragma unroll
-        for (int i = 0; i < kPerWave; i++) {
-            const int piece = i * NW + wave;
-            if (i * NW >= from && i * NW < to) buf_load_lds16(r, at + piece * 1024, lane * 16, piece * 1024);
+        for (int t = 0; t < (kWhole ? KSP : 1); t++) {
+            const int tile = st * KSP + (kWhole ? t : wave / kHalf);
+            // past the last tile: no bytes
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)(rec0 + tile * rec_step), 0, tile <= kt1 - kt0 ? (int)block_bytes(HD, ES) : 0, kBufWord3);
+            const int tt = kWhole ? t : wave / kHalf;
+            uint8_t* at = lds + (v ? P::v_at(st, tt) : P::k_at(st, tt)) + first_piece * 1024;
+#pragma unroll
+            for (int i = 0; i < (kWhole ? kWhole : 1); i++)
+                buf_load_lds16(r, at + i * NW * 1024, first_piece * 1024 + lane * 16, (v ? TB : 0) + i * NW * 1024);
+            // the last half kilobyte (the other half: no such bytes)
+            if (!v && (kWhole ? wave == t : first_piece == 0)) buf_load_lds16(r, lds + P::meta_at(st, tt), lane * 16, 2 * TB);
         }
-        // the last half kilobyte (the other half: no such bytes)
-        if (to == kPieces && wave == 0) buf_load_lds16(r, at + kPieces * 1024, lane * 16, kPieces * 1024);
     };
-    stage(kt0, 0, kPieces);
+    auto stage_k = [&](int st) { stage(st, false); };
+    auto stage_v = [&](int st) { stage(st, true); };
+    stage_k(0);
+    if (DS == 1) stage_v(0);
 
     // ---- q ----
     op q[NS][KS];
@@ -327,136 +366,243 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
         if (a.scale == 0.0f) fq = 1.0f;
     }
 
-    f16_t o[NT] = {};
-    float m = -FLT_MAX, l = 0.0f;
-    for (int kt = kt0; kt <= kt1; kt++) {
-        const uint8_t* at = lds + (P::STAGES == 2 ? (kt & 1) * P::STAGE : 0);
-        // this wave's copies have landed, then everyone's; and all are done with the tile before
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        lds_barrier();
-        if (P::STAGES == 2 && kt < kt1) stage(kt + 1, 0, kPieces);
-        const bool work = kt >= my0 && kt <= my1;
-        f16_t sc = {}, sx = {};
-        if (work) {
+    // one wave a SIMD: q and o stay in the accumulation registers, from which
+    // products take them as well (left to itself the compiler moves them there
+    // and back for every tile)
+    constexpr bool kAcc = T == G4_F32 && HD >= 256;
+    if constexpr (kAcc) {
+#pragma unroll
+        for (int k = 0; k < NS; k++)
 #pragma unroll
             for (int i = 0; i < KS; i++) {
-                const op k0 = *reinterpret_cast<const op*>(at + (part * KS + i) * 1024 + lane * 16);
-                sc = mfma32(k0, q[0][i], sc);
-                if constexpr (NS == 2) {
-                    const op k1 = *reinterpret_cast<const op*>(at + 64 * HD + (part * KS + i) * 1024 + lane * 16);
-                    sx = mfma32(k0, q[1][i], sx);
-                    sx = mfma32(k1, q[0][i], sx);
-                }
+                asm("" : "+a"(q[k][i]));
             }
-            if constexpr (NS == 2) sc += sx;
-        }
-        if constexpr (DS == 2) {
-            f4_t* box = reinterpret_cast<f4_t*>(lds + P::STAGE * P::STAGES);
-            if (work) {
+    }
+    f16_t o[NT] = {};
+    float m = -FLT_MAX, l = 0.0f;
+    f16_t sc;
+    op p[NS][2];
+    auto scores = [&](int st) {
+        const uint8_t* at = lds + P::k_at(st, kp) + lane * 16;
+        sc = f16_t{};
+        f16_t sx = {};
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    box[(wave * 4 + i) * 64 + lane] = f4_t{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+        for (int i = 0; i < KS; i++) {
+            const op k0 = *reinterpret_cast<const op*>(at + (part * KS + i) * 1024);
+            sc = mfma32(k0, q[0][i], sc);
+            if constexpr (NS == 2) {
+                const op k1 = *reinterpret_cast<const op*>(at + 64 * HD + (part * KS + i) * 1024);
+                sx = mfma32(k0, q[1][i], sx);
+                sx = mfma32(k1, q[0][i], sx);
             }
-            lds_barrier();   // K is done with, too
-            if (kt < kt1) stage(kt + 1, 0, kPieces / 2);
-            if (work) {
+        }
+        if constexpr (NS == 2) sc += sx;
+    };
+    auto weights = [&](int st, int kt) {
+        const float* meta = reinterpret_cast<const float*>(lds + P::meta_at(st, kp));
+        const unsigned* mk = reinterpret_cast<const unsigned*>(meta) + kMetaMask / 4;
+        const unsigned marks = __builtin_amdgcn_readfirstlane(mk[0] | mk[1]);
+        float vinv[16];
+        if constexpr (T == G4_F32) {
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const float4 fk = *reinterpret_cast<const float4*>(meta + 8 * b + 4 * h);
+                const float4 ve = *reinterpret_cast<const float4*>(meta + kMetaVExp / 4 + 8 * b + 4 * h);
+                const float4 vi = *reinterpret_cast<const float4*>(meta + kMetaVInv / 4 + 8 * b + 4 * h);
+                const float f[4] = {fk.x, fk.y, fk.z, fk.w}, e[4] = {ve.x, ve.y, ve.z, ve.w}, v[4] = {vi.x, vi.y, vi.z, vi.w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const f4_t y = box[((wave ^ 1) * 4 + i) * 64 + lane];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) sc[4 * i + j] += y[j];
+                    sc[4 * b + i] = __builtin_fmaf(sc[4 * b + i], fq * f[i], e[i]);
+                    vinv[4 * b + i] = v[i];
                 }
             }
         }
-        if (work) {
-            const float* meta = reinterpret_cast<const float*>(at + 64 * HD * ES);
-            const unsigned* mk = reinterpret_cast<const unsigned*>(meta) + kMetaMask / 4;
-            const unsigned marks = __builtin_amdgcn_readfirstlane(mk[0] | mk[1]);
-            float vinv[16];
+        if (marks) {
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (marks >> (8 * (r >> 2) + 4 * h + (r & 3)) & 1) sc[r] = __uint_as_float(0x7fc00000u);
+        }
+        if (kt < full0 || kt > full1) {
+            const int hi = row - kt * 32 - 4 * h, lo = wfirst - kt * 32 - 4 * h;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int key = 8 * (r >> 2) + (r & 3);
+                if (key > hi || key < lo) sc[r] = -INFINITY;
+            }
+        }
+        float top = sc[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) top = fmaxf(top, sc[r]);
+        if constexpr (T != G4_F32) top *= fq;
+        if (__any(top > m + kSlack)) {
+            top = fmaxf(top, shfl_xor(top, 32));
+            top = fmaxf(top, m);
+            const float f = exp2f(m - top);
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < NT; i++) o[i] *= f;
+        }
+        const float base = m - kLift;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float x = sc[8 * t + j];
+                w[j] = __builtin_amdgcn_exp2f(T == G4_F32 ? x - base : __builtin_fmaf(x, fq, -base));
+                if constexpr (T == G4_F32) l = __builtin_fmaf(w[j], vinv[8 * t + j], l);
+                else l += w[j];
+            }
             if constexpr (T == G4_F32) {
+                h2v_t hi[4], lo[4];
 #pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const float4 fk = *reinterpret_cast<const float4*>(meta + 8 * b + 4 * h);
-                    const float4 ve = *reinterpret_cast<const float4*>(meta + kMetaVExp / 4 + 8 * b + 4 * h);
-                    const float4 vi = *reinterpret_cast<const float4*>(meta + kMetaVInv / 4 + 8 * b + 4 * h);
-                    const float f[4] = {fk.x, fk.y, fk.z, fk.w}, e[4] = {ve.x, ve.y, ve.z, ve.w}, v[4] = {vi.x, vi.y, vi.z, vi.w};
+                for (int j = 0; j < 4; j++) split2(w[2 * j], w[2 * j + 1], 1.0f, hi[j], lo[j]);
+                __builtin_memcpy(&p[0][t], hi, 16);
+                __builtin_memcpy(&p[1][t], lo, 16);
+            } else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        sc[4 * b + i] = __builtin_fmaf(sc[4 * b + i], fq * f[i], e[i]);
-                        vinv[4 * b + i] = v[i];
-                    }
-                }
+                for (int j = 0; j < 8; j++) p[0][t][j] = (E)w[j];
             }
-            if (marks) {
+        }
+    };
+    auto values = [&](int st) {
+        const uint8_t* at = lds + P::v_at(st, kp) + lane * 16;
 #pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (marks >> (8 * (r >> 2) + 4 * h + (r & 3)) & 1) sc[r] = __uint_as_float(0x7fc00000u);
-            }
-            if (kt < full0 || kt > full1) {
-                const int hi = row - kt * 32 - 4 * h, lo = wfirst - kt * 32 - 4 * h;
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int key = 8 * (r >> 2) + (r & 3);
-                    if (key > hi || key < lo) sc[r] = -INFINITY;
-                }
-            }
-            float top = sc[0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) top = fmaxf(top, sc[r]);
-            if constexpr (T != G4_F32) top *= fq;
-            if (__any(top > m + kSlack)) {
-                top = fmaxf(top, shfl_xor(top, 32));
-                top = fmaxf(top, m);
-                const float f = exp2f(m - top);
-                m = top;
-                l *= f;
-#pragma unroll
-                for (int i = 0; i < NT; i++) o[i] *= f;
-            }
-            const float base = m - kLift;
-            op p[NS][2];
+        for (int i = 0; i < NT; i++)
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                float w[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float x = sc[8 * t + j];
-                    w[j] = __builtin_amdgcn_exp2f(T == G4_F32 ? x - base : __builtin_fmaf(x, fq, -base));
-                    if constexpr (T == G4_F32) l = __builtin_fmaf(w[j], vinv[8 * t + j], l);
-                    else l += w[j];
+                const uint8_t* v = at + ((part * NT + i) * 2 + t) * 1024;
+                const op v0 = *reinterpret_cast<const op*>(v);
+                o[i] = mfma32(v0, p[0][t], o[i]);
+                if constexpr (NS == 2) {
+                    o[i] = mfma32(v0, p[1][t], o[i]);
+                    o[i] = mfma32(*reinterpret_cast<const op*>(v + 64 * HD), p[0][t], o[i]);
                 }
-                if constexpr (T == G4_F32) {
-                    h2v_t hi[4], lo[4];
+            }
+    };
+
+    if constexpr (DS == 1) {
+        // this wave's copies have landed, then everyone's; and all are done
+        // with the stage before (waves 4 .. 7 but for its V, which has three
+        // places)
+        auto turn = [&](int st) {
+            wait_vm<0>();
+            lds_barrier();
+            if (st + 1 < stages) {
+                stage_k(st + 1);
+                stage_v(st + 1);
+            }
+        };
+        int st = 0;
+        for (; st < s0; st++) turn(st);
+        if (KSP == 1 || kp == 0) {
+            for (; st < s1; st++) {
+                turn(st);
+                scores(st);
+                weights(st, kt0 + st * KSP + kp);
+                values(st);
+            }
+        } else if (s0 < s1) {
+            turn(st);
+            scores(st);
+            weights(st, kt0 + st * KSP + kp);
+            for (st++; st < s1; st++) {
+                turn(st);
+                values(st - 1);
+                scores(st);
+                weights(st, kt0 + st * KSP + kp);
+            }
+            if (st < stages) turn(st);
+            values(s1 - 1);
+            st++;
+        }
+        for (; st < stages; st++) turn(st);
+    } else {
+        // a tile's turn up to its scores, and from there on; both waves of a job
+        // take part in the same ones
+        f4_t* box = reinterpret_cast<f4_t*>(lds + P::XCH);
+        auto begin = [&](int st) {
+            wait_vm<0>();
+            lds_barrier();   // K is there, V of the tile before done with
+            stage_v(st);
+        };
+        auto middle = [&](int st) {
+            lds_barrier();   // K is done with, the partial scores there
+            if (st + 1 < stages) stage_k(st + 1);
+        };
+        auto end = [&](int st) {
+            // all copies but those of the next K (and, wave 0, its factors)
+            if (st + 1 >= stages) wait_vm<0>();
+            else if (wave == 0) wait_vm<kShare + 1>();
+            else wait_vm<kShare>();
+            lds_barrier();   // V is there
+        };
+        int st = 0;
+        for (; st < s0; st++) {
+            begin(st);
+            middle(st);
+            end(st);
+        }
+        for (; st < s1; st++) {
+            begin(st);
+            scores(st);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) split2(w[2 * j], w[2 * j + 1], 1.0f, hi[j], lo[j]);
-                    __builtin_memcpy(&p[0][t], hi, 16);
-                    __builtin_memcpy(&p[1][t], lo, 16);
-                } else {
+            for (int i = 0; i < 4; i++)
+                box[(wave * 4 + i) * 64 + lane] = f4_t{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+            middle(st);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) p[0][t][j] = (E)w[j];
-                }
+            for (int i = 0; i < 4; i++) {
+                const f4_t y = box[((wave ^ 1) * 4 + i) * 64 + lane];
+#pragma unroll
+                for (int j = 0; j < 4; j++) sc[4 * i + j] += y[j];
+            }
+            weights(st, kt0 + st);
+            end(st);
+            values(st);
+        }
+        for (; st < stages; st++) {
+            begin(st);
+            middle(st);
+            end(st);
+        }
+    }
+
+    if constexpr (KSP == 2) {
+        // waves 4 .. 7 hand their sums to waves 0 .. 3
+        wait_vm<0>();
+        lds_barrier();
+        float* ml = reinterpret_cast<float*>(lds + NJ * HD * 128) + slot * 64 + col * 2;
+        f4_t* box = reinterpret_cast<f4_t*>(lds) + slot * HD * 8 + lane;
+        l += shfl_xor(l, 32);
+        if (kp == 1) {
+            if (h == 0) {
+                ml[0] = m;
+                ml[1] = l;
             }
 #pragma unroll
             for (int i = 0; i < NT; i++)
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const uint8_t* v = at + 32 * HD * ES + ((part * NT + i) * 2 + t) * 1024 + lane * 16;
-                    const op v0 = *reinterpret_cast<const op*>(v);
-                    o[i] = mfma32(v0, p[0][t], o[i]);
-                    if constexpr (NS == 2) {
-                        o[i] = mfma32(v0, p[1][t], o[i]);
-                        o[i] = mfma32(*reinterpret_cast<const op*>(v + 64 * HD), p[0][t], o[i]);
-                    }
-                }
+                for (int b = 0; b < 4; b++)
+                    box[(i * 4 + b) * 64] = f4_t{o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
         }
-        if constexpr (P::STAGES == 1) {
-            lds_barrier();   // V is done with
-            if (kt < kt1) stage(kt + 1, kPieces / 2, kPieces);
-        }
+        lds_barrier();
+        if (kp == 1) return;
+        const float m1 = ml[0], l1 = ml[1], top = fmaxf(m, m1);
+        const float f0 = exp2f(m - top), f1 = exp2f(m1 - top);
+        l = l * f0 + l1 * f1;
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const f4_t y = box[(i * 4 + b) * 64];
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[i][4 * b + j] = o[i][4 * b + j] * f0 + y[j] * f1;
+            }
+    } else {
+        l += shfl_xor(l, 32);
     }
-
     if (!mine || row >= n) return;
-    l += shfl_xor(l, 32);
     const float f = 1.0f / l;
     E* out = (E*)a.out + (size_t)(r0 + row) * a.out_stride + (size_t)head * HD + part * (HD / DS);
 #pragma unroll
