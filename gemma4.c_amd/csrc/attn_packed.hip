@@ -94,9 +94,9 @@ __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
     __shared__ __align__(16) uint8_t img[64 * HD];         // one half (hi or lo) of K or V
     __shared__ unsigned marks;
     const unsigned id = blockIdx.x;
-    const int s = unit_seq(a.cu, a.n_seqs, 1, 5, 1, id);
-    const int r0 = a.cu[s], r1 = a.cu[s + 1];
-    const unsigned b = id - unit_base(a.cu, s, 1, 5, 1);
+    const SeqAt sq = find_seq(a.cu, nullptr, a.n_seqs, 1, 5, 1, id);
+    const int r0 = sq.r0, r1 = sq.r1;
+    const unsigned b = id - (((unsigned)r0 >> 5) + (unsigned)sq.s);
     if (r0 < 0 || r1 <= r0 || r1 > a.m || b >= (unsigned)((r1 - r0 + 31) >> 5)) return;
     const int row0 = r0 + (int)b * 32, rows = r1 - row0 < 32 ? r1 - row0 : 32;
     const bool is_v = blockIdx.z;
@@ -210,6 +210,70 @@ __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
     if (tid == 0) reinterpret_cast<unsigned*>(meta)[kMetaMask / 4 + is_v] = marks;
 }
 
+// ---- few rows: one launch, fp32 throughout --------------------------------------
+// A workgroup a row and head, a wave a key at a time: a hundredth of the
+// products' rate, without the latency of a second launch and of tiles.  Taken
+// where rows x keys x heads cannot pass 2^18 however the rows fall into
+// sequences.  One sequence, 8 heads, fp32 / bf16, this against the other: 128
+// rows of 256 14.0 / 15.4 against 27.1 / 18.8 us, 192 rows 21.7 / 23.5 against
+// 32.4 / 20.3, 256 rows 42.7 / 47.2 against 36.6 / 21.9; 128 rows of 512 18.8 /
+// 19.9 against 38.6 / 27.0.
+constexpr double kFewPairs = 1 << 18;
+template <int T, int HD>
+__global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedArgs a) {
+    typedef typename Kind<T>::t E;
+    constexpr int N = HD / 64;
+    const int row = blockIdx.x, h = blockIdx.y, kvh = h / a.group;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float red[4][HD + 2];
+    const SeqAt sq = find_seq(a.cu, nullptr, a.n_seqs, 1, 0, 0, (unsigned)row);
+    const int r0 = sq.r0, r1 = sq.r1;
+    if (r0 < 0 || r1 > a.m || row < r0 || row >= r1) return;
+    const int first = a.window > 0 && row - r0 >= a.window ? row + 1 - a.window : r0;
+    const E* K = (const E*)a.k + (size_t)kvh * HD;
+    const E* V = (const E*)a.v + (size_t)kvh * HD;
+    float q[N], o[N] = {}, m = -FLT_MAX, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        q[i] = (float)((const E*)a.q)[(size_t)row * a.q_stride + (size_t)h * HD + i * 64 + lane] * (a.scale * kLog2e);
+    for (int t = first + wave; t <= row; t += 4) {
+        float x = 0.0f, v[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            x = __builtin_fmaf(q[i], (float)K[(size_t)t * a.kv_stride + i * 64 + lane], x);
+            v[i] = (float)V[(size_t)t * a.kv_stride + i * 64 + lane];
+        }
+        x = wave_sum(x);
+        const float mn = fmaxf(m, x), f = exp2f(m - mn), w = exp2f(x - mn);
+        l = l * f + w;
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] = __builtin_fmaf(w, v[i], o[i] * f);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) red[wave][i * 64 + lane] = o[i];
+    if (lane == 0) {
+        red[wave][HD] = m;
+        red[wave][HD + 1] = l;
+    }
+    lds_sync();
+    float top = red[0][HD], f[4], den = 0.0f;
+#pragma unroll
+    for (int w = 1; w < 4; w++) top = fmaxf(top, red[w][HD]);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        f[w] = exp2f(red[w][HD] - top);
+        den += f[w] * red[w][HD + 1];
+    }
+    E* out = (E*)a.out + (size_t)row * a.out_stride + (size_t)h * HD;
+    for (int d = threadIdx.x; d < HD; d += 256) {
+        float num = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) num += f[w] * red[w][d];
+        out[d] = (E)(num / den);
+    }
+}
+
 // ---- second launch ------------------------------------------------------------------
 // A wave's job is 32 rows of one q head; a workgroup takes NJ consecutive jobs
 // of a kv head (the heads of 32 rows, then the next 32 rows), which share its
@@ -245,9 +309,66 @@ struct Plan {
     static __device__ __forceinline__ int meta_at(int st, int kp) { return META + ((st & 1) * KSP + kp) * 1024; }
 };
 
+// the order of a run of products and the LDS reads of their operands: AHEAD
+// operands are on their way before the first product, then each step's NM
+// products are followed by the NR reads of a later step.  (Reads take longer
+// than a product; left to itself the compiler issues two at a time.)
+template <int STEPS, int AHEAD, int NM, int NR>
+__device__ __forceinline__ void order_products() {
+    constexpr int A = AHEAD < STEPS ? AHEAD : STEPS;
+    __builtin_amdgcn_sched_group_barrier(0x100, A * NR, 0);   // LDS reads
+#pragma unroll
+    for (int i = 0; i < STEPS - A; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, NM, 0);     // products
+        __builtin_amdgcn_sched_group_barrier(0x100, NR, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, A * NM, 0);
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// The u-th of all workgroups of a kv head, those with the most keys first: a
+// sequence's c-th workgroup has the more keys the larger c is (up to the
+// window), whatever sequence it is, so they go by c, downwards, and by
+// sequence.  Up to 64 sequences, one a lane.  (In the order of the sequences a
+// launch of one and a half rounds takes two: prompts of 100 to 2048 rows with
+// a window of 512, fp32, 8 heads of 256: 120 -> 80 us.)
+__device__ __forceinline__ bool longest_first(const PackedArgs& a, int nj, unsigned u, int& s, unsigned& c) {
+    const int lane = threadIdx.x & 63;
+    unsigned units = 0;
+    if (lane < a.n_seqs) {
+        const int r0 = a.cu[lane], r1 = a.cu[lane + 1];
+        if (r0 >= 0 && r1 > r0 && r1 <= a.m) units = (unsigned)(((long)((r1 - r0 + 31) >> 5) * a.group + nj - 1) / nj);
+    }
+    // workgroups of all sequences from their c-th on
+    auto from = [&](unsigned c) {
+        unsigned x = units > c ? units - c : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
+        return (unsigned)__builtin_amdgcn_readfirstlane(x);
+    };
+    if (u >= from(0)) return false;
+    unsigned most = units;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const unsigned x = __shfl_xor(most, d, 64);
+        most = x > most ? x : most;
+    }
+    // the largest c with more than u from it on
+    unsigned lo = 0, hi = __builtin_amdgcn_readfirstlane(most);
+    while (hi - lo > 1) {
+        const unsigned mid = (lo + hi) >> 1;
+        if (from(mid) > u) lo = mid;
+        else hi = mid;
+    }
+    c = lo;
+    unsigned long long have = __ballot(units > c);
+    for (unsigned k = u - from(c + 1); k; k--) have &= have - 1;
+    s = __builtin_ctzll(have);
+    return true;
 }
 
 template <int T, int HD>
@@ -265,11 +386,17 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % DS, kp = wave / (NJ * DS);
 
     // ---- whose rows ----
-    const unsigned id = blockIdx.x, kvh = id % (unsigned)a.n_kv, u = (gridDim.x - 1 - id) / (unsigned)a.n_kv;
-    const int s = unit_seq(a.cu, a.n_seqs, a.group, P::LGROWS, a.extra, u);
+    const unsigned id = blockIdx.x, kvh = id % (unsigned)a.n_kv, u = id / (unsigned)a.n_kv;
+    int s;
+    unsigned c;
+    if (a.n_seqs <= 64) {
+        if (!longest_first(a, NJ, u, s, c)) return;
+    } else {
+        s = unit_seq(a.cu, a.n_seqs, a.group, P::LGROWS, a.extra, gridDim.x / a.n_kv - 1 - u);
+        c = gridDim.x / a.n_kv - 1 - u - unit_base(a.cu, s, a.group, P::LGROWS, a.extra);
+    }
     const int r0 = a.cu[s], r1 = a.cu[s + 1], n = r1 - r0;
     if (r0 < 0 || n <= 0 || r1 > a.m) return;
-    const unsigned c = u - unit_base(a.cu, s, a.group, P::LGROWS, a.extra);
     const long jobs = (long)((n + 31) >> 5) * a.group, job0 = (long)c * NJ;
     if (job0 >= jobs) return;
     const long jl = job0 + NJ < jobs ? job0 + NJ - 1 : jobs - 1;
@@ -396,6 +523,7 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
                 sx = mfma32(k1, q[0][i], sx);
             }
         }
+        order_products<KS, 3, NS == 2 ? 3 : 1, NS>();
         if constexpr (NS == 2) sc += sx;
     };
     auto weights = [&](int st, int kt) {
@@ -480,6 +608,7 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
                     o[i] = mfma32(*reinterpret_cast<const op*>(v + 64 * HD), p[0][t], o[i]);
                 }
             }
+        order_products<2 * NT, 3, NS == 2 ? 3 : 1, NS>();
     };
 
     if constexpr (DS == 1) {
@@ -619,6 +748,11 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
 template <int T, int HD>
 int launch_packed(PackedArgs a) {
     typedef Plan<T, HD> P;
+    const double keys = a.window > 0 && a.window < a.m ? a.window : a.m;
+    if ((double)a.m * keys * a.n_heads <= kFewPairs) {
+        hipLaunchKernelGGL((attn_packed_few_kernel<T, HD>), dim3(a.m, a.n_heads), dim3(256), 0, g4_stream(), a);
+        return g4_check_launch("attn_packed_few_kernel");
+    }
     static bool done = false;
     if (!done) {
         // more than 64 KB of LDS has to be asked for once

@@ -84,6 +84,32 @@ __device__ __forceinline__ int unit_seq(const int* __restrict__ cu, int n, int m
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
+// that sequence with its rows and (lens given) its length.  Up to 64 sequences
+// all of it is in the lanes after one round trip to memory.
+struct SeqAt {
+    int s, r0, r1, len;
+};
+__device__ __forceinline__ SeqAt find_seq(const int* __restrict__ cu, const int* __restrict__ lens, int n, int mul, int lg,
+                                          int extra, unsigned u) {
+    SeqAt r;
+    if (n <= 64) {
+        const int lane = threadIdx.x & 63, i = lane < n ? lane : n - 1;
+        const int c0 = cu[i], c1 = cu[i + 1], len = lens ? lens[i] : 0;
+        const unsigned base = (unsigned)(((unsigned long long)(unsigned)c0 * (unsigned)mul) >> lg) + (unsigned)extra * (unsigned)i;
+        const int c = __popcll(__ballot(lane < n && base <= u));
+        r.s = c > 0 ? c - 1 : 0;
+        r.r0 = __builtin_amdgcn_readlane(c0, r.s);
+        r.r1 = __builtin_amdgcn_readlane(c1, r.s);
+        r.len = __builtin_amdgcn_readlane(len, r.s);
+    } else {
+        r.s = unit_seq(cu, n, mul, lg, extra, u);
+        r.r0 = cu[r.s];
+        r.r1 = cu[r.s + 1];
+        r.len = lens ? lens[r.s] : 0;
+    }
+    return r;
+}
+
 // host: the arguments every entry point of the cache checks alike
 int kv_pool_check(const char* who, KvPool* o, const void* kp, const void* vp, int type, int n_pages, int page, int n_kv,
                   int hd, const int* table, int table_stride);

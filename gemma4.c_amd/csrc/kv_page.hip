@@ -42,31 +42,24 @@ struct RowArgs {
 // most (n + 30) / 16 blocks, so the shares never overlap and no prefix sum is
 // needed; units past a sequence's last block have nothing to do.
 struct Unit {
+    int s, at;         // sequence, position of the block's token 0
     int t0, t1;        // tokens of the block that take part
     int row;           // row of token 0 of the block (may lie before the first row)
-    int page;          // -1: the table's entry is not a page
-    size_t block;
-    size_t scale;      // index of token 0's scale
 };
 
 __device__ __forceinline__ bool find_unit(const RowArgs& a, Unit& u) {
     const unsigned id = blockIdx.x;
-    const int s = unit_seq(a.cu, a.n_seqs, 1, 4, 2, id);
-    const int r0 = a.cu[s], r1 = a.cu[s + 1], len = a.lens[s];
-    if (r0 < 0 || r1 <= r0 || r1 > a.m || r1 - r0 > len || !a.p.fits(len)) return false;
-    const int pos0 = len - (r1 - r0);
-    const unsigned b = id - unit_base(a.cu, s, 1, 4, 2);
-    const int first = pos0 >> 4, blocks = ((len - 1) >> 4) - first + 1;
+    const SeqAt q = find_seq(a.cu, a.lens, a.n_seqs, 1, 4, 2, id);
+    if (q.r0 < 0 || q.r1 <= q.r0 || q.r1 > a.m || q.r1 - q.r0 > q.len || !a.p.fits(q.len)) return false;
+    const int pos0 = q.len - (q.r1 - q.r0);
+    const unsigned b = id - (((unsigned)q.r0 >> 4) + 2u * (unsigned)q.s);
+    const int first = pos0 >> 4, blocks = ((q.len - 1) >> 4) - first + 1;
     if (b >= (unsigned)blocks) return false;
-    const int at = (first + (int)b) << 4;
-    u.t0 = pos0 > at ? pos0 - at : 0;
-    u.t1 = len - at < 16 ? len - at : 16;
-    u.row = r0 + (at - pos0);
-    u.page = a.p.page_of(s, at);
-    if (u.page >= 0) {
-        u.block = a.p.block_of(u.page, blockIdx.y, at);
-        u.scale = u.block * 16;
-    }
+    u.s = q.s;
+    u.at = (first + (int)b) << 4;
+    u.t0 = pos0 > u.at ? pos0 - u.at : 0;
+    u.t1 = q.len - u.at < 16 ? q.len - u.at : 16;
+    u.row = q.r0 + (u.at - pos0);
     return true;
 }
 
@@ -118,25 +111,35 @@ __global__ __launch_bounds__(256) void kv_store_kernel(RowArgs a) {
     typedef RowMap<HD> M;
     __shared__ __align__(16) uint8_t img[16 * HD * ES];
     Unit u;
-    if (!find_unit(a, u) || u.page < 0) return;
+    if (!find_unit(a, u)) return;
+    const int page = a.p.page_of(u.s, u.at);   // on its way beside the rows
     const bool is_v = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* __restrict__ src = (is_v ? a.v : a.k) + (size_t)blockIdx.y * HD;
-    uint8_t* pool = is_v ? a.p.vp : a.p.kp;
     const int sub = lane / M::LPR, col = lane % M::LPR;
+    // whether any of a pass's rows of this wave takes part
+    auto in_use = [&](int i) {
+        const int t = (i * 4 + __builtin_amdgcn_readfirstlane(wave)) * M::RPW;
+        return t + M::RPW > u.t0 && t < u.t1;
+    };
     float4 x[M::PASS][M::VPL];
 #pragma unroll
     for (int i = 0; i < M::PASS; i++) {
         const int t = (i * 4 + wave) * M::RPW + sub;
+        if (!in_use(i)) continue;
         // rows that take no part read the block's first row in their place
         const int r = u.row + (t >= u.t0 && t < u.t1 ? t : u.t0);
 #pragma unroll
         for (int k = 0; k < M::VPL; k++)
             x[i][k] = *reinterpret_cast<const float4*>(src + (size_t)r * a.kv_stride + (k * M::LPR + col) * 4);
     }
+    if (page < 0) return;
+    uint8_t* pool = is_v ? a.p.vp : a.p.kp;
+    const size_t block = a.p.block_of(page, blockIdx.y, u.at);
 #pragma unroll
     for (int i = 0; i < M::PASS; i++) {
         const int t = (i * 4 + wave) * M::RPW + sub;
+        if (!in_use(i)) continue;
         float d = 1.0f;
         if (TYPE == G4_KV_Q8) {
             // as integers, magnitudes keep their order and infinities and NaN come last
@@ -157,7 +160,7 @@ __global__ __launch_bounds__(256) void kv_store_kernel(RowArgs a) {
             }
             d = top < 0x7f800000u ? __uint_as_float(top) / 127.0f : __uint_as_float(0x7fc00000u);
             if (col == 0 && t >= u.t0 && t < u.t1)
-                reinterpret_cast<float*>(pool + a.p.scale_off)[u.scale + t] = d;
+                reinterpret_cast<float*>(pool + a.p.scale_off)[block * 16 + t] = d;
         }
 #pragma unroll
         for (int k = 0; k < M::VPL; k++) {
@@ -180,7 +183,7 @@ __global__ __launch_bounds__(256) void kv_store_kernel(RowArgs a) {
         }
     }
     lds_sync();
-    uint8_t* out = pool + u.block * (16 * HD * ES);
+    uint8_t* out = pool + block * (16 * HD * ES);
     for (int x0 = tid; x0 < HD * ES; x0 += 256) {
         if (is_v) {
             const int t = (x0 >> 4 & 3) * 4;   // the piece's first token
@@ -190,8 +193,11 @@ __global__ __launch_bounds__(256) void kv_store_kernel(RowArgs a) {
                 const T* from = reinterpret_cast<const T*>(img + x0 * 16);
                 T* to = reinterpret_cast<T*>(out + x0 * 16);
 #pragma unroll
-                for (int j = 0; j < 16 / ES; j++)
-                    if (t + j % 4 >= u.t0 && t + j % 4 < u.t1) to[j] = from[j];
+                for (int k = 0; k < 4; k++)
+                    if (t + k >= u.t0 && t + k < u.t1) {
+#pragma unroll
+                        for (int j = 0; j < 4 / ES; j++) to[4 * j + k] = from[4 * j + k];
+                    }
             }
         } else {
             const int t = x0 & 15;
@@ -213,18 +219,18 @@ __global__ __launch_bounds__(256) void kv_load_kernel(RowArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     float* __restrict__ dst = (is_v ? a.v : a.k) + (size_t)blockIdx.y * HD;
     const uint8_t* pool = is_v ? a.p.vp : a.p.kp;
-    if (u.page >= 0) {
-        const uint8_t* in = pool + u.block * (16 * HD * ES);
-        for (int x0 = tid; x0 < HD * ES; x0 += 256)
-            reinterpret_cast<uint4*>(img)[x0] = reinterpret_cast<const uint4*>(in)[x0];
-    }
+    const int page = a.p.page_of(u.s, u.at);
+    const size_t block = a.p.block_of(page < 0 ? 0 : page, blockIdx.y, u.at);
+    const uint8_t* in = pool + block * (16 * HD * ES);
+    for (int x0 = tid; x0 < HD * ES; x0 += 256)
+        reinterpret_cast<uint4*>(img)[x0] = reinterpret_cast<const uint4*>(in)[x0];
     const int sub = lane / M::LPR, col = lane % M::LPR;
     float d[M::PASS];
 #pragma unroll
     for (int i = 0; i < M::PASS; i++) {
         const int t = (i * 4 + wave) * M::RPW + sub;
-        d[i] = u.page < 0 ? __uint_as_float(0x7fc00000u)   // rows of a page that is none: NaN
-               : TYPE == G4_KV_Q8 ? reinterpret_cast<const float*>(pool + a.p.scale_off)[u.scale + t] : 1.0f;
+        d[i] = TYPE == G4_KV_Q8 ? reinterpret_cast<const float*>(pool + a.p.scale_off)[block * 16 + t] : 1.0f;
+        if (page < 0) d[i] = __uint_as_float(0x7fc00000u);   // rows of a page that is none: NaN
     }
     lds_sync();
 #pragma unroll
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(256) void kv_load_kernel(RowArgs a) {
                 const T q = *reinterpret_cast<const T*>(img + (is_v ? kv_v_byte<ES>(t, c + j) : kv_k_byte<ES>(t, c + j)));
                 e[j] = Elem<TYPE>::back(q);
                 if (TYPE == G4_KV_Q8) e[j] *= d[i];
-                if (u.page < 0) e[j] = d[i];
+                if (page < 0) e[j] = d[i];
             }
             *reinterpret_cast<float4*>(dst + (size_t)(u.row + t) * a.kv_stride + c) = make_float4(e[0], e[1], e[2], e[3]);
         }
