@@ -753,11 +753,13 @@ int launch_packed(PackedArgs a) {
         hipLaunchKernelGGL((attn_packed_few_kernel<T, HD>), dim3(a.m, a.n_heads), dim3(256), 0, g4_stream(), a);
         return g4_check_launch("attn_packed_few_kernel");
     }
-    static bool done = false;
-    if (!done) {
-        // more than 64 KB of LDS has to be asked for once
+    // more than 64 KB of LDS has to be asked for, once on each device
+    static unsigned long long asked = 0;
+    int dev = 0;
+    G4_HIP(hipGetDevice(&dev));
+    if (dev >= 64 || !(asked >> dev & 1)) {
         G4_HIP(hipFuncSetAttribute((const void*)attn_packed_kernel<T, HD>, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS));
-        done = true;
+        if (dev < 64) asked |= 1ull << dev;
     }
     hipLaunchKernelGGL((packed_layout_kernel<T, HD>), dim3(a.m / 32 + a.n_seqs, a.n_kv, 2), dim3(256), 0, g4_stream(), a);
     // a sequence of n rows has ceil(ceil(n / 32) group / NJ) units, at most

@@ -128,9 +128,10 @@ __device__ __forceinline__ int unit_wg(unsigned long long u, unsigned long long 
     return (int)w;
 }
 
-// floats of a partial result: [head][hd] sums, then each head's maximum and weight sum
+// floats of a partial result: [head][hd] sums, then each head's maximum and
+// weight sum (16-byte aligned)
 __host__ __device__ inline size_t part_floats(int group, int hd) {
-    return (size_t)(group < kHeadsWG ? group : kHeadsWG) * (hd + 2);
+    return ((size_t)(group < kHeadsWG ? group : kHeadsWG) * (hd + 2) + 3) & ~(size_t)3;
 }
 
 // ---- operands ------------------------------------------------------------------
@@ -570,6 +571,15 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
     const int np = few ? tiles : w1 - w0 + 1, gh = a.group < kHeadsWG ? a.group : kHeadsWG;
     const size_t pf = part_floats(a.group, HD);
     auto slot = [&](int i) { return a.part + ((size_t)(few ? unit_wg(u0 + i, n) : w0 + i) * 2 + (i == 0)) * pf; };
+    // the first pieces' sums are on their way while the factors are found
+    const int c = tid % LPR, gr = tid / LPR;
+    auto sums = [&](int i, float4 (&y)[8]) {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            y[k] = reinterpret_cast<const float4*>(slot(i + k * GR < np ? i + k * GR : 0) + col * HD + blockIdx.z * D)[c];
+    };
+    float4 y[8];
+    sums(gr, y);
     // maxima, factors, weight sums: pieces tid and tid + 256
     float m[2], l[2], top = -INFINITY;
 #pragma unroll
@@ -600,24 +610,17 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
     if ((tid & 63) == 0) wred[tid >> 6] = sum;
     lds_sync();
     sum = (wred[0] + wred[1]) + (wred[2] + wred[3]);
-    const int c = tid % LPR, gr = tid / LPR;
     float4 x = make_float4(0, 0, 0, 0);
     for (int i = gr; i < np; i += 8 * GR) {
-        float4 y[8];
-        float f[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int j = i + k * GR < np ? i + k * GR : gr;
-            y[k] = reinterpret_cast<const float4*>(slot(j) + col * HD + blockIdx.z * D)[c];
-            f[k] = i + k * GR < np ? fac[j] : 0.0f;
-        }
+        if (i > gr) sums(i, y);
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             if (i + k * GR >= np) continue;
-            x.x = fmaf(f[k], y[k].x, x.x);
-            x.y = fmaf(f[k], y[k].y, x.y);
-            x.z = fmaf(f[k], y[k].z, x.z);
-            x.w = fmaf(f[k], y[k].w, x.w);
+            const float f = fac[i + k * GR];
+            x.x = __builtin_fmaf(f, y[k].x, x.x);
+            x.y = __builtin_fmaf(f, y[k].y, x.y);
+            x.z = __builtin_fmaf(f, y[k].z, x.z);
+            x.w = __builtin_fmaf(f, y[k].w, x.w);
         }
     }
     acc[tid] = x;

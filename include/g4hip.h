@@ -445,7 +445,7 @@ int g4_kv_page_load(const void *kp, const void *vp, int type, int n_pages, int p
  * the cache holds are exact, their sums fp32.  lens[s] = 0 gives zeros; a page
  * outside the pool or a length past the table gives NaN in that sequence's row.
  * Where what a head sees holds infinities or NaN, its output is what the
- * formula gives or NaN.  part: g4_attn_decode_paged_part_bytes() bytes that no
+ * formula gives or NaN.  out may not overlap q.  part: g4_attn_decode_paged_part_bytes() bytes that no
  * call running at the same time uses (its contents need not be kept).  q, out,
  * part 16-byte aligned, strides multiples of 4. */
 size_t g4_attn_decode_paged_part_bytes(int n_heads, int n_kv, int hd);
@@ -455,8 +455,13 @@ int g4_attn_decode_paged(const float *q, int q_stride, const void *kp, const voi
 /* The attention block (main.c:1909-1950) of every row of whole prompts: row i
  * of a sequence sees that sequence's rows max(0, i + 1 - window) .. i (window
  * 0: 0 .. i).  q, k, v, out rows of one type, G4_F32, G4_F16 or G4_BF16, their
- * strides in elements (16-byte aligned rows).  Rows of out past cu[n_seqs] and
- * those of sequences whose cu does not fit are left as they are.  work:
+ * strides in elements (16-byte aligned rows).  F32: products of operands met
+ * within 2^-22 of themselves or 2^-39 of their row's largest, fp32 sums; F16,
+ * BF16: exact products, weights rounded to the type, fp32 sums (few rows: fp32
+ * throughout).  Rows of out past cu[n_seqs] and those of sequences whose cu
+ * does not fit are left as they are.  Where what a row's head sees holds
+ * infinities or NaN, its output is what the formula gives or NaN; what it does
+ * not see never matters.  work:
  * g4_attn_prompt_packed_work_bytes() bytes that no call running at the same
  * time uses (its contents need not be kept); out may not overlap the inputs. */
 size_t g4_attn_prompt_packed_work_bytes(int type, int n_seqs, int m, int n_kv, int hd);

@@ -527,3 +527,190 @@ def test_serving(lib):
             want, bound = pn.attention(qs[t:].reshape(steps, n_heads, hd), hk.reshape(-1, n_kv, hd),
                                        hv.reshape(-1, n_kv, hd), first[t:], scale)
             assert (np.abs(o[t:] - want) <= bound).all()
+
+
+def same_bits(a, b):
+    return np.array_equal(a.view(np.uint8), b.view(np.uint8))
+
+
+class Stream:
+    """work on a created library stream"""
+
+    def __init__(self, lib):
+        self.lib = lib
+
+    def __enter__(self):
+        p = C.c_void_p()
+        self.lib.g4_stream_create(C.byref(p))
+        self.p = p.value
+        self.lib.g4_set_stream(self.p)
+        return self
+
+    def __exit__(self, *exc):
+        self.lib.g4_sync()
+        self.lib.g4_set_stream(None)
+        self.lib.g4_stream_destroy(self.p)
+
+
+@pytest.mark.parametrize("kind", [pn.BF16, pn.Q8])
+def test_graph_of_steps(lib, kind):
+    """A step (store, decode attention) captured once and replayed while the lengths grow: every replay equals the
+    eager calls bit for bit, the program's own work running in between."""
+    rng = np.random.default_rng(300)
+    hd, n_heads, n_kv, page, steps = 128, 8, 2, 16, 6
+    n = [0, 33, 500, 14]
+    total = [t + steps for t in n]
+    table, pages = pn.page_table(rng, total, page)
+    hist = rows(rng, sum(n), n_kv, hd)
+    step = [(rows(rng, 4, n_heads, hd), rows(rng, 4, n_kv, hd), rows(rng, 4, n_kv, hd)) for _ in range(steps)]
+    results = []
+    for captured in (False, True):
+        with Stream(lib):
+            c = Cache(lib, rng, kind, hd, n_kv, page, None, table=table, pages=pages)
+            c.store(hist, hist[::-1].copy(), n, n)
+            dq, dk, dv = (filled(lib, a.nbytes) for a in step[0])
+            lens, cu = filled(lib, 16), dbuf(lib, pn.starts([1] * 4))
+            out = filled(lib, 4 * n_heads * hd * 4)
+            part = filled(lib, lib.L.g4_attn_decode_paged_part_bytes(n_heads, n_kv, hd))
+
+            def run():
+                lib.g4_kv_page_store(*c.args(), dk.ptr, dv.ptr, n_kv * hd, cu.ptr, lens.ptr, 4, 4)
+                lib.g4_attn_decode_paged(dq.ptr, n_heads * hd, *c.args(), lens.ptr, 4, 200, n_heads, F(0.1), part.ptr,
+                                         out.ptr, n_heads * hd)
+
+            graph = None
+            if captured:
+                lens.write(np.array(total, np.int32))
+                lib.g4_graph_begin()
+                run()
+                g = C.c_void_p()
+                lib.g4_graph_end(C.byref(g))
+                graph = g.value
+            got = []
+            for i, (q, k, v) in enumerate(step):
+                dq.write(q)
+                dk.write(k)
+                dv.write(v)
+                lens.write(np.array([t + i + 1 for t in n], np.int32))
+                if graph:
+                    lib.g4_graph_launch(graph)
+                else:
+                    run()
+                lib.g4_sync()
+                got.append(out.to_array(np.float32))
+                c.load([t + i + 1 for t in n], [t + i + 1 for t in n])
+            results.append(np.stack(got))
+            if graph:
+                lib.g4_graph_destroy(graph)
+    assert np.isfinite(results[0]).all() and same_bits(*results)
+
+
+@pytest.mark.parametrize("kind,hd", [(pn.F32, 256), (pn.BF16, 256), (pn.F32, 512), (pn.F16, 512), (pn.BF16, 64)])
+def test_graph_of_prompts(lib, kind, hd):
+    """A prompt batch captured once and replayed with other prompts and other lengths: each replay equals the eager call"""
+    rng = np.random.default_rng(301)
+    n_heads, n_kv, m, scale = 8, 2, 420, 0.07
+    es = 4 if kind == pn.F32 else 2
+    batches = [[200, 219, 1], [420, 0, 0], [33, 300, 60], [0, 5, 0]]
+    data = [tuple(cast(rows(rng, m, h, hd), kind)[0] for h in (n_heads, n_kv, n_kv)) for _ in batches]
+    with Stream(lib):
+        dq, dk, dv = (filled(lib, a.nbytes) for a in data[0])
+        cu, out = filled(lib, 16), filled(lib, m * n_heads * hd * es)
+        work = filled(lib, lib.L.g4_attn_prompt_packed_work_bytes(kind, 3, m, n_kv, hd))
+
+        def run():
+            lib.g4_attn_prompt_packed(dq.ptr, n_heads * hd, dk.ptr, dv.ptr, n_kv * hd, out.ptr, n_heads * hd, kind, cu.ptr, 3,
+                                      m, 100, n_heads, n_kv, hd, F(scale), work.ptr)
+
+        def batch(i, call):
+            for d, a in zip((dq, dk, dv), data[i]):
+                d.write(a)
+            cu.write(pn.starts(batches[i]))
+            lib.g4_memset(out.ptr, 0x3F, out.nbytes)
+            call()
+            lib.g4_sync()
+            return out.to_array(np.uint8)
+
+        want = [batch(i, run) for i in range(len(batches))]
+        cu.write(pn.starts(batches[0]))
+        lib.g4_graph_begin()
+        run()
+        g = C.c_void_p()
+        lib.g4_graph_end(C.byref(g))
+        for i in (2, 0, 1, 3, 2):
+            assert same_bits(batch(i, lambda: lib.g4_graph_launch(g.value)), want[i]), i
+        lib.g4_graph_destroy(g.value)
+
+
+def test_calls_one_after_the_other(lib):
+    """Calls of other sizes that share part and work, none of which waits: each result is its own"""
+    rng = np.random.default_rng(302)
+    hd, n_kv, n_heads, page = 128, 2, 8, 32
+    part = filled(lib, lib.L.g4_attn_decode_paged_part_bytes(n_heads, n_kv, hd))
+    cases = []
+    for lens in ([4000, 3], [70], [0, 0, 900], [1]):
+        c = Cache(lib, rng, pn.F16, hd, n_kv, page, lens)
+        x = rows(rng, sum(lens), n_kv, hd)
+        c.store(x, x, lens, lens)
+        q = rows(rng, len(lens), n_heads, hd)
+        cases.append((c, dbuf(lib, q), dbuf(lib, np.array(lens, np.int32)), filled(lib, q.nbytes),
+                      run_decode(lib, c, q, lens, n_heads, 0, 0.1)))
+    for _ in range(3):
+        for c, dq, dl, out, _want in cases:
+            lib.g4_attn_decode_paged(dq.ptr, n_heads * hd, *c.args(), dl.ptr, dl.nbytes // 4, 0, n_heads, F(0.1), part.ptr,
+                                     out.ptr, n_heads * hd)
+    lib.g4_sync()
+    for c, dq, dl, out, want in cases:
+        assert same_bits(out.to_array(np.float32).reshape(want.shape), want)
+
+
+def test_offsets_past_32_bits(lib):
+    """pages at the end of pools of 5 GB and more"""
+    rng = np.random.default_rng(303)
+    for kind, hd, n_kv, page, pages in ((pn.F32, 512, 2, 64, 20000), (pn.Q8, 512, 2, 256, 21000)):
+        lens = [150, 61]
+        need = [-(-t // page) for t in lens]
+        table = np.full((2, max(need)), -1, np.int32)
+        at = pages
+        for s, c in enumerate(need):
+            for i in range(c):
+                at -= 1
+                table[s, i] = at
+        c = Cache(lib, rng, kind, hd, n_kv, page, None, table=table, pages=pages)
+        assert c.k.nbytes > 1 << 32
+        k, v = rows(rng, sum(lens), n_kv, hd), rows(rng, sum(lens), n_kv, hd)
+        c.store(k, v, lens, lens)
+        gk, gv = c.load(lens, lens)
+        hk, hv = pn.held(k, kind, hd), pn.held(v, kind, hd)
+        assert same(gk, hk) and same(gv, hv)
+        q = rows(rng, 2, 4, hd)
+        got = run_decode(lib, c, q, lens, 4, 0, 0.04).reshape(2, 4, hd)
+        cu = pn.starts(lens)
+        for s, t in enumerate(lens):
+            r = slice(cu[s], cu[s + 1])
+            want, bound = pn.attention(q[s].reshape(1, 4, hd), hk[r].reshape(t, n_kv, hd), hv[r].reshape(t, n_kv, hd), [0],
+                                       0.04)
+            within(np.abs(got[s] - want[0]), bound[0], s)
+
+
+def test_shared_pages(lib):
+    """two sequences with the same first pages (a common prefix) and tails of their own"""
+    rng = np.random.default_rng(304)
+    hd, n_kv, page = 64, 1, 16
+    table = np.array([[0, 1, 2, 3], [0, 1, 4, 5]], np.int32)
+    c = Cache(lib, rng, pn.BF16, hd, n_kv, page, None, table=table, pages=6)
+    a, b = rows(rng, 50, n_kv, hd), rows(rng, 60, n_kv, hd)
+    b[:32] = a[:32]
+    c.store(a, a, [50], [50])                       # sequence 0 with the prefix
+    second = Cache.__new__(Cache)
+    second.__dict__.update(c.__dict__)
+    second.table, second.dtable = table[1:], dbuf(lib, table[1:])
+    second.store(b[32:], b[32:], [28], [60])        # the other's tail
+    gk, gv = c.load([50, 60], [50, 60])
+    assert same(gk, pn.held(np.concatenate([a, b]), pn.BF16, hd)) and same(gv, gk)
+
+
+def test_prompt_lengths(lib):
+    """sequences of 1 to 136 rows one after the other, a window that ends inside tiles, three heads on a kv head"""
+    for kind in (pn.F32, pn.BF16):
+        check_prompt(lib, 305, kind, 64, 6, 2, list(range(1, 141, 9)), window=33)
