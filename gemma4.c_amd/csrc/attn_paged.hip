@@ -23,6 +23,7 @@ struct PagedArgs {
     int q_stride, out_stride, n_seqs, window, n_heads;
     int group, ngrp;   // q heads a kv head, workgroup columns' groups of them
     int lead;          // units in front of an item's tiles
+    int whole;         // a workgroup an item, nothing to join
     float scale;
 };
 
@@ -230,17 +231,39 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned w = blockIdx.x;
-    const Line ln = find_line(a, [&](unsigned long long n) { return (n * w) >> kLgWG; }, -1, red);
-    unsigned long long cur = (ln.total * w) >> kLgWG;
-    const unsigned long long end = (ln.total * (w + 1)) >> kLgWG;
-    if (cur >= end) return;
     const int rep = a.p.n_kv * a.ngrp;
-    int s = __builtin_amdgcn_readfirstlane(ln.s);
-    int first_tile, len = __builtin_amdgcn_readfirstlane(ln.len);
-    int tiles = seq_tiles(a, len, first_tile);
-    const unsigned long long off = cur - ln.before * rep;   // unit within the sequence's items
-    int item = __builtin_amdgcn_readfirstlane((int)(off / (unsigned)(tiles + a.lead)));
-    int unit = __builtin_amdgcn_readfirstlane((int)(off - (unsigned long long)item * (tiles + a.lead)));
+    unsigned long long cur, end;
+    int s, len, item, unit;
+    if (a.whole) {
+        s = (int)(w / (unsigned)rep);
+        item = (int)w - s * rep;
+        len = __builtin_amdgcn_readfirstlane(a.lens[s]);
+        unit = 0;
+        cur = 0;
+        end = ~0ull;
+    } else {
+        const Line ln = find_line(a, [&](unsigned long long n) { return (n * w) >> kLgWG; }, -1, red);
+        cur = (ln.total * w) >> kLgWG;
+        end = (ln.total * (w + 1)) >> kLgWG;
+        if (cur >= end) return;
+        s = __builtin_amdgcn_readfirstlane(ln.s);
+        len = __builtin_amdgcn_readfirstlane(ln.len);
+        int f;
+        const unsigned per = (unsigned)(seq_tiles(a, len, f) + a.lead);
+        const unsigned long long off = cur - ln.before * rep;   // unit within the sequence's items
+        item = __builtin_amdgcn_readfirstlane((int)(off / per));
+        unit = __builtin_amdgcn_readfirstlane((int)(off - (unsigned long long)item * per));
+    }
+    int first_tile, tiles = seq_tiles(a, len, first_tile);
+    if (a.whole && tiles == 0) {
+        // no keys: zeros; a length that does not fit: NaN
+        const float x = len == 0 ? 0.0f : __uint_as_float(0x7fc00000u);
+        const int kvh = item / a.ngrp, hg = item - kvh * a.ngrp;
+        const int nh = a.group - hg * kHeadsWG < kHeadsWG ? a.group - hg * kHeadsWG : kHeadsWG;
+        float* to = a.out + (size_t)s * a.out_stride + (size_t)(kvh * a.group + hg * kHeadsWG) * HD;
+        for (int i = tid; i < nh * HD / 4; i += 256) reinterpret_cast<float4*>(to)[i] = make_float4(x, x, x, x);
+        return;
+    }
     while (true) {
         const unsigned long long left = end - cur;
         const int unit1 = left < (unsigned long long)(tiles + a.lead - unit) ? unit + (int)left : tiles + a.lead;
@@ -526,7 +549,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
             lds_sync();   // the sums' place takes q again
         }
         cur += (unsigned)(unit1 - unit);
-        if (cur >= end) break;
+        if (a.whole || cur >= end) break;
         unit = 0;
         if (++item == rep) {
             item = 0;
@@ -642,6 +665,10 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
 template <int TYPE, int HD>
 void launch_paged(const PagedArgs& a) {
     constexpr int NL = HD * CacheType<TYPE>::ES / 16, R = 4, D = NL < R ? NL : R;
+    if (a.whole) {
+        hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D>), dim3(a.n_seqs * a.p.n_kv * a.ngrp), dim3(256), 0, g4_stream(), a);
+        return;
+    }
     hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D>), dim3(kPagedWG), dim3(256), 0, g4_stream(), a);
     if (a.n_heads * a.n_seqs < 256)
         hipLaunchKernelGGL((attn_paged_join_kernel<HD, 64>), dim3(a.n_heads, a.n_seqs, HD / 64), dim3(256), 0, g4_stream(), a);
@@ -685,6 +712,16 @@ extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp
     a.group = n_heads / n_kv;
     a.ngrp = (a.group + kHeadsWG - 1) / kHeadsWG;
     a.lead = n_seqs * n_kv * a.ngrp > 64 ? 3 : 0;
+    // Where a sequence cannot have more than 256 keys to look at (fp32: 128), by
+    // its table or the window, a workgroup takes an item whole and there is
+    // nothing to join: two rounds of the four waves cost less than the second
+    // launch.  bf16, head_dim 256, 2 kv heads, 1 / 64 / 200 sequences of 200
+    // keys: 8.4 / 11.2 / 17.6 us whole, 11.9 / 15.9 / 29.0 split; one of 500:
+    // 12.1 and 12.0; fp32 of 512, one of 64 keys 18.3 and 21.6, of 200 28.1
+    // and 22.0.
+    long most = (long)table_stride * page;
+    if (window > 0 && window < most) most = window;
+    a.whole = most <= (type == G4_F32 ? 128 : 256);
     if (type == G4_F32) launch_paged<G4_F32>(a, hd);
     else if (type == G4_F16) launch_paged<G4_F16>(a, hd);
     else if (type == G4_BF16) launch_paged<G4_BF16>(a, hd);
