@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedArgs a) {
 template <int T, int HD>
 struct Plan {
     static constexpr int ES = Kind<T>::ES;
-    static constexpr int DS = HD == 512 ? 2 : 1;
+    static constexpr int DS = HD == 512 ? 2 : 1;                     // fp32 at 512: attn_packed_wide_kernel
     static constexpr int NW = T == G4_F32 ? 4 : 8;                   // waves; 8: two a SIMD
     static constexpr int KSP = NW == 8 && DS == 1 ? 2 : 1;           // tiles at a time
     static constexpr int NJ = NW / DS / KSP, LGROWS = NJ == 4 ? 7 : 6;   // 32 NJ = 2^LGROWS rows
@@ -371,6 +371,36 @@ __device__ __forceinline__ bool longest_first(const PackedArgs& a, int nj, unsig
     return true;
 }
 
+// a workgroup's sequence and jobs
+struct Share {
+    int r0, n;                  // the sequence's first row, its rows
+    unsigned kvh, block0;       // its first block of K and V
+    long job0, jobs, jl;        // the first job, the sequence's, the last of the workgroup
+};
+__device__ __forceinline__ bool find_share(const PackedArgs& a, int nj, int lg, Share& o) {
+    const unsigned id = blockIdx.x, u = id / (unsigned)a.n_kv;
+    o.kvh = id % (unsigned)a.n_kv;
+    int s;
+    unsigned c;
+    if (a.n_seqs <= 64) {
+        if (!longest_first(a, nj, u, s, c)) return false;
+    } else {
+        const unsigned back = gridDim.x / a.n_kv - 1 - u;   // a sequence's longest first
+        s = unit_seq(a.cu, a.n_seqs, a.group, lg, a.extra, back);
+        c = back - unit_base(a.cu, s, a.group, lg, a.extra);
+    }
+    const int r1 = a.cu[s + 1];
+    o.r0 = a.cu[s];
+    o.n = r1 - o.r0;
+    if (o.r0 < 0 || r1 <= o.r0 || r1 > a.m) return false;
+    o.block0 = unit_base(a.cu, s, 1, 5, 1);
+    o.jobs = (long)((o.n + 31) >> 5) * a.group;
+    o.job0 = (long)c * nj;
+    if (o.job0 >= o.jobs) return false;
+    o.jl = o.job0 + nj < o.jobs ? o.job0 + nj - 1 : o.jobs - 1;
+    return true;
+}
+
 template <int T, int HD>
 __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void attn_packed_kernel(PackedArgs a) {
     typedef Plan<T, HD> P;
@@ -385,21 +415,11 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % DS, kp = wave / (NJ * DS);
 
-    // ---- whose rows ----
-    const unsigned id = blockIdx.x, kvh = id % (unsigned)a.n_kv, u = id / (unsigned)a.n_kv;
-    int s;
-    unsigned c;
-    if (a.n_seqs <= 64) {
-        if (!longest_first(a, NJ, u, s, c)) return;
-    } else {
-        s = unit_seq(a.cu, a.n_seqs, a.group, P::LGROWS, a.extra, gridDim.x / a.n_kv - 1 - u);
-        c = gridDim.x / a.n_kv - 1 - u - unit_base(a.cu, s, a.group, P::LGROWS, a.extra);
-    }
-    const int r0 = a.cu[s], r1 = a.cu[s + 1], n = r1 - r0;
-    if (r0 < 0 || n <= 0 || r1 > a.m) return;
-    const long jobs = (long)((n + 31) >> 5) * a.group, job0 = (long)c * NJ;
-    if (job0 >= jobs) return;
-    const long jl = job0 + NJ < jobs ? job0 + NJ - 1 : jobs - 1;
+    Share sh;
+    if (!find_share(a, NJ, P::LGROWS, sh)) return;
+    const int r0 = sh.r0, n = sh.n;
+    const long job0 = sh.job0, jobs = sh.jobs, jl = sh.jl;
+    const unsigned kvh = sh.kvh;
     const int slot = wave / DS % NJ;
     const bool mine = job0 + slot < jobs;
     const long job = mine ? job0 + slot : jl;
@@ -416,7 +436,7 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
 
     // ---- tiles on their way into LDS: stage st has the tiles kt0 + KSP st + (0 .. KSP - 1) ----
     const int stages = (kt1 - kt0) / KSP + 1;
-    const uint8_t* rec0 = a.work + ((size_t)(unit_base(a.cu, s, 1, 5, 1) + kt0) * a.n_kv + kvh) * block_bytes(HD, ES);
+    const uint8_t* rec0 = a.work + ((size_t)(sh.block0 + kt0) * a.n_kv + kvh) * block_bytes(HD, ES);
     const size_t rec_step = (size_t)a.n_kv * block_bytes(HD, ES);
     constexpr int kShare = kHalf * KSP / NW;              // pieces a wave copies of a stage's K, of its V
     constexpr int kWhole = kHalf / NW;                    // of one tile's (0: half the waves have a tile each)
@@ -448,23 +468,21 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     float fq = fabsf(a.scale) * kLog2e;
     const E* qr = (const E*)a.q + (size_t)(r0 + (row < n ? row : n - 1)) * a.q_stride + (size_t)head * HD;
     if constexpr (T == G4_F32) {
-        float4 x[DS][KS][2];
+        float4 x[KS][2];
         unsigned top = 0;
 #pragma unroll
-        for (int p = 0; p < DS; p++)
+        for (int i = 0; i < KS; i++)
 #pragma unroll
-            for (int i = 0; i < KS; i++)
+            for (int j = 0; j < 2; j++) {
+                const float4 y = reinterpret_cast<const float4*>(qr + i * 16 + h * 8)[j];
+                x[i][j] = y;
+                const float e[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float4 y = reinterpret_cast<const float4*>(qr + (p == 0 ? part : 1 - part) * (HD / DS) + i * 16 + h * 8)[j];
-                    x[p][i][j] = y;
-                    const float e[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const unsigned m = __float_as_uint(e[k]) & 0x7fffffffu;
-                        top = m > top ? m : top;
-                    }
+                for (int k = 0; k < 4; k++) {
+                    const unsigned m = __float_as_uint(e[k]) & 0x7fffffffu;
+                    top = m > top ? m : top;
                 }
+            }
         const unsigned o = __shfl_xor(top, 32, 64);
         top = o > top ? o : top;
         const int e = (int)(top >> 23) > kLowK ? (int)(top >> 23) : kLowK;
@@ -474,10 +492,10 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             h2v_t hi[4], lo[4];
-            split2(x[0][i][0].x, x[0][i][0].y, sf, hi[0], lo[0]);
-            split2(x[0][i][0].z, x[0][i][0].w, sf, hi[1], lo[1]);
-            split2(x[0][i][1].x, x[0][i][1].y, sf, hi[2], lo[2]);
-            split2(x[0][i][1].z, x[0][i][1].w, sf, hi[3], lo[3]);
+            split2(x[i][0].x, x[i][0].y, sf, hi[0], lo[0]);
+            split2(x[i][0].z, x[i][0].w, sf, hi[1], lo[1]);
+            split2(x[i][1].x, x[i][1].y, sf, hi[2], lo[2]);
+            split2(x[i][1].z, x[i][1].w, sf, hi[3], lo[3]);
             __builtin_memcpy(&q[0][i], hi, 16);
             __builtin_memcpy(&q[1][i], lo, 16);
         }
@@ -745,6 +763,258 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
         }
 }
 
+// ---- fp32 at head_dim 512 ------------------------------------------------------------
+// q and o of a job's 512 dims take two waves' registers.  Each wave computes
+// the scores of 16 of a tile's 32 keys over all dims (q whole: the 256
+// accumulation registers) and their weights, and adds all 32 keys' values to
+// half the dims; the weights meet in LDS, with the maxima they stand for.  The
+// maxima are whole numbers, so that weights of one are brought to another's by
+// an exact power of two, which after the first tiles is 1.  Against halving
+// the dims of both products (partial scores of all keys in LDS, weights
+// computed twice, one barrier more) ...
+// K and V of a tile have one place each: the next K is on its way during the
+// second product, V during the first.
+struct Wide {
+    static constexpr int HD = 512, TB = 32 * HD * 4, NJ = 2;
+    static constexpr int META = 2 * TB, PW = META + 2048, MX = PW + NJ * 4096, LDS = MX + NJ * 2 * 32 * 8;
+};
+__global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) {
+    constexpr int HD = Wide::HD, TB = Wide::TB, NJ = Wide::NJ, KS = HD / 32, NT = HD / 64;
+    constexpr float kSlack = 4.0f, kLift = 11.0f;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5, c16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave & 1, slot = wave >> 1;
+    Share sh;
+    if (!find_share(a, NJ, 6, sh)) return;
+    const bool mine = sh.job0 + slot < sh.jobs;
+    const long job = mine ? sh.job0 + slot : sh.jl;
+    const int jt = (int)(job / a.group), head = (int)sh.kvh * a.group + (int)(job - (long)jt * a.group);
+    auto first_key = [&](int r) { return a.window > 0 && r >= a.window ? r + 1 - a.window : 0; };
+    const int kt0 = first_key((int)(sh.job0 / a.group) * 32) >> 5, kt1 = (int)(sh.jl / a.group);
+    const int my0 = (first_key(jt * 32) >> 5) - kt0, my1 = jt - kt0;
+    const int s0 = mine && my0 > 0 ? my0 : 0, s1 = mine && my1 >= 0 ? my1 + 1 : s0;
+    const int full0 = (first_key(jt * 32 + 31) + 31) >> 5, full1 = jt - 1;
+    const int stages = kt1 - kt0 + 1;
+    const uint8_t* rec0 = a.work + ((size_t)(sh.block0 + kt0) * a.n_kv + sh.kvh) * block_bytes(HD, 4);
+    const size_t rec_step = (size_t)a.n_kv * block_bytes(HD, 4);
+    auto stage = [&](int st, bool v) {
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc((void*)(rec0 + st * rec_step), 0, (int)block_bytes(HD, 4), kBufWord3);
+        uint8_t* at = lds + (v ? TB : 0) + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < TB / 4096; i++) buf_load_lds16(r, at + i * 4096, wave * 1024 + lane * 16, (v ? TB : 0) + i * 4096);
+        if (!v && wave == 0) buf_load_lds16(r, lds + Wide::META + (st & 1) * 1024, lane * 16, 2 * TB);
+    };
+    stage(0, false);
+
+    // ---- q: rows c16 and 16 + c16, steps of 32 dims, 8 of them a lane ----
+    h8_t q[2][2][KS];
+    float fq[2];
+    int row2[2], wf2[2];
+#pragma unroll
+    for (int ct = 0; ct < 2; ct++) {
+        row2[ct] = jt * 32 + 16 * ct + c16;
+        wf2[ct] = first_key(row2[ct]);
+        const float* qr = (const float*)a.q + (size_t)(sh.r0 + (row2[ct] < sh.n ? row2[ct] : sh.n - 1)) * a.q_stride + (size_t)head * HD;
+        float4 x[KS][2];
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                x[i][j] = reinterpret_cast<const float4*>(qr + i * 32 + g * 8)[j];
+                const float e[4] = {x[i][j].x, x[i][j].y, x[i][j].z, x[i][j].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const unsigned b = __float_as_uint(e[k]) & 0x7fffffffu;
+                    top = b > top ? b : top;
+                }
+            }
+#pragma unroll
+        for (int d = 16; d < 64; d <<= 1) {
+            const unsigned o = __shfl_xor(top, d, 64);
+            top = o > top ? o : top;
+        }
+        const int e = (int)(top >> 23) > kLowK ? (int)(top >> 23) : kLowK;
+        float sf = row_scale(e < 255 ? e : 254);
+        fq[ct] = fabsf(a.scale) * kLog2e * (e < 255 ? row_scale_inv(e) : __uint_as_float(0x7fc00000u));
+        if (a.scale < 0.0f) sf = -sf;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            h2v_t hi[4], lo[4];
+            split2(x[i][0].x, x[i][0].y, sf, hi[0], lo[0]);
+            split2(x[i][0].z, x[i][0].w, sf, hi[1], lo[1]);
+            split2(x[i][1].x, x[i][1].y, sf, hi[2], lo[2]);
+            split2(x[i][1].z, x[i][1].w, sf, hi[3], lo[3]);
+            __builtin_memcpy(&q[0][ct][i], hi, 16);
+            __builtin_memcpy(&q[1][ct][i], lo, 16);
+            asm("" : "+a"(q[0][ct][i]));
+            asm("" : "+a"(q[1][ct][i]));
+        }
+    }
+
+    f16_t o[NT] = {};
+    float m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {}, mo = -FLT_MAX;   // of rows row2, and of row col: what o stands for
+    // the job's weights: [step of 16 keys][hi, lo][lane] 16 bytes; maxima: [part][row]
+    uint8_t* pw = lds + Wide::PW + slot * 4096;
+    float* mx = reinterpret_cast<float*>(lds + Wide::MX) + slot * 64;
+    auto scores = [&](int st) {
+        const int kt = kt0 + st;
+        const uint8_t* at = lds + (g >> 1) * 1024 + ((g & 1) * 32 + 16 * part + c16) * 16;
+        f4_t sc[2] = {}, sx[2] = {};
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const h8_t k0 = *reinterpret_cast<const h8_t*>(at + i * 2048), k1 = *reinterpret_cast<const h8_t*>(at + 64 * HD + i * 2048);
+#pragma unroll
+            for (int ct = 0; ct < 2; ct++) sc[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[0][ct][i], sc[ct], 0, 0, 0);
+#pragma unroll
+            for (int ct = 0; ct < 2; ct++) sx[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[1][ct][i], sx[ct], 0, 0, 0);
+#pragma unroll
+            for (int ct = 0; ct < 2; ct++) sx[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[0][ct][i], sx[ct], 0, 0, 0);
+        }
+        order_products<KS, 3, 6, 2>();
+        // ---- weights of keys 16 part + 4 g .. + 3 ----
+        const float* meta = reinterpret_cast<const float*>(lds + Wide::META + (st & 1) * 1024);
+        const int key0 = 16 * part + 4 * g;
+        const unsigned* mk = reinterpret_cast<const unsigned*>(meta) + kMetaMask / 4;
+        const unsigned marks = __builtin_amdgcn_readfirstlane(mk[0] | mk[1]);
+        const float4 fk = *reinterpret_cast<const float4*>(meta + key0), ve = *reinterpret_cast<const float4*>(meta + kMetaVExp / 4 + key0),
+                     vi = *reinterpret_cast<const float4*>(meta + kMetaVInv / 4 + key0);
+        const float f[4] = {fk.x, fk.y, fk.z, fk.w}, e[4] = {ve.x, ve.y, ve.z, ve.w}, v[4] = {vi.x, vi.y, vi.z, vi.w};
+        float y[2][4], top[2];
+#pragma unroll
+        for (int ct = 0; ct < 2; ct++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[ct][r] = __builtin_fmaf(sc[ct][r] + sx[ct][r], fq[ct] * f[r], e[r]);
+            if (marks) {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (marks >> (key0 + r) & 1) y[ct][r] = __uint_as_float(0x7fc00000u);
+            }
+            if (kt < full0 || kt > full1) {
+                const int hi = row2[ct] - kt * 32 - key0, lo = wf2[ct] - kt * 32 - key0;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (r > hi || r < lo) y[ct][r] = -INFINITY;
+            }
+            top[ct] = fmaxf(fmaxf(y[ct][0], y[ct][1]), fmaxf(y[ct][2], y[ct][3]));
+        }
+        if (__any(top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
+#pragma unroll
+            for (int ct = 0; ct < 2; ct++) {
+                float t = fmaxf(top[ct], shfl_xor(top[ct], 16));
+                t = fmaxf(ceilf(fmaxf(t, shfl_xor(t, 32))), m[ct]);
+                l[ct] *= exp2f(m[ct] - t);
+                m[ct] = t;
+            }
+        }
+#pragma unroll
+        for (int ct = 0; ct < 2; ct++) {
+            const float base = m[ct] - kLift;
+            float w[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                w[r] = __builtin_amdgcn_exp2f(y[ct][r] - base);
+                l[ct] = __builtin_fmaf(w[r], v[r], l[ct]);
+            }
+            h2v_t hi[2], lo[2];
+            split2(w[0], w[1], 1.0f, hi[0], lo[0]);
+            split2(w[2], w[3], 1.0f, hi[1], lo[1]);
+            // lane 32 h + row of step `part` takes keys 4 h .. + 3 and 8 + 4 h .. + 3 of the 16
+            uint8_t* to = pw + part * 2048 + ((g & 1) * 32 + 16 * ct + c16) * 16 + (g >> 1) * 8;
+            *reinterpret_cast<uint2*>(to) = make_uint2(h2_bits(hi[0]), h2_bits(hi[1]));
+            *reinterpret_cast<uint2*>(to + 1024) = make_uint2(h2_bits(lo[0]), h2_bits(lo[1]));
+            if (g == 0) mx[part * 32 + 16 * ct + c16] = m[ct];
+        }
+    };
+    auto values = [&]() {
+        h8_t p[2][2];   // [hi, lo][step]
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) p[k][t] = *reinterpret_cast<const h8_t*>(pw + t * 2048 + k * 1024 + lane * 16);
+        const float ma = mx[col], mb = mx[32 + col], top = fmaxf(ma, mb);
+        if (__any(ma != mb || top != mo)) {
+            const float fo = exp2f(mo - top);
+            mo = top;
+            // by 2^-24 at most at a time, fp16's smallest number
+            auto scale = [&](float d, int t) {
+                const _Float16 f0 = (_Float16)exp2f(fmaxf(d, -24.0f)), f1 = (_Float16)exp2f(fminf(d + 24.0f, 0.0f));
+#pragma unroll
+                for (int k = 0; k < 2; k++) p[k][t] = p[k][t] * f0 * f1;
+            };
+            scale(ma - top, 0);
+            scale(mb - top, 1);
+#pragma unroll
+            for (int i = 0; i < NT; i++) o[i] *= fo;
+#pragma unroll
+            for (int ct = 0; ct < 2; ct++) {
+                const float t = fmaxf(mx[16 * ct + c16], mx[32 + 16 * ct + c16]);
+                l[ct] *= exp2f(m[ct] - t);
+                m[ct] = t;
+            }
+        }
+        const uint8_t* at = lds + TB + part * NT * 2048 + lane * 16;
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const uint8_t* v = at + (i * 2 + t) * 1024;
+                const h8_t v0 = *reinterpret_cast<const h8_t*>(v);
+                o[i] = mfma32(v0, p[0][t], o[i]);
+                o[i] = mfma32(v0, p[1][t], o[i]);
+                o[i] = mfma32(*reinterpret_cast<const h8_t*>(v + 64 * HD), p[0][t], o[i]);
+            }
+        order_products<2 * NT, 3, 3, 2>();
+    };
+
+    auto begin = [&](int st) {
+        wait_vm<0>();
+        lds_barrier();   // K is there, V and the weights of the tile before are done with
+        stage(st, true);
+    };
+    auto middle = [&](int st) {
+        wait_vm<0>();
+        lds_barrier();   // V and the weights are there, K is done with
+        if (st + 1 < stages) stage(st + 1, false);
+    };
+    int st = 0;
+    for (; st < s0; st++) {
+        begin(st);
+        middle(st);
+    }
+    for (; st < s1; st++) {
+        begin(st);
+        scores(st);
+        middle(st);
+        values();
+    }
+    for (; st < stages; st++) {
+        begin(st);
+        middle(st);
+    }
+
+    // ---- the two waves' weight sums ----
+    float* ls = reinterpret_cast<float*>(lds + Wide::MX) + 128 + slot * 64;
+#pragma unroll
+    for (int ct = 0; ct < 2; ct++) {
+        l[ct] += shfl_xor(l[ct], 16);
+        l[ct] += shfl_xor(l[ct], 32);
+        if (g == 0) ls[part * 32 + 16 * ct + c16] = l[ct];
+    }
+    lds_barrier();
+    const int row = jt * 32 + col;
+    if (!mine || row >= sh.n) return;
+    const float f = 1.0f / (ls[col] + ls[32 + col]);
+    float* out = (float*)a.out + (size_t)(sh.r0 + row) * a.out_stride + (size_t)head * HD + part * (HD / 2);
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+            *reinterpret_cast<f4_t*>(out + i * 32 + 8 * b + 4 * h) =
+                f4_t{o[i][4 * b] * f, o[i][4 * b + 1] * f, o[i][4 * b + 2] * f, o[i][4 * b + 3] * f};
+}
+
 template <int T, int HD>
 int launch_packed(PackedArgs a) {
     typedef Plan<T, HD> P;
@@ -754,11 +1024,16 @@ int launch_packed(PackedArgs a) {
         return g4_check_launch("attn_packed_few_kernel");
     }
     // more than 64 KB of LDS has to be asked for, once on each device
+    constexpr bool kWide = T == G4_F32 && HD == 512;
+    constexpr int kLds = kWide ? Wide::LDS : P::LDS, kThreads = 64 * P::NW;
+    void (*kernel)(PackedArgs);
+    if constexpr (kWide) kernel = attn_packed_wide_kernel;
+    else kernel = attn_packed_kernel<T, HD>;
     static unsigned long long asked = 0;
     int dev = 0;
     G4_HIP(hipGetDevice(&dev));
     if (dev >= 64 || !(asked >> dev & 1)) {
-        G4_HIP(hipFuncSetAttribute((const void*)attn_packed_kernel<T, HD>, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS));
+        G4_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
         if (dev < 64) asked |= 1ull << dev;
     }
     hipLaunchKernelGGL((packed_layout_kernel<T, HD>), dim3(a.m / 32 + a.n_seqs, a.n_kv, 2), dim3(256), 0, g4_stream(), a);
@@ -766,7 +1041,7 @@ int launch_packed(PackedArgs a) {
     // n group / (32 NJ) + extra
     a.extra = (31 * a.group + 32 * (P::NJ - 1) + 32 * P::NJ - 1) / (32 * P::NJ);
     const size_t units = (((size_t)a.m * a.group) >> P::LGROWS) + (size_t)a.extra * a.n_seqs;
-    hipLaunchKernelGGL((attn_packed_kernel<T, HD>), dim3((unsigned)(units * a.n_kv)), dim3(64 * P::NW), P::LDS, g4_stream(), a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(units * a.n_kv)), dim3(kThreads), kLds, g4_stream(), a);
     return g4_check_launch("attn_packed_kernel");
 }
 template <int T>
