@@ -309,10 +309,10 @@ struct Plan {
     static __device__ __forceinline__ int meta_at(int st, int kp) { return META + ((st & 1) * KSP + kp) * 1024; }
 };
 
-// the order of a run of products and the LDS reads of their operands: AHEAD
-// operands are on their way before the first product, then each step's NM
-// products are followed by the NR reads of a later step.  (Reads take longer
-// than a product; left to itself the compiler issues two at a time.)
+// asks for an order of a run of products and the LDS reads of their operands:
+// AHEAD steps' reads before the first product, then each step's NM products
+// followed by the NR reads of a later step (fp32 256: 931 -> 868 us over four
+// prompts of 4096)
 template <int STEPS, int AHEAD, int NM, int NR>
 __device__ __forceinline__ void order_products() {
     constexpr int A = AHEAD < STEPS ? AHEAD : STEPS;
@@ -323,6 +323,26 @@ __device__ __forceinline__ void order_products() {
         __builtin_amdgcn_sched_group_barrier(0x100, NR, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x8, A * NM, 0);
+}
+
+// A run of STEPS steps of products whose operands are read from LDS AHEAD steps
+// before: read(i, x) reads step i's operands, use(i, x) multiplies them.  The
+// scheduling barriers hold the reads where they are, where one wave a SIMD has
+// registers for it (fp32 512: 2056 -> 1886 us over four prompts of 4096; the
+// two-wave kernels lose 4-8 % by it).
+template <typename X, int STEPS, int AHEAD, typename Read, typename Use>
+__device__ __forceinline__ void run_products(Read read, Use use) {
+    constexpr int N = (AHEAD < STEPS ? AHEAD : STEPS - 1) + 1;
+    X x[N];
+#pragma unroll
+    for (int i = 0; i < N - 1; i++) read(i, x[i]);
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        if (i + N - 1 < STEPS) read(i + N - 1, x[(i + N - 1) % N]);
+        __builtin_amdgcn_sched_barrier(0);
+        use(i, x[i % N]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 template <int N>
@@ -771,7 +791,10 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
 // maxima are whole numbers, so that weights of one are brought to another's by
 // an exact power of two, which after the first tiles is 1.  Against halving
 // the dims of both products (partial scores of all keys in LDS, weights
-// computed twice, one barrier more) ...
+// computed twice, one barrier more): 2441 -> 1886 us over four prompts of 4096
+// with the reads ahead, 292 TFLOP/s.  Bound by its copies to LDS, 128 KB a
+// tile and 64 rows at 55 bytes/ns a CU (half of the time by themselves), and by
+// the products; more rows do not fit the registers.
 // K and V of a tile have one place each: the next K is on its way during the
 // second product, V during the first.
 struct Wide {
@@ -856,23 +879,28 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
     f16_t o[NT] = {};
     float m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {}, mo = -FLT_MAX;   // of rows row2, and of row col: what o stands for
     // the job's weights: [step of 16 keys][hi, lo][lane] 16 bytes; maxima: [part][row]
+    struct Ops {
+        h8_t x[2];
+    };
     uint8_t* pw = lds + Wide::PW + slot * 4096;
     float* mx = reinterpret_cast<float*>(lds + Wide::MX) + slot * 64;
     auto scores = [&](int st) {
         const int kt = kt0 + st;
         const uint8_t* at = lds + (g >> 1) * 1024 + ((g & 1) * 32 + 16 * part + c16) * 16;
         f4_t sc[2] = {}, sx[2] = {};
+        run_products<Ops, KS, 3>(
+            [&](int i, Ops& k) {
+                k.x[0] = *reinterpret_cast<const h8_t*>(at + i * 2048);
+                k.x[1] = *reinterpret_cast<const h8_t*>(at + 64 * HD + i * 2048);
+            },
+            [&](int i, const Ops& k) {
 #pragma unroll
-        for (int i = 0; i < KS; i++) {
-            const h8_t k0 = *reinterpret_cast<const h8_t*>(at + i * 2048), k1 = *reinterpret_cast<const h8_t*>(at + 64 * HD + i * 2048);
+                for (int ct = 0; ct < 2; ct++) sc[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.x[0], q[0][ct][i], sc[ct], 0, 0, 0);
 #pragma unroll
-            for (int ct = 0; ct < 2; ct++) sc[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[0][ct][i], sc[ct], 0, 0, 0);
+                for (int ct = 0; ct < 2; ct++) sx[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.x[0], q[1][ct][i], sx[ct], 0, 0, 0);
 #pragma unroll
-            for (int ct = 0; ct < 2; ct++) sx[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[1][ct][i], sx[ct], 0, 0, 0);
-#pragma unroll
-            for (int ct = 0; ct < 2; ct++) sx[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[0][ct][i], sx[ct], 0, 0, 0);
-        }
-        order_products<KS, 3, 6, 2>();
+                for (int ct = 0; ct < 2; ct++) sx[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.x[1], q[0][ct][i], sx[ct], 0, 0, 0);
+            });
         // ---- weights of keys 16 part + 4 g .. + 3 ----
         const float* meta = reinterpret_cast<const float*>(lds + Wide::META + (st & 1) * 1024);
         const int key0 = 16 * part + 4 * g;
@@ -955,17 +983,17 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
             }
         }
         const uint8_t* at = lds + TB + part * NT * 2048 + lane * 16;
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint8_t* v = at + (i * 2 + t) * 1024;
-                const h8_t v0 = *reinterpret_cast<const h8_t*>(v);
-                o[i] = mfma32(v0, p[0][t], o[i]);
-                o[i] = mfma32(v0, p[1][t], o[i]);
-                o[i] = mfma32(*reinterpret_cast<const h8_t*>(v + 64 * HD), p[0][t], o[i]);
-            }
-        order_products<2 * NT, 3, 3, 2>();
+        run_products<Ops, 2 * NT, 2>(
+            [&](int i, Ops& v) {
+                v.x[0] = *reinterpret_cast<const h8_t*>(at + i * 1024);
+                v.x[1] = *reinterpret_cast<const h8_t*>(at + 64 * HD + i * 1024);
+            },
+            [&](int i, const Ops& v) {
+                f16_t& s = o[i >> 1];
+                s = mfma32(v.x[0], p[0][i & 1], s);
+                s = mfma32(v.x[0], p[1][i & 1], s);
+                s = mfma32(v.x[1], p[0][i & 1], s);
+            });
     };
 
     auto begin = [&](int st) {
