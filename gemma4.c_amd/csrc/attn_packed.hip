@@ -350,6 +350,17 @@ __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// of all 64 lanes, by lane moves within rows of 16 and four reads across them
+template <typename Op>
+__device__ __forceinline__ unsigned wave_reduce(unsigned v, Op op) {
+    v = op(v, (unsigned)dpp_i<kDppXor1>((int)v));
+    v = op(v, (unsigned)dpp_i<kDppXor2>((int)v));
+    v = op(v, (unsigned)dpp_i<kDppHalfMirror>((int)v));
+    v = op(v, (unsigned)dpp_i<kDppMirror>((int)v));
+    auto at = [&](int l) { return (unsigned)__builtin_amdgcn_readlane((int)v, l); };
+    return op(op(at(0), at(16)), op(at(32), at(48)));
+}
+
 // The u-th of all workgroups of a kv head, those with the most keys first: a
 // sequence's c-th workgroup has the more keys the larger c is (up to the
 // window), whatever sequence it is, so they go by c, downwards, and by
@@ -365,20 +376,11 @@ __device__ __forceinline__ bool longest_first(const PackedArgs& a, int nj, unsig
     }
     // workgroups of all sequences from their c-th on
     auto from = [&](unsigned c) {
-        unsigned x = units > c ? units - c : 0;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
-        return (unsigned)__builtin_amdgcn_readfirstlane(x);
+        return wave_reduce(units > c ? units - c : 0, [](unsigned x, unsigned y) { return x + y; });
     };
     if (u >= from(0)) return false;
-    unsigned most = units;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const unsigned x = __shfl_xor(most, d, 64);
-        most = x > most ? x : most;
-    }
     // the largest c with more than u from it on
-    unsigned lo = 0, hi = __builtin_amdgcn_readfirstlane(most);
+    unsigned lo = 0, hi = wave_reduce(units, [](unsigned x, unsigned y) { return x > y ? x : y; });
     while (hi - lo > 1) {
         const unsigned mid = (lo + hi) >> 1;
         if (from(mid) > u) lo = mid;
