@@ -13,7 +13,9 @@ int kv_pool_check(const char* who, KvPool* o, const void* kp, const void* vp, in
     G4_CHECK(kv_elem_size(type), G4_ERR_TYPE, "%s: unsupported cache type %d", who, type);
     G4_CHECK_ARG(bytes, "%s: bad pool (%d pages of %d tokens, %d kv heads of %d)", who, n_pages, page, n_kv, hd);
     G4_CHECK_ARG(kp && vp && table && al16(kp) && al16(vp), "%s: null or unaligned pool", who);
-    G4_CHECK_ARG(table_stride > 0, "%s: table_stride %d", who, table_stride);
+    // positions and sums over 64 sequences stay within 32 bits
+    G4_CHECK_ARG(table_stride > 0 && (long)table_stride * page <= 1 << 30, "%s: table_stride %d (2^30 positions at most)", who,
+                 table_stride);
     o->kp = (uint8_t*)kp;
     o->vp = (uint8_t*)vp;
     o->table = table;

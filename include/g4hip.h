@@ -411,7 +411,7 @@ int g4_softmax(float *x, int n);
  *     rint(x / d) (codes 0 if d is 0), read back as code * d; a head that holds
  *     an infinity or NaN reads back as NaN.
  * table (device): table[s * table_stride + i] is the page of positions
- * i * page .. of sequence s.  Entries that no position in use needs are not
+ * i * page .. of sequence s (2^30 positions at most).  Entries that no position in use needs are not
  * read.  Pages are never looked at past a sequence's length, so what is left
  * there by others (infinities, NaN) does not matter.
  * Packed rows: sequence s has rows cu[s] .. cu[s+1]-1 (cu: n_seqs + 1
@@ -456,7 +456,8 @@ int g4_attn_decode_paged(const float *q, int q_stride, const void *kp, const voi
  * of a sequence sees that sequence's rows max(0, i + 1 - window) .. i (window
  * 0: 0 .. i).  q, k, v, out rows of one type, G4_F32, G4_F16 or G4_BF16, their
  * strides in elements (16-byte aligned rows).  F32: products of operands met
- * within 2^-22 of themselves or 2^-39 of their row's largest, fp32 sums; F16,
+ * within 2^-22 of themselves or 2^-39 of their row's largest (a weight times its
+ * V row: 2^-35 of the largest such product), fp32 sums; F16,
  * BF16: exact products, weights rounded to the type, fp32 sums (few rows: fp32
  * throughout).  Rows of out past cu[n_seqs] and those of sequences whose cu
  * does not fit are left as they are.  Where what a row's head sees holds

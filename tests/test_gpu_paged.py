@@ -44,10 +44,11 @@ def filled(lib, nbytes, byte=0xFF):
 class Cache:
     """two pools and the pages of a batch of sequences"""
 
-    def __init__(self, lib, rng, kind, hd, n_kv, page, lens, table=None, pages=None):
+    def __init__(self, lib, rng, kind, hd, n_kv, page, lens, table=None, pages=None, extra=2):
+        """extra: table entries past the longest sequence's; many of them and the work is split whatever the lengths"""
         self.lib, self.kind, self.hd, self.n_kv, self.page = lib, kind, hd, n_kv, page
         if table is None:
-            table, pages = pn.page_table(rng, lens, page)
+            table, pages = pn.page_table(rng, lens, page, extra=extra)
         self.table, self.pages = np.ascontiguousarray(table, np.int32), pages
         size = lib.L.g4_kv_pool_bytes(kind, pages, page, n_kv, hd)
         self.k, self.v = filled(lib, size), filled(lib, size)
@@ -299,9 +300,17 @@ def test_decode_long(lib, kind, hd):
 
 
 def test_decode_many(lib):
-    """more sequences than workgroups"""
+    """more sequences than workgroups, short throughout and with some long ones; the most there may be"""
     rng = np.random.default_rng(71)
     check_decode(lib, 71, pn.BF16, 64, 2, 2, 16, [int(x) for x in rng.integers(0, 40, 700)])
+    check_decode(lib, 71, pn.BF16, 64, 2, 2, 16, [int(x) for x in rng.integers(0, 40, 300)] + [900, 0, 1300])
+    check_decode(lib, 71, pn.Q8, 64, 1, 1, 16, [int(x) for x in rng.integers(0, 6, 4095)] + [700])
+
+
+def test_decode_splits(lib):
+    """numbers of tiles on either side of what one workgroup, all of them and one round take"""
+    for lens in ([32 * 511], [32 * 512 + 1], [32 * 513], [32 * 2048 - 31], [33] * 64, [65] * 65, [300] * 33, [1] * 63 + [5000]):
+        check_decode(lib, 79, pn.BF16, 64, 1, 1, 64, lens, window=0, gain=1.0)
 
 
 def test_decode_strides(lib):
@@ -309,12 +318,13 @@ def test_decode_strides(lib):
     check_decode(lib, 72, pn.F16, 256, 8, 2, 32, [40, 3, 77], extra=12)
 
 
-def test_decode_pages_outside(lib):
+@pytest.mark.parametrize("extra", [2, 40])
+def test_decode_pages_outside(lib, extra):
     """a page outside the pool or a length past the table: NaN in that sequence's row and nowhere else"""
     rng = np.random.default_rng(73)
     hd, page = 64, 16
     for kind in pn.TYPES:
-        c = Cache(lib, rng, kind, hd, 1, page, [40, 40, 40, 40])
+        c = Cache(lib, rng, kind, hd, 1, page, [40, 40, 40, 40], extra=extra)
         x = rows(rng, 160, 1, hd)
         c.store(x, x, [40] * 4, [40] * 4)
         q = rows(rng, 4, 2, hd)
@@ -328,13 +338,14 @@ def test_decode_pages_outside(lib):
         assert same(d[0], a[0]) and np.isfinite(d[1]).all() and np.isnan(d[2]).all() and same(d[3], a[3])
 
 
+@pytest.mark.parametrize("extra", [2, 40])
 @pytest.mark.parametrize("kind", [pn.F32, pn.F16, pn.BF16])
-def test_decode_not_finite(lib, kind):
+def test_decode_not_finite(lib, kind, extra):
     """infinities and NaN at positions that are not seen change nothing; seen, they make their heads NaN or
     infinite and no others"""
     rng = np.random.default_rng(74)
     hd, n_kv, page, t = 128, 2, 32, 90
-    c = Cache(lib, rng, kind, hd, n_kv, page, [128, 128])
+    c = Cache(lib, rng, kind, hd, n_kv, page, [128, 128], extra=extra)
     k, v = rows(rng, 256, n_kv, hd), rows(rng, 256, n_kv, hd)
     k2, v2 = k.copy(), v.copy()
     for a in (k2, v2):      # past the length, before the window
@@ -714,3 +725,62 @@ def test_prompt_lengths(lib):
     """sequences of 1 to 136 rows one after the other, a window that ends inside tiles, three heads on a kv head"""
     for kind in (pn.F32, pn.BF16):
         check_prompt(lib, 305, kind, 64, 6, 2, list(range(1, 141, 9)), window=33)
+
+
+@pytest.mark.parametrize("hd,window", [(256, 0), (512, 0), (512, 40), (128, 40)])
+def test_prompt_magnitudes(lib, hd, window):
+    """fp32 rows whose sizes differ by 2^60 from key to key and by 2^20 within a row: what a row does not see, and what
+    has next to no weight, costs it no precision, and a key of large scores moves the maximum far at once"""
+    rng = np.random.default_rng(400 + hd)
+    n_heads, n_kv, n = 4, 2, [300, 130]
+    m, cu = sum(n), pn.starts(n)
+    q, k, v = (rows(rng, m, h, hd) for h in (n_heads, n_kv, n_kv))
+    v *= np.exp2(rng.integers(-30, 31, (m, n_kv * hd // 64))).repeat(64, 1).astype(np.float32)
+    v *= np.exp2(rng.integers(-10, 11, v.shape)).astype(np.float32)
+    k *= np.exp2(rng.integers(-6, 3, (m, 1))).astype(np.float32)
+    k[rng.integers(0, m, 12)] *= np.float32(20)         # scores far from the others', up and down
+    v[7] = 0
+    v[200] = 0
+    k[31] = 0
+    scale = hd ** -0.5
+    _, got = run_prompt(lib, q, k, v, pn.F32, cu, m, window, n_heads, n_kv, hd, scale)
+    for s, t in enumerate(n):
+        r = slice(cu[s], cu[s + 1])
+        first = [max(0, i + 1 - window) if window else 0 for i in range(t)]
+        want, bound = pn.attention(q[r].reshape(t, n_heads, hd), k[r].reshape(t, n_kv, hd), v[r].reshape(t, n_kv, hd), first,
+                                   scale)
+        # Added for rows this wide: an element of V is met within 2^-39 of its row's largest; and a weight times its V
+        # row's power of two is held as two fp16, the largest of them at 2^11 or more (2^15 at most) and each within
+        # 2^-25, half of fp16's smallest step: times V's scaled elements, below 2^15, that is 2^-10 a key where the
+        # largest key stands for 2^11 * 2^14 at least: 2^-35 of the largest weight * row for each key that is seen.
+        big = np.abs(v[r].reshape(t, n_kv, hd)).max(-1).repeat(n_heads // n_kv, 1).astype(np.float64)
+        for i in range(t):
+            seen = slice(first[i], i + 1)
+            for h in range(n_heads):
+                sc = scale * (k[r].reshape(t, n_kv, hd)[seen, h // 2].astype(np.float64) @ q[cu[s] + i].reshape(n_heads, hd)[h])
+                p = np.exp(sc - sc.max())
+                pb = p * big[seen, h]
+                bound[i, h] += (2.0 ** -38 * pb.sum() + 2.0 ** -35 * len(p) * pb.max()) / p.sum()
+        within(np.abs(got[r].reshape(t, n_heads, hd) - want), bound, s)
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+def test_decode_magnitudes(lib, hd):
+    """the same for one token over an fp32 cache, whose products are exact whatever the sizes"""
+    rng = np.random.default_rng(410)
+    n_heads, n_kv, lens = 4, 2, [300, 1500]
+    m = sum(lens)
+    k, v = rows(rng, m, n_kv, hd), rows(rng, m, n_kv, hd)
+    v *= np.exp2(rng.integers(-30, 31, v.shape)).astype(np.float32)
+    k *= np.exp2(rng.integers(-6, 3, (m, 1))).astype(np.float32)
+    k[rng.integers(0, m, 12)] *= np.float32(20)
+    c = Cache(lib, rng, pn.F32, hd, n_kv, 16, lens)
+    c.store(k, v, lens, lens)
+    q = rows(rng, 2, n_heads, hd)
+    got = run_decode(lib, c, q, lens, n_heads, 0, hd ** -0.5).reshape(2, n_heads, hd)
+    cu = pn.starts(lens)
+    for s, t in enumerate(lens):
+        r = slice(cu[s], cu[s + 1])
+        want, bound = pn.attention(q[s].reshape(1, n_heads, hd), k[r].reshape(t, n_kv, hd), v[r].reshape(t, n_kv, hd), [0],
+                                   hd ** -0.5)
+        within(np.abs(got[s] - want[0]), bound[0], s)

@@ -43,7 +43,7 @@ def rows_call(fn, **kw):
 
 ROWS_BAD = [dict(kp=None), dict(vp=None), dict(table=None), dict(k=None), dict(v=None), dict(cu=None), dict(lens=None),
             dict(kp=P + 8), dict(vp=P + 4), dict(k=P + 4), dict(v=P + 8), dict(n_pages=0), dict(page=24), dict(n_kv=0),
-            dict(hd=200), dict(ts=0), dict(stride=508), dict(stride=514), dict(stride=-512), dict(n=0), dict(n=4097),
+            dict(hd=200), dict(ts=0), dict(ts=(1 << 26) + 1), dict(stride=508), dict(stride=514), dict(stride=-512), dict(n=0), dict(n=4097),
             dict(m=0), dict(m=-4)]
 
 
@@ -70,7 +70,7 @@ def decode_call(**kw):
 DECODE_BAD = [dict(q=None), dict(kp=None), dict(vp=None), dict(table=None), dict(lens=None), dict(part=None), dict(out=None),
               dict(q=P + 4), dict(out=P + 8), dict(part=P + 4), dict(qs=2044), dict(qs=2050), dict(os=2040), dict(os=2049),
               dict(heads=7), dict(heads=0), dict(n_kv=0), dict(hd=192), dict(page=0), dict(n=0), dict(n=5000),
-              dict(window=-1), dict(ts=-1)]
+              dict(window=-1), dict(ts=-1), dict(page=4096, ts=1 << 20)]
 
 
 @pytest.mark.parametrize("bad", DECODE_BAD, ids=str)
