@@ -291,9 +291,9 @@ __global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedArgs a) {
 // put it off to the next tile.  Their sums meet at the end, in LDS.  (8191 rows
 // in bf16, 8 heads of 256: 404 us with eight jobs a workgroup in step, 333 so.)
 // What bounds it: the matrix cores under the card's power limit.  Four prompts
-// of 4096 rows, 8 heads of 256 (128: 32): bf16 306-372 us from card to card,
-// 740-900 TFLOP/s at 2.0-2.1 GHz where an 8192^3 library product reaches 1182;
-// fp32 868-950 us, 290-317 TFLOP/s and three times as many products.  Copies to
+// of 4096 rows, 8 heads of 256 (128: 32): bf16 300-370 us from card to card,
+// 745-910 TFLOP/s at 2.0-2.1 GHz where an 8192^3 library product reaches 1182;
+// fp32 815-900 us, 305-337 TFLOP/s and three times as many products.  Copies to
 // LDS alone (55 bytes/ns a CU) would take 155 and 305 us.  Three independent
 // sums instead of two, the next tile's scores computed beside this tile's
 // weights and wave priorities around the products changed nothing or lost.
@@ -308,7 +308,10 @@ struct Plan {
     static constexpr int TB = 32 * HD * ES;
     static constexpr int NK = DS == 2 ? 1 : 2 * KSP, NV = DS == 2 ? 1 : KSP == 2 ? 5 : 2;
     static constexpr int META = (NK + NV) * TB, XCH = META + 2 * KSP * 1024;
-    static constexpr int LDS = XCH + (DS == 2 ? NW * 4096 : 0);
+    static constexpr int RB = HD / DS * ES;                          // bytes of a wave's part of a row
+    static constexpr int NEED = XCH + (DS == 2 ? NW * 4096 : 0);     // DS 2: partial scores
+    static constexpr int ROWS = KSP == 1 ? NW * 32 * RB : 0;         // the output's rows
+    static constexpr int LDS = NEED > ROWS ? NEED : ROWS;
     static constexpr int JOIN = NJ * (HD * 128 + 256);               // sums of waves 4 .. 7
     static_assert(LDS <= 160 * 1024 && NJ * DS * KSP == NW && (KSP == 1 || JOIN <= LDS), "LDS");
     static __device__ __forceinline__ int k_at(int st, int kp) { return DS == 2 ? 0 : ((st & 1) * KSP + kp) * TB; }
@@ -402,6 +405,66 @@ __device__ __forceinline__ bool longest_first(const PackedArgs& a, int nj, unsig
     return true;
 }
 
+// between a wave's own LDS accesses, which the CU keeps in order: for the compiler
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Rows to and from memory go through LDS as whole lines: an instruction costs
+// the CU's address unit four cycles for every 128-byte line it touches, and the
+// operands' own order (16 bytes of each of 32 rows) touches 32 of them: 16000
+// cycles for a workgroup's q and as many for its output, of the 95000 that 17
+// tiles take.  (Prompts of 100 to 2048 rows with a window of 512, 8 heads of
+// 256: fp32 86 -> 79 us, bf16 51 -> 44 us.)  Chunk c (16 bytes) of row r lies in
+// slot c ^ r, so that neither order has bank conflicts.
+template <int C>
+__device__ __forceinline__ int row_slot(int r, int c) {
+    return (r * C + (c ^ (r & (C < 32 ? C - 1 : 31)))) * 16;
+}
+// N rows of C chunks each, from `first` on, by one wave: at(r) is row r's
+// address, box takes C chunks a row
+template <int C, int N, typename At>
+__device__ __forceinline__ void rows_to_lds(uint8_t* box, int first, At at) {
+    constexpr int K = N * C / 64;
+    const int lane = threadIdx.x & 63;
+    f4_t x[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int p = k * 64 + lane;
+        x[k] = reinterpret_cast<const f4_t*>(at(first + p / C))[p % C];
+    }
+    wave_lds_order();
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int p = k * 64 + lane;
+        *reinterpret_cast<f4_t*>(box + row_slot<C>(first + p / C, p % C)) = x[k];
+    }
+    wave_lds_order();
+}
+// the other way: 32 rows of C chunks, the first n of them
+template <int C, typename At>
+__device__ __forceinline__ void rows_from_lds(const uint8_t* box, int n, At at) {
+    constexpr int K = C / 2, B = K < 16 ? K : 16;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));   // addresses of its own: none kept from rows_to_lds over all tiles
+    wave_lds_order();
+#pragma unroll
+    for (int k = 0; k < K; k += B) {
+        f4_t x[B];
+#pragma unroll
+        for (int i = 0; i < B; i++) {
+            const int p = (k + i) * 64 + lane;
+            x[i] = *reinterpret_cast<const f4_t*>(box + row_slot<C>(p / C, p % C));
+        }
+#pragma unroll
+        for (int i = 0; i < B; i++) {
+            const int p = (k + i) * 64 + lane;
+            if (p / C < n) reinterpret_cast<f4_t*>(at(p / C))[p % C] = x[i];
+        }
+    }
+}
+
 // a workgroup's sequence and jobs
 struct Share {
     int r0, n;                  // the sequence's first row, its rows
@@ -473,14 +536,16 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     constexpr int kWhole = kHalf / NW;                    // of one tile's (0: half the waves have a tile each)
     static_assert(kHalf * KSP % NW == 0 && (kWhole || kShare == 1), "shares");
     const int first_piece = kWhole ? wave : wave % kHalf;
+    // past the last tile: no bytes
+    auto tile_rsrc = [&](int tile) {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(rec0 + tile * rec_step), 0,
+                                                 tile <= kt1 - kt0 ? (int)block_bytes(HD, ES) : 0, kBufWord3);
+    };
     auto stage = [&](int st, bool v) {
 #pragma unroll
         for (int t = 0; t < (kWhole ? KSP : 1); t++) {
-            const int tile = st * KSP + (kWhole ? t : wave / kHalf);
-            // past the last tile: no bytes
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                (void*)(rec0 + tile * rec_step), 0, tile <= kt1 - kt0 ? (int)block_bytes(HD, ES) : 0, kBufWord3);
             const int tt = kWhole ? t : wave / kHalf;
+            const __amdgpu_buffer_rsrc_t r = tile_rsrc(st * KSP + tt);
             uint8_t* at = lds + (v ? P::v_at(st, tt) : P::k_at(st, tt)) + first_piece * 1024;
 #pragma unroll
             for (int i = 0; i < (kWhole ? kWhole : 1); i++)
@@ -494,26 +559,43 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     stage_k(0);
     if (DS == 1) stage_v(0);
 
-    // ---- q ----
+    // ---- q, through places in LDS that the first stage leaves free ----
     op q[NS][KS];
     float fq = fabsf(a.scale) * kLog2e;
-    const E* qr = (const E*)a.q + (size_t)(r0 + (row < n ? row : n - 1)) * a.q_stride + (size_t)head * HD;
+    constexpr int kPasses = KSP == 2 ? 1 : 2, kChunks = P::RB / 16 / kPasses, kSteps = KS / kPasses;
+    // fp32: half of the second K and V places each; 16 bits: the second K places
+    // and free V ones, a job's rows by its two waves; DS 2: V and the partial scores
+    uint8_t* box = lds + (KSP == 2 ? (slot < 2 ? 2 + slot : slot == 2 ? 5 : 7) * TB
+                          : DS == 1 ? (wave < 2 ? TB : 2 * TB) + wave * (TB / 2)
+                          : wave < 4 ? TB + wave * (TB / 4) : P::XCH + (wave - 4) * (TB / 4));
+    auto q_row = [&](int pass) {
+        return [=](int r) {
+            const int i = jt * 32 + r < n ? jt * 32 + r : n - 1;
+            return (const uint8_t*)((const E*)a.q + (size_t)(r0 + i) * a.q_stride + (size_t)head * HD + part * (HD / DS)) +
+                   pass * kChunks * 16;
+        };
+    };
+    auto chunk = [&](int c) { return box + row_slot<kChunks>(col, c); };
     if constexpr (T == G4_F32) {
         float4 x[KS][2];
         unsigned top = 0;
 #pragma unroll
-        for (int i = 0; i < KS; i++)
+        for (int pass = 0; pass < 2; pass++) {
+            rows_to_lds<kChunks, 32>(box, 0, q_row(pass));
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const float4 y = reinterpret_cast<const float4*>(qr + i * 16 + h * 8)[j];
-                x[i][j] = y;
-                const float e[4] = {y.x, y.y, y.z, y.w};
+            for (int i = 0; i < kSteps; i++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const unsigned m = __float_as_uint(e[k]) & 0x7fffffffu;
-                    top = m > top ? m : top;
+                for (int j = 0; j < 2; j++) {
+                    const float4 y = *reinterpret_cast<const float4*>(chunk(i * 4 + h * 2 + j));
+                    x[pass * kSteps + i][j] = y;
+                    const float e[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const unsigned m = __float_as_uint(e[k]) & 0x7fffffffu;
+                        top = m > top ? m : top;
+                    }
                 }
-            }
+        }
         const unsigned o = __shfl_xor(top, 32, 64);
         top = o > top ? o : top;
         const int e = (int)(top >> 23) > kLowK ? (int)(top >> 23) : kLowK;
@@ -533,15 +615,23 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     } else {
         const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
-        for (int i = 0; i < KS; i++) {
-            uint4 x = *reinterpret_cast<const uint4*>(qr + part * (HD / DS) + i * 16 + h * 8);
-            if (a.scale == 0.0f) x = make_uint4(0, 0, 0, 0);
-            x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-            q[0][i] = __builtin_bit_cast(op, x);
+        for (int pass = 0; pass < kPasses; pass++) {
+            if constexpr (KSP == 2) {
+                rows_to_lds<kChunks, 16>(box, kp * 16, q_row(pass));
+                lds_barrier();
+            } else {
+                rows_to_lds<kChunks, 32>(box, 0, q_row(pass));
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; i++) {
+                uint4 x = *reinterpret_cast<const uint4*>(chunk(i * 2 + h));
+                if (a.scale == 0.0f) x = make_uint4(0, 0, 0, 0);
+                x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                q[0][pass * kSteps + i] = __builtin_bit_cast(op, x);
+            }
         }
         if (a.scale == 0.0f) fq = 1.0f;
     }
-
     // one wave a SIMD: q and o stay in the accumulation registers, from which
     // products take them as well (left to itself the compiler moves them there
     // and back for every tile)
@@ -558,22 +648,42 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     float m = -FLT_MAX, l = 0.0f;
     f16_t sc;
     op p[NS][2];
+    struct Ops {
+        op x[NS];
+    };
+    // kFeed: the next tile's copies are issued between the products, one a step
+    // (by themselves the 65 KB of an fp32 tile of 256 dims take the CU's address
+    // unit 1000 of a tile's 6500 cycles, which nothing else would use), those
+    // past the last tile as well: they have no bytes, and a branch costs more
+    constexpr bool kFeed = NS == 2;
     auto scores = [&](int st) {
         const uint8_t* at = lds + P::k_at(st, kp) + lane * 16;
         sc = f16_t{};
         f16_t sx = {};
+        if constexpr (kFeed) {
+            const __amdgpu_buffer_rsrc_t r = tile_rsrc(st + 1);
+            uint8_t* to[2] = {lds + P::k_at(st + 1, 0) + wave * 1024, lds + P::v_at(st + 1, 0) + wave * 1024};
+            run_products<Ops, KS, 2>(
+                [&](int i, Ops& k) {
 #pragma unroll
-        for (int i = 0; i < KS; i++) {
-            const op k0 = *reinterpret_cast<const op*>(at + (part * KS + i) * 1024);
-            sc = mfma32(k0, q[0][i], sc);
-            if constexpr (NS == 2) {
-                const op k1 = *reinterpret_cast<const op*>(at + 64 * HD + (part * KS + i) * 1024);
-                sx = mfma32(k0, q[1][i], sx);
-                sx = mfma32(k1, q[0][i], sx);
-            }
+                    for (int j = 0; j < NS; j++) k.x[j] = *reinterpret_cast<const op*>(at + j * 64 * HD + i * 1024);
+                },
+                [&](int i, const Ops& k) {
+                    sc = mfma32(k.x[0], q[0][i], sc);
+#pragma unroll
+                    for (int j = i * 2 * kShare / KS; j < (i + 1) * 2 * kShare / KS; j++)
+                        buf_load_lds16(r, to[j / kShare] + j % kShare * NW * 1024, wave * 1024 + lane * 16,
+                                       j / kShare * TB + j % kShare * NW * 1024);
+                    if (i == KS - 1 && wave == 0) buf_load_lds16(r, lds + P::meta_at(st + 1, 0), lane * 16, 2 * TB);
+                    sx = mfma32(k.x[0], q[1][i], sx);
+                    sx = mfma32(k.x[1], q[0][i], sx);
+                });
+            sc += sx;
+        } else {
+#pragma unroll
+            for (int i = 0; i < KS; i++) sc = mfma32(*reinterpret_cast<const op*>(at + (part * KS + i) * 1024), q[0][i], sc);
+            order_products<KS, 3, 1, 1>();
         }
-        order_products<KS, 3, NS == 2 ? 3 : 1, NS>();
-        if constexpr (NS == 2) sc += sx;
     };
     auto weights = [&](int st, int kt) {
         const float* meta = reinterpret_cast<const float*>(lds + P::meta_at(st, kp));
@@ -645,57 +755,62 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     };
     auto values = [&](int st) {
         const uint8_t* at = lds + P::v_at(st, kp) + lane * 16;
+        if constexpr (NS == 2) {
+            run_products<Ops, 2 * NT, 2>(
+                [&](int i, Ops& v) {
 #pragma unroll
-        for (int i = 0; i < NT; i++)
+                    for (int j = 0; j < NS; j++) v.x[j] = *reinterpret_cast<const op*>(at + j * 64 * HD + i * 1024);
+                },
+                [&](int i, const Ops& v) {
+                    f16_t& s = o[i >> 1];
+                    s = mfma32(v.x[0], p[0][i & 1], s);
+                    s = mfma32(v.x[0], p[1][i & 1], s);
+                    s = mfma32(v.x[1], p[0][i & 1], s);
+                });
+        } else {
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint8_t* v = at + ((part * NT + i) * 2 + t) * 1024;
-                const op v0 = *reinterpret_cast<const op*>(v);
-                o[i] = mfma32(v0, p[0][t], o[i]);
-                if constexpr (NS == 2) {
-                    o[i] = mfma32(v0, p[1][t], o[i]);
-                    o[i] = mfma32(*reinterpret_cast<const op*>(v + 64 * HD), p[0][t], o[i]);
-                }
-            }
-        order_products<2 * NT, 3, NS == 2 ? 3 : 1, NS>();
+            for (int i = 0; i < 2 * NT; i++)
+                o[i >> 1] = mfma32(*reinterpret_cast<const op*>(at + (part * NT * 2 + i) * 1024), p[0][i & 1], o[i >> 1]);
+            order_products<2 * NT, 3, 1, 1>();
+        }
     };
 
     if constexpr (DS == 1) {
         // this wave's copies have landed, then everyone's; and all are done
         // with the stage before (waves 4 .. 7 but for its V, which has three
         // places)
-        auto turn = [&](int st) {
+        auto turn = [&](int st, bool feed) {
             wait_vm<0>();
             lds_barrier();
-            if (st + 1 < stages) {
+            if (!feed && st + 1 < stages) {
                 stage_k(st + 1);
                 stage_v(st + 1);
             }
         };
         int st = 0;
-        for (; st < s0; st++) turn(st);
+        for (; st < s0; st++) turn(st, false);
         if (KSP == 1 || kp == 0) {
             for (; st < s1; st++) {
-                turn(st);
+                turn(st, kFeed);
                 scores(st);
                 weights(st, kt0 + st * KSP + kp);
                 values(st);
             }
         } else if (s0 < s1) {
-            turn(st);
+            turn(st, false);
             scores(st);
             weights(st, kt0 + st * KSP + kp);
             for (st++; st < s1; st++) {
-                turn(st);
+                turn(st, false);
                 values(st - 1);
                 scores(st);
                 weights(st, kt0 + st * KSP + kp);
             }
-            if (st < stages) turn(st);
+            if (st < stages) turn(st, false);
             values(s1 - 1);
             st++;
         }
-        for (; st < stages; st++) turn(st);
+        for (; st < stages; st++) turn(st, false);
     } else {
         // a tile's turn up to its scores, and from there on; both waves of a job
         // take part in the same ones
@@ -780,9 +895,16 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     } else {
         l += shfl_xor(l, 32);
     }
-    if (!mine || row >= n) return;
+    // ---- the output's rows, where K and V (16 bits: this wave's other sums) were ----
+    if (KSP == 1) {
+        wait_vm<0>();
+        lds_barrier();
+    }
+    if (!mine) return;
+    wave_lds_order();
     const float f = 1.0f / l;
-    E* out = (E*)a.out + (size_t)(r0 + row) * a.out_stride + (size_t)head * HD + part * (HD / DS);
+    constexpr int kRow = P::RB / 16;
+    uint8_t* rows = lds + (KSP == 2 ? slot * HD * 128 : wave * 32 * P::RB);
 #pragma unroll
     for (int i = 0; i < NT; i++)
 #pragma unroll
@@ -790,8 +912,12 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
             E y[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) y[j] = (E)(o[i][4 * b + j] * f);
-            __builtin_memcpy(__builtin_assume_aligned(out + i * 32 + 8 * b + 4 * h, 4 * ES), y, 4 * ES);
+            uint8_t* to = rows + (ES == 4 ? row_slot<kRow>(col, i * 8 + 2 * b + h) : row_slot<kRow>(col, i * 4 + b) + h * 8);
+            __builtin_memcpy(__builtin_assume_aligned(to, 4 * ES), y, 4 * ES);
         }
+    rows_from_lds<kRow>(rows, n - jt * 32, [&](int r) {
+        return (uint8_t*)((E*)a.out + (size_t)(r0 + jt * 32 + r) * a.out_stride + (size_t)head * HD + part * (HD / DS));
+    });
 }
 
 // ---- fp32 at head_dim 512 ------------------------------------------------------------
@@ -803,9 +929,10 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
 // an exact power of two, which after the first tiles is 1.  Against halving
 // the dims of both products (partial scores of all keys in LDS, weights
 // computed twice, one barrier more): 2441 -> 1886 us over four prompts of 4096
-// with the reads ahead, 292 TFLOP/s.  Bound by its copies to LDS, 128 KB a
-// tile and 64 rows at 55 bytes/ns a CU (half of the time by themselves), and by
-// the products; more rows do not fit the registers.
+// with the reads ahead, 1790 with q and the output as whole lines, 307 TFLOP/s.
+// Bound by its copies to LDS, 128 KB a tile and 64 rows at 55 bytes/ns a CU
+// (half of the time by themselves), and by the products; more rows do not fit
+// the registers.
 // K and V of a tile have one place each: the next K is on its way during the
 // second product, V during the first.
 struct Wide {
@@ -839,9 +966,14 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
         for (int i = 0; i < TB / 4096; i++) buf_load_lds16(r, at + i * 4096, wave * 1024 + lane * 16, (v ? TB : 0) + i * 4096);
         if (!v && wave == 0) buf_load_lds16(r, lds + Wide::META + (st & 1) * 1024, lane * 16, 2 * TB);
     };
-    stage(0, false);
-
-    // ---- q: rows c16 and 16 + c16, steps of 32 dims, 8 of them a lane ----
+    // ---- q: rows c16 and 16 + c16, steps of 32 dims, 8 of them a lane; half of
+    // the job's rows by each of its waves through LDS ----
+    uint8_t* box = lds + slot * 32 * HD * 4;
+    rows_to_lds<HD / 4, 16>(box, part * 16, [&](int r) {
+        const int i = jt * 32 + r < sh.n ? jt * 32 + r : sh.n - 1;
+        return (const uint8_t*)((const float*)a.q + (size_t)(sh.r0 + i) * a.q_stride + (size_t)head * HD);
+    });
+    lds_barrier();
     h8_t q[2][2][KS];
     float fq[2];
     int row2[2], wf2[2];
@@ -849,14 +981,13 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
     for (int ct = 0; ct < 2; ct++) {
         row2[ct] = jt * 32 + 16 * ct + c16;
         wf2[ct] = first_key(row2[ct]);
-        const float* qr = (const float*)a.q + (size_t)(sh.r0 + (row2[ct] < sh.n ? row2[ct] : sh.n - 1)) * a.q_stride + (size_t)head * HD;
         float4 x[KS][2];
         unsigned top = 0;
 #pragma unroll
         for (int i = 0; i < KS; i++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                x[i][j] = reinterpret_cast<const float4*>(qr + i * 32 + g * 8)[j];
+                x[i][j] = *reinterpret_cast<const float4*>(box + row_slot<HD / 4>(16 * ct + c16, i * 8 + g * 2 + j));
                 const float e[4] = {x[i][j].x, x[i][j].y, x[i][j].z, x[i][j].w};
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -887,6 +1018,8 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
         }
     }
 
+    lds_barrier();   // q has been read
+    stage(0, false);
     f16_t o[NT] = {};
     float m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {}, mo = -FLT_MAX;   // of rows row2, and of row col: what o stands for
     // the job's weights: [step of 16 keys][hi, lo][lane] 16 bytes; maxima: [part][row]
@@ -1042,16 +1175,18 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
         if (g == 0) ls[part * 32 + 16 * ct + c16] = l[ct];
     }
     lds_barrier();
-    const int row = jt * 32 + col;
-    if (!mine || row >= sh.n) return;
+    if (!mine) return;
     const float f = 1.0f / (ls[col] + ls[32 + col]);
-    float* out = (float*)a.out + (size_t)(sh.r0 + row) * a.out_stride + (size_t)head * HD + part * (HD / 2);
+    uint8_t* rows = lds + wave * 32 * HD * 2;
 #pragma unroll
     for (int i = 0; i < NT; i++)
 #pragma unroll
         for (int b = 0; b < 4; b++)
-            *reinterpret_cast<f4_t*>(out + i * 32 + 8 * b + 4 * h) =
+            *reinterpret_cast<f4_t*>(rows + row_slot<HD / 8>(col, i * 8 + 2 * b + h)) =
                 f4_t{o[i][4 * b] * f, o[i][4 * b + 1] * f, o[i][4 * b + 2] * f, o[i][4 * b + 3] * f};
+    rows_from_lds<HD / 8>(rows, sh.n - jt * 32, [&](int r) {
+        return (uint8_t*)((float*)a.out + (size_t)(sh.r0 + jt * 32 + r) * a.out_stride + (size_t)head * HD + part * (HD / 2));
+    });
 }
 
 template <int T, int HD>
