@@ -929,7 +929,8 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
 // an exact power of two, which after the first tiles is 1.  Against halving
 // the dims of both products (partial scores of all keys in LDS, weights
 // computed twice, one barrier more): 2441 -> 1886 us over four prompts of 4096
-// with the reads ahead, 1790 with q and the output as whole lines, 307 TFLOP/s.
+// with the reads ahead, 1780 with q and the output as whole lines, 1640 with the
+// copies between the products, 335 TFLOP/s.
 // Bound by its copies to LDS, 128 KB a tile and 64 rows at 55 bytes/ns a CU
 // (half of the time by themselves), and by the products; more rows do not fit
 // the registers.
@@ -958,13 +959,22 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
     const int stages = kt1 - kt0 + 1;
     const uint8_t* rec0 = a.work + ((size_t)(sh.block0 + kt0) * a.n_kv + sh.kvh) * block_bytes(HD, 4);
     const size_t rec_step = (size_t)a.n_kv * block_bytes(HD, 4);
+    // past the last tile: no bytes
+    auto tile_rsrc = [&](int st) {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(rec0 + st * rec_step), 0, st < stages ? (int)block_bytes(HD, 4) : 0,
+                                                 kBufWord3);
+    };
+    // a wave's of a tile's K, of its V, issued between its first kFeed steps of
+    // products (all before the products 1780 us, over 4, 8, 16 steps 1695, 1640, 1652)
+    constexpr int kCopies = TB / 4096, kFeed = 8;
+    auto copy = [&](const __amdgpu_buffer_rsrc_t r, int st, bool v, int i) {
+        buf_load_lds16(r, lds + (v ? TB : 0) + wave * 1024 + i * 4096, wave * 1024 + lane * 16, (v ? TB : 0) + i * 4096);
+        if (!v && i == 0 && wave == 0) buf_load_lds16(r, lds + Wide::META + (st & 1) * 1024, lane * 16, 2 * TB);
+    };
     auto stage = [&](int st, bool v) {
-        const __amdgpu_buffer_rsrc_t r =
-            __builtin_amdgcn_make_buffer_rsrc((void*)(rec0 + st * rec_step), 0, (int)block_bytes(HD, 4), kBufWord3);
-        uint8_t* at = lds + (v ? TB : 0) + wave * 1024;
+        const __amdgpu_buffer_rsrc_t r = tile_rsrc(st);
 #pragma unroll
-        for (int i = 0; i < TB / 4096; i++) buf_load_lds16(r, at + i * 4096, wave * 1024 + lane * 16, (v ? TB : 0) + i * 4096);
-        if (!v && wave == 0) buf_load_lds16(r, lds + Wide::META + (st & 1) * 1024, lane * 16, 2 * TB);
+        for (int i = 0; i < kCopies; i++) copy(r, st, v, i);
     };
     // ---- q: rows c16 and 16 + c16, steps of 32 dims, 8 of them a lane; half of
     // the job's rows by each of its waves through LDS ----
@@ -1032,6 +1042,7 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
         const int kt = kt0 + st;
         const uint8_t* at = lds + (g >> 1) * 1024 + ((g & 1) * 32 + 16 * part + c16) * 16;
         f4_t sc[2] = {}, sx[2] = {};
+        const __amdgpu_buffer_rsrc_t r = tile_rsrc(st);
         run_products<Ops, KS, 3>(
             [&](int i, Ops& k) {
                 k.x[0] = *reinterpret_cast<const h8_t*>(at + i * 2048);
@@ -1040,6 +1051,9 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
             [&](int i, const Ops& k) {
 #pragma unroll
                 for (int ct = 0; ct < 2; ct++) sc[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.x[0], q[0][ct][i], sc[ct], 0, 0, 0);
+                if (i < kFeed)
+#pragma unroll
+                    for (int j = i * kCopies / kFeed; j < (i + 1) * kCopies / kFeed; j++) copy(r, st, true, j);
 #pragma unroll
                 for (int ct = 0; ct < 2; ct++) sx[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.x[0], q[1][ct][i], sx[ct], 0, 0, 0);
 #pragma unroll
@@ -1099,7 +1113,8 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
             if (g == 0) mx[part * 32 + 16 * ct + c16] = m[ct];
         }
     };
-    auto values = [&]() {
+    auto values = [&](int next) {
+        const __amdgpu_buffer_rsrc_t r = tile_rsrc(next);
         h8_t p[2][2];   // [hi, lo][step]
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -1135,36 +1150,37 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
             [&](int i, const Ops& v) {
                 f16_t& s = o[i >> 1];
                 s = mfma32(v.x[0], p[0][i & 1], s);
+                if (i < kFeed)
+#pragma unroll
+                    for (int j = i * kCopies / kFeed; j < (i + 1) * kCopies / kFeed; j++) copy(r, next, false, j);
                 s = mfma32(v.x[0], p[1][i & 1], s);
                 s = mfma32(v.x[1], p[0][i & 1], s);
             });
     };
 
-    auto begin = [&](int st) {
+    auto begin = [&]() {
         wait_vm<0>();
         lds_barrier();   // K is there, V and the weights of the tile before are done with
-        stage(st, true);
     };
-    auto middle = [&](int st) {
+    auto middle = [&]() {
         wait_vm<0>();
         lds_barrier();   // V and the weights are there, K is done with
-        if (st + 1 < stages) stage(st + 1, false);
+    };
+    auto pass = [&](int st) {
+        begin();
+        stage(st, true);
+        middle();
+        stage(st + 1, false);
     };
     int st = 0;
-    for (; st < s0; st++) {
-        begin(st);
-        middle(st);
-    }
+    for (; st < s0; st++) pass(st);
     for (; st < s1; st++) {
-        begin(st);
+        begin();
         scores(st);
-        middle(st);
-        values();
+        middle();
+        values(st + 1);
     }
-    for (; st < stages; st++) {
-        begin(st);
-        middle(st);
-    }
+    for (; st < stages; st++) pass(st);
 
     // ---- the two waves' weight sums ----
     float* ls = reinterpret_cast<float*>(lds + Wide::MX) + 128 + slot * 64;
@@ -1174,6 +1190,7 @@ __global__ __launch_bounds__(256, 1) void attn_packed_wide_kernel(PackedArgs a) 
         l[ct] += shfl_xor(l[ct], 32);
         if (g == 0) ls[part * 32 + 16 * ct + c16] = l[ct];
     }
+    wait_vm<0>();
     lds_barrier();
     if (!mine) return;
     const float f = 1.0f / (ls[col] + ls[32 + col]);
