@@ -11,7 +11,7 @@ namespace {
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kLgWG = 9, kPagedWG = 1 << kLgWG;   // workgroups that share the work, two a CU
-constexpr int kHeadsWG = 16;                                // q heads of a workgroup: the columns of a product
+constexpr int kHeadsWG = 16;                      // q heads of a workgroup: the columns of a product
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct PagedArgs {
@@ -221,9 +221,10 @@ __device__ __forceinline__ void mfma_terms(const b8_t (&a)[NT], const b8_t (&b)[
 // terms of a step come from LDS.  Bound by the cache's bytes where there are
 // many: 40 sequences of 2000 to 30000 keys, 8 q heads on 2 kv heads of 256,
 // bf16 150 us (5.4 TB/s; a plain read 6.25), fp32 5.4, codes 4.75; of 512, codes
-// 5.0, fp32 5.2.  DEPTH loads of 1 KB are in flight a wave: 4, 8 and 16 are
-// equally fast while nothing spills, and at head_dim 512 (codes, 190 us with
-// 32 in flight) the spills and moves cost more than the depth gives (155).
+// 5.0, fp32 4.8.  DEPTH loads of 1 KB are in flight a wave, 4 for 16-bit caches
+// and 8 for the others: fp16 of 512, one sequence of 32768 keys, 34 us with 4
+// and 35 with 8; fp32 of 512 163 and 154, codes of 512 161 and 155, fp32 of 256
+// 145 and 144.  More costs registers and gives nothing (codes of 512, 16: 215).
 template <int TYPE, int HD, int DEPTH>
 __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
     constexpr int ES = CacheType<TYPE>::ES, NT = CacheType<TYPE>::NT;
@@ -278,76 +279,76 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
         const int unit1 = left < (unsigned long long)(tiles + a.lead - unit) ? unit + (int)left : tiles + a.lead;
         const int tile0 = unit > a.lead ? unit - a.lead : 0, tile1 = unit1 - a.lead;
         if (tile1 > tile0) {
-        const int kvh = item / a.ngrp, hg = item - kvh * a.ngrp;
-        const int nh = a.group - hg * kHeadsWG < kHeadsWG ? a.group - hg * kHeadsWG : kHeadsWG;
-        const int head0 = kvh * a.group + hg * kHeadsWG;
-        const int first = a.window > 0 && len > a.window ? len - a.window : 0;
+            const int kvh = item / a.ngrp, hg = item - kvh * a.ngrp;
+            const int nh = a.group - hg * kHeadsWG < kHeadsWG ? a.group - hg * kHeadsWG : kHeadsWG;
+            const int head0 = kvh * a.group + hg * kHeadsWG;
+            const int first = a.window > 0 && len > a.window ? len - a.window : 0;
 
-        // ---- where a tile's two blocks are; one without a key in use is not read ----
-        bool bad = false;
-        auto pages = [&](int tile, bool on, int (&pg)[2]) {
-            const int pos = (first_tile + tile) << 5;
-            pg[0] = pg[1] = -1;
-            if (on && first - pos < 16) {
-                pg[0] = __builtin_amdgcn_readfirstlane(a.p.page_of(s, pos));
-                bad = bad || pg[0] < 0;
-            }
-            if (on && len - pos > 16) {
-                pg[1] = __builtin_amdgcn_readfirstlane(a.p.page_of(s, pos + 16));
-                bad = bad || pg[1] < 0;
-            }
-        };
-        auto block = [&](int tile, const int (&pg)[2], int i) {
-            return a.p.block_of(pg[i] < 0 ? 0 : pg[i], kvh, ((first_tile + tile) << 5) + 16 * i);
-        };
-        auto rsrc = [&](const uint8_t* pool, int tile, const int (&pg)[2], __amdgpu_buffer_rsrc_t (&r)[2]) {
+            // ---- where a tile's two blocks are; one without a key in use is not read ----
+            bool bad = false;
+            auto pages = [&](int tile, bool on, int (&pg)[2]) {
+                const int pos = (first_tile + tile) << 5;
+                pg[0] = pg[1] = -1;
+                if (on && first - pos < 16) {
+                    pg[0] = __builtin_amdgcn_readfirstlane(a.p.page_of(s, pos));
+                    bad = bad || pg[0] < 0;
+                }
+                if (on && len - pos > 16) {
+                    pg[1] = __builtin_amdgcn_readfirstlane(a.p.page_of(s, pos + 16));
+                    bad = bad || pg[1] < 0;
+                }
+            };
+            auto block = [&](int tile, const int (&pg)[2], int i) {
+                return a.p.block_of(pg[i] < 0 ? 0 : pg[i], kvh, ((first_tile + tile) << 5) + 16 * i);
+            };
+            auto rsrc = [&](const uint8_t* pool, int tile, const int (&pg)[2], __amdgpu_buffer_rsrc_t (&r)[2]) {
 #pragma unroll
-            for (int i = 0; i < 2; i++)
-                r[i] = __builtin_amdgcn_make_buffer_rsrc((void*)(pool + block(tile, pg, i) * (16 * HD * ES)), 0,
-                                                         pg[i] < 0 ? 0 : 16 * HD * ES, kBufWord3);
-        };
-        // load i of a tile: K pieces in the order of the product steps, then V pieces, blocks in turn
-        auto load = [&](int i, const __amdgpu_buffer_rsrc_t (&k)[2], const __amdgpu_buffer_rsrc_t (&v)[2]) {
-            if (i < 2 * KC) {
-                const int b = i / CPS & 1, c = i / (2 * CPS) * CPS + i % CPS;
-                return buf_load16(k[b], lane * 16, c * 1024);
-            }
-            return buf_load16(v[i & 1], lane * 16, (i - 2 * KC) / 2 * 1024);
-        };
-        int tile = tile0 + wave, pg[2], npg[2];
-        uint4 ring[DEPTH];
-        __amdgpu_buffer_rsrc_t kr[2], vr[2], kn[2], vn[2];
-        pages(tile, tile < tile1, pg);
-        rsrc(a.p.kp, tile, pg, kr);
-        rsrc(a.p.vp, tile, pg, vr);
+                for (int i = 0; i < 2; i++)
+                    r[i] = __builtin_amdgcn_make_buffer_rsrc((void*)(pool + block(tile, pg, i) * (16 * HD * ES)), 0,
+                                                             pg[i] < 0 ? 0 : 16 * HD * ES, kBufWord3);
+            };
+            // load i of a tile: K pieces in the order of the product steps, then V pieces, blocks in turn
+            auto load = [&](int i, const __amdgpu_buffer_rsrc_t (&k)[2], const __amdgpu_buffer_rsrc_t (&v)[2]) {
+                if (i < 2 * KC) {
+                    const int b = i / CPS & 1, c = i / (2 * CPS) * CPS + i % CPS;
+                    return buf_load16(k[b], lane * 16, c * 1024);
+                }
+                return buf_load16(v[i & 1], lane * 16, (i - 2 * KC) / 2 * 1024);
+            };
+            int tile = tile0 + wave, pg[2], npg[2];
+            uint4 ring[DEPTH];
+            __amdgpu_buffer_rsrc_t kr[2], vr[2], kn[2], vn[2];
+            pages(tile, tile < tile1, pg);
+            rsrc(a.p.kp, tile, pg, kr);
+            rsrc(a.p.vp, tile, pg, vr);
 #pragma unroll
-        for (int i = 0; i < DEPTH; i++) ring[i] = load(i, kr, vr);
+            for (int i = 0; i < DEPTH; i++) ring[i] = load(i, kr, vr);
 
-        // ---- q, times scale log2(e), as three terms in the products' order ----
-        const float qs = a.scale * kLog2e;
-        for (int x = tid; x < STEPS * 64; x += 256) {
-            const int st = x >> 6, l = x & 63, lg = l >> 4, lc = l & 15;
-            float4 q0 = make_float4(0, 0, 0, 0), q1 = q0;
-            if (lc < nh) {
-                const float* qr = a.q + (size_t)s * a.q_stride + (size_t)(head0 + lc) * HD;
-                const int d0 = ES == 4 ? st * 32 + lg * 4 : ES == 2 ? st * 32 + lg * 8 : (st >> 1) * 64 + lg * 16 + (st & 1) * 8;
-                q0 = *reinterpret_cast<const float4*>(qr + d0);
-                q1 = *reinterpret_cast<const float4*>(qr + d0 + (ES == 4 ? 16 : 4));
-            }
-            uint32_t t[4][3];
-            split_pair<3>(q0.x * qs, q0.y * qs, t[0]);
-            split_pair<3>(q0.z * qs, q0.w * qs, t[1]);
-            split_pair<3>(q1.x * qs, q1.y * qs, t[2]);
-            split_pair<3>(q1.z * qs, q1.w * qs, t[3]);
+            // ---- q, times scale log2(e), as three terms in the products' order ----
+            const float qs = a.scale * kLog2e;
+            for (int x = tid; x < STEPS * 64; x += 256) {
+                const int st = x >> 6, l = x & 63, lg = l >> 4, lc = l & 15;
+                float4 q0 = make_float4(0, 0, 0, 0), q1 = q0;
+                if (lc < nh) {
+                    const float* qr = a.q + (size_t)s * a.q_stride + (size_t)(head0 + lc) * HD;
+                    const int d0 = ES == 4 ? st * 32 + lg * 4 : ES == 2 ? st * 32 + lg * 8 : (st >> 1) * 64 + lg * 16 + (st & 1) * 8;
+                    q0 = *reinterpret_cast<const float4*>(qr + d0);
+                    q1 = *reinterpret_cast<const float4*>(qr + d0 + (ES == 4 ? 16 : 4));
+                }
+                uint32_t t[4][3];
+                split_pair<3>(q0.x * qs, q0.y * qs, t[0]);
+                split_pair<3>(q0.z * qs, q0.w * qs, t[1]);
+                split_pair<3>(q1.x * qs, q1.y * qs, t[2]);
+                split_pair<3>(q1.z * qs, q1.w * qs, t[3]);
 #pragma unroll
-            for (int k = 0; k < 3; k++)
-                reinterpret_cast<uint4*>(buf)[(st * 3 + k) * 64 + l] = make_uint4(t[0][k], t[1][k], t[2][k], t[3][k]);
-        }
-        lds_sync();
+                for (int k = 0; k < 3; k++)
+                    reinterpret_cast<uint4*>(buf)[(st * 3 + k) * 64 + l] = make_uint4(t[0][k], t[1][k], t[2][k], t[3][k]);
+            }
+            lds_sync();
 
-        // ---- the wave's tiles ----
-        f4_t o[NTILE] = {};
-        float m = -INFINITY, l = 0.0f;
+            // ---- the wave's tiles ----
+            f4_t o[NTILE] = {};
+            float m = -INFINITY, l = 0.0f;
             for (; tile < tile1; tile += 4) {
                 // past the last tile the loads have no bytes to read
                 pages(tile + 4, tile + 4 < tile1, npg);
@@ -488,73 +489,73 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
                 }
             }
 
-        // ---- the four waves' sums: 2, 3 -> 0, 1 -> 0 ----
-        l += shfl_xor(l, 16);
-        l += shfl_xor(l, 32);
-        if (bad) l = __uint_as_float(0x7fc00000u);
-        float top = m, sum = l;
-        const bool alone = tile1 - tile0 == 1;   // wave 0 had the only tile
-        f4_t* box = reinterpret_cast<f4_t*>(buf) + (wave & 1) * NTILE * 64 + lane;
-        if (!alone) {
-            if (g == 0) {
-                mls[0][wave][col] = m;
-                mls[1][wave][col] = l;
-            }
-            lds_sync();   // q is no longer needed
-            float mine = 0.0f;
-            top = -INFINITY;
-            sum = 0.0f;
+            // ---- the four waves' sums: 2, 3 -> 0, 1 -> 0 ----
+            l += shfl_xor(l, 16);
+            l += shfl_xor(l, 32);
+            if (bad) l = __uint_as_float(0x7fc00000u);
+            float top = m, sum = l;
+            const bool alone = tile1 - tile0 == 1;   // wave 0 had the only tile
+            f4_t* box = reinterpret_cast<f4_t*>(buf) + (wave & 1) * NTILE * 64 + lane;
+            if (!alone) {
+                if (g == 0) {
+                    mls[0][wave][col] = m;
+                    mls[1][wave][col] = l;
+                }
+                lds_sync();   // q is no longer needed
+                float mine = 0.0f;
+                top = -INFINITY;
+                sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) top = fmaxf(top, mls[0][i][col]);
+                for (int i = 0; i < 4; i++) top = fmaxf(top, mls[0][i][col]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float mi = mls[0][i][col], f = mi == top ? 1.0f : exp2f(mi - top);
-                sum += f * mls[1][i][col];
-                if (i == wave) mine = f;
-            }
+                for (int i = 0; i < 4; i++) {
+                    const float mi = mls[0][i][col], f = mi == top ? 1.0f : exp2f(mi - top);
+                    sum += f * mls[1][i][col];
+                    if (i == wave) mine = f;
+                }
 #pragma unroll
-            for (int i = 0; i < NTILE; i++) o[i] *= mine;
-            if (wave >= 2) {
-#pragma unroll
-                for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
-            }
-            lds_sync();
-            if (wave < 2) {
-#pragma unroll
-                for (int i = 0; i < NTILE; i++) o[i] += box[i * 64];
-                if (wave == 1) {
+                for (int i = 0; i < NTILE; i++) o[i] *= mine;
+                if (wave >= 2) {
 #pragma unroll
                     for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
                 }
-            }
-            lds_sync();
-            if (wave == 0) {
+                lds_sync();
+                if (wave < 2) {
 #pragma unroll
-                for (int i = 0; i < NTILE; i++) o[i] += box[(NTILE + i) * 64];
-            }
-        }
-        if (wave == 0 && col < nh) {
-            const bool whole = tile0 == 0 && tile1 == tiles;
-            float* to;
-            float f = 1.0f;
-            if (whole) {
-                to = a.out + (size_t)s * a.out_stride + (size_t)(head0 + col) * HD;
-                f = 1.0f / sum;
-            } else {
-                float* slot = a.part + ((size_t)w * 2 + (tile0 == 0)) * part_floats(a.group, HD);
-                to = slot + col * HD;
-                if (g == 0) {
-                    slot += (a.group < kHeadsWG ? a.group : kHeadsWG) * HD;
-                    slot[2 * col] = top;
-                    slot[2 * col + 1] = sum;
+                    for (int i = 0; i < NTILE; i++) o[i] += box[i * 64];
+                    if (wave == 1) {
+#pragma unroll
+                        for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
+                    }
+                }
+                lds_sync();
+                if (wave == 0) {
+#pragma unroll
+                    for (int i = 0; i < NTILE; i++) o[i] += box[(NTILE + i) * 64];
                 }
             }
+            if (wave == 0 && col < nh) {
+                const bool whole = tile0 == 0 && tile1 == tiles;
+                float* to;
+                float f = 1.0f;
+                if (whole) {
+                    to = a.out + (size_t)s * a.out_stride + (size_t)(head0 + col) * HD;
+                    f = 1.0f / sum;
+                } else {
+                    float* slot = a.part + ((size_t)w * 2 + (tile0 == 0)) * part_floats(a.group, HD);
+                    to = slot + col * HD;
+                    if (g == 0) {
+                        slot += (a.group < kHeadsWG ? a.group : kHeadsWG) * HD;
+                        slot[2 * col] = top;
+                        slot[2 * col + 1] = sum;
+                    }
+                }
 #pragma unroll
-            for (int i = 0; i < NTILE; i++) {
-                const f4_t r = o[i] * f;
-                *reinterpret_cast<f4_t*>(to + i * 16 + g * 4) = r;
+                for (int i = 0; i < NTILE; i++) {
+                    const f4_t r = o[i] * f;
+                    *reinterpret_cast<f4_t*>(to + i * 16 + g * 4) = r;
+                }
             }
-        }
             lds_sync();   // the sums' place takes q again
         }
         cur += (unsigned)(unit1 - unit);
@@ -674,7 +675,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
 
 template <int TYPE, int HD>
 void launch_paged(const PagedArgs& a) {
-    constexpr int NL = HD * CacheType<TYPE>::ES / 16, R = 4, D = NL < R ? NL : R;
+    constexpr int ES = CacheType<TYPE>::ES, NL = HD * ES / 16, R = ES == 2 ? 4 : 8, D = NL < R ? NL : R;
     if (a.whole) {
         hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D>), dim3(a.n_seqs * a.p.n_kv * a.ngrp), dim3(256), 0, g4_stream(), a);
         return;
