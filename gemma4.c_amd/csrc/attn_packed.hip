@@ -19,6 +19,8 @@
 #include <float.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "g4_kvpage.h"
 #include "g4_tile.h"
 
@@ -1214,13 +1216,20 @@ int launch_packed(PackedArgs a) {
         hipLaunchKernelGGL((attn_packed_few_kernel<T, HD>), dim3(a.m, a.n_heads), dim3(256), 0, g4_stream(), a);
         return g4_check_launch("attn_packed_few_kernel");
     }
-    // more than 64 KB of LDS has to be asked for, once on each device
+    // a sequence of n rows has ceil(ceil(n / 32) group / NJ) units, at most
+    // n group / (32 NJ) + extra
+    a.extra = (31 * a.group + 32 * (P::NJ - 1) + 32 * P::NJ - 1) / (32 * P::NJ);
+    const size_t units = (((size_t)a.m * a.group) >> P::LGROWS) + (size_t)a.extra * a.n_seqs;
     constexpr bool kWide = T == G4_F32 && HD == 512;
     constexpr int kLds = kWide ? Wide::LDS : P::LDS, kThreads = 64 * P::NW;
+    G4_CHECK_ARG(kv_grid_fits(units * a.n_kv, kThreads) && kv_grid_fits((size_t)a.m / 32 + a.n_seqs, 256),
+                 "g4_attn_prompt_packed: %d rows of %d sequences, %d heads: more than one launch takes", a.m, a.n_seqs,
+                 a.n_heads);
     void (*kernel)(PackedArgs);
     if constexpr (kWide) kernel = attn_packed_wide_kernel;
     else kernel = attn_packed_kernel<T, HD>;
-    static unsigned long long asked = 0;
+    // more than 64 KB of LDS has to be asked for, once on each device
+    static std::atomic<unsigned long long> asked{0};
     int dev = 0;
     G4_HIP(hipGetDevice(&dev));
     if (dev >= 64 || !(asked >> dev & 1)) {
@@ -1228,10 +1237,6 @@ int launch_packed(PackedArgs a) {
         if (dev < 64) asked |= 1ull << dev;
     }
     hipLaunchKernelGGL((packed_layout_kernel<T, HD>), dim3(a.m / 32 + a.n_seqs, a.n_kv, 2), dim3(256), 0, g4_stream(), a);
-    // a sequence of n rows has ceil(ceil(n / 32) group / NJ) units, at most
-    // n group / (32 NJ) + extra
-    a.extra = (31 * a.group + 32 * (P::NJ - 1) + 32 * P::NJ - 1) / (32 * P::NJ);
-    const size_t units = (((size_t)a.m * a.group) >> P::LGROWS) + (size_t)a.extra * a.n_seqs;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(units * a.n_kv)), dim3(kThreads), kLds, g4_stream(), a);
     return g4_check_launch("attn_packed_kernel");
 }

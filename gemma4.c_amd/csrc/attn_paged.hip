@@ -732,7 +732,7 @@ extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp
     // and 22.0.
     long most = (long)table_stride * page;
     if (window > 0 && window < most) most = window;
-    a.whole = most <= (type == G4_F32 ? 128 : 256);
+    a.whole = most <= (type == G4_F32 ? 128 : 256) && kv_grid_fits((size_t)n_seqs * n_kv * a.ngrp, 256);
     if (type == G4_F32) launch_paged<G4_F32>(a, hd);
     else if (type == G4_F16) launch_paged<G4_F16>(a, hd);
     else if (type == G4_BF16) launch_paged<G4_BF16>(a, hd);

@@ -110,6 +110,9 @@ __device__ __forceinline__ SeqAt find_seq(const int* __restrict__ cu, const int*
     return r;
 }
 
+// host: whether a launch may have that many workgroups
+inline bool kv_grid_fits(size_t wgs, int threads) { return wgs < ((size_t)1 << 32) / threads; }
+
 // host: the arguments every entry point of the cache checks alike
 int kv_pool_check(const char* who, KvPool* o, const void* kp, const void* vp, int type, int n_pages, int page, int n_kv,
                   int hd, const int* table, int table_stride);

@@ -284,6 +284,7 @@ int page_rows(const char* who, RowArgs& a, const void* kp, const void* vp, int t
                  "%s: kv_stride %d (a multiple of 4, n_kv * hd at least)", who, a.kv_stride);
     G4_CHECK_ARG(a.n_seqs > 0 && a.n_seqs <= kKvMaxSeqs && a.m > 0, "%s: %d rows of %d sequences (1 to %d)", who, a.m,
                  a.n_seqs, kKvMaxSeqs);
+    G4_CHECK_ARG(kv_grid_fits((size_t)a.m / 16 + 2 * a.n_seqs, 256), "%s: %d rows: more than one launch takes", who, a.m);
     if (type == G4_F32) launch_rows<G4_F32>(a, hd, store);
     else if (type == G4_F16) launch_rows<G4_F16>(a, hd, store);
     else if (type == G4_BF16) launch_rows<G4_BF16>(a, hd, store);

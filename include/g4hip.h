@@ -411,12 +411,13 @@ int g4_softmax(float *x, int n);
  *     rint(x / d) (codes 0 if d is 0), read back as code * d; a head that holds
  *     an infinity or NaN reads back as NaN.
  * table (device): table[s * table_stride + i] is the page of positions
- * i * page .. of sequence s (2^30 positions at most).  Entries that no position in use needs are not
- * read.  Pages are never looked at past a sequence's length, so what is left
- * there by others (infinities, NaN) does not matter.
+ * i * page .. of sequence s (2^30 positions at most).  Entries that no position
+ * in use needs are not read.  Pages are never looked at past a sequence's
+ * length, so what is left there by others (infinities, NaN) does not matter.
  * Packed rows: sequence s has rows cu[s] .. cu[s+1]-1 (cu: n_seqs + 1
  * ascending device ints, cu[n_seqs] <= m); m is the number of rows the
- * buffers hold.  Rows of no sequence are neither read nor written.
+ * buffers hold.  Rows of no sequence are neither read nor written.  More rows,
+ * sequences and heads than the 2^32 threads of a launch can take are refused.
  * ------------------------------------------------------------------------- */
 /* bytes of one pool; 0 if a size or the type is not one of the above */
 size_t g4_kv_pool_bytes(int type, int n_pages, int page, int n_kv, int hd);
@@ -445,9 +446,10 @@ int g4_kv_page_load(const void *kp, const void *vp, int type, int n_pages, int p
  * the cache holds are exact, their sums fp32.  lens[s] = 0 gives zeros; a page
  * outside the pool or a length past the table gives NaN in that sequence's row.
  * Where what a head sees holds infinities or NaN, its output is what the
- * formula gives or NaN.  out may not overlap q.  part: g4_attn_decode_paged_part_bytes() bytes that no
- * call running at the same time uses (its contents need not be kept).  q, out,
- * part 16-byte aligned, strides multiples of 4. */
+ * formula gives or NaN.  out may not overlap q.  part:
+ * g4_attn_decode_paged_part_bytes() bytes that no call running at the same time
+ * uses (its contents need not be kept).  q, out, part 16-byte aligned, strides
+ * multiples of 4. */
 size_t g4_attn_decode_paged_part_bytes(int n_heads, int n_kv, int hd);
 int g4_attn_decode_paged(const float *q, int q_stride, const void *kp, const void *vp, int type, int n_pages, int page,
                          int n_kv, int hd, const int *table, int table_stride, const int *lens, int n_seqs, int window,

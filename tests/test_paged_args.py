@@ -113,3 +113,20 @@ def test_prompt_type():
         assert prompt_call(type=t) == g4.G4_ERR_TYPE
     assert L.g4_attn_prompt_packed_work_bytes(g4.KV_Q8, 3, 10, 2, 256) == 0
     assert L.g4_attn_prompt_packed_work_bytes(g4.BF16, 3, 10, 2, 256) > 0
+
+
+@pytest.mark.parametrize("fn", ["g4_kv_page_store", "g4_kv_page_load"])
+@pytest.mark.parametrize("m", [(1 << 28), (1 << 31) - 1])
+def test_rows_past_a_launch(fn, m):
+    # a workgroup of 256 threads for every 16 rows: 2^32 threads
+    assert rows_call(fn, m=m) == g4.G4_ERR_ARG
+    assert fn in msg() and "launch" in msg()
+
+
+@pytest.mark.parametrize("kw", [dict(m=(1 << 31) - 1), dict(m=1 << 30, type=g4.F16),
+                                dict(n=4096, heads=65535, n_kv=65535, hd=64, qs=65535 * 64, ks=65535 * 64, os=65535 * 64),
+                                dict(m=1 << 20, heads=65535, n_kv=1, hd=64, qs=65535 * 64, ks=64, os=65535 * 64, type=g4.BF16)],
+                         ids=str)
+def test_prompt_past_a_launch(kw):
+    assert prompt_call(**kw) == g4.G4_ERR_ARG
+    assert "g4_attn_prompt_packed" in msg() and "launch" in msg()
