@@ -85,8 +85,9 @@ constexpr int kLowV = 51;    // sums of 2^-e stay in range
 
 // ---- first launch: K and V into blocks -----------------------------------------
 // blockIdx: block, kv head, K or V.  Sequence s has the blocks (cu[s] >> 5) + s
-// and on.  Bytes and latency: 8191 rows of 2 x 256 in bf16 10 us (3.3 TB/s read
-// and written), 7022 of 2 x 512 in fp32 29 us (4.0).
+// and on.  Bytes and latency (the starts, the rows, the stores are a chain):
+// 8191 rows of 2 x 256 in bf16 9.4 us (3.6 TB/s read and written), 7022 of 2 x
+// 512 in fp32 26 us (4.4).
 template <int T, int HD>
 __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
     typedef typename Kind<T>::t E;
@@ -105,18 +106,22 @@ __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
     const bool is_v = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int sub = lane / LPR, col = lane % LPR;
+    // V: a thread has G keys next to each other, which it writes at once (one at
+    // a time: 9.9 and 27.5 us)
+    constexpr int G = PASS < 4 ? PASS : 4;
+    auto key = [&](int i) { return is_v ? (wave * RPW + sub) * PASS + i : (i * 4 + wave) * RPW + sub; };
     // LDS slot of lane l's 16 bytes of a piece: the lanes of a row write to
     // one slot of many pieces (K) or to every 4th or 8th slot (V), all on the
     // same banks without the exchange
     auto swz = [&](int piece, int l) {
-        return piece * 64 + (is_v ? l ^ (l >> 3 & 3) ^ (piece >> 1 & 1) << 2 : l ^ ((piece * 2 + (l >> 5)) & 7));
+        return piece * 64 + (is_v ? l ^ (l >> 3 & 3) ^ (piece >> 1 & 1) ^ (piece & 4) : l ^ ((piece * 2 + (l >> 5)) & 7));
     };
     const E* src = (const E*)(is_v ? a.v : a.k) + (size_t)blockIdx.y * HD;
     if (tid == 0) marks = 0;
     uint4 x[PASS][VPL];
 #pragma unroll
     for (int i = 0; i < PASS; i++) {
-        const int t = (i * 4 + wave) * RPW + sub;
+        const int t = key(i);
         const size_t r = row0 + (t < rows ? t : 0);
 #pragma unroll
         for (int k = 0; k < VPL; k++)
@@ -129,7 +134,7 @@ __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
     float sc[PASS];
 #pragma unroll
     for (int i = 0; i < PASS; i++) {
-        const int t = (i * 4 + wave) * RPW + sub;
+        const int t = key(i);
         // the row's largest magnitude, as integers: infinities and NaN come last
         unsigned top = 0;
 #pragma unroll
@@ -169,42 +174,57 @@ __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
             }
         }
     }
+    // VW halves (hi or lo) of a thread's row i, dims c ..
+    auto halves = [&](int i, int k, int half, uint16_t (&e)[VW]) {
+        const unsigned w[4] = {x[i][k].x, x[i][k].y, x[i][k].z, x[i][k].w};
+        if constexpr (T == G4_F32) {
+#pragma unroll
+            for (int j = 0; j < VW; j += 2) {
+                h2v_t hi, lo;
+                split2(__uint_as_float(w[j]), __uint_as_float(w[j + 1]), sc[i], hi, lo);
+                const unsigned y = __builtin_bit_cast(unsigned, half ? lo : hi);
+                e[j] = (uint16_t)y;
+                e[j + 1] = (uint16_t)(y >> 16);
+            }
+        } else {
+            __builtin_memcpy(e, w, 16);
+        }
+    };
 #pragma unroll
     for (int half = 0; half < NS; half++) {
         if (half) lds_sync();   // the first half has been read
+        if (is_v) {
 #pragma unroll
-        for (int i = 0; i < PASS; i++) {
-            const int t = (i * 4 + wave) * RPW + sub;
+            for (int i = 0; i < PASS; i += G)
 #pragma unroll
-            for (int k = 0; k < VPL; k++) {
-                const int c = (k * LPR + col) * VW;
-                uint16_t e[VW];
-                const unsigned w[4] = {x[i][k].x, x[i][k].y, x[i][k].z, x[i][k].w};
-                if constexpr (T == G4_F32) {
+                for (int k = 0; k < VPL; k++) {
+                    uint16_t e[G][VW];
 #pragma unroll
-                    for (int j = 0; j < VW; j += 2) {
-                        h2v_t hi, lo;
-                        split2(__uint_as_float(w[j]), __uint_as_float(w[j + 1]), sc[i], hi, lo);
-                        const unsigned y = __builtin_bit_cast(unsigned, half ? lo : hi);
-                        e[j] = (uint16_t)y;
-                        e[j + 1] = (uint16_t)(y >> 16);
-                    }
-                } else {
-                    __builtin_memcpy(e, w, 16);
-                }
-                if (is_v) {
-                    // key t = 16 u + 8 b + 4 h + i
+                    for (int r = 0; r < G; r++) halves(i + r, k, half, e[r]);
+                    // key t = 16 u + 8 b + 4 h + r
+                    const int t = key(i), c = (k * LPR + col) * VW;
                     const int u = t >> 4, h = t >> 2 & 1, slot = (t >> 3 & 1) * 4 + (t & 3);
 #pragma unroll
                     for (int j = 0; j < VW; j++) {
                         const int d = c + j;
-                        *reinterpret_cast<uint16_t*>(img + swz((d >> 5) * 2 + u, h * 32 + (d & 31)) * 16 + slot * 2) = e[j];
+                        uint16_t y[G];
+#pragma unroll
+                        for (int r = 0; r < G; r++) y[r] = e[r][j];
+                        __builtin_memcpy(__builtin_assume_aligned(img + swz((d >> 5) * 2 + u, h * 32 + (d & 31)) * 16 + slot * 2, G * 2),
+                                         y, G * 2);
                     }
-                } else {
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PASS; i++)
+#pragma unroll
+                for (int k = 0; k < VPL; k++) {
+                    const int t = key(i), c = (k * LPR + col) * VW;
+                    uint16_t e[VW];
+                    halves(i, k, half, e);
                     __builtin_memcpy(__builtin_assume_aligned(img + swz(c >> 4, (c >> 3 & 1) * 32 + t) * 16 + (c & 7) * 2, VW * 2), e,
                                      VW * 2);
                 }
-            }
         }
         lds_sync();
         for (int i = tid; i < 4 * HD; i += 256)
