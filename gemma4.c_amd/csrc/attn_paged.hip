@@ -221,10 +221,11 @@ __device__ __forceinline__ void mfma_terms(const b8_t (&a)[NT], const b8_t (&b)[
 // terms of a step come from LDS.  Bound by the cache's bytes where there are
 // many: 40 sequences of 2000 to 30000 keys, 8 q heads on 2 kv heads of 256,
 // bf16 150 us (5.4 TB/s; a plain read 6.25), fp32 5.4, codes 4.75; of 512, codes
-// 5.0, fp32 4.8.  DEPTH loads of 1 KB are in flight a wave, 4 for 16-bit caches
-// and 8 for the others: fp16 of 512, one sequence of 32768 keys, 34 us with 4
-// and 35 with 8; fp32 of 512 163 and 154, codes of 512 161 and 155, fp32 of 256
-// 145 and 144.  More costs registers and gives nothing (codes of 512, 16: 215).
+// 5.0, fp32 4.9.  DEPTH loads of 1 KB are in flight a wave: 8, which one
+// sequence of 200 keys out of HBM needs (bf16 of 256: 17 us with 4, 13 with 8,
+// 12 with 16; of 512: 25 and 20), or 4 where 16-bit caches of 512 are split
+// (fp16, one sequence of 32768 keys: 32 us with 4, 34 with 8).  More costs
+// registers: codes of 512, 48 sequences, 155 us with 8, 215 with 16.
 template <int TYPE, int HD, int DEPTH>
 __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
     constexpr int ES = CacheType<TYPE>::ES, NT = CacheType<TYPE>::NT;
@@ -234,7 +235,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
     constexpr int NL = 4 * KC, STEPS = HD / 32, NTILE = HD / 16, TPC = 4 / ES;   // TPC: 16-dim tiles of a V piece
     constexpr bool kKOnly = DEPTH <= 2 * KC;              // loads ahead of a tile's end are the next one's K
     static_assert(NL % DEPTH == 0, "ring");
-    constexpr int kQBytes = STEPS * 3 * 1024, kSumBytes = 2 * NTILE * 1024;
+    constexpr int kRounds = NTILE > 16 ? 2 : 1, NR = NTILE / kRounds, NW = NR / 4;   // tiles a round, a wave's of them
+    constexpr int kQBytes = STEPS * 3 * 1024, kSumBytes = 4 * NR * 1024;
     __shared__ __align__(16) uint8_t buf[kQBytes > kSumBytes ? kQBytes : kSumBytes];
     __shared__ unsigned long long red[6];
     __shared__ float mls[2][4][kHeadsWG];
@@ -244,9 +246,28 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
     const int rep = a.p.n_kv * a.ngrp;
     unsigned long long cur, end;
     int s, len, item, unit;
+    // an item's q, 8 dims of a step and head a thread, on its way while the
+    // pages are looked up where the registers allow it
+    constexpr int QN = (STEPS + 3) / 4;
+    constexpr bool kEarlyQ = HD < 512 || (ES == 2 && DEPTH <= 4);
+    float4 qx[QN][2];
+    auto load_q = [&]() {
+        const int kvh = item / a.ngrp, h0 = (item - kvh * a.ngrp) * kHeadsWG;
+        const int nh = a.group - h0 < kHeadsWG ? a.group - h0 : kHeadsWG;
+        const int h = kvh * a.group + h0 + (col < nh ? col : nh - 1);
+        const float* qr = a.q + (size_t)s * a.q_stride + (size_t)h * HD;
+#pragma unroll
+        for (int i = 0; i < QN; i++) {
+            const int st = STEPS % 4 ? (i * 4 + wave) % STEPS : i * 4 + wave;
+            const int d0 = ES == 4 ? st * 32 + g * 4 : ES == 2 ? st * 32 + g * 8 : (st >> 1) * 64 + g * 16 + (st & 1) * 8;
+            qx[i][0] = *reinterpret_cast<const float4*>(qr + d0);
+            qx[i][1] = *reinterpret_cast<const float4*>(qr + d0 + (ES == 4 ? 16 : 4));
+        }
+    };
     if (a.whole) {
         s = (int)(w / (unsigned)rep);
         item = (int)w - s * rep;
+        if (kEarlyQ) load_q();
         len = __builtin_amdgcn_readfirstlane(a.lens[s]);
         unit = 0;
         cur = 0;
@@ -263,6 +284,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
         const unsigned long long off = cur - ln.before * rep;   // unit within the sequence's items
         item = __builtin_amdgcn_readfirstlane((int)(off / per));
         unit = __builtin_amdgcn_readfirstlane((int)(off - (unsigned long long)item * per));
+        if (kEarlyQ) load_q();
     }
     int first_tile, tiles = seq_tiles(a, len, first_tile);
     if (a.whole && tiles == 0) {
@@ -325,16 +347,14 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
             for (int i = 0; i < DEPTH; i++) ring[i] = load(i, kr, vr);
 
             // ---- q, times scale log2(e), as three terms in the products' order ----
+            if (!kEarlyQ) load_q();
             const float qs = a.scale * kLog2e;
-            for (int x = tid; x < STEPS * 64; x += 256) {
-                const int st = x >> 6, l = x & 63, lg = l >> 4, lc = l & 15;
-                float4 q0 = make_float4(0, 0, 0, 0), q1 = q0;
-                if (lc < nh) {
-                    const float* qr = a.q + (size_t)s * a.q_stride + (size_t)(head0 + lc) * HD;
-                    const int d0 = ES == 4 ? st * 32 + lg * 4 : ES == 2 ? st * 32 + lg * 8 : (st >> 1) * 64 + lg * 16 + (st & 1) * 8;
-                    q0 = *reinterpret_cast<const float4*>(qr + d0);
-                    q1 = *reinterpret_cast<const float4*>(qr + d0 + (ES == 4 ? 16 : 4));
-                }
+#pragma unroll
+            for (int i = 0; i < QN; i++) {
+                const int st = i * 4 + wave;
+                if (st >= STEPS) continue;
+                float4 q0 = qx[i][0], q1 = qx[i][1];
+                if (col >= nh) q0 = q1 = make_float4(0, 0, 0, 0);
                 uint32_t t[4][3];
                 split_pair<3>(q0.x * qs, q0.y * qs, t[0]);
                 split_pair<3>(q0.z * qs, q0.w * qs, t[1]);
@@ -342,7 +362,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
                 split_pair<3>(q1.z * qs, q1.w * qs, t[3]);
 #pragma unroll
                 for (int k = 0; k < 3; k++)
-                    reinterpret_cast<uint4*>(buf)[(st * 3 + k) * 64 + l] = make_uint4(t[0][k], t[1][k], t[2][k], t[3][k]);
+                    reinterpret_cast<uint4*>(buf)[(st * 3 + k) * 64 + lane] = make_uint4(t[0][k], t[1][k], t[2][k], t[3][k]);
             }
             lds_sync();
 
@@ -489,71 +509,60 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
                 }
             }
 
-            // ---- the four waves' sums: 2, 3 -> 0, 1 -> 0 ----
+            // ---- the four waves' sums, a quarter of the dims by each (one wave after
+            // another: bf16 of 256, one sequence of 203 keys, 8.7 -> 8.0 us with q's part) ----
             l += shfl_xor(l, 16);
             l += shfl_xor(l, 32);
             if (bad) l = __uint_as_float(0x7fc00000u);
-            float top = m, sum = l;
-            const bool alone = tile1 - tile0 == 1;   // wave 0 had the only tile
-            f4_t* box = reinterpret_cast<f4_t*>(buf) + (wave & 1) * NTILE * 64 + lane;
-            if (!alone) {
+            const bool whole = tile0 == 0 && tile1 == tiles;
+            float* slot = a.part + ((size_t)w * 2 + (tile0 == 0)) * part_floats(a.group, HD);
+            float* to = whole ? a.out + (size_t)s * a.out_stride + (size_t)(head0 + col) * HD : slot + col * HD;
+            float* stats = slot + (a.group < kHeadsWG ? a.group : kHeadsWG) * HD + 2 * col;
+            if (tile1 - tile0 == 1) {   // wave 0 had the only tile
+                if (wave == 0 && col < nh) {
+                    const float f = whole ? 1.0f / l : 1.0f;
+#pragma unroll
+                    for (int i = 0; i < NTILE; i++) {
+                        const f4_t r = o[i] * f;
+                        *reinterpret_cast<f4_t*>(to + i * 16 + g * 4) = r;
+                    }
+                    if (!whole && g == 0) *reinterpret_cast<float2*>(stats) = make_float2(m, l);
+                }
+            } else {
                 if (g == 0) {
                     mls[0][wave][col] = m;
                     mls[1][wave][col] = l;
                 }
                 lds_sync();   // q is no longer needed
-                float mine = 0.0f;
-                top = -INFINITY;
-                sum = 0.0f;
+                f4_t* box = reinterpret_cast<f4_t*>(buf) + lane;
+                float f[4], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) top = fmaxf(top, mls[0][i][col]);
+                for (int r = 0; r < kRounds; r++) {
+                    if (r) lds_sync();
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float mi = mls[0][i][col], f = mi == top ? 1.0f : exp2f(mi - top);
-                    sum += f * mls[1][i][col];
-                    if (i == wave) mine = f;
-                }
+                    for (int i = 0; i < NR; i++) box[(wave * NR + i) * 64] = o[r * NR + i];
+                    if (r == 0) {
 #pragma unroll
-                for (int i = 0; i < NTILE; i++) o[i] *= mine;
-                if (wave >= 2) {
+                        for (int i = 0; i < 4; i++) top = fmaxf(top, f[i] = mls[0][i][col]);
 #pragma unroll
-                    for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
-                }
-                lds_sync();
-                if (wave < 2) {
+                        for (int i = 0; i < 4; i++) {
+                            f[i] = f[i] == top ? 1.0f : exp2f(f[i] - top);
+                            sum += f[i] * mls[1][i][col];
+                        }
+                        if (!whole && wave == 0 && g == 0 && col < nh) *reinterpret_cast<float2*>(stats) = make_float2(top, sum);
+                        const float x = whole ? 1.0f / sum : 1.0f;
 #pragma unroll
-                    for (int i = 0; i < NTILE; i++) o[i] += box[i * 64];
-                    if (wave == 1) {
-#pragma unroll
-                        for (int i = 0; i < NTILE; i++) box[i * 64] = o[i];
+                        for (int i = 0; i < 4; i++) f[i] *= x;
                     }
-                }
-                lds_sync();
-                if (wave == 0) {
+                    lds_sync();
 #pragma unroll
-                    for (int i = 0; i < NTILE; i++) o[i] += box[(NTILE + i) * 64];
-                }
-            }
-            if (wave == 0 && col < nh) {
-                const bool whole = tile0 == 0 && tile1 == tiles;
-                float* to;
-                float f = 1.0f;
-                if (whole) {
-                    to = a.out + (size_t)s * a.out_stride + (size_t)(head0 + col) * HD;
-                    f = 1.0f / sum;
-                } else {
-                    float* slot = a.part + ((size_t)w * 2 + (tile0 == 0)) * part_floats(a.group, HD);
-                    to = slot + col * HD;
-                    if (g == 0) {
-                        slot += (a.group < kHeadsWG ? a.group : kHeadsWG) * HD;
-                        slot[2 * col] = top;
-                        slot[2 * col + 1] = sum;
+                    for (int i = 0; i < NW; i++) {
+                        const int t = wave * NW + i;
+                        f4_t y = box[t * 64] * f[0];
+#pragma unroll
+                        for (int k = 1; k < 4; k++) y += box[(k * NR + t) * 64] * f[k];
+                        if (col < nh) *reinterpret_cast<f4_t*>(to + (r * NR + t) * 16 + g * 4) = y;
                     }
-                }
-#pragma unroll
-                for (int i = 0; i < NTILE; i++) {
-                    const f4_t r = o[i] * f;
-                    *reinterpret_cast<f4_t*>(to + i * 16 + g * 4) = r;
                 }
             }
             lds_sync();   // the sums' place takes q again
@@ -568,6 +577,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
                 tiles = seq_tiles(a, len, first_tile);
             } while (tiles == 0);
         }
+        if (kEarlyQ) load_q();
     }
 }
 
@@ -675,9 +685,9 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
 
 template <int TYPE, int HD>
 void launch_paged(const PagedArgs& a) {
-    constexpr int ES = CacheType<TYPE>::ES, NL = HD * ES / 16, R = ES == 2 ? 4 : 8, D = NL < R ? NL : R;
+    constexpr int ES = CacheType<TYPE>::ES, NL = HD * ES / 16, W = NL < 8 ? NL : 8, D = ES == 2 && HD == 512 ? 4 : W;
     if (a.whole) {
-        hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D>), dim3(a.n_seqs * a.p.n_kv * a.ngrp), dim3(256), 0, g4_stream(), a);
+        hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, W>), dim3(a.n_seqs * a.p.n_kv * a.ngrp), dim3(256), 0, g4_stream(), a);
         return;
     }
     hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D>), dim3(kPagedWG), dim3(256), 0, g4_stream(), a);
