@@ -234,18 +234,22 @@ __global__ __launch_bounds__(256) void packed_layout_kernel(PackedArgs a) {
 }
 
 // ---- few rows: one launch, fp32 throughout --------------------------------------
-// A workgroup a row and head, a wave a key at a time: a hundredth of the
-// products' rate, without the latency of a second launch and of tiles.  Taken
-// where rows x keys x heads cannot pass 2^18 however the rows fall into
+// A workgroup a row and head, a wave a few keys at a time (one: 64 rows of 256
+// 6.4 us against 5.2; four q heads of a kv head together, 7.9): a hundredth of
+// the products' rate, without the latency of a second launch and of tiles.
+// Taken where rows x keys x heads cannot pass 2^18 however the rows fall into
 // sequences.  One sequence, 8 heads, fp32 / bf16, this against the other: 128
-// rows of 256 14.0 / 15.4 against 27.1 / 18.8 us, 192 rows 21.7 / 23.5 against
-// 32.4 / 20.3, 256 rows 42.7 / 47.2 against 36.6 / 21.9; 128 rows of 512 18.8 /
-// 19.9 against 38.6 / 27.0.
+// rows of 256 12.3 / 13.3 against 24.2 / 15.0 us, 192 rows 18.2 / 19.4 against
+// 28.7 / 16.6, 256 rows 38 / 42 against 33 / 18.7; 128 rows of 512 20.6 / 16.0
+// against 30.3 / 20.9.
 constexpr double kFewPairs = 1 << 18;
 template <int T, int HD>
 __global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedArgs a) {
     typedef typename Kind<T>::t E;
-    constexpr int N = HD / 64;
+    constexpr int N = HD / 64, KB = N * sizeof(E) <= 16 ? 4 : 2;   // a lane's dims; keys at a time
+    struct alignas(N * sizeof(E) < 16 ? N * sizeof(E) : 16) Dims {
+        E x[N];
+    };
     const int row = blockIdx.x, h = blockIdx.y, kvh = h / a.group;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __shared__ float red[4][HD + 2];
@@ -253,28 +257,46 @@ __global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedArgs a) {
     const int r0 = sq.r0, r1 = sq.r1;
     if (r0 < 0 || r1 > a.m || row < r0 || row >= r1) return;
     const int first = a.window > 0 && row - r0 >= a.window ? row + 1 - a.window : r0;
-    const E* K = (const E*)a.k + (size_t)kvh * HD;
-    const E* V = (const E*)a.v + (size_t)kvh * HD;
+    auto dims = [&](const void* x, int stride, int r, int head) {
+        return reinterpret_cast<const Dims*>((const E*)x + (size_t)r * stride + (size_t)head * HD)[lane];
+    };
+    const Dims qx = dims(a.q, a.q_stride, row, h);
     float q[N], o[N] = {}, m = -FLT_MAX, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; i++)
-        q[i] = (float)((const E*)a.q)[(size_t)row * a.q_stride + (size_t)h * HD + i * 64 + lane] * (a.scale * kLog2e);
-    for (int t = first + wave; t <= row; t += 4) {
-        float x = 0.0f, v[N];
+    for (int i = 0; i < N; i++) q[i] = (float)qx.x[i] * (a.scale * kLog2e);
+    for (int t0 = first + wave * KB; t0 <= row; t0 += 4 * KB) {
+        Dims k[KB], v[KB];
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            x = __builtin_fmaf(q[i], (float)K[(size_t)t * a.kv_stride + i * 64 + lane], x);
-            v[i] = (float)V[(size_t)t * a.kv_stride + i * 64 + lane];
+        for (int j = 0; j < KB; j++) {
+            const int t = t0 + j <= row ? t0 + j : row;
+            k[j] = dims(a.k, a.kv_stride, t, kvh);
+            v[j] = dims(a.v, a.kv_stride, t, kvh);
         }
-        x = wave_sum(x);
-        const float mn = fmaxf(m, x), f = exp2f(m - mn), w = exp2f(x - mn);
-        l = l * f + w;
+        float x[KB], mn = m;
+#pragma unroll
+        for (int j = 0; j < KB; j++) {
+            x[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; i++) x[j] = __builtin_fmaf(q[i], (float)k[j].x[i], x[j]);
+            x[j] = wave_sum(x[j]);
+            if (t0 + j > row) x[j] = -INFINITY;
+            mn = fmaxf(mn, x[j]);
+        }
+        const float f = exp2f(m - mn);
+        l *= f;
         m = mn;
 #pragma unroll
-        for (int i = 0; i < N; i++) o[i] = __builtin_fmaf(w, v[i], o[i] * f);
+        for (int i = 0; i < N; i++) o[i] *= f;
+#pragma unroll
+        for (int j = 0; j < KB; j++) {
+            const float w = exp2f(x[j] - mn);
+            l += w;
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = __builtin_fmaf(w, (float)v[j].x[i], o[i]);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < N; i++) red[wave][i * 64 + lane] = o[i];
+    for (int i = 0; i < N; i++) red[wave][lane * N + i] = o[i];
     if (lane == 0) {
         red[wave][HD] = m;
         red[wave][HD + 1] = l;
