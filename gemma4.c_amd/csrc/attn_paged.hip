@@ -53,6 +53,22 @@ __device__ __forceinline__ int seq_units(const PagedArgs& a, int len) {
     return t ? t + a.lead : 0;
 }
 
+// inclusive prefix sums over a wave: within rows of 16 by lane moves (lane -
+// 1, 2, 4, 8, nothing from before the row), then the totals of the rows before
+template <int CTRL>
+__device__ __forceinline__ unsigned row_shr(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ unsigned wave_prefix(unsigned v) {
+    v += row_shr<0x111>(v);
+    v += row_shr<0x112>(v);
+    v += row_shr<0x114>(v);
+    v += row_shr<0x118>(v);
+    auto at = [&](int l) { return (unsigned)__builtin_amdgcn_readlane((int)v, l); };
+    const unsigned a = at(15), b = a + at(31), c = b + at(47), row = (threadIdx.x & 63) >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
+}
+
 struct Line {
     unsigned long long total;   // N, all units
     unsigned long long before;  // units of one (kv head, heads) before sequence s
@@ -70,12 +86,7 @@ __device__ __forceinline__ Line find_line(const PagedArgs& a, At at, int of_seq,
     if (a.n_seqs <= 64) {
         const int len = lane < a.n_seqs ? a.lens[lane] : 0;
         const unsigned t = seq_units(a, len);   // 64 times 2^26 and less
-        unsigned x = t;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const unsigned o = __shfl_up(x, d, 64);
-            if (lane >= d) x += o;
-        }
+        const unsigned x = wave_prefix(t);
         Line r;
         r.total = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(x, 63) * rep;
         const unsigned long long u = at(r.total);
@@ -282,7 +293,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
         int f;
         const unsigned per = (unsigned)(seq_tiles(a, len, f) + a.lead);
         const unsigned long long off = cur - ln.before * rep;   // unit within the sequence's items
-        item = __builtin_amdgcn_readfirstlane((int)(off / per));
+        item = __builtin_amdgcn_readfirstlane(off >> 32 ? (int)(off / per) : (int)((unsigned)off / per));
         unit = __builtin_amdgcn_readfirstlane((int)(off - (unsigned long long)item * per));
         if (kEarlyQ) load_q();
     }
