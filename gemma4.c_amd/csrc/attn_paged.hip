@@ -744,16 +744,19 @@ extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp
     a.group = n_heads / n_kv;
     a.ngrp = (a.group + kHeadsWG - 1) / kHeadsWG;
     a.lead = n_seqs * n_kv * a.ngrp > 64 ? 3 : 0;
-    // Where a sequence cannot have more than 256 keys to look at (fp32: 128), by
-    // its table or the window, a workgroup takes an item whole and there is
-    // nothing to join: two rounds of the four waves cost less than the second
-    // launch.  bf16, head_dim 256, 2 kv heads, 1 / 64 / 200 sequences of 200
-    // keys: 8.4 / 11.2 / 17.6 us whole, 11.9 / 15.9 / 29.0 split; one of 500:
-    // 12.1 and 12.0; fp32 of 512, one of 64 keys 18.3 and 21.6, of 200 28.1
-    // and 22.0.
+    // Where a sequence cannot have more keys to look at than that, by its table
+    // or the window, a workgroup takes an item whole and there is nothing to
+    // join: some rounds of the four waves cost less than the second launch.
+    // head_dim 256, 2 kv heads, 1 / 64 / 200 sequences: bf16, 250 keys 7.7 / 8.7
+    // / 19.6 us whole, 11.2 / 15.0 / 30.5 split, 500 keys 11.1 / 16.9 / 37.5 and
+    // 11.5 / 19.7 / 43.8; codes, 500 keys 13.6 / 14.4 / 22.5 and 12.1 / 17.4 / 34.7;
+    // fp32, 250 keys 15.5 / 18.2 / 41.1 and 14.8 / 21.2 / 48.2, 380 keys 20.7 / 21.8
+    // / 53.7 and 15.0 / 27.2 / 65.8.  Of 512: bf16, 250 keys 12.4 and 13.9 (one),
+    // 380 keys 15.1 and 14.0; fp32, 120 keys 16.8 and 21.0, 250 keys 26.3 and 21.3.
     long most = (long)table_stride * page;
     if (window > 0 && window < most) most = window;
-    a.whole = most <= (type == G4_F32 ? 128 : 256) && kv_grid_fits((size_t)n_seqs * n_kv * a.ngrp, 256);
+    const int cap = type == G4_F32 ? 256 : 512, fit = (type == G4_F32 ? 65536 : 131072) / hd;
+    a.whole = most <= (fit < cap ? fit : cap) && kv_grid_fits((size_t)n_seqs * n_kv * a.ngrp, 256);
     if (type == G4_F32) launch_paged<G4_F32>(a, hd);
     else if (type == G4_F16) launch_paged<G4_F16>(a, hd);
     else if (type == G4_BF16) launch_paged<G4_BF16>(a, hd);

@@ -313,6 +313,28 @@ def test_decode_splits(lib):
         check_decode(lib, 79, pn.BF16, 64, 1, 1, 64, lens, window=0, gain=1.0)
 
 
+@pytest.mark.parametrize("kind,hd", [(pn.F32, 64), (pn.F32, 512), (pn.BF16, 256), (pn.BF16, 512), (pn.Q8, 128), (pn.Q8, 512)])
+def test_decode_whole_or_split(lib, kind, hd):
+    """tables and windows on either side of the keys up to which a workgroup takes a sequence whole"""
+    for most in (128, 256, 512):
+        check_decode(lib, 80, kind, hd, 8, 2, 16, [most - 33, most - 1, 1, 90])              # 16 or 32 entries past it
+        check_decode(lib, 81, kind, hd, 8, 2, 16, [most - 32, 0, 17], window=0)
+        for w in (most, most + 1):
+            check_decode(lib, 82, kind, hd, 8, 2, 32, [700, most, most + 1, 5], window=w)
+
+
+def test_decode_split_extremes(lib):
+    """what the tests of heads and of extremes see, beside a sequence too long to be taken whole"""
+    for kind in (pn.F32, pn.BF16, pn.Q8):
+        check_decode(lib, 83, kind, 128, 4, 2, 16, [50, 300, 900], gain=60.0, scale=1.0)
+        check_decode(lib, 84, kind, 128, 4, 2, 16, [50, 300, 900], gain=0.0, scale=1.0)
+        check_decode(lib, 85, kind, 128, 4, 2, 16, [50, 300, 900], scale=-0.09)
+    for n_heads, n_kv in ((1, 1), (12, 1), (17, 1), (40, 2)):
+        for kind, hd in ((pn.BF16, 128), (pn.Q8, 256)):
+            check_decode(lib, 86 + n_heads, kind, hd, n_heads, n_kv, 32, [5, 130, 900, 64, 1])
+            check_decode(lib, 87 + n_heads, kind, hd, n_heads, n_kv, 32, [5, 130, 900, 64, 1], window=600)
+
+
 def test_decode_strides(lib):
     """q and out rows wider than their heads"""
     check_decode(lib, 72, pn.F16, 256, 8, 2, 32, [40, 3, 77], extra=12)
