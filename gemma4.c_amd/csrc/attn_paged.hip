@@ -23,7 +23,7 @@ struct PagedArgs {
     int q_stride, out_stride, n_seqs, window, n_heads;
     int group, ngrp;   // q heads a kv head, workgroup columns' groups of them
     int lead;          // units in front of an item's tiles
-    int whole;         // a workgroup an item, nothing to join
+    int whole;         // 4, 8: a workgroup of so many waves an item, nothing to join; 0: split
     float scale;
 };
 
@@ -237,8 +237,9 @@ __device__ __forceinline__ void mfma_terms(const b8_t (&a)[NT], const b8_t (&b)[
 // 12 with 16; of 512: 25 and 20), or 4 where 16-bit caches of 512 are split
 // (fp16, one sequence of 32768 keys: 32 us with 4, 34 with 8).  More costs
 // registers: codes of 512, 48 sequences, 155 us with 8, 215 with 16.
-template <int TYPE, int HD, int DEPTH>
-__global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
+// WAVES 8: items taken whole, half the rounds
+template <int TYPE, int HD, int DEPTH, int WAVES>
+__global__ __launch_bounds__((64 * WAVES), 2) void attn_paged_kernel(PagedArgs a) {
     constexpr int ES = CacheType<TYPE>::ES, NT = CacheType<TYPE>::NT;
     constexpr int KC = HD * ES / 64;                      // 1 KB pieces of a 16-token block
     constexpr int CPS = ES == 4 ? 2 : 1;                  // pieces of a product step of 32 dims (ES 1: half a piece)
@@ -246,11 +247,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
     constexpr int NL = 4 * KC, STEPS = HD / 32, NTILE = HD / 16, TPC = 4 / ES;   // TPC: 16-dim tiles of a V piece
     constexpr bool kKOnly = DEPTH <= 2 * KC;              // loads ahead of a tile's end are the next one's K
     static_assert(NL % DEPTH == 0, "ring");
-    constexpr int kRounds = NTILE > 16 ? 2 : 1, NR = NTILE / kRounds, NW = NR / 4;   // tiles a round, a wave's of them
-    constexpr int kQBytes = STEPS * 3 * 1024, kSumBytes = 4 * NR * 1024;
+    constexpr int kRounds = NTILE > 16 ? 2 : 1, NR = NTILE / kRounds;            // rounds of joining NR dim tiles,
+    constexpr int NW = NR > WAVES ? NR / WAVES : 1;                              // NW of them a wave
+    constexpr int kQBytes = STEPS * 3 * 1024, kSumBytes = WAVES * NR * 1024;
     __shared__ __align__(16) uint8_t buf[kQBytes > kSumBytes ? kQBytes : kSumBytes];
     __shared__ unsigned long long red[6];
-    __shared__ float mls[2][4][kHeadsWG];
+    __shared__ float mls[2][WAVES][kHeadsWG];
+    const bool items = WAVES == 8 || a.whole;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned w = blockIdx.x;
@@ -259,7 +262,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
     int s, len, item, unit;
     // an item's q, 8 dims of a step and head a thread, on its way while the
     // pages are looked up where the registers allow it
-    constexpr int QN = (STEPS + 3) / 4;
+    constexpr int QN = (STEPS + WAVES - 1) / WAVES;
     constexpr bool kEarlyQ = HD < 512 || (ES == 2 && DEPTH <= 4);
     float4 qx[QN][2];
     auto load_q = [&]() {
@@ -269,13 +272,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
         const float* qr = a.q + (size_t)s * a.q_stride + (size_t)h * HD;
 #pragma unroll
         for (int i = 0; i < QN; i++) {
-            const int st = STEPS % 4 ? (i * 4 + wave) % STEPS : i * 4 + wave;
+            const int st = STEPS % WAVES ? (i * WAVES + wave) % STEPS : i * WAVES + wave;
             const int d0 = ES == 4 ? st * 32 + g * 4 : ES == 2 ? st * 32 + g * 8 : (st >> 1) * 64 + g * 16 + (st & 1) * 8;
             qx[i][0] = *reinterpret_cast<const float4*>(qr + d0);
             qx[i][1] = *reinterpret_cast<const float4*>(qr + d0 + (ES == 4 ? 16 : 4));
         }
     };
-    if (a.whole) {
+    if (items) {
         s = (int)(w / (unsigned)rep);
         item = (int)w - s * rep;
         if (kEarlyQ) load_q();
@@ -298,13 +301,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
         if (kEarlyQ) load_q();
     }
     int first_tile, tiles = seq_tiles(a, len, first_tile);
-    if (a.whole && tiles == 0) {
+    if (items && tiles == 0) {
         // no keys: zeros; a length that does not fit: NaN
         const float x = len == 0 ? 0.0f : __uint_as_float(0x7fc00000u);
         const int kvh = item / a.ngrp, hg = item - kvh * a.ngrp;
         const int nh = a.group - hg * kHeadsWG < kHeadsWG ? a.group - hg * kHeadsWG : kHeadsWG;
         float* to = a.out + (size_t)s * a.out_stride + (size_t)(kvh * a.group + hg * kHeadsWG) * HD;
-        for (int i = tid; i < nh * HD / 4; i += 256) reinterpret_cast<float4*>(to)[i] = make_float4(x, x, x, x);
+        for (int i = tid; i < nh * HD / 4; i += 64 * WAVES) reinterpret_cast<float4*>(to)[i] = make_float4(x, x, x, x);
         return;
     }
     while (true) {
@@ -362,7 +365,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
             const float qs = a.scale * kLog2e;
 #pragma unroll
             for (int i = 0; i < QN; i++) {
-                const int st = i * 4 + wave;
+                const int st = i * WAVES + wave;
                 if (st >= STEPS) continue;
                 float4 q0 = qx[i][0], q1 = qx[i][1];
                 if (col >= nh) q0 = q1 = make_float4(0, 0, 0, 0);
@@ -380,12 +383,12 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
             // ---- the wave's tiles ----
             f4_t o[NTILE] = {};
             float m = -INFINITY, l = 0.0f;
-            for (; tile < tile1; tile += 4) {
+            for (; tile < tile1; tile += WAVES) {
                 // past the last tile the loads have no bytes to read
-                pages(tile + 4, tile + 4 < tile1, npg);
+                pages(tile + WAVES, tile + WAVES < tile1, npg);
                 if (!kKOnly) {
-                    rsrc(a.p.kp, tile + 4, npg, kn);
-                    rsrc(a.p.vp, tile + 4, npg, vn);
+                    rsrc(a.p.kp, tile + WAVES, npg, kn);
+                    rsrc(a.p.vp, tile + WAVES, npg, vn);
                 }
                 float ksc[8], vsc[8];
                 if (TYPE == G4_KV_Q8) {
@@ -482,7 +485,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
                     const int key = pos + 16 * (i >> 2) + (i & 3);
                     keep[i] = key >= first && key < len ? 0xffffffffu : 0u;
                 }
-                if (kKOnly) rsrc(a.p.kp, tile + 4, npg, kn);
+                if (kKOnly) rsrc(a.p.kp, tile + WAVES, npg, kn);
 #pragma unroll
                 for (int c = 0; c < KC; c++) {
                     uint4 y[2];
@@ -511,7 +514,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if (kKOnly) rsrc(a.p.vp, tile + 4, npg, vn);
+                if (kKOnly) rsrc(a.p.vp, tile + WAVES, npg, vn);
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
                     kr[b] = kn[b];
@@ -520,8 +523,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
                 }
             }
 
-            // ---- the four waves' sums, a quarter of the dims by each (one wave after
-            // another: bf16 of 256, one sequence of 203 keys, 8.7 -> 8.0 us with q's part) ----
+            // ---- the waves' sums, a part of the dims by each (one wave after another,
+            // bf16 of 256, one sequence of 203 keys: 8.7 -> 8.0 us with q's loads ahead) ----
             l += shfl_xor(l, 16);
             l += shfl_xor(l, 32);
             if (bad) l = __uint_as_float(0x7fc00000u);
@@ -546,7 +549,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
                 }
                 lds_sync();   // q is no longer needed
                 f4_t* box = reinterpret_cast<f4_t*>(buf) + lane;
-                float f[4], top = -INFINITY, sum = 0.0f;
+                float f[WAVES], top = -INFINITY, sum = 0.0f;
 #pragma unroll
                 for (int r = 0; r < kRounds; r++) {
                     if (r) lds_sync();
@@ -554,24 +557,25 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
                     for (int i = 0; i < NR; i++) box[(wave * NR + i) * 64] = o[r * NR + i];
                     if (r == 0) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) top = fmaxf(top, f[i] = mls[0][i][col]);
+                        for (int i = 0; i < WAVES; i++) top = fmaxf(top, f[i] = mls[0][i][col]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
+                        for (int i = 0; i < WAVES; i++) {
                             f[i] = f[i] == top ? 1.0f : exp2f(f[i] - top);
                             sum += f[i] * mls[1][i][col];
                         }
                         if (!whole && wave == 0 && g == 0 && col < nh) *reinterpret_cast<float2*>(stats) = make_float2(top, sum);
                         const float x = whole ? 1.0f / sum : 1.0f;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) f[i] *= x;
+                        for (int i = 0; i < WAVES; i++) f[i] *= x;
                     }
                     lds_sync();
 #pragma unroll
                     for (int i = 0; i < NW; i++) {
                         const int t = wave * NW + i;
+                        if (t >= NR) break;
                         f4_t y = box[t * 64] * f[0];
 #pragma unroll
-                        for (int k = 1; k < 4; k++) y += box[(k * NR + t) * 64] * f[k];
+                        for (int k = 1; k < WAVES; k++) y += box[(k * NR + t) * 64] * f[k];
                         if (col < nh) *reinterpret_cast<f4_t*>(to + (r * NR + t) * 16 + g * 4) = y;
                     }
                 }
@@ -579,7 +583,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_kernel(PagedArgs a) {
             lds_sync();   // the sums' place takes q again
         }
         cur += (unsigned)(unit1 - unit);
-        if (a.whole || cur >= end) break;
+        if (items || cur >= end) break;
         unit = 0;
         if (++item == rep) {
             item = 0;
@@ -698,10 +702,14 @@ template <int TYPE, int HD>
 void launch_paged(const PagedArgs& a) {
     constexpr int ES = CacheType<TYPE>::ES, NL = HD * ES / 16, W = NL < 8 ? NL : 8, D = ES == 2 && HD == 512 ? 4 : W;
     if (a.whole) {
-        hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, W>), dim3(a.n_seqs * a.p.n_kv * a.ngrp), dim3(256), 0, g4_stream(), a);
+        const int items = a.n_seqs * a.p.n_kv * a.ngrp;
+        if (a.whole == 8)
+            hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, W, 8>), dim3(items), dim3(512), 0, g4_stream(), a);
+        else
+            hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, W, 4>), dim3(items), dim3(256), 0, g4_stream(), a);
         return;
     }
-    hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D>), dim3(kPagedWG), dim3(256), 0, g4_stream(), a);
+    hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D, 4>), dim3(kPagedWG), dim3(256), 0, g4_stream(), a);
     if (a.n_heads * a.n_seqs < 256)
         hipLaunchKernelGGL((attn_paged_join_kernel<HD, 64>), dim3(a.n_heads, a.n_seqs, HD / 64), dim3(256), 0, g4_stream(), a);
     else
@@ -746,17 +754,20 @@ extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp
     a.lead = n_seqs * n_kv * a.ngrp > 64 ? 3 : 0;
     // Where a sequence cannot have more keys to look at than that, by its table
     // or the window, a workgroup takes an item whole and there is nothing to
-    // join: some rounds of the four waves cost less than the second launch.
-    // head_dim 256, 2 kv heads, 1 / 64 / 200 sequences: bf16, 250 keys 7.7 / 8.7
-    // / 19.6 us whole, 11.2 / 15.0 / 30.5 split, 500 keys 11.1 / 16.9 / 37.5 and
-    // 11.5 / 19.7 / 43.8; codes, 500 keys 13.6 / 14.4 / 22.5 and 12.1 / 17.4 / 34.7;
-    // fp32, 250 keys 15.5 / 18.2 / 41.1 and 14.8 / 21.2 / 48.2, 380 keys 20.7 / 21.8
-    // / 53.7 and 15.0 / 27.2 / 65.8.  Of 512: bf16, 250 keys 12.4 and 13.9 (one),
-    // 380 keys 15.1 and 14.0; fp32, 120 keys 16.8 and 21.0, 250 keys 26.3 and 21.3.
+    // join: some rounds of its waves cost less than the second launch.
+    // head_dim 256, 2 kv heads, 1 / 64 / 200 sequences: bf16, 250 keys 6.8 / 7.8
+    // / 19.7 us whole, 11.2 / 15.0 / 30.5 split, 500 keys 9.1 / 18.4 / 37.5 and
+    // 11.5 / 19.7 / 43.8; codes, 500 keys 11.5 / 12.4 / 22.0 and 12.1 / 17.4 / 34.7;
+    // fp32, 250 keys 11.8 / 18.1 / 41 and 14.8 / 21.2 / 48.2.  Of 512: bf16, 250
+    // keys 10.5 and 13.9 (one); fp32, 120 keys 16.8 and 21.0, 250 keys with four
+    // waves 26.3 and 21.3.  Eight waves where each such workgroup has a CU and more
+    // than a round of four to do: against four, one sequence of 250 keys 6.8
+    // and 7.6 us in bf16, 11.8 and 15.5 in fp32; 64 of 500 keys 18.4 and 17.1.
     long most = (long)table_stride * page;
     if (window > 0 && window < most) most = window;
     const int cap = type == G4_F32 ? 256 : 512, fit = (type == G4_F32 ? 65536 : 131072) / hd;
-    a.whole = most <= (fit < cap ? fit : cap) && kv_grid_fits((size_t)n_seqs * n_kv * a.ngrp, 256);
+    const size_t items = (size_t)n_seqs * n_kv * a.ngrp;
+    a.whole = most > (fit < cap ? fit : cap) || !kv_grid_fits(items, 256) ? 0 : items <= 256 && most > 128 ? 8 : 4;
     if (type == G4_F32) launch_paged<G4_F32>(a, hd);
     else if (type == G4_F16) launch_paged<G4_F16>(a, hd);
     else if (type == G4_BF16) launch_paged<G4_BF16>(a, hd);
