@@ -335,8 +335,8 @@ __global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedArgs a) {
 // put it off to the next tile.  Their sums meet at the end, in LDS.  (8191 rows
 // in bf16, 8 heads of 256: 404 us with eight jobs a workgroup in step, 333 so.)
 // What bounds it: the matrix cores under the card's power limit.  Four prompts
-// of 4096 rows, 8 heads of 256 (128: 32): bf16 300-370 us from card to card,
-// 745-910 TFLOP/s at 2.0-2.1 GHz where an 8192^3 library product reaches 1182;
+// of 4096 rows, 8 heads of 256 (128: 32): bf16 293-370 us from card to card,
+// 745-940 TFLOP/s at 1.75-2.1 GHz where an 8192^3 library product reaches 1182;
 // fp32 815-900 us, 305-337 TFLOP/s and three times as many products.  Copies to
 // LDS alone (55 bytes/ns a CU) would take 155 and 305 us.  Three independent
 // sums instead of two, the next tile's scores computed beside this tile's
