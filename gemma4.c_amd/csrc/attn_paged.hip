@@ -228,8 +228,10 @@ __device__ __forceinline__ void mfma_terms(const b8_t (&a)[NT], const b8_t (&b)[
 // dims).  The cache's layout has each lane's K and V operands in 16
 // consecutive bytes, so keys and values go from memory to the products through
 // registers alone: no LDS, no barrier and no lane exchange but the one of the
-// running maximum, which moves only when a score passes it by 2^8.  The q
-// terms of a step come from LDS.  Bound by the cache's bytes where there are
+// running maximum m.  It is put 2^8 above the largest score and moves only when
+// one passes it, so that weights are at most 1 and their sums with V finite
+// wherever the keys times the largest V are.  The q terms of a step come from
+// LDS.  Bound by the cache's bytes where there are
 // many: 40 sequences of 2000 to 30000 keys, 8 q heads on 2 kv heads of 256,
 // bf16 150 us (5.4 TB/s; a plain read 6.25), fp32 5.4, codes 4.75; of 512, codes
 // 5.0, fp32 4.9.  DEPTH loads of 1 KB are in flight a wave: 8, which one
@@ -451,10 +453,10 @@ __global__ __launch_bounds__((64 * WAVES), 2) void attn_paged_kernel(PagedArgs a
                     x[i] = key >= first && key < len ? y : -INFINITY;
                     top = fmaxf(top, x[i]);
                 }
-                if (__any(top > m + 8.0f)) {
+                if (__any(top > m)) {
                     top = fmaxf(top, shfl_xor(top, 16));
                     top = fmaxf(top, shfl_xor(top, 32));
-                    top = fmaxf(top, m);
+                    top = fmaxf(top + 8.0f, m);
                     const float f = top == m ? 1.0f : exp2f(m - top);
                     m = top;
                     l *= f;

@@ -445,6 +445,8 @@ int g4_kv_page_load(const void *kp, const void *vp, int type, int n_pages, int p
  * whatever the cache's type: the products of q and of the weights with what
  * the cache holds are exact, their sums fp32.  lens[s] = 0 gives zeros; a page
  * outside the pool or a length past the table gives NaN in that sequence's row.
+ * Weights are summed before the division: |V| times the keys a row sees has to
+ * stay below fp32's largest number, scores (and q times attn_scale) as well.
  * Where what a head sees holds infinities or NaN, its output is what the
  * formula gives or NaN.  out may not overlap q.  part:
  * g4_attn_decode_paged_part_bytes() bytes that no call running at the same time
