@@ -353,8 +353,8 @@ __global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedArgs a) {
 // of a kv head (the heads of 32 rows, then the next 32 rows), which share its
 // tiles of 32 keys in LDS.  S^T = K Q^T (rows keys, columns q rows): a lane
 // holds 16 of a row's 32 scores, which are, as they stand, its operand of
-// O^T += V^T P^T.  The running maximum moves only when a score passes it by
-// 2^8 (fp32: 2^4).  DS 2 (head_dim 512, whose q and o would not fit a wave's
+// O^T += V^T P^T.  The running maximum moves only when a score passes it (bf16,
+// where it stands 2^8 above the largest; fp16, fp32: by 2^8, 2^4).  DS 2 (head_dim 512, whose q and o would not fit a wave's
 // registers): a job's dims are halved over two waves, whose partial scores
 // meet in LDS; K and V of a tile have one place each, and the next tile's K is
 // on its way while V is worked on, and the other way round.
@@ -576,7 +576,10 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
     constexpr int ES = P::ES, NS = Kind<T>::NS, NW = P::NW, DS = P::DS, NJ = P::NJ, KSP = P::KSP, TB = P::TB;
     constexpr int KS = HD / 16 / DS, NT = HD / 32 / DS;   // a wave's product steps and 32-dim tiles
     constexpr int kHalf = TB / 1024;                      // KB of a tile's K, of its V
-    constexpr float kSlack = T == G4_F32 ? 4.0f : 8.0f;
+    // how far a score may pass the maximum before it moves, and how far above the
+    // largest score it is put.  bf16, whose V goes as far as fp32: weights are at
+    // most 1; fp16's smallest numbers ask for large weights, and its V cannot overflow
+    constexpr float kSlack = T == G4_F32 ? 4.0f : T == G4_F16 ? 8.0f : 0.0f, kRaise = T == G4_BF16 ? 8.0f : 0.0f;
     constexpr float kLift = T == G4_F32 ? 11.0f : 0.0f;   // fp16 weights: 2^11 above their fp32 size
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
@@ -796,7 +799,7 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
         if constexpr (T != G4_F32) top *= fq;
         if (__any(top > m + kSlack)) {
             top = fmaxf(top, shfl_xor(top, 32));
-            top = fmaxf(top, m);
+            top = fmaxf(top + kRaise, m);
             const float f = exp2f(m - top);
             if constexpr (T == G4_F32) l = move_sum(l, m - top);
             else l *= f;

@@ -463,7 +463,8 @@ int g4_attn_decode_paged(const float *q, int q_stride, const void *kp, const voi
  * within 2^-22 of themselves or 2^-39 of their row's largest (a weight times its
  * V row: 2^-35 of the largest such product), fp32 sums; F16,
  * BF16: exact products, weights rounded to the type, fp32 sums (few rows: fp32
- * throughout).  Rows of out past cu[n_seqs] and those of sequences whose cu
+ * throughout); BF16 and few rows: |V| times the keys a row sees has to stay below
+ * fp32's largest number, with every type scores as well.  Rows of out past cu[n_seqs] and those of sequences whose cu
  * does not fit are left as they are.  Where what a row's head sees holds
  * infinities or NaN, its output is what the formula gives or NaN; what it does
  * not see never matters.  work:

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import paged_np as pn
-from test_gpu_paged import rows, run_prompt, within
+from test_gpu_paged import cast, rows, run_prompt, within
 
 pytestmark = pytest.mark.gpu
 
@@ -23,6 +23,14 @@ def lib():
 
 def in_tiles(m, window, heads):
     assert m * (min(m, window) if window else m) * heads > FEW
+
+
+def rounded(kind, want, bound, v):
+    """16 bits: the bound with weights and results rounded to the type, as the types' test derives it"""
+    if kind == pn.F32:
+        return bound
+    big = np.abs(v).max()
+    return bound + pn.HALF[kind] * (np.abs(want) + 1.01 * big) + 2.0 ** -25 * len(v) * big
 
 
 def fp32_bound(q, k, v, want_bound, first, scale):
@@ -79,3 +87,23 @@ def test_values_far_apart(lib, hd, top, big_first):
     v[rng.integers(0, t, 9)] = 0
     check_far(lib, hd, k, v, 3.0)
     check_far(lib, hd, np.concatenate([k] * 3), np.concatenate([v] * 3), 3.0, window=70)
+
+
+@pytest.mark.parametrize("hd", [64, 256, 512])
+def test_values_at_the_limit(lib, hd):
+    """bf16 V so large that the keys together stay just below fp32's largest number, under scores that rise by 2^7.9 from
+    one of a wave's tiles to the next"""
+    t, n_heads, n_kv, top = 400, 8, 2, 119
+    in_tiles(t, 0, n_heads)
+    assert t * 2.0 ** top < float(np.finfo(np.float32).max) < t * 2.0 ** (top + 1)
+    k = np.zeros((t, n_kv, hd), np.float32)
+    for i in range(t):
+        k[i, :, :i // 64] = 1
+    v = np.full((t, n_kv * hd), 2.0 ** top, np.float32)
+    v *= np.random.default_rng(580).choice(np.array([1, -1], np.float32), n_kv * hd)
+    q = np.zeros((t, n_heads, hd), np.float32)
+    q[:, :, :16] = 5.46875
+    _, got = run_prompt(lib, *(cast(x.reshape(t, -1), pn.BF16)[0] for x in (q, k, v)), pn.BF16, [0, t], t, 0, n_heads, n_kv, hd,
+                        1.0)
+    want, bound = pn.attention(q, k, v.reshape(t, n_kv, hd), [0] * t, 1.0)
+    within(np.abs(got.reshape(t, n_heads, hd) - want), rounded(pn.BF16, want, bound, v), hd)
