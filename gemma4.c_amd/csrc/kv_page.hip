@@ -302,7 +302,8 @@ extern "C" size_t g4_kv_pool_bytes(int type, int n_pages, int page, int n_kv, in
     if (!es || n_pages < 1 || page < 16 || page > kKvMaxPage || (page & (page - 1)) || n_kv < 1 || n_kv > 65535 ||
         (hd != 64 && hd != 128 && hd != 256 && hd != 512))
         return 0;
-    const size_t rows = (size_t)n_pages * page * n_kv;
+    const size_t rows = (size_t)n_pages * page * n_kv;   // below 2^59
+    if (rows > (SIZE_MAX >> 1) / ((size_t)hd * es + 4)) return 0;
     return rows * hd * es + (type == G4_KV_Q8 ? rows * 4 : 0);
 }
 

@@ -130,3 +130,18 @@ def test_rows_past_a_launch(fn, m):
 def test_prompt_past_a_launch(kw):
     assert prompt_call(**kw) == g4.G4_ERR_ARG
     assert "g4_attn_prompt_packed" in msg() and "launch" in msg()
+
+
+@pytest.mark.parametrize("pool", [(g4.F32, (1 << 31) - 1, 4096, 65535, 512), (g4.F32, 1 << 28, 4096, 8192, 512),
+                                  (g4.F32, 1 << 30, 4096, 4096, 512), (g4.KV_Q8, (1 << 31) - 1, 4096, 65535, 512),
+                                  (g4.BF16, 1 << 30, 4096, 4096, 512)], ids=str)
+def test_pools_past_an_address(pool):
+    """sizes that 64 bits do not hold are no pool, and not the size of what is left of them"""
+    assert pool[1] * pool[2] * pool[3] * pool[4] * (1 if pool[0] == g4.KV_Q8 else 2) >= 1 << 63
+    assert L.g4_kv_pool_bytes(*pool) == 0
+    kind, pages, page, n_kv, hd = pool
+    for fn in ("g4_kv_page_store", "g4_kv_page_load"):
+        assert rows_call(fn, type=kind, n_pages=pages, page=page, n_kv=n_kv, hd=hd, stride=1 << 30) == g4.G4_ERR_ARG
+        assert "bad pool" in msg()
+    assert decode_call(type=kind, n_pages=pages, page=page, n_kv=n_kv, hd=hd, heads=n_kv) == g4.G4_ERR_ARG
+    assert "bad pool" in msg()
