@@ -700,15 +700,26 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedArgs a) {
     }
 }
 
+// keys up to which a workgroup takes an item whole (figures: g4_attn_decode_paged),
+// and those of a round of four waves, past which it has eight
+constexpr int kRound = 128;
+constexpr int whole_keys(int type, int hd) {
+    const int cap = type == G4_F32 ? 256 : 512, fit = (type == G4_F32 ? 65536 : 131072) / hd;
+    return fit < cap ? fit : cap;
+}
+
 template <int TYPE, int HD>
 void launch_paged(const PagedArgs& a) {
     constexpr int ES = CacheType<TYPE>::ES, NL = HD * ES / 16, W = NL < 8 ? NL : 8, D = ES == 2 && HD == 512 ? 4 : W;
     if (a.whole) {
         const int items = a.n_seqs * a.p.n_kv * a.ngrp;
-        if (a.whole == 8)
-            hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, W, 8>), dim3(items), dim3(512), 0, g4_stream(), a);
-        else
-            hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, W, 4>), dim3(items), dim3(256), 0, g4_stream(), a);
+        if constexpr (whole_keys(TYPE, HD) > kRound) {
+            if (a.whole == 8) {
+                hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, W, 8>), dim3(items), dim3(512), 0, g4_stream(), a);
+                return;
+            }
+        }
+        hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, W, 4>), dim3(items), dim3(256), 0, g4_stream(), a);
         return;
     }
     hipLaunchKernelGGL((attn_paged_kernel<TYPE, HD, D, 4>), dim3(kPagedWG), dim3(256), 0, g4_stream(), a);
@@ -767,9 +778,8 @@ extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp
     // and 7.6 us in bf16, 11.8 and 15.5 in fp32; 64 of 500 keys 18.4 and 17.1.
     long most = (long)table_stride * page;
     if (window > 0 && window < most) most = window;
-    const int cap = type == G4_F32 ? 256 : 512, fit = (type == G4_F32 ? 65536 : 131072) / hd;
     const size_t items = (size_t)n_seqs * n_kv * a.ngrp;
-    a.whole = most > (fit < cap ? fit : cap) || !kv_grid_fits(items, 256) ? 0 : items <= 256 && most > 128 ? 8 : 4;
+    a.whole = most > whole_keys(type, hd) || !kv_grid_fits(items, 256) ? 0 : items <= 256 && most > kRound ? 8 : 4;
     if (type == G4_F32) launch_paged<G4_F32>(a, hd);
     else if (type == G4_F16) launch_paged<G4_F16>(a, hd);
     else if (type == G4_BF16) launch_paged<G4_BF16>(a, hd);
