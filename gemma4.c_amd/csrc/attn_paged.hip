@@ -33,11 +33,18 @@ struct PagedArgs {
 // it costs to begin and to end an item.  All items' units form one line,
 // sequences in order, and workgroup w takes the units N w / 512 .. N (w + 1) /
 // 512 - 1 of it, whatever the lengths are: a long sequence is spread over many
-// workgroups, several short ones share one.  (64 sequences of 1 to 8192 keys,
-// window 512, fp32: 35 us without the lead units, a workgroup of short items
-// outliving the others; 18 with 3 of them, equal with 4, 31 with 1.  Up to 64
-// items there are none: over one sequence of 32768 keys they would give some
-// workgroups a second round, 34 against 28 us.)
+// workgroups, several short ones share one.  Without lead units a workgroup of
+// short items outlives the others (the kernel, 64 sequences of 1 to 8192 keys,
+// window 512, fp32: 35 us without, 17 with 3 of them, equal with 4, 31 with 1).
+// One sequence has none: its items are alike, there is nothing to even out, and
+// they would only give some workgroups a further round.  us with 0 / 3 lead
+// units, both launches, 2 kv heads: fp16 of 512, one sequence of 32768 keys 32 /
+// 39, of 20000 27 / 27; 2 to 8 ragged ones 38 / 28, 39 / 30, 37 / 28, 69 / 67;
+// one of 20011 beside two of 700 31 / 27, beside eight 40 / 29.  bf16 of 256, one of
+// 32768 beside 8, 24, 40, 100 of 10 to 300: 26 / 23, 28 / 23, 35 / 27, 37 / 30;
+// window 700, 8, 24, 40, 100 sequences: 12 / 13, 18 / 15, 22 / 18, 34 / 33.  What
+// loses are several sequences whose tiles divide by the workgroups by chance: fp16
+// of 512, 2, 4, 8 of 32768 each 52 / 57, 104 / 113, 194 / 202.
 
 // tiles of a sequence and its first one; 0 tiles: an empty sequence or a
 // length that does not fit
@@ -764,7 +771,7 @@ extern "C" int g4_attn_decode_paged(const float* q, int q_stride, const void* kp
     a.n_seqs = n_seqs; a.window = window; a.n_heads = n_heads; a.scale = attn_scale;
     a.group = n_heads / n_kv;
     a.ngrp = (a.group + kHeadsWG - 1) / kHeadsWG;
-    a.lead = n_seqs * n_kv * a.ngrp > 64 ? 3 : 0;
+    a.lead = n_seqs > 1 ? 3 : 0;
     // Where a sequence cannot have more keys to look at than that, by its table
     // or the window, a workgroup takes an item whole and there is nothing to
     // join: some rounds of its waves cost less than the second launch.

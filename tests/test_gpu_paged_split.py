@@ -70,7 +70,8 @@ def test_heads(lib, kind, hd, n_heads, n_kv):
 
 @pytest.mark.parametrize("kind,hd", [(pn.F16, 256), (pn.F32, 128), (pn.Q8, 512)])
 def test_few_items(lib, kind, hd):
-    """whole heads joined with no lead units (64 items and fewer), parts of 64 dims with them (more than 64)"""
+    """whole heads joined in few items, one sequence's (no lead units) among them, and parts of 64 dims in many"""
+    check(lib, 623, kind, hd, 288, 2, 16, [2100], joined=True)
     check(lib, 620, kind, hd, 16, 1, 16, ragged(620, 20, 2500), joined=True)
     check(lib, 621, kind, hd, 3, 1, 16, ragged(621, 70, 700), joined=False)
     check(lib, 622, kind, hd, 2, 2, 16, ragged(622, 90, 700), joined=False)
