@@ -416,7 +416,8 @@ int g4_softmax(float *x, int n);
  * length, so what is left there by others (infinities, NaN) does not matter.
  * Packed rows: sequence s has rows cu[s] .. cu[s+1]-1 (cu: n_seqs + 1
  * ascending device ints, cu[n_seqs] <= m); m is the number of rows the
- * buffers hold.  Rows of no sequence are neither read nor written.  More rows,
+ * buffers hold.  Rows of no sequence are neither read nor written; where cu
+ * does not ascend, sequences beside the place may be skipped.  More rows,
  * sequences and heads than the 2^32 threads of a launch can take are refused.
  * ------------------------------------------------------------------------- */
 /* bytes of one pool; 0 if a size or the type is not one of the above */
@@ -459,15 +460,20 @@ int g4_attn_decode_paged(const float *q, int q_stride, const void *kp, const voi
 /* The attention block (main.c:1909-1950) of every row of whole prompts: row i
  * of a sequence sees that sequence's rows max(0, i + 1 - window) .. i (window
  * 0: 0 .. i).  q, k, v, out rows of one type, G4_F32, G4_F16 or G4_BF16, their
- * strides in elements (16-byte aligned rows).  F32: products of operands met
- * within 2^-22 of themselves or 2^-39 of their row's largest (a weight times its
- * V row: 2^-35 of the largest such product), fp32 sums; F16,
- * BF16: exact products, weights rounded to the type, fp32 sums (few rows: fp32
- * throughout); BF16 and few rows: |V| times the keys a row sees has to stay below
- * fp32's largest number, with every type scores as well.  Rows of out past cu[n_seqs] and those of sequences whose cu
- * does not fit are left as they are.  Where what a row's head sees holds
- * infinities or NaN, its output is what the formula gives or NaN; what it does
- * not see never matters.  work:
+ * strides in elements (16-byte aligned rows).  Rows of out past cu[n_seqs] and
+ * those of sequences whose cu does not fit are left as they are.
+ *   F32: products of operands met within 2^-22 of themselves or 2^-39 of their
+ * row's largest (V also 2^-115; a weight times its V row: 2^-35 of the largest
+ * such product), fp32 sums.
+ *   F16, BF16: exact products, fp32 sums, weights rounded to the type before they
+ * multiply V: against 64 bits the result is off by about 1.25 times what its own
+ * rounding to the type costs.
+ *   Few rows (rows x keys x heads up to 2^18, keys: m or the window): fp32 throughout, so that a batch
+ * that grows past it is rounded as above from there on.
+ *   BF16 and few rows: |V| times the keys a row sees has to stay below fp32's
+ * largest number; with every type scores as well.
+ * Where what a row's head sees holds infinities or NaN, its output is what the
+ * formula gives or NaN; what it does not see does not matter beyond rounding.  work:
  * g4_attn_prompt_packed_work_bytes() bytes that no call running at the same
  * time uses (its contents need not be kept); out may not overlap the inputs. */
 size_t g4_attn_prompt_packed_work_bytes(int type, int n_seqs, int m, int n_kv, int hd);
