@@ -825,11 +825,12 @@ __global__ __launch_bounds__((64 * Plan<T, HD>::NW), (Plan<T, HD>::NW / 4)) void
                 __builtin_memcpy(&p[0][t], hi, 16);
                 __builtin_memcpy(&p[1][t], lo, 16);
             } else {
-                // Rounded to the type, the operand's, while l keeps fp32: the one product
-                // instead of two of hi + lo.  8191 rows in bf16, 8 heads of 256: 283 us
-                // with an error of 0.00205 of the norm, against 399 and 0.00166, which is
-                // the output's own rounding; of 512, four prompts of 4096, 622 (0.00211)
-                // against 828 (0.00166).
+                // Rounded to the type, the operand's, while l keeps fp32: bf16, 8191 rows, 8
+                // heads of 256, 283 us with an error of 0.00205 of the norm, where the
+                // output's own rounding alone makes 0.00166.  That is reached by two
+                // products, of hi and lo, in 399 us, or by fp16 weights and V rows with
+                // exponents as in fp32 in 328 (more instructions a key, the SIMD's
+                // registers spent); of 512, four prompts of 4096: 622 (0.00211), 828, 684.
 #pragma unroll
                 for (int j = 0; j < 8; j++) p[0][t][j] = (E)w[j];
             }
