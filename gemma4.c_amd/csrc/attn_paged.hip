@@ -38,13 +38,16 @@ struct PagedArgs {
 // window 512, fp32: 35 us without, 17 with 3 of them, equal with 4, 31 with 1).
 // One sequence has none: its items are alike, there is nothing to even out, and
 // they would only give some workgroups a further round.  us with 0 / 3 lead
-// units, both launches, 2 kv heads: fp16 of 512, one sequence of 32768 keys 32 /
-// 39, of 20000 27 / 27; 2 to 8 ragged ones 38 / 28, 39 / 30, 37 / 28, 69 / 67;
-// one of 20011 beside two of 700 31 / 27, beside eight 40 / 29.  bf16 of 256, one of
-// 32768 beside 8, 24, 40, 100 of 10 to 300: 26 / 23, 28 / 23, 35 / 27, 37 / 30;
-// window 700, 8, 24, 40, 100 sequences: 12 / 13, 18 / 15, 22 / 18, 34 / 33.  What
-// loses are several sequences whose tiles divide by the workgroups by chance: fp16
-// of 512, 2, 4, 8 of 32768 each 52 / 57, 104 / 113, 194 / 202.
+// units, both launches, 2 kv heads:
+//   fp16 of 512: one sequence of 32768 keys 32 / 39, of 20000 27 / 27; two, four,
+//   six, eight of 700 to 28000 38 / 28, 37 / 28, 71 / 67, 51 / 43; one of 20011
+//   beside two of 700 31 / 27, beside eight 40 / 29;
+//   bf16 of 256: one of 32768 beside 8, 24, 40, 100 of 10 to 300 26 / 23, 28 / 23,
+//   35 / 27, 37 / 30; window 700, 8, 24, 40, 100 sequences 12 / 13, 18 / 15,
+//   22 / 18, 34 / 33.
+// Against it are a few sequences whose tiles divide by the workgroups by chance:
+// fp16 of 512, two, four, eight of 32768 52 / 57, 104 / 113, 194 / 202, four of 2000
+// 20 / 26, and one of nine batches of two to four ragged ones, 22 / 27.
 
 // tiles of a sequence and its first one; 0 tiles: an empty sequence or a
 // length that does not fit

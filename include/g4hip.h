@@ -471,7 +471,8 @@ int g4_attn_decode_paged(const float *q, int q_stride, const void *kp, const voi
  *   Few rows (rows x keys x heads up to 2^18, keys: m or the window): fp32 throughout, so that a batch
  * that grows past it is rounded as above from there on.
  *   BF16 and few rows: |V| times the keys a row sees has to stay below fp32's
- * largest number; with every type scores as well.
+ * largest number; with every type scores and q times attn_scale as well (F32: a q
+ * row's largest times a K row's largest times attn_scale).
  * Where what a row's head sees holds infinities or NaN, its output is what the
  * formula gives or NaN; what it does not see does not matter beyond rounding.  work:
  * g4_attn_prompt_packed_work_bytes() bytes that no call running at the same
