@@ -355,9 +355,10 @@ __global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedArgs a) {
 // holds 16 of a row's 32 scores, which are, as they stand, its operand of
 // O^T += V^T P^T.  The running maximum moves only when a score passes it (bf16,
 // where it stands 2^8 above the largest; fp16, fp32: by 2^8, 2^4).  DS 2
-// (head_dim 512, whose q and o would not fit a wave's registers): a job's dims are halved over two waves, whose partial scores
-// meet in LDS; K and V of a tile have one place each, and the next tile's K is
-// on its way while V is worked on, and the other way round.
+// (head_dim 512, whose q and o would not fit a wave's registers): a job's dims
+// are halved over two waves, whose partial scores meet in LDS; K and V of a tile
+// have one place each, and the next tile's K is on its way while V is worked on,
+// and the other way round.
 // KSP 2 (16 bits): the two waves of a SIMD are given the same job and every
 // other tile, so that there are twice the workgroups, half as long, and the
 // one does its second product while the other is at its weights: waves 4 .. 7
