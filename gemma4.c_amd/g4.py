@@ -111,6 +111,8 @@ _SIGS = {
     "g4_kv_pool_bytes": (SZ, [I, I, I, I, I]),
     "g4_kv_page_store": (I, [VP, VP, I, I, I, I, I, VP, I, VP, VP, I, VP, VP, I, I]),
     "g4_kv_page_load": (I, [VP, VP, I, I, I, I, I, VP, I, VP, VP, I, VP, VP, I, I]),
+    "g4_qkv_post_seqs": (I, [VP, I, VP, I, VP, VP, I, VP, I, I, VP, I, VP, VP, I, I, VP, I, I, F, VP, VP, I, I]),
+    "g4_kv_page_append": (I, [VP, VP, I, I, I, I, I, VP, I, VP, VP, I, VP, VP, I, VP, I, VP, I, I, VP, I, I, F, VP, VP, I, I]),
     "g4_attn_decode_paged_part_bytes": (SZ, [I, I, I]),
     "g4_attn_decode_paged": (I, [VP, I, VP, VP, I, I, I, I, I, VP, I, VP, I, I, I, F, VP, VP, I]),
     "g4_attn_prompt_packed_work_bytes": (SZ, [I, I, I, I, I]),

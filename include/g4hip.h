@@ -439,6 +439,36 @@ int g4_kv_page_store(void *kp, void *vp, int type, int n_pages, int page, int n_
 int g4_kv_page_load(const void *kp, const void *vp, int type, int n_pages, int page, int n_kv, int hd, const int *table,
                     int table_stride, float *k, float *v, int kv_stride, const int *cu, const int *lens, int n_seqs,
                     int m);
+/* What stands between the projections and the attention (main.c:1886-1900),
+ * for the packed rows of all sequences: g4_qkv_post_rows at the position of
+ * each row, lens[s] - n + i for row i of the n of sequence s.  q heads: norm
+ * with q_norm and rotation; k heads: norm with k_norm and rotation; v heads:
+ * norm without weight.  q, k, v: fp32 rows as the projections leave them,
+ * strides in elements; q or k (with v) may be null: only the other's rows.
+ * Outputs: rows of `type` (G4_F32; G4_F16, G4_BF16: rounded to nearest even),
+ * as g4_attn_prompt_packed, g4_attn_chunk_paged and (fp32) the cache take
+ * them; fp32 rows may go where they came from (same pointer and stride).
+ * rope_tab: n_rot / 2 (cos, sin) pairs for each of the positions 0 ..
+ * tab_rows - 1, as g4_rope_table_rows(rope_tab, 0, tab_rows, n_rot, ...)
+ * fills it once.  For head_dim 256 and 512 fp32 results are bit for bit those of
+ * g4_qkv_post_rows with the same table row.  A sequence whose cu or lens do
+ * not fit (n > lens, rows past m, lens past tab_rows) is skipped.  All rows
+ * and weights 16-byte aligned, input strides multiples of 4, output strides
+ * of 16 bytes; rope_tab 8-byte aligned. */
+int g4_qkv_post_seqs(const float *q, int q_stride, const float *q_norm, int n_heads, const float *k, const float *v,
+                     int kv_stride, const float *k_norm, int n_kv, int hd, void *q_out, int q_out_stride, void *k_out,
+                     void *v_out, int kv_out_stride, int type, const float *rope_tab, int tab_rows, int n_rot, float eps,
+                     const int *cu, const int *lens, int n_seqs, int m);
+/* The same with K and V going straight into their pages: g4_qkv_post_seqs to
+ * fp32 rows and g4_kv_page_store of them in one launch, bit for bit.  q
+ * (nullable: K and V alone) becomes rows q_out of q_type.  A sequence is
+ * skipped (its q rows too) where either of the two skips it; K and V rows of
+ * pages outside the pool are dropped. */
+int g4_kv_page_append(void *kp, void *vp, int type, int n_pages, int page, int n_kv, int hd, const int *table,
+                      int table_stride, const float *k, const float *v, int kv_stride, const float *k_norm, const float *q,
+                      int q_stride, const float *q_norm, int n_heads, void *q_out, int q_out_stride, int q_type,
+                      const float *rope_tab, int tab_rows, int n_rot, float eps, const int *cu, const int *lens,
+                      int n_seqs, int m);
 /* The attention block (main.c:1909-1950) of one token of every sequence: q
  * row s (n_heads * hd floats, q_stride apart) over positions
  * max(0, lens[s] - window) .. lens[s] - 1 (window 0: all), the token's own K/V
