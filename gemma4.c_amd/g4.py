@@ -115,6 +115,8 @@ _SIGS = {
     "g4_kv_page_append": (I, [VP, VP, I, I, I, I, I, VP, I, VP, VP, I, VP, VP, I, VP, I, VP, I, I, VP, I, I, F, VP, VP, I, I]),
     "g4_attn_decode_paged_part_bytes": (SZ, [I, I, I]),
     "g4_attn_decode_paged": (I, [VP, I, VP, VP, I, I, I, I, I, VP, I, VP, I, I, I, F, VP, VP, I]),
+    "g4_attn_chunk_paged_part_bytes": (SZ, [I, I, I, I]),
+    "g4_attn_chunk_paged": (I, [VP, I, I, VP, VP, I, I, I, I, I, VP, I, VP, VP, I, I, I, I, F, VP, VP, I]),
     "g4_attn_prompt_packed_work_bytes": (SZ, [I, I, I, I, I]),
     "g4_attn_prompt_packed": (I, [VP, I, VP, VP, I, VP, I, I, VP, I, I, I, I, I, I, F, VP]),
     "g4_emb_lookup": (I, [VP, VP, I, I, I, I]),

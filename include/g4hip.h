@@ -512,6 +512,36 @@ int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void
                           int out_stride, int type, const int *cu, int n_seqs, int m, int window, int n_heads, int n_kv,
                           int hd, float attn_scale, void *work);
 
+/* The attention block (main.c:1909-1950) of chunks of new rows of every
+ * sequence (a later turn, a prompt in pieces, drafts to be checked, one token
+ * each, side by side) over the cache, where the rows' own K and V are stored
+ * already (g4_kv_page_append): row i of the n of sequence s is position
+ * p = lens[s] - n + i and sees max(0, p + 1 - window) .. p (window 0: 0 .. p).
+ * q and out: rows of q_type, strides in elements (16-byte aligned rows):
+ *   G4_F32 over a cache of any type: operands of the products as in
+ * g4_attn_prompt_packed's F32 over a cache of that type, three terms of q over
+ * BF16 and codes (exact) and weights within 2^-17, F16: q within 2^-22 of itself
+ * or 2^-39 of its row's largest, weights 2^-22; fp32 sums.
+ *   G4_F16 over F16, G4_BF16 over BF16 or G4_KV_Q8: exact products of q, fp32
+ * sums, weights (times the scale of a token's codes) rounded to the type before
+ * they multiply V.
+ * Rows of out past cu[n_seqs] and those of sequences whose cu or lens do not
+ * fit (n > lens, rows past m, positions past the table) are left as they are.
+ * A row that sees a page outside the pool becomes NaN.  Pages, and within a page
+ * tokens, that no row of the sequence sees do not matter, whatever they hold;
+ * what a row does not see does not change it, infinities and NaN included.
+ * |V| times the keys a row sees has to stay below fp32's largest number, scores
+ * (and q times attn_scale) as well.  Where what a row's head sees holds
+ * infinities or NaN, its output is what the formula gives or NaN.  out may not
+ * overlap q.  part: g4_attn_chunk_paged_part_bytes() bytes (m: this call's or
+ * more) that no call running at the same time uses (its contents need not be
+ * kept). */
+size_t g4_attn_chunk_paged_part_bytes(int m, int n_heads, int n_kv, int hd);
+int g4_attn_chunk_paged(const void *q, int q_stride, int q_type, const void *kp, const void *vp, int type, int n_pages,
+                        int page, int n_kv, int hd, const int *table, int table_stride, const int *cu, const int *lens,
+                        int n_seqs, int m, int window, int n_heads, float attn_scale, void *part, void *out,
+                        int out_stride);
+
 /* ---------------------------------------------------------------------------
  * Step glue (main.c:1696-1778, 1988-1993, 2045-2049)
  * ------------------------------------------------------------------------- */
