@@ -1,18 +1,13 @@
 // attn_paged.hip -- attention of one new token of every sequence over the
 // paged KV cache.
-#include <math.h>
-
+#include "g4_attn_tile.h"
 #include "g4_kvpage.h"
-#include "g4_tile.h"
 
 namespace g4 {
 namespace {
 
-typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
-
 constexpr int kLgWG = 9, kPagedWG = 1 << kLgWG;   // workgroups that share the work, two a CU
 constexpr int kHeadsWG = 16;                      // q heads of a workgroup: the columns of a product
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct PagedArgs {
     KvPool p;
@@ -161,26 +156,6 @@ __host__ __device__ inline size_t part_floats(int group, int hd) {
 }
 
 // ---- operands ------------------------------------------------------------------
-// A float is the sum of three bf16: its leading 8, middle 8 and last 8 bits.
-// Every product of two such terms is exact, so that matrix instructions on 16
-// bits give the fp32 product.
-__device__ __forceinline__ uint32_t hi_halves(uint32_t x0, uint32_t x1) { return __builtin_amdgcn_perm(x1, x0, 0x07060302u); }
-__device__ __forceinline__ float rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-template <int NT>
-__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&t)[NT]) {
-#pragma unroll
-    for (int i = 0; i < NT; i++) {
-        t[i] = hi_halves(__float_as_uint(x0), __float_as_uint(x1));
-        if (i + 1 < NT) {
-            x0 = rest(x0);
-            x1 = rest(x1);
-        }
-    }
-}
-__device__ __forceinline__ b8_t as_b8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __builtin_bit_cast(b8_t, make_uint4(a, b, c, d));
-}
-
 template <int TYPE>
 struct CacheType;
 template <>

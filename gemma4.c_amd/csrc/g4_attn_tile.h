@@ -1,6 +1,7 @@
 // g4_attn_tile.h -- what the attention kernels on 32 x 32 x 16 products share:
-// the scales of split fp32 rows and what weights lose by them, the order of
-// products and LDS reads, rows to and from memory through LDS.
+// fp32 operands as sums of terms of 16 bits, the scales of split rows and what
+// weights lose by them, the order of products and LDS reads, rows to and from
+// memory through LDS.
 #pragma once
 #include <float.h>
 #include <math.h>
@@ -18,6 +19,26 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ f16_t mfma32(h8_t a, h8_t b, f16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f16_t mfma32(b8_t a, b8_t b, f16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// A float is the sum of three bf16: its leading 8, middle 8 and last 8 bits.
+// Every product of two such terms is exact, so that matrix instructions on 16
+// bits give the fp32 product.
+__device__ __forceinline__ uint32_t hi_halves(uint32_t x0, uint32_t x1) { return __builtin_amdgcn_perm(x1, x0, 0x07060302u); }
+__device__ __forceinline__ float rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+template <int NT>
+__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&t)[NT]) {
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        t[i] = hi_halves(__float_as_uint(x0), __float_as_uint(x1));
+        if (i + 1 < NT) {
+            x0 = rest(x0);
+            x1 = rest(x1);
+        }
+    }
+}
+__device__ __forceinline__ b8_t as_b8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_bit_cast(b8_t, make_uint4(a, b, c, d));
+}
 
 // biased exponent of a row's largest magnitude -> the scale that brings it
 // to [2^14, 2^15) and its inverse; low: the smallest exponent told apart
