@@ -1,10 +1,16 @@
 // attn_chunk.hip -- attention of chunks of new rows of every sequence over the
 // paged KV cache, which holds their own keys and values already.
+#include <atomic>
+
 #include "g4_attn_tile.h"
 #include "g4_kvpage.h"
 
 namespace g4 {
 namespace {
+
+constexpr int kShares = 256;   // workgroups that share the work, one a CU
+constexpr int kLead = 64;      // keys that stand for what it costs to begin and to end an item
+constexpr int kLeast = 96;     // no smaller share than this
 
 struct ChunkArgs {
     KvPool p;
@@ -15,147 +21,1117 @@ struct ChunkArgs {
     float* part;
     int q_stride, out_stride, n_seqs, m, window, n_heads;
     int group;      // q heads a kv head
+    int gh, ngrp;   // of these, a workgroup's; groups of them
+    int rpi;        // rows of an item
+    int cols;       // columns of a partial result, a multiple of 32
     float scale;
 };
 
-template <int T>
-struct Row;   // element of q and output rows
-template <>
-struct Row<G4_F32> { typedef float t; };
-template <>
-struct Row<G4_F16> { typedef _Float16 t; };
-template <>
-struct Row<G4_BF16> { typedef __bf16 t; };
-template <int T>
-struct Cached { static constexpr int ES = T == G4_F32 ? 4 : T == G4_KV_Q8 ? 1 : 2; };
+// ---- shares of the work ------------------------------------------------------
+// An item is up to rpi rows of a sequence, a kv head and up to gh of its q
+// heads: at most a workgroup's columns.  Its measure is the keys it looks at
+// (rpi rows counted whole) and kLead.  All items form one line, by sequence,
+// kv head, group of heads and row, and share w of W takes the measure N w / W
+// .. N (w + 1) / W - 1 of it, whatever the lengths are: a few rows of a long
+// sequence are spread over many workgroups, short sequences share one.  The
+// line's sums over a sequence's items are closed forms.
 
-// element i of a register's worth of cached elements (16-bit and fp32 values, codes)
-template <int T>
-__device__ __forceinline__ float cached(const uint32_t* w, int i) {
-    if constexpr (T == G4_F32) return __uint_as_float(w[i]);
-    else if constexpr (T == G4_F16) return hbits_to_f32(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
-    else if constexpr (T == G4_BF16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
-    else return (float)(int8_t)(w[i >> 2] >> (8 * (i & 3)));
+typedef unsigned long long u64;
+
+struct Seq {
+    int r0, n, hist;   // first row, rows (0: none, or what does not fit), earlier positions
+};
+__device__ __forceinline__ Seq seq_of(const ChunkArgs& a, int r0, int r1, int len) {
+    Seq q = {r0, r1 - r0, len - (r1 - r0)};
+    if (r0 < 0 || r1 <= r0 || r1 > a.m || q.n > len || !a.p.fits(len)) q.n = 0;
+    return q;
 }
-// N elements that lie next to each other
-template <int T, int N>
-__device__ __forceinline__ void load_cached(const uint8_t* at, float (&x)[N]) {
-    constexpr int B = N * Cached<T>::ES;
-    uint32_t w[(B + 3) / 4];
-    if constexpr (B >= 16) {
-#pragma unroll
-        for (int i = 0; i < B / 16; i++) {
-            // 16 bytes are next to each other in a block, the next 16 are a token's next lane's
-            const uint4 y = *reinterpret_cast<const uint4*>(at + i * 256);
-            w[4 * i] = y.x; w[4 * i + 1] = y.y; w[4 * i + 2] = y.z; w[4 * i + 3] = y.w;
-        }
-    } else if constexpr (B == 8) {
-        const uint2 y = *reinterpret_cast<const uint2*>(at);
-        w[0] = y.x; w[1] = y.y;
-    } else if constexpr (B == 4) {
-        w[0] = *reinterpret_cast<const uint32_t*>(at);
-    } else if constexpr (B == 2) {
-        w[0] = *reinterpret_cast<const uint16_t*>(at);
-    } else {
-        w[0] = *at;
+__device__ __forceinline__ int seq_items(const ChunkArgs& a, const Seq& q) {
+    return (int)(((unsigned)q.n + a.rpi - 1) / (unsigned)a.rpi);
+}
+__device__ __forceinline__ int first_key(const ChunkArgs& a, int pos) {
+    return a.window > 0 && pos >= a.window ? pos + 1 - a.window : 0;
+}
+// measure of item i, and of the first c items: hist + (i + 1) rpi keys while
+// the window does not pass the first of them, window - 1 + rpi from there on
+__device__ __forceinline__ u64 item_measure(const ChunkArgs& a, const Seq& q, int i) {
+    const u64 row = (u64)i * a.rpi;
+    if (a.window > 0 && q.hist + row >= (u64)a.window) return (u64)kLead + a.window - 1 + a.rpi;
+    return kLead + q.hist + row + a.rpi;
+}
+__device__ __forceinline__ u64 items_measure(const ChunkArgs& a, const Seq& q, int c) {
+    u64 whole = c;
+    if (a.window > 0) {
+        whole = q.hist < a.window ? (u64)((unsigned)(a.window - 1 - q.hist) / (unsigned)a.rpi) + 1 : 0;
+        if (whole > (u64)c) whole = c;
     }
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = cached<T>(w, i);
+    return (u64)c * kLead + whole * q.hist + (u64)a.rpi * (whole * (whole + 1) / 2) +
+           (c - whole) * ((u64)a.rpi + a.window - 1);
 }
 
-// One wave: one q row's head (dims lane * N .. + N - 1, times scale log2(e))
-// over positions first .. last of sequence s, `step` times four at a time
-// from the four that hold position at on; adds to the running maximum m, sum
-// l and o.  fp32 throughout; only the positions asked for have a part, so
-// that infinities and NaN elsewhere do not matter; where a page is none: NaN.
-template <int TC, int HD>
-__device__ void row_keys(const KvPool& p, int s, int kvh, int first, int last, int at, int step, const float (&q)[HD / 64],
-                         float& m, float& l, float (&o)[HD / 64]) {
-    constexpr int ES = Cached<TC>::ES, N = HD / 64;
+// a place on the line
+struct Place {
+    int s, rep, item;   // sequence, kv head and group of heads, item
+    Seq q;
+    u64 x, size;        // where in the item, the item's measure
+};
+struct Line {
+    u64 total;
+    unsigned shares;    // W
+    // where share w begins: N w / W without overflow
+    __device__ __forceinline__ u64 at(unsigned w) const { return total / shares * w + total % shares * w / shares; }
+};
+__device__ __forceinline__ Line line_of(u64 total) {
+    const u64 most = total / kLeast;
+    return {total, most < 1 ? 1u : most < kShares ? (unsigned)most : (unsigned)kShares};
+}
+
+// of all 64 lanes of a wave
+__device__ __forceinline__ u64 wave_scan(u64 v) {
     const int lane = threadIdx.x & 63;
-    for (int t0 = at & ~3; t0 <= last; t0 += 4 * step) {
-        const int page = p.page_of(s, t0);
-        const size_t block = p.block_of(page < 0 ? 0 : page, kvh, t0), off = block * (16 * HD * ES);
-        const uint8_t* kb = p.kp + off;
-        const uint8_t* vb = p.vp + off;
-        const float* ks = reinterpret_cast<const float*>(p.kp + p.scale_off) + block * 16 + (t0 & 15);
-        const float* vs = reinterpret_cast<const float*>(p.vp + p.scale_off) + block * 16 + (t0 & 15);
-        float x[4], v[N][4], mn = m;
 #pragma unroll
-        for (int i = 0; i < N; i++) load_cached<TC, 4>(vb + kv_v_byte<ES>(t0 & 15, lane * N + i), v[i]);
+    for (int d = 1; d < 64; d <<= 1) {
+        const u64 o = __shfl_up(v, d, 64);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+__device__ __forceinline__ u64 lane_u64(u64 v, int l) {
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)v, l);
+}
+
+// The line, and the place at(line) on it, by all NT threads of a workgroup
+// (red: NT / 64 + 3 words of LDS): up to 64 sequences each wave by itself,
+// after one round trip to memory.  false: no such place.
+template <int NT, typename At>
+__device__ __forceinline__ bool find_place(const ChunkArgs& a, At at, Line& line, Place& o, u64* red) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const unsigned rep = a.p.n_kv * a.ngrp;
+    u64 before, u;
+    if (a.n_seqs <= 64) {
+        const int i = lane < a.n_seqs ? lane : a.n_seqs - 1;
+        const Seq q = seq_of(a, a.cu[i], a.cu[i + 1], a.lens[i]);
+        const u64 mine = lane < a.n_seqs && q.n ? items_measure(a, q, seq_items(a, q)) : 0, x = wave_scan(mine);
+        line = line_of(lane_u64(x, 63) * rep);
+        u = at(line);
+        const u64 past = __ballot(x * rep > u);
+        if (!past) return false;
+        o.s = __builtin_ctzll(past);
+        before = lane_u64(x - mine, o.s);
+        o.q.r0 = __builtin_amdgcn_readlane(q.r0, o.s);
+        o.q.n = __builtin_amdgcn_readlane(q.n, o.s);
+        o.q.hist = __builtin_amdgcn_readlane(q.hist, o.s);
+    } else {
+        constexpr int NWV = NT / 64;
+        const int per = (a.n_seqs + NT - 1) / NT, s0 = tid * per;
+        auto measure = [&](int s) {
+            const Seq q = seq_of(a, a.cu[s], a.cu[s + 1], a.lens[s]);
+            return q.n ? items_measure(a, q, seq_items(a, q)) : (u64)0;
+        };
+        u64 sum = 0;
+        for (int i = 0; i < per; i++)
+            if (s0 + i < a.n_seqs) sum += measure(s0 + i);
+        const u64 x = wave_scan(sum);
+        if (lane == 63) red[wave] = x;
+        if (tid == 0) red[NWV] = ~(u64)0;
+        lds_sync();
+        u64 b = x - sum, all = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float k[N];
-            load_cached<TC, N>(kb + kv_k_byte<ES>((t0 & 15) + j, lane * N), k);
-            x[j] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < N; i++) x[j] = __builtin_fmaf(q[i], k[i], x[j]);
-            x[j] = wave_sum(x[j]);
-            if (TC == G4_KV_Q8) x[j] *= ks[j];
-            if (page < 0) x[j] = __uint_as_float(0x7fc00000u);
-            if (t0 + j < first || t0 + j > last) x[j] = -INFINITY;
-            mn = fmaxf(mn, x[j]);
+        for (int w = 0; w < NWV; w++) {
+            if (w < wave) b += red[w];
+            all += red[w];
         }
-        const float f = exp2f(m - mn);
-        l *= f;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < N; i++) o[i] *= f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (t0 + j < first || t0 + j > last) continue;
-            const float w = exp2f(x[j] - mn);
-            l += w;
-#pragma unroll
-            for (int i = 0; i < N; i++) o[i] = __builtin_fmaf(w, TC == G4_KV_Q8 ? v[i][j] * vs[j] : v[i][j], o[i]);
+        line = line_of(all * rep);
+        u = at(line);
+        if (u >= b * rep && u < (b + sum) * rep) {
+            int s = s0;
+            for (;; s++) {
+                const u64 v = measure(s);
+                if (u < (b + v) * rep) break;
+                b += v;
+            }
+            red[NWV] = b;
+            red[NWV + 1] = (unsigned)s;
         }
+        lds_sync();
+        before = red[NWV];
+        if (before == ~(u64)0) return false;
+        o.s = __builtin_amdgcn_readfirstlane((int)red[NWV + 1]);
+        before = lane_u64(before, 0);
+        o.q = seq_of(a, a.cu[o.s], a.cu[o.s + 1], a.lens[o.s]);
+        lds_sync();
+    }
+    const int items = seq_items(a, o.q);
+    const u64 one = items_measure(a, o.q, items), off = u - before * rep;
+    o.rep = __builtin_amdgcn_readfirstlane((int)(off / one));
+    const u64 y = off - (u64)o.rep * one;
+    // the last item that begins at y or before: 64 candidates a step
+    int lo = 0, n = items;
+    while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const bool in = (long)lane * step < n && items_measure(a, o.q, lo + lane * step) <= y;
+        const int c = __popcll(__ballot(in));
+        lo += (c > 0 ? c - 1 : 0) * step;
+        n = items - lo < step ? items - lo : step;
+    }
+    o.item = __builtin_amdgcn_readfirstlane(lo);
+    o.x = lane_u64(y - items_measure(a, o.q, o.item), 0);
+    o.size = lane_u64(item_measure(a, o.q, o.item), 0);
+    return true;
+}
+
+// an item's rows, keys and 32-key tiles
+struct Item {
+    int row0, rows, kfirst, klast, kt0, tiles;
+    __device__ __forceinline__ Item(const ChunkArgs& a, const Place& p) {
+        row0 = p.item * a.rpi;
+        rows = p.q.n - row0 < a.rpi ? p.q.n - row0 : a.rpi;
+        kfirst = first_key(a, p.q.hist + row0);
+        klast = p.q.hist + row0 + rows - 1;
+        kt0 = kfirst >> 5;
+        tiles = (klast >> 5) - kt0 + 1;
+    }
+    // the tile that a share which begins at x of the item begins with
+    __device__ __forceinline__ int tile_at(u64 x, u64 size) const {
+        if (x >= size) return tiles;
+        const int t = (int)((kfirst + (x > kLead ? x - kLead : 0)) >> 5) - kt0;
+        return t < tiles ? t : tiles;
+    }
+};
+// floats of a partial result: 32 columns at a time in the order of a wave's
+// registers, then each column's maximum and weight sum
+__host__ __device__ inline size_t part_floats(int cols, int hd) { return (size_t)cols * (hd + 2); }
+
+// ---- types ----------------------------------------------------------------------
+// TQ: rows, TC: cache.  NQ, NK, NP: terms of q, of K (and V), of the weights.
+// REG: tiles go through registers, where they are put into other numbers
+// (codes into bf16, fp32 into halves); the others go from the pages to LDS.
+template <int TQ, int TC>
+struct Mode {
+    static constexpr int ES = TC == G4_F32 ? 4 : TC == G4_KV_Q8 ? 1 : 2;
+    static constexpr bool kHalf = TC == G4_F32 || TC == G4_F16;     // fp16 operands
+    static constexpr bool F = TC == G4_F32, Q8 = TC == G4_KV_Q8, REG = F || Q8;
+    static constexpr int NQ = TQ != G4_F32 ? 1 : kHalf ? 2 : 3, NK = F ? 2 : 1, NP = TQ != G4_F32 ? 1 : 2;
+    // a score is the sum of products as it stands, times log2(e) scale
+    static constexpr bool kRaw = !F && !Q8 && NQ < 3;
+    // how far a score may pass the maximum before it moves, and how far above the
+    // largest score it is put.  bf16, whose V goes as far as fp32: weights are at
+    // most 1; fp16's smallest numbers ask for large weights, and its V cannot overflow
+    static constexpr float kSlack = !kHalf ? 0.0f : NQ == 1 ? 8.0f : 4.0f, kRaise = kHalf ? 0.0f : 8.0f;
+    static constexpr float kLift = kHalf && NQ > 1 ? 11.0f : 0.0f;   // fp16 terms: 2^11 above their fp32 size
+};
+template <int T>
+struct RowElem;
+template <>
+struct RowElem<G4_F32> { typedef float t; };
+template <>
+struct RowElem<G4_F16> { typedef _Float16 t; };
+template <>
+struct RowElem<G4_BF16> { typedef __bf16 t; };
+template <bool HALF>
+struct OpOf { typedef b8_t t; };
+template <>
+struct OpOf<true> { typedef h8_t t; };
+
+// A wave's job is 32 columns (row, q head) of an item; a workgroup's jobs share
+// its tiles of 32 keys in LDS.  S^T = K Q^T (rows keys, columns q rows): a lane
+// holds 16 of a column's 32 scores, which are, as they stand, its operand of
+// O^T += V^T P^T.  DS 2 (head_dim 512): a job's dims are halved over two waves,
+// whose partial scores meet in LDS; KSP 2: the two waves of a SIMD have the same
+// job and every other tile, waves 4 .. 7 their second product a tile later.
+template <int TQ, int TC, int HD>
+struct Plan {
+    typedef Mode<TQ, TC> M;
+    static constexpr int DS = HD == 512 ? 2 : 1;
+    static constexpr int NW = M::NQ == 1 ? 8 : 4;                    // waves; 8: two a SIMD
+    static constexpr int KSP = NW == 8 && DS == 1 ? 2 : 1;           // tiles at a time
+    static constexpr int NJ = NW / DS / KSP, COLS = 32 * NJ;
+    // LDS: K and V of a tile are TB bytes each
+    static constexpr int TB = 64 * HD * M::NK;
+    static constexpr int NKP = DS == 2 ? 1 : 2 * KSP, NVP = DS == 2 ? 1 : KSP == 2 ? 5 : 2;
+    static constexpr int META = (NKP + NVP) * TB, XCH = META + 2 * KSP * 512;
+    static constexpr int RB = HD / DS * (TQ == G4_F32 ? 4 : 2);      // bytes of a wave's part of a row
+    static constexpr int END = XCH + (DS == 2 ? NW * 4096 : 0);      // DS 2: partial scores
+    static constexpr int ROWS = (KSP == 1 ? NW : 0) * 32 * RB;       // the output's rows
+    static constexpr int JOIN = KSP == 2 ? NJ * (HD * 128 + 256) : 0;   // sums of waves 4 .. 7
+    static constexpr int TOP0 = END > ROWS ? END : ROWS, TOP = TOP0 > JOIN ? TOP0 : JOIN;
+    static constexpr int RED = (TOP + 15) / 16 * 16, LDS = RED + 128;
+    static_assert(LDS <= 160 * 1024 && NJ * DS * KSP == NW, "LDS");
+    // staging: a unit is a 16-token block of K or V; WPU waves have one
+    static constexpr int UNITS = 4 * KSP, WPU = NW / UNITS, KC = HD * M::ES / 64, PCS = KC / WPU;
+    static_assert(PCS * WPU == KC, "pieces");
+    static __device__ __forceinline__ int k_at(int st, int kp) { return DS == 2 ? 0 : ((st & 1) * KSP + kp) * TB; }
+    static __device__ __forceinline__ int v_at(int st, int kp) {
+        return (NKP + (DS == 2 ? 0 : kp == 0 ? st & 1 : 2 + st % 3)) * TB;
+    }
+    static __device__ __forceinline__ int meta_at(int st, int kp) { return META + ((st & 1) * KSP + kp) * 512; }
+};
+// a tile's 512 bytes beside it: 32 factors of K (fp32: 2^e, codes: scales), 32 of V
+// (exponents, scales), fp32: 2^-e; marks of each block's keys that make a score
+// NaN; fp32: the weight sums below which lost_weight is asked for
+constexpr int kMetaV = 128, kMetaInv = 256, kMetaMarks = 384, kMetaLost = 392;
+
+template <int TQ, int TC, int HD>
+__global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW / 4)) void attn_chunk_kernel(ChunkArgs a) {
+    typedef Plan<TQ, TC, HD> P;
+    typedef Mode<TQ, TC> M;
+    typedef typename RowElem<TQ>::t E;
+    typedef typename OpOf<M::kHalf>::t op;
+    constexpr int NW = P::NW, DS = P::DS, NJ = P::NJ, KSP = P::KSP, TB = P::TB, KC = P::KC, PCS = P::PCS;
+    constexpr int NQ = M::NQ, NK = M::NK, NP = M::NP, ES = M::ES;
+    constexpr int KS = HD / 16 / DS, NT = HD / 32 / DS;   // a wave's product steps and 32-dim tiles
+    extern __shared__ __align__(16) uint8_t lds[];
+    u64* red = reinterpret_cast<u64*>(lds + P::RED);
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % DS, kp = wave / (NJ * DS), slot = wave / DS % NJ;
+    // this wave's share of the staging: tile of a stage, K or V, block of the tile, which pieces
+    const int unit = wave % P::UNITS, ut = unit >> 2, uv = unit >> 1 & 1, ub = unit & 1, piece0 = wave / P::UNITS * PCS;
+    const int t16 = lane & 15, g = lane >> 4;
+
+    Line line;
+    Place at;
+    unsigned share = 0;
+    if (!find_place<64 * NW>(
+            a,
+            [&](const Line& l) {
+                // neighbours on the line, which look at the same keys, to one XCD
+                share = l.shares == kShares ? (blockIdx.x & 7) * (kShares / 8) + (blockIdx.x >> 3) : blockIdx.x;
+                return share < l.shares ? l.at(share) : ~(u64)0 / (a.p.n_kv * a.ngrp) / 2 * (a.p.n_kv * a.ngrp);
+            },
+            line, at, red))
+        return;
+    u64 left = line.at(share + 1) - line.at(share);
+
+    while (left > 0) {
+        const u64 take = left < at.size - at.x ? left : at.size - at.x;
+        const Item it(a, at);
+        const int tile0 = it.tile_at(at.x, at.size), tile1 = it.tile_at(at.x + take, at.size);
+        if (tile0 < tile1) {
+            const int kvh = at.rep / a.ngrp, hg = at.rep - kvh * a.ngrp;
+            const int nh = a.group - hg * a.gh < a.gh ? a.group - hg * a.gh : a.gh;    // heads there are
+            const int head0 = kvh * a.group + hg * a.gh;
+            const int ncols = it.rows * nh;
+            const bool mine = slot * 32 < ncols;
+            // column j: row j / nh, head j % nh; columns past the last repeat it
+            auto col_row = [&](int j, int& hh) {
+                j = j < ncols ? j : ncols - 1;
+                const int r = (int)((unsigned)j / (unsigned)nh);
+                hh = j - r * nh;
+                return it.row0 + r;
+            };
+            int unused;
+            const int pos = at.q.hist + col_row(slot * 32 + col, unused), kf = first_key(a, pos);
+            // tiles that every column of the job sees whole: full0 .. full1
+            const int jfirst = at.q.hist + col_row(slot * 32, unused), jlast = at.q.hist + col_row(slot * 32 + 31, unused);
+            const int full0 = (first_key(a, jlast) + 31) >> 5, full1 = ((jfirst + 1) >> 5) - 1;
+            const int ktb = it.kt0 + tile0;                          // the piece's first tile
+            const int ntile = tile1 - tile0, stages = (ntile + KSP - 1) / KSP;
+
+            // ---- tiles on their way into LDS: stage st has the tiles ktb + KSP st + (0 .. KSP - 1) ----
+            // the page of this wave's block, -1: not a page, -2: nobody looks at it
+            auto page_at = [&](int st) {
+                const int t = st * KSP + ut, key = (ktb + t) * 32 + ub * 16;
+                if (t >= ntile || key + 15 < it.kfirst || key > it.klast) return -2;
+                return __builtin_amdgcn_readfirstlane(a.p.page_of(at.s, key));
+            };
+            auto block_at = [&](int st, int pg) {
+                return a.p.block_of(pg < 0 ? 0 : pg, kvh, (ktb + st * KSP + ut) * 32 + ub * 16);
+            };
+            auto block_rsrc = [&](size_t block, int pg) {
+                return __builtin_amdgcn_make_buffer_rsrc((void*)((uv ? a.p.vp : a.p.kp) + block * (16 * HD * ES)), 0,
+                                                         pg < 0 ? 0 : 16 * HD * ES, kBufWord3);
+            };
+            // tokens of this wave's block that somebody looks at, as bits
+            auto block_use = [&](int st) {
+                const int key = (ktb + st * KSP + ut) * 32 + ub * 16;
+                unsigned u = 0xffffu;
+                if (it.kfirst > key) u &= it.kfirst - key < 16 ? 0xffffu << (it.kfirst - key) : 0u;
+                if (it.klast < key + 15) u &= it.klast >= key ? 0xffffu >> (15 - (it.klast - key)) : 0u;
+                return u;
+            };
+            uint8_t* const mine_meta = lds + kMetaMarks + ub * 4;
+            int pg = page_at(0);
+            // straight to LDS (K or V, as this wave has it)
+            auto copy = [&](int st) {
+                const __amdgpu_buffer_rsrc_t r = block_rsrc(block_at(st, pg), pg);
+                uint8_t* to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut)) + (ub * KC + piece0) * 1024;
+#pragma unroll
+                for (int i = 0; i < PCS; i++) buf_load_lds16(r, to + i * 1024, piece0 * 1024 + lane * 16, i * 1024);
+                if (uv && piece0 == 0 && lane == 0) *reinterpret_cast<unsigned*>(mine_meta + P::meta_at(st, ut)) = pg == -1 ? 0xffffu : 0u;
+                pg = page_at(st + 1);
+            };
+            // through registers
+            uint4 raw[M::REG ? PCS : 1];
+            float raw_scale = 0.0f;
+            int raw_pg = 0;
+            auto fetch = [&](int st) {
+                const size_t block = block_at(st, pg);
+                const __amdgpu_buffer_rsrc_t r = block_rsrc(block, pg);
+#pragma unroll
+                for (int i = 0; i < PCS; i++) raw[i] = buf_load16(r, piece0 * 1024 + lane * 16, i * 1024);
+                if (M::Q8) raw_scale = reinterpret_cast<const float*>((uv ? a.p.vp : a.p.kp) + a.p.scale_off)[block * 16 + t16];
+                raw_pg = pg;
+                pg = page_at(st + 1);
+            };
+            auto put = [&](int st) {
+                uint8_t* to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut));
+                float* meta = reinterpret_cast<float*>(lds + P::meta_at(st, ut));
+                const unsigned use = block_use(st);
+                unsigned marks = raw_pg == -1 ? 0xffffu : 0u;
+                if constexpr (M::Q8) {
+                    const bool on = use >> t16 & 1 && raw_pg >= 0;
+                    // scales that are not finite: of heads with infinities or NaN
+                    const bool bad = on && !(fabsf(raw_scale) < INFINITY);
+                    marks |= (unsigned)__ballot(bad && g == 0) & 0xffffu;
+                    if (g == 0 && piece0 == 0) meta[(uv ? kMetaV / 4 : 0) + ub * 16 + t16] = on && !bad ? raw_scale : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < PCS; i++) {
+                        const int c = piece0 + i;
+                        const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                        unsigned y[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const int c0 = (int8_t)(w[k >> 1] >> (k & 1 ? 16 : 0)), c1 = (int8_t)(w[k >> 1] >> (k & 1 ? 24 : 8));
+                            y[k] = hi_halves(__float_as_uint((float)c0), __float_as_uint((float)c1));
+                        }
+                        if (uv) {
+                            // dims 64 c + 16 k + t16 of tokens 4 g .. 4 g + 3
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                *reinterpret_cast<uint2*>(to + ((2 * c + (k >> 1)) * 2 + ub) * 1024 +
+                                                          ((g & 1) * 32 + (k & 1) * 16 + t16) * 16 + (g >> 1) * 8) =
+                                    make_uint2(y[2 * k], y[2 * k + 1]);
+                        } else {
+                            // dims 64 c + 16 g .. + 15 of token t16
+#pragma unroll
+                            for (int k = 0; k < 2; k++)
+                                *reinterpret_cast<uint4*>(to + (4 * c + g) * 1024 + (k * 32 + ub * 16 + t16) * 16) =
+                                    make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                        }
+                    }
+                } else if constexpr (M::F) {
+                    if (!uv) {
+                        // dims 16 i + 4 g .. + 3 of token t16
+                        unsigned top = 0;
+#pragma unroll
+                        for (int i = 0; i < PCS; i++) {
+                            const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                            for (int k = 0; k < 4; k++) top = (w[k] & 0x7fffffffu) > top ? w[k] & 0x7fffffffu : top;
+                        }
+#pragma unroll
+                        for (int d = 16; d < 64; d <<= 1) {
+                            const unsigned o = __shfl_xor(top, d, 64);
+                            top = o > top ? o : top;
+                        }
+                        int e = (int)(top >> 23) > kLowK ? (int)(top >> 23) : kLowK;
+                        const bool bad = e == 255;
+                        if (bad) e = kLowK;
+                        marks |= (unsigned)__ballot(bad && g == 0 && (use >> t16 & 1)) & 0xffffu;
+                        const float sf = row_scale(e);
+                        if (g == 0) meta[ub * 16 + t16] = row_scale_inv(e);
+#pragma unroll
+                        for (int i = 0; i < PCS; i++) {
+                            h2v_t hi[2], lo[2];
+                            split2(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y), sf, hi[0], lo[0]);
+                            split2(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w), sf, hi[1], lo[1]);
+                            uint8_t* w = to + i * 1024 + ((g >> 1) * 32 + ub * 16 + t16) * 16 + (g & 1) * 8;
+                            *reinterpret_cast<uint2*>(w) = make_uint2(h2_bits(hi[0]), h2_bits(hi[1]));
+                            *reinterpret_cast<uint2*>(w + 64 * HD) = make_uint2(h2_bits(lo[0]), h2_bits(lo[1]));
+                        }
+                    } else {
+                        // dim 16 i + t16 of tokens 4 g .. 4 g + 3
+                        unsigned top[4] = {};
+#pragma unroll
+                        for (int i = 0; i < PCS; i++) {
+                            const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                            for (int k = 0; k < 4; k++) top[k] = (w[k] & 0x7fffffffu) > top[k] ? w[k] & 0x7fffffffu : top[k];
+                        }
+                        float sf[4];
+                        int low = 113;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+#pragma unroll
+                            for (int d = 1; d < 16; d <<= 1) {
+                                const unsigned o = __shfl_xor(top[k], d, 64);
+                                top[k] = o > top[k] ? o : top[k];
+                            }
+                            int e = (int)(top[k] >> 23) > kLowV ? (int)(top[k] >> 23) : kLowV;
+                            const bool on = use >> (4 * g + k) & 1, bad = e == 255;
+                            if (bad || !on) e = kLowV;
+                            // rows that nobody looks at, or that are not finite: zeros
+                            if (bad || !on) {
+#pragma unroll
+                                for (int i = 0; i < PCS; i++) {
+                                    if (k == 0) raw[i].x = 0;
+                                    else if (k == 1) raw[i].y = 0;
+                                    else if (k == 2) raw[i].z = 0;
+                                    else raw[i].w = 0;
+                                }
+                            }
+                            const u64 b = __ballot(bad && on && t16 == 0);   // lanes 0, 16, 32, 48: tokens k, 4 + k, ..
+#pragma unroll
+                            for (int j = 0; j < 4; j++) marks |= (unsigned)(b >> (16 * j) & 1) << (4 * j + k);
+                            sf[k] = row_scale(e);
+                            if (on && e - 141 < low) low = e - 141;
+                            if (t16 == 0) {
+                                meta[kMetaV / 4 + ub * 16 + 4 * g + k] = (float)(e - 141);
+                                meta[kMetaInv / 4 + ub * 16 + 4 * g + k] = sf[k];
+                            }
+                        }
+                        int o = __shfl_xor(low, 16, 64);
+                        low = o < low ? o : low;
+                        o = __shfl_xor(low, 32, 64);
+                        low = o < low ? o : low;
+                        if (lane == 0) meta[kMetaLost / 4 + ub] = __builtin_ldexpf(1.0f, 48 - 126 - low);
+#pragma unroll
+                        for (int i = 0; i < PCS; i++) {
+                            h2v_t hi[2], lo[2];
+                            split2(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y), sf[0], sf[1], hi[0], lo[0]);
+                            split2(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w), sf[2], sf[3], hi[1], lo[1]);
+                            uint8_t* w = to + ((i >> 1) * 2 + ub) * 1024 + ((g & 1) * 32 + (i & 1) * 16 + t16) * 16 + (g >> 1) * 8;
+                            *reinterpret_cast<uint2*>(w) = make_uint2(h2_bits(hi[0]), h2_bits(hi[1]));
+                            *reinterpret_cast<uint2*>(w + 64 * HD) = make_uint2(h2_bits(lo[0]), h2_bits(lo[1]));
+                        }
+                    }
+                }
+                // K's and V's marks have a word each: [K or V][block]
+                if (piece0 == 0 && lane == 0) reinterpret_cast<unsigned*>(meta)[kMetaMarks / 4 + (uv ? 0 : 4) + ub] = marks;
+            };
+
+            // ---- q: 32 columns' rows through places in LDS that the first stage leaves free ----
+            op q[NQ][KS];
+            float fq = fabsf(a.scale) * kLog2e;
+            constexpr int kBox = KSP == 2 ? TB : DS == 1 ? TB / 2 : TB / 4, kPasses = 32 * P::RB / kBox;
+            constexpr int kChunks = P::RB / 16 / kPasses, kSteps = KS / kPasses;
+            static_assert(kBox == 32 * kChunks * 16 && kSteps * kPasses == KS, "q");
+            uint8_t* box = lds + (KSP == 2 ? (slot < 2 ? 2 + slot : slot == 2 ? 5 : 7) * TB
+                                  : DS == 1 ? (wave < 2 ? TB : 2 * TB) + wave * (TB / 2)
+                                  : wave < 4 ? TB + wave * (TB / 4) : P::XCH + (wave - 4) * (TB / 4));
+            auto q_row = [&](int pass) {
+                return [=](int r) {
+                    int hh;
+                    const int row = col_row(slot * 32 + r, hh);
+                    return (const uint8_t*)((const E*)a.q + (size_t)(at.q.r0 + row) * a.q_stride + (size_t)(head0 + hh) * HD +
+                                            part * (HD / DS)) + pass * kChunks * 16;
+                };
+            };
+            auto chunk = [&](int c) { return box + row_slot<kChunks>(col, c); };
+            auto load_q = [&]() {
+                if constexpr (TQ != G4_F32) {
+                    const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+                    for (int pass = 0; pass < kPasses; pass++) {
+                        if constexpr (KSP == 2) {
+                            rows_to_lds<kChunks, 16>(box, kp * 16, q_row(pass));
+                            lds_barrier();
+                        } else {
+                            rows_to_lds<kChunks, 32>(box, 0, q_row(pass));
+                        }
+#pragma unroll
+                        for (int i = 0; i < kSteps; i++) {
+                            uint4 x = *reinterpret_cast<const uint4*>(chunk(i * 2 + h));
+                            if (a.scale == 0.0f) x = make_uint4(0, 0, 0, 0);
+                            x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                            q[0][pass * kSteps + i] = __builtin_bit_cast(op, x);
+                        }
+                    }
+                    if (a.scale == 0.0f) fq = 1.0f;
+                } else if constexpr (NQ == 3) {
+                    // times scale log2(e), as three terms: the float itself
+                    const float qs = a.scale * kLog2e;
+#pragma unroll
+                    for (int pass = 0; pass < kPasses; pass++) {
+                        rows_to_lds<kChunks, 32>(box, 0, q_row(pass));
+#pragma unroll
+                        for (int i = 0; i < kSteps; i++) {
+                            const float4 x = *reinterpret_cast<const float4*>(chunk(i * 4 + h * 2));
+                            const float4 y = *reinterpret_cast<const float4*>(chunk(i * 4 + h * 2 + 1));
+                            uint32_t t[4][3];
+                            split_pair<3>(x.x * qs, x.y * qs, t[0]);
+                            split_pair<3>(x.z * qs, x.w * qs, t[1]);
+                            split_pair<3>(y.x * qs, y.y * qs, t[2]);
+                            split_pair<3>(y.z * qs, y.w * qs, t[3]);
+#pragma unroll
+                            for (int k = 0; k < NQ; k++) {
+                                const uint4 z = make_uint4(t[0][k], t[1][k], t[2][k], t[3][k]);
+                                q[k][pass * kSteps + i] = __builtin_bit_cast(op, z);
+                            }
+                        }
+                    }
+                    fq = 1.0f;
+                } else {
+                    float4 x[KS][2];
+                    unsigned top = 0;
+#pragma unroll
+                    for (int pass = 0; pass < kPasses; pass++) {
+                        rows_to_lds<kChunks, 32>(box, 0, q_row(pass));
+#pragma unroll
+                        for (int i = 0; i < kSteps; i++)
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                const float4 y = *reinterpret_cast<const float4*>(chunk(i * 4 + h * 2 + j));
+                                x[pass * kSteps + i][j] = y;
+                                const float e[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    const unsigned b = __float_as_uint(e[k]) & 0x7fffffffu;
+                                    top = b > top ? b : top;
+                                }
+                            }
+                    }
+                    unsigned o = __shfl_xor(top, 32, 64);
+                    top = o > top ? o : top;
+                    if constexpr (DS == 2) {
+                        // of both halves: the partial scores have to be of one scale
+                        unsigned* xch = reinterpret_cast<unsigned*>(lds + P::XCH);
+                        xch[wave * 64 + lane] = top;
+                        lds_barrier();
+                        o = xch[(wave ^ 1) * 64 + lane];
+                        top = o > top ? o : top;
+                    }
+                    const int e = (int)(top >> 23) > kLowK ? (int)(top >> 23) : kLowK;
+                    float sf = row_scale(e < 255 ? e : 254);
+                    fq *= e < 255 ? row_scale_inv(e) : __uint_as_float(0x7fc00000u);
+                    if (a.scale < 0.0f) sf = -sf;
+                    if (a.scale == 0.0f) {   // a score of -infinity times fq has to stay one
+                        sf = 0.0f;
+                        fq = e < 255 ? 1.0f : fq;
+                    }
+#pragma unroll
+                    for (int i = 0; i < KS; i++) {
+                        h2v_t hi[4], lo[4];
+                        split2(x[i][0].x, x[i][0].y, sf, hi[0], lo[0]);
+                        split2(x[i][0].z, x[i][0].w, sf, hi[1], lo[1]);
+                        split2(x[i][1].x, x[i][1].y, sf, hi[2], lo[2]);
+                        split2(x[i][1].z, x[i][1].w, sf, hi[3], lo[3]);
+                        __builtin_memcpy(&q[0][i], hi, 16);
+                        __builtin_memcpy(&q[1][i], lo, 16);
+                    }
+                }
+            };
+
+            // ---- first stage, q ----
+            if constexpr (M::REG) {
+                fetch(0);
+                load_q();
+                if constexpr (DS == 2) {
+                    lds_barrier();   // the boxes have been read
+                    if (!uv) {
+                        put(0);
+                        fetch(1);
+                    }
+                } else {
+                    put(0);
+                    fetch(1);
+                }
+            } else {
+                if (DS == 1 || !uv) copy(0);
+                load_q();
+                if (DS == 2) lds_barrier();
+            }
+            f16_t o[NT] = {};
+            float m = -FLT_MAX, l = 0.0f;
+            f16_t sc;
+            op p[NP][2];
+            struct Ops {
+                op x[NK];
+            };
+            // lane's place in a tile
+            const int kbase = M::REG ? lane * 16 : (col >> 4) * KC * 1024 + h * 256 + (col & 15) * 16;
+            const int vbase = M::REG ? lane * 16 : (h * 16 + (col & 15)) * 16 + (col >> 4) * 8;
+            auto read_k = [&](const uint8_t* from, int i, Ops& k) {
+                const int s = part * KS + i;
+#pragma unroll
+                for (int j = 0; j < NK; j++)
+                    k.x[j] = *reinterpret_cast<const op*>(from + kbase + (M::REG ? j * 64 * HD + s * 1024 : (s >> 1) * 1024 + (s & 1) * 512));
+            };
+            auto read_v = [&](const uint8_t* from, int i, Ops& v) {
+                const int s = part * NT * 2 + i;
+                if constexpr (M::REG) {
+#pragma unroll
+                    for (int j = 0; j < NK; j++) v.x[j] = *reinterpret_cast<const op*>(from + vbase + j * 64 * HD + s * 1024);
+                } else {
+                    const uint8_t* x = from + vbase + (s & 1) * KC * 1024 + (s >> 1) * 1024;
+                    const uint2 y = *reinterpret_cast<const uint2*>(x), z = *reinterpret_cast<const uint2*>(x + 512);
+                    v.x[0] = __builtin_bit_cast(op, make_uint4(y.x, y.y, z.x, z.y));
+                }
+            };
+            auto scores = [&](int st) {
+                const uint8_t* from = lds + P::k_at(st, kp);
+                sc = f16_t{};
+                if constexpr (NQ == 1) {
+#pragma unroll
+                    for (int i = 0; i < KS; i++) {
+                        Ops k;
+                        read_k(from, i, k);
+                        sc = mfma32(k.x[0], q[0][i], sc);
+                    }
+                    order_products<KS, 3, 1, 1>();
+                } else {
+                    f16_t sx = {};
+                    run_products<Ops, KS, 2>([&](int i, Ops& k) { read_k(from, i, k); },
+                                             [&](int i, const Ops& k) {
+                                                 sc = mfma32(k.x[0], q[0][i], sc);
+#pragma unroll
+                                                 for (int j = 1; j < NQ; j++) sx = mfma32(k.x[0], q[j][i], sx);
+                                                 if constexpr (NK == 2) sx = mfma32(k.x[1], q[0][i], sx);
+                                             });
+                    sc += sx;
+                }
+            };
+            auto weights = [&](int st) {
+                const int kt = ktb + st * KSP + kp;
+                const float* meta = reinterpret_cast<const float*>(lds + P::meta_at(st, kp));
+                const unsigned* mk = reinterpret_cast<const unsigned*>(meta) + kMetaMarks / 4;
+                unsigned marks = mk[0] | mk[1] << 16;
+                if (M::REG) marks |= mk[4] | mk[5] << 16;
+                marks = __builtin_amdgcn_readfirstlane(marks);
+                float fv[16];       // codes: V's scales, fp32: 2^-e
+                if constexpr (M::REG) {
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        const float4 xk = *reinterpret_cast<const float4*>(meta + 8 * b + 4 * h);
+                        const float4 xv = *reinterpret_cast<const float4*>(meta + kMetaV / 4 + 8 * b + 4 * h);
+                        const float k[4] = {xk.x, xk.y, xk.z, xk.w}, v[4] = {xv.x, xv.y, xv.z, xv.w};
+                        if constexpr (M::F) {
+                            const float4 xi = *reinterpret_cast<const float4*>(meta + kMetaInv / 4 + 8 * b + 4 * h);
+                            const float vi[4] = {xi.x, xi.y, xi.z, xi.w};
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                sc[4 * b + i] = __builtin_fmaf(sc[4 * b + i], fq * k[i], v[i]);
+                                fv[4 * b + i] = vi[i];
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                sc[4 * b + i] *= NQ == 3 ? k[i] : fq * k[i];
+                                fv[4 * b + i] = v[i];
+                            }
+                        }
+                    }
+                }
+                if (marks) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (marks >> (8 * (r >> 2) + 4 * h + (r & 3)) & 1) sc[r] = __uint_as_float(0x7fc00000u);
+                }
+                if (kt < full0 || kt > full1) {
+                    const int hi = pos - kt * 32 - 4 * h, lo = kf - kt * 32 - 4 * h;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int key = 8 * (r >> 2) + (r & 3);
+                        if (key > hi || key < lo) sc[r] = -INFINITY;
+                    }
+                }
+                float top = sc[0];
+#pragma unroll
+                for (int r = 1; r < 16; r++) top = fmaxf(top, sc[r]);
+                if constexpr (M::kRaw) top *= fq;
+                if (__any(top > m + M::kSlack)) {
+                    top = fmaxf(top, shfl_xor(top, 32));
+                    top = fmaxf(top + M::kRaise, m);
+                    const float f = exp2f(m - top);
+                    if constexpr (M::F) l = move_sum(l, m - top);
+                    else l *= f;
+                    m = top;
+#pragma unroll
+                    for (int i = 0; i < NT; i++) o[i] *= f;
+                }
+                const float base = m - M::kLift;
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float x = sc[8 * t + j];
+                        w[j] = __builtin_amdgcn_exp2f(M::kRaw ? __builtin_fmaf(x, fq, -base) : x - base);
+                        if constexpr (M::F) l = __builtin_fmaf(w[j], fv[8 * t + j], l);
+                        else l += w[j];
+                        if constexpr (M::Q8) w[j] *= fv[8 * t + j];
+                    }
+                    if constexpr (NP == 1) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) p[0][t][j] = (E)w[j];
+                    } else if constexpr (M::kHalf) {
+                        h2v_t hi[4], lo[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) split2(w[2 * j], w[2 * j + 1], 1.0f, hi[j], lo[j]);
+                        __builtin_memcpy(&p[0][t], hi, 16);
+                        __builtin_memcpy(&p[1][t], lo, 16);
+                    } else {
+                        // two terms, each rounded to nearest: within 2^-18 of the weight
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            p[0][t][j] = (__bf16)w[j];
+                            p[1][t][j] = (__bf16)(w[j] - (float)p[0][t][j]);
+                        }
+                    }
+                }
+                if constexpr (M::F) {
+                    const float lost = __uint_as_float(__builtin_amdgcn_readfirstlane(
+                        __float_as_uint(fmaxf(meta[kMetaLost / 4], meta[kMetaLost / 4 + 1]))));
+                    if (__any(l < lost)) {
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const int key = 8 * (r >> 2) + 4 * h + (r & 3);
+                            l += lost_weight(sc[r] - base, meta[kMetaV / 4 + key], fv[r]);
+                        }
+                    }
+                }
+            };
+            auto values = [&](int st) {
+                const uint8_t* from = lds + P::v_at(st, kp);
+                if constexpr (NP == 1) {
+#pragma unroll
+                    for (int i = 0; i < 2 * NT; i++) {
+                        Ops v;
+                        read_v(from, i, v);
+                        o[i >> 1] = mfma32(v.x[0], p[0][i & 1], o[i >> 1]);
+                    }
+                    order_products<2 * NT, 3, 1, 1>();
+                } else {
+                    run_products<Ops, 2 * NT, 2>([&](int i, Ops& v) { read_v(from, i, v); },
+                                                 [&](int i, const Ops& v) {
+                                                     f16_t& s = o[i >> 1];
+                                                     s = mfma32(v.x[0], p[0][i & 1], s);
+                                                     s = mfma32(v.x[0], p[1][i & 1], s);
+                                                     if constexpr (NK == 2) s = mfma32(v.x[1], p[0][i & 1], s);
+                                                 });
+                }
+            };
+            // Tiles that came straight from the pages: V of tokens that nobody looks at
+            // becomes zeros (whatever is there: a weight of 0 times it has to be 0), and
+            // where a result was not finite (careful) so do infinities and NaN, whose keys
+            // are marked: a column that sees one gets the score NaN, the others the bits
+            // they would have without it.
+            auto clean = [&](int st, bool careful) {
+                if (M::REG || !uv || piece0 != 0) return;
+                const unsigned use = block_use(st);
+                uint8_t* v = lds + P::v_at(st, ut) + ub * KC * 1024;
+                unsigned seen = 0;
+                for (int i = lane; i < KC * 64; i += 64) {
+                    uint4 x = *reinterpret_cast<const uint4*>(v + i * 16);
+                    const int t0 = (i >> 4 & 3) * 4;
+                    unsigned w[4] = {x.x, x.y, x.z, x.w};
+                    constexpr unsigned kInf = TC == G4_F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int t = t0 + (k & 3);
+                        const unsigned sh = 16 * (k & 1), e = w[k >> 1] >> sh & kInf;
+                        const bool bad = careful && e == kInf;
+                        if (bad || !(use >> t & 1)) w[k >> 1] &= ~(0xffffu << sh);
+                        if (bad && use >> t & 1) seen |= 1u << t;
+                    }
+                    *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                if (careful && seen) atomicOr(reinterpret_cast<unsigned*>(mine_meta + P::meta_at(st, ut)), seen);
+            };
+            // whether a stage has tokens that nobody looks at
+            auto ragged = [&](int st) {
+                const int k0 = (ktb + st * KSP) * 32, k1 = (st + 1) * KSP < ntile ? k0 + 32 * KSP - 1 : (ktb + ntile) * 32 - 1;
+                return k0 < it.kfirst || k1 > it.klast;
+            };
+
+            for (bool careful = false;; careful = true) {
+                if constexpr (DS == 1) {
+                    // this wave's copies have landed, then everyone's; and all are done
+                    // with the stage before (waves 4 .. 7 but for its V, which has three
+                    // places)
+                    auto turn = [&](int st) {
+                        if constexpr (M::REG) {
+                            lds_barrier();
+                            if (st + 1 < stages) {
+                                put(st + 1);
+                                fetch(st + 2);
+                            }
+                        } else {
+                            wait_vm<0>();
+                            lds_barrier();
+                            if (careful || ragged(st)) {
+                                clean(st, careful);
+                                lds_barrier();
+                            }
+                            if (st + 1 < stages) copy(st + 1);
+                        }
+                    };
+                    int st = 0;
+                    if (KSP == 1 || kp == 0) {
+                        for (; st < stages; st++) {
+                            turn(st);
+                            scores(st);
+                            weights(st);
+                            values(st);
+                        }
+                    } else {
+                        turn(st);
+                        if (kp < ntile) {
+                            scores(st);
+                            weights(st);
+                        }
+                        for (st++; st < stages; st++) {
+                            turn(st);
+                            values(st - 1);
+                            if (st * KSP + kp < ntile) {
+                                scores(st);
+                                weights(st);
+                            }
+                        }
+                        if ((stages - 1) * KSP + kp < ntile) values(stages - 1);
+                    }
+                } else {
+                    f4_t* xch = reinterpret_cast<f4_t*>(lds + P::XCH);
+                    for (int st = 0; st < stages; st++) {
+                        if constexpr (!M::REG) wait_vm<0>();
+                        lds_barrier();   // K is there, V of the tile before done with
+                        if (uv) {
+                            if constexpr (M::REG) {
+                                put(st);
+                                fetch(st + 1);
+                            } else {
+                                copy(st);
+                            }
+                        }
+                        scores(st);
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            xch[(wave * 4 + i) * 64 + lane] = f4_t{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+                        if constexpr (!M::REG) {
+                            if (uv) wait_vm<0>();
+                        }
+                        lds_barrier();   // K is done with, the partial scores and V are there
+                        if constexpr (!M::REG) {
+                            if (careful || ragged(st)) {
+                                clean(st, careful);
+                                lds_barrier();
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const f4_t y = xch[((wave ^ 1) * 4 + i) * 64 + lane];
+#pragma unroll
+                            for (int j = 0; j < 4; j++) sc[4 * i + j] += y[j];
+                        }
+                        weights(st);
+                        if (!uv && st + 1 < stages) {
+                            if constexpr (M::REG) {
+                                put(st + 1);
+                                fetch(st + 2);
+                            } else {
+                                copy(st + 1);
+                            }
+                        }
+                        values(st);
+                    }
+                }
+                // ---- a result that is not finite: once more, carefully ----
+                if (M::REG || careful) break;
+                float z = 0.0f * l;
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) z = __builtin_fmaf(0.0f, o[i][r], z);
+                unsigned* votes = reinterpret_cast<unsigned*>(red);
+                const bool odd = __any(!(z == 0.0f));
+                if (lane == 0) votes[wave] = odd;
+                wait_vm<0>();
+                lds_barrier();
+                unsigned any = 0;
+#pragma unroll
+                for (int w = 0; w < NW; w++) any |= votes[w];
+                if (!__builtin_amdgcn_readfirstlane(any)) break;
+#pragma unroll
+                for (int i = 0; i < NT; i++) o[i] = f16_t{};
+                m = -FLT_MAX;
+                l = 0.0f;
+                pg = page_at(0);
+                if (DS == 1 || !uv) copy(0);
+            }
+
+            const bool whole = tile0 == 0 && tile1 == it.tiles;
+            l += shfl_xor(l, 32);
+            wait_vm<0>();
+            lds_barrier();
+            if constexpr (KSP == 2) {
+                // waves 4 .. 7 hand their sums to waves 0 .. 3
+                float* ml = reinterpret_cast<float*>(lds + NJ * HD * 128) + slot * 64 + col * 2;
+                f4_t* sums = reinterpret_cast<f4_t*>(lds) + slot * HD * 8 + lane;
+                if (kp == 1) {
+                    if (h == 0) {
+                        ml[0] = m;
+                        ml[1] = l;
+                    }
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int b = 0; b < 4; b++)
+                            sums[(i * 4 + b) * 64] = f4_t{o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
+                }
+                lds_barrier();
+                if (kp == 0) {
+                    const float m1 = ml[0], l1 = ml[1], top = fmaxf(m, m1);
+                    const float f0 = exp2f(m - top), f1 = exp2f(m1 - top);
+                    l = l * f0 + l1 * f1;
+                    m = top;
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int b = 0; b < 4; b++) {
+                            const f4_t y = sums[(i * 4 + b) * 64];
+#pragma unroll
+                            for (int j = 0; j < 4; j++) o[i][4 * b + j] = o[i][4 * b + j] * f0 + y[j] * f1;
+                        }
+                }
+            }
+            if (mine && kp == 0) {
+                if (whole) {
+                    // ---- the output's rows, where K and V (KSP 2: this wave's other sums) were ----
+                    wave_lds_order();
+                    const float f = 1.0f / l;
+                    constexpr int kRow = P::RB / 16;
+                    uint8_t* rows = lds + (KSP == 2 ? slot * HD * 128 : wave * 32 * P::RB);
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int b = 0; b < 4; b++) {
+                            E y[4];
+#pragma unroll
+                            for (int j = 0; j < 4; j++) y[j] = (E)(o[i][4 * b + j] * f);
+                            uint8_t* to = rows + (TQ == G4_F32 ? row_slot<kRow>(col, i * 8 + 2 * b + h)
+                                                               : row_slot<kRow>(col, i * 4 + b) + h * 8);
+                            __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(E)), y, 4 * sizeof(E));
+                        }
+                    rows_from_lds<kRow>(rows, ncols - slot * 32, [&](int r) {
+                        int hh;
+                        const int row = col_row(slot * 32 + r, hh);
+                        return (uint8_t*)((E*)a.out + (size_t)(at.q.r0 + row) * a.out_stride + (size_t)(head0 + hh) * HD +
+                                          part * (HD / DS));
+                    });
+                } else {
+                    float* to = a.part + (size_t)(share * 2 + (tile0 == 0)) * part_floats(a.cols, HD);
+                    f4_t* sums = reinterpret_cast<f4_t*>(to) + (size_t)(slot * DS + part) * NT * 256 + lane;
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int b = 0; b < 4; b++)
+                            sums[(i * 4 + b) * 64] = f4_t{o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
+                    if (part == 0 && h == 0)
+                        *reinterpret_cast<float2*>(to + (size_t)a.cols * HD + (slot * 32 + col) * 2) = make_float2(m, l);
+                }
+            }
+            lds_barrier();   // LDS is the next item's
+        }
+        left -= take;
+        if (!left) break;
+        // ---- the next item ----
+        at.x = 0;
+        if (++at.item >= seq_items(a, at.q)) {
+            at.item = 0;
+            if (++at.rep == a.p.n_kv * a.ngrp) {
+                at.rep = 0;
+                do {
+                    if (++at.s >= a.n_seqs) return;
+                    at.q = seq_of(a, a.cu[at.s], a.cu[at.s + 1], a.lens[at.s]);
+                } while (at.q.n == 0);
+            }
+        }
+        at.size = item_measure(a, at.q, at.item);
     }
 }
 
-// ---- one launch, fp32 throughout: a workgroup a row and head ------------------
-template <int TQ, int TC, int HD>
-__global__ __launch_bounds__(256) void attn_chunk_row_kernel(ChunkArgs a) {
-    typedef typename Row<TQ>::t E;
-    constexpr int N = HD / 64;
-    const int row = blockIdx.x, h = blockIdx.y, kvh = h / a.group;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __shared__ float red[4][HD + 2];
-    const SeqAt sq = find_seq(a.cu, a.lens, a.n_seqs, 1, 0, 0, (unsigned)row);
-    if (sq.r0 < 0 || sq.r1 > a.m || row < sq.r0 || row >= sq.r1 || sq.r1 - sq.r0 > sq.len || !a.p.fits(sq.len)) return;
-    const int last = sq.len - sq.r1 + row, first = a.window > 0 && last >= a.window ? last + 1 - a.window : 0;
-    const E* qr = (const E*)a.q + (size_t)row * a.q_stride + (size_t)h * HD + lane * N;
-    float q[N], o[N] = {}, m = -FLT_MAX, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; i++) q[i] = (float)qr[i] * (a.scale * kLog2e);
-    row_keys<TC, HD>(a.p, sq.s, kvh, first, last, (first & ~3) + 4 * wave, 4, q, m, l, o);
-#pragma unroll
-    for (int i = 0; i < N; i++) red[wave][lane * N + i] = o[i];
-    if (lane == 0) {
-        red[wave][HD] = m;
-        red[wave][HD + 1] = l;
+// ---- second launch: items of more than one share ---------------------------------
+// blockIdx: border between two shares, 32 columns, 128 dims (64 where there are
+// no more).  The first border inside an item joins its pieces, with the weights
+// 2^(m_i - max m).
+template <int TQ, int HD>
+__global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
+    typedef typename RowElem<TQ>::t E;
+    constexpr int D = HD < 128 ? HD : 128, V = D / 32;     // dims, 16-byte values of a thread
+    __shared__ u64 red[8];
+    Line line;
+    Place at;
+    const unsigned w = blockIdx.x + 1;
+    const int slot = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
+    if (!find_place<256>(a, [&](const Line& l) { return w < l.shares ? l.at(w) : ~(u64)0 / (a.p.n_kv * a.ngrp) / 2 * (a.p.n_kv * a.ngrp); },
+                         line, at, red))
+        return;
+    const u64 start = line.at(w) - at.x, end = start + at.size;      // the item's place on the line
+    if (at.x == 0 || line.at(w - 1) > start) return;                 // an item's start, or not the first border in it
+    const Item it(a, at);
+    const int kvh = at.rep / a.ngrp, hg = at.rep - kvh * a.ngrp;
+    const int nh = a.group - hg * a.gh < a.gh ? a.group - hg * a.gh : a.gh, ncols = it.rows * nh;
+    if (slot * 32 >= ncols) return;
+    // piece i is share w - 1 + i's: tiles from edge(i) to edge(i + 1)
+    auto edge = [&](int i) {
+        if (i == 0) return 0;
+        const u64 u = w - 1 + i < line.shares ? line.at(w - 1 + i) : line.total;
+        return u >= end ? it.tiles : it.tile_at(u - start, at.size);
+    };
+    auto piece = [&](int i) { return a.part + (size_t)((w - 1 + i) * 2 + (edge(i) == 0)) * part_floats(a.cols, HD); };
+    // the pieces that have tiles; one alone has been written
+    int pieces = 0, some = 0;
+    for (int e = 0; e < it.tiles; pieces++) {
+        const int e1 = edge(pieces + 1);
+        some += e1 > e;
+        e = e1;
     }
-    lds_sync();
-    float top = red[0][HD], f[4], den = 0.0f;
+    if (some < 2) return;
+    const size_t ml = (size_t)a.cols * HD + (slot * 32 + col) * 2;
+    float top = -FLT_MAX;
+    for (int i = 0; i < pieces; i++)
+        if (edge(i) < edge(i + 1)) top = fmaxf(top, piece(i)[ml]);
+    f4_t x[V] = {};
+    float l = 0.0f;
+    for (int i = 0; i < pieces; i++) {
+        if (edge(i) >= edge(i + 1)) continue;
+        const float* from = piece(i);
+        const float2 y = *reinterpret_cast<const float2*>(from + ml);
+        const float f = exp2f(y.x - top);
+        l += f * y.y;
+        const f4_t* sums = reinterpret_cast<const f4_t*>(from) + (size_t)slot * HD * 8 + z * D * 8 + tid;
 #pragma unroll
-    for (int w = 1; w < 4; w++) top = fmaxf(top, red[w][HD]);
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        f[w] = exp2f(red[w][HD] - top);
-        den += f[w] * red[w][HD + 1];
+        for (int k = 0; k < V; k++) x[k] += sums[k * 256] * f;
     }
-    E* out = (E*)a.out + (size_t)row * a.out_stride + (size_t)h * HD;
-    for (int d = threadIdx.x; d < HD; d += 256) {
-        float num = 0.0f;
+    if (slot * 32 + col >= ncols) return;
+    const int r = (int)((unsigned)(slot * 32 + col) / (unsigned)nh), hh = slot * 32 + col - r * nh;
+    E* out = (E*)a.out + (size_t)(at.q.r0 + it.row0 + r) * a.out_stride + (size_t)(kvh * a.group + hg * a.gh + hh) * HD + z * D;
+    const float f = 1.0f / l;
 #pragma unroll
-        for (int w = 0; w < 4; w++) num += f[w] * red[w][d];
-        out[d] = (E)(num / den);
+    for (int k = 0; k < V; k++) {
+        // registers 4 b .. + 3 of 32-dim tile k: dims 8 b + 4 h .. + 3
+        const int d = k * 32 + (tid >> 6) * 8 + 4 * h;
+        const E y[4] = {(E)(x[k][0] * f), (E)(x[k][1] * f), (E)(x[k][2] * f), (E)(x[k][3] * f)};
+        __builtin_memcpy(__builtin_assume_aligned(out + d, 4 * sizeof(E)), y, 4 * sizeof(E));
     }
 }
 
+// columns of a workgroup, and what follows from it
+void set_columns(ChunkArgs& a, int cols) {
+    a.gh = a.group < cols ? a.group : cols;
+    a.ngrp = (a.group + a.gh - 1) / a.gh;
+    a.rpi = cols / a.gh;
+    const long used = (long)a.m * a.gh;
+    a.cols = used < cols ? (int)((used + 31) / 32 * 32) : cols;
+}
+
 template <int TQ, int TC, int HD>
-int launch_chunk(const ChunkArgs& a) {
-    hipLaunchKernelGGL((attn_chunk_row_kernel<TQ, TC, HD>), dim3(a.m, a.n_heads), dim3(256), 0, g4_stream(), a);
-    return g4_check_launch("attn_chunk_row_kernel");
+int launch_chunk(ChunkArgs a) {
+    typedef Plan<TQ, TC, HD> P;
+    set_columns(a, P::COLS);
+    auto kernel = attn_chunk_kernel<TQ, TC, HD>;
+    // more than 64 KB of LDS has to be asked for, once on each device
+    static std::atomic<unsigned long long> asked{0};
+    int dev = 0;
+    G4_HIP(hipGetDevice(&dev));
+    if (dev >= 64 || !(asked >> dev & 1)) {
+        G4_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS));
+        if (dev < 64) asked |= 1ull << dev;
+    }
+    hipLaunchKernelGGL(kernel, dim3(kShares), dim3(64 * P::NW), P::LDS, g4_stream(), a);
+    hipLaunchKernelGGL((attn_chunk_join_kernel<TQ, HD>), dim3(kShares - 1, a.cols / 32, HD < 128 ? 1 : HD / 128), dim3(256), 0,
+                       g4_stream(), a);
+    return g4_check_launch("attn_chunk_kernel");
 }
 template <int TQ, int TC>
 int launch_chunk(const ChunkArgs& a, int hd) {
@@ -173,7 +1149,10 @@ using namespace g4;
 extern "C" size_t g4_attn_chunk_paged_part_bytes(int m, int n_heads, int n_kv, int hd) {
     if (m < 1 || n_heads < 1 || n_heads > 65535 || n_kv < 1 || n_heads % n_kv || (hd != 64 && hd != 128 && hd != 256 && hd != 512))
         return 0;
-    return 16;
+    // two partial results of each share
+    const int group = n_heads / n_kv, cols = 128, gh = group < cols ? group : cols;
+    const long used = (long)m * gh;
+    return (size_t)kShares * 2 * part_floats(used < cols ? (int)((used + 31) / 32 * 32) : cols, hd) * 4;
 }
 
 extern "C" int g4_attn_chunk_paged(const void* q, int q_stride, int q_type, const void* kp, const void* vp, int type,
@@ -192,7 +1171,7 @@ extern "C" int g4_attn_chunk_paged(const void* q, int q_stride, int q_type, cons
     G4_CHECK_ARG(q && cu && lens && part && out && al16(q) && al16(part) && al16(out), "%s: null or unaligned pointer", who);
     G4_CHECK_ARG(q_stride % (16 / es) == 0 && q_stride / hd >= n_heads && out_stride % (16 / es) == 0 && out_stride / hd >= n_heads,
                  "%s: strides %d, %d (multiples of %d, n_heads * hd at least)", who, q_stride, out_stride, 16 / es);
-    G4_CHECK_ARG(n_seqs > 0 && n_seqs <= kKvMaxSeqs && m > 0 && kv_grid_fits(m, 256), "%s: %d rows of %d sequences (1 to %d)", who, m,
+    G4_CHECK_ARG(n_seqs > 0 && n_seqs <= kKvMaxSeqs && m > 0, "%s: %d rows of %d sequences (1 to %d)", who, m,
                  n_seqs, kKvMaxSeqs);
     a.q = q; a.out = out; a.cu = cu; a.lens = lens; a.part = (float*)part; a.q_stride = q_stride; a.out_stride = out_stride;
     a.n_seqs = n_seqs; a.m = m; a.window = window; a.n_heads = n_heads; a.scale = attn_scale;

@@ -49,8 +49,9 @@ def bound_of(bound, want, q, k, v, qk, ck, scale):
         return bound + 2.0 ** -17 * big         # weights as two bf16 terms
     # operands within 2^-22 of themselves or 2^-39 of their row's largest (F32: q and K, and the smaller terms' product
     # left out): a score is off by that of sum |q| |k|, its weight by twice it; weights and V 2^-22 each
-    mags = np.abs(scale) * (np.abs(q).max((0, 1)) @ np.abs(k).max((0, 1)))
-    low = np.abs(scale) * 2.0 ** -39 * k.shape[-1] * np.abs(q).max() * np.abs(k).max()
+    kv = np.repeat(np.abs(k), q.shape[1] // k.shape[1], 1)
+    mags = np.abs(scale) * np.einsum("rhd,khd->rhk", np.abs(q), kv, optimize=True).max(-1)[..., None]
+    low = np.abs(scale) * 2.0 ** -39 * k.shape[-1] * np.abs(q).max(-1, keepdims=True) * np.abs(k).max()
     each = 3 if ck == pn.F32 else 1
     return bound + each * (2 * (2.0 ** -22 * mags + 2 * low) + 2.0 ** -22 + 2.0 ** -39) * big
 
