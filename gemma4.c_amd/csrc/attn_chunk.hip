@@ -8,7 +8,7 @@
 namespace g4 {
 namespace {
 
-constexpr int kShares = 256;   // workgroups that share the work, one a CU
+constexpr int kLgShares = 8, kShares = 1 << kLgShares;   // workgroups that share the work, one a CU
 constexpr int kLead = 64;      // keys that stand for what it costs to begin and to end an item
 constexpr int kLeast = 96;     // no smaller share than this
 
@@ -77,15 +77,19 @@ struct Place {
 };
 struct Line {
     u64 total;
-    unsigned shares;    // W
+    int lg;             // W = 2^lg
     // where share w begins: N w / W without overflow
-    __device__ __forceinline__ u64 at(unsigned w) const { return total / shares * w + total % shares * w / shares; }
+    __device__ __forceinline__ u64 at(unsigned w) const {
+        return (total >> lg) * w + (((unsigned)total & ((1u << lg) - 1)) * w >> lg);
+    }
 };
 __device__ __forceinline__ Line line_of(u64 total) {
-    const u64 most = total / kLeast;
-    return {total, most < 1 ? 1u : most < kShares ? (unsigned)most : (unsigned)kShares};
+    int lg = 0;
+    while (lg < kLgShares && (total >> (lg + 1)) >= kLeast) lg++;
+    return {total, lg};
 }
 
+constexpr u64 kNowhere = ~(u64)0;
 // of all 64 lanes of a wave
 __device__ __forceinline__ u64 wave_scan(u64 v) {
     const int lane = threadIdx.x & 63;
@@ -163,7 +167,11 @@ __device__ __forceinline__ bool find_place(const ChunkArgs& a, At at, Line& line
     }
     const int items = seq_items(a, o.q);
     const u64 one = items_measure(a, o.q, items), off = u - before * rep;
-    o.rep = __builtin_amdgcn_readfirstlane((int)(off / one));
+    // the quotient, whose double is off by one at most
+    int r = (int)((double)off / (double)one);
+    if ((u64)r * one > off) r--;
+    else if ((u64)(r + 1) * one <= off) r++;
+    o.rep = __builtin_amdgcn_readfirstlane(r);
     const u64 y = off - (u64)o.rep * one;
     // the last item that begins at y or before: 64 candidates a step
     int lo = 0, n = items;
@@ -282,11 +290,10 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
     constexpr int KS = HD / 16 / DS, NT = HD / 32 / DS;   // a wave's product steps and 32-dim tiles
     extern __shared__ __align__(16) uint8_t lds[];
     u64* red = reinterpret_cast<u64*>(lds + P::RED);
-    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % DS, kp = wave / (NJ * DS), slot = wave / DS % NJ;
     // this wave's share of the staging: tile of a stage, K or V, block of the tile, which pieces
     const int unit = wave % P::UNITS, ut = unit >> 2, uv = unit >> 1 & 1, ub = unit & 1, piece0 = wave / P::UNITS * PCS;
-    const int t16 = lane & 15, g = lane >> 4;
 
     Line line;
     Place at;
@@ -295,8 +302,8 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             a,
             [&](const Line& l) {
                 // neighbours on the line, which look at the same keys, to one XCD
-                share = l.shares == kShares ? (blockIdx.x & 7) * (kShares / 8) + (blockIdx.x >> 3) : blockIdx.x;
-                return share < l.shares ? l.at(share) : ~(u64)0 / (a.p.n_kv * a.ngrp) / 2 * (a.p.n_kv * a.ngrp);
+                share = l.lg == kLgShares ? (blockIdx.x & 7) * (kShares / 8) + (blockIdx.x >> 3) : blockIdx.x;
+                return share >> l.lg ? kNowhere : l.at(share);
             },
             line, at, red))
         return;
@@ -307,15 +314,24 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
         const Item it(a, at);
         const int tile0 = it.tile_at(at.x, at.size), tile1 = it.tile_at(at.x + take, at.size);
         if (tile0 < tile1) {
+            // every part of an item's work has a lane number of its own, so that no
+            // address derived from it is kept in a register over the others
+            auto own_lane = [&]() {
+                int x = tid & 63;
+                asm volatile("" : "+v"(x));
+                return x;
+            };
+            const int lane = own_lane(), col = lane & 31, h = lane >> 5, t16 = lane & 15, g = lane >> 4;
             const int kvh = at.rep / a.ngrp, hg = at.rep - kvh * a.ngrp;
             const int nh = a.group - hg * a.gh < a.gh ? a.group - hg * a.gh : a.gh;    // heads there are
             const int head0 = kvh * a.group + hg * a.gh;
             const int ncols = it.rows * nh;
             const bool mine = slot * 32 < ncols;
             // column j: row j / nh, head j % nh; columns past the last repeat it
+            const unsigned inv_nh = (65535u + nh) / (unsigned)nh;   // j < 128: j / nh exactly
             auto col_row = [&](int j, int& hh) {
                 j = j < ncols ? j : ncols - 1;
-                const int r = (int)((unsigned)j / (unsigned)nh);
+                const int r = (int)((unsigned)j * inv_nh >> 16);
                 hh = j - r * nh;
                 return it.row0 + r;
             };
@@ -328,11 +344,19 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             const int ntile = tile1 - tile0, stages = (ntile + KSP - 1) / KSP;
 
             // ---- tiles on their way into LDS: stage st has the tiles ktb + KSP st + (0 .. KSP - 1) ----
-            // the page of this wave's block, -1: not a page, -2: nobody looks at it
-            auto page_at = [&](int st) {
+            // The page of this wave's block of a stage, -1: not a page, -2: nobody looks
+            // at it.  It is asked for a stage ahead: waiting for it would mean waiting
+            // for every load before it.
+            int asked_page = 0;
+            bool asked = false;
+            auto ask_page = [&](int st) {
                 const int t = st * KSP + ut, key = (ktb + t) * 32 + ub * 16;
-                if (t >= ntile || key + 15 < it.kfirst || key > it.klast) return -2;
-                return __builtin_amdgcn_readfirstlane(a.p.page_of(at.s, key));
+                asked = t < ntile && key + 15 >= it.kfirst && key <= it.klast;
+                if (asked) asked_page = a.p.table[(size_t)at.s * a.p.table_stride + (key >> a.p.lgpage)];
+            };
+            auto take_page = [&]() {
+                const int p = __builtin_amdgcn_readfirstlane(asked_page);
+                return !asked ? -2 : p >= 0 && p < a.p.n_pages ? p : -1;
             };
             auto block_at = [&](int st, int pg) {
                 return a.p.block_of(pg < 0 ? 0 : pg, kvh, (ktb + st * KSP + ut) * 32 + ub * 16);
@@ -350,28 +374,30 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 return u;
             };
             uint8_t* const mine_meta = lds + kMetaMarks + ub * 4;
-            int pg = page_at(0);
+            ask_page(0);
             // straight to LDS (K or V, as this wave has it)
             auto copy = [&](int st) {
+                const int pg = take_page();
                 const __amdgpu_buffer_rsrc_t r = block_rsrc(block_at(st, pg), pg);
                 uint8_t* to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut)) + (ub * KC + piece0) * 1024;
 #pragma unroll
                 for (int i = 0; i < PCS; i++) buf_load_lds16(r, to + i * 1024, piece0 * 1024 + lane * 16, i * 1024);
                 if (uv && piece0 == 0 && lane == 0) *reinterpret_cast<unsigned*>(mine_meta + P::meta_at(st, ut)) = pg == -1 ? 0xffffu : 0u;
-                pg = page_at(st + 1);
+                ask_page(st + 1);
             };
             // through registers
             uint4 raw[M::REG ? PCS : 1];
             float raw_scale = 0.0f;
             int raw_pg = 0;
             auto fetch = [&](int st) {
+                const int pg = take_page();
                 const size_t block = block_at(st, pg);
                 const __amdgpu_buffer_rsrc_t r = block_rsrc(block, pg);
 #pragma unroll
                 for (int i = 0; i < PCS; i++) raw[i] = buf_load16(r, piece0 * 1024 + lane * 16, i * 1024);
                 if (M::Q8) raw_scale = reinterpret_cast<const float*>((uv ? a.p.vp : a.p.kp) + a.p.scale_off)[block * 16 + t16];
                 raw_pg = pg;
-                pg = page_at(st + 1);
+                ask_page(st + 1);
             };
             auto put = [&](int st) {
                 uint8_t* to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut));
@@ -517,17 +543,18 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                                             part * (HD / DS)) + pass * kChunks * 16;
                 };
             };
-            auto chunk = [&](int c) { return box + row_slot<kChunks>(col, c); };
             auto load_q = [&]() {
+                const int lane = own_lane(), col = lane & 31, h = lane >> 5;
+                auto chunk = [&](int c) { return box + row_slot<kChunks>(col, c); };
                 if constexpr (TQ != G4_F32) {
                     const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
                     for (int pass = 0; pass < kPasses; pass++) {
                         if constexpr (KSP == 2) {
-                            rows_to_lds<kChunks, 16>(box, kp * 16, q_row(pass));
+                            rows_to_lds<kChunks, 16>(box, kp * 16, q_row(pass), lane);
                             lds_barrier();
                         } else {
-                            rows_to_lds<kChunks, 32>(box, 0, q_row(pass));
+                            rows_to_lds<kChunks, 32>(box, 0, q_row(pass), lane);
                         }
 #pragma unroll
                         for (int i = 0; i < kSteps; i++) {
@@ -543,7 +570,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     const float qs = a.scale * kLog2e;
 #pragma unroll
                     for (int pass = 0; pass < kPasses; pass++) {
-                        rows_to_lds<kChunks, 32>(box, 0, q_row(pass));
+                        rows_to_lds<kChunks, 32>(box, 0, q_row(pass), lane);
 #pragma unroll
                         for (int i = 0; i < kSteps; i++) {
                             const float4 x = *reinterpret_cast<const float4*>(chunk(i * 4 + h * 2));
@@ -566,7 +593,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     unsigned top = 0;
 #pragma unroll
                     for (int pass = 0; pass < kPasses; pass++) {
-                        rows_to_lds<kChunks, 32>(box, 0, q_row(pass));
+                        rows_to_lds<kChunks, 32>(box, 0, q_row(pass), lane);
 #pragma unroll
                         for (int i = 0; i < kSteps; i++)
 #pragma unroll
@@ -883,8 +910,9 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 } else {
                     f4_t* xch = reinterpret_cast<f4_t*>(lds + P::XCH);
                     for (int st = 0; st < stages; st++) {
-                        if constexpr (!M::REG) wait_vm<0>();
-                        lds_barrier();   // K is there, V of the tile before done with
+                        // K is there, V of the tile before done with
+                        if (!M::REG && !uv) wait_vm<0>();
+                        lds_barrier();
                         if (uv) {
                             if constexpr (M::REG) {
                                 put(st);
@@ -897,14 +925,13 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
 #pragma unroll
                         for (int i = 0; i < 4; i++)
                             xch[(wave * 4 + i) * 64 + lane] = f4_t{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
-                        if constexpr (!M::REG) {
-                            if (uv) wait_vm<0>();
-                        }
-                        lds_barrier();   // K is done with, the partial scores and V are there
-                        if constexpr (!M::REG) {
-                            if (careful || ragged(st)) {
-                                clean(st, careful);
-                                lds_barrier();
+                        lds_barrier();   // K is done with, the partial scores (and V out of registers) there
+                        if (!uv && st + 1 < stages) {
+                            if constexpr (M::REG) {
+                                put(st + 1);
+                                fetch(st + 2);
+                            } else {
+                                copy(st + 1);
                             }
                         }
 #pragma unroll
@@ -913,14 +940,18 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
 #pragma unroll
                             for (int j = 0; j < 4; j++) sc[4 * i + j] += y[j];
                         }
+                        // marks have to be there before the weights
+                        const bool special = !M::REG && (careful || ragged(st));
+                        if (special) {
+                            if (uv) wait_vm<0>();
+                            lds_barrier();
+                            clean(st, careful);
+                            lds_barrier();
+                        }
                         weights(st);
-                        if (!uv && st + 1 < stages) {
-                            if constexpr (M::REG) {
-                                put(st + 1);
-                                fetch(st + 2);
-                            } else {
-                                copy(st + 1);
-                            }
+                        if (!M::REG && !special) {
+                            if (uv) wait_vm<0>();
+                            lds_barrier();   // V is there
                         }
                         values(st);
                     }
@@ -945,10 +976,12 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 for (int i = 0; i < NT; i++) o[i] = f16_t{};
                 m = -FLT_MAX;
                 l = 0.0f;
-                pg = page_at(0);
+                ask_page(0);
                 if (DS == 1 || !uv) copy(0);
             }
 
+            {
+            const int lane = own_lane(), col = lane & 31, h = lane >> 5;
             const bool whole = tile0 == 0 && tile1 == it.tiles;
             l += shfl_xor(l, 32);
             wait_vm<0>();
@@ -1020,6 +1053,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                         *reinterpret_cast<float2*>(to + (size_t)a.cols * HD + (slot * 32 + col) * 2) = make_float2(m, l);
                 }
             }
+            }
             lds_barrier();   // LDS is the next item's
         }
         left -= take;
@@ -1053,7 +1087,7 @@ __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
     Place at;
     const unsigned w = blockIdx.x + 1;
     const int slot = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
-    if (!find_place<256>(a, [&](const Line& l) { return w < l.shares ? l.at(w) : ~(u64)0 / (a.p.n_kv * a.ngrp) / 2 * (a.p.n_kv * a.ngrp); },
+    if (!find_place<256>(a, [&](const Line& l) { return w >> l.lg ? kNowhere : l.at(w); },
                          line, at, red))
         return;
     const u64 start = line.at(w) - at.x, end = start + at.size;      // the item's place on the line
@@ -1062,29 +1096,39 @@ __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
     const int kvh = at.rep / a.ngrp, hg = at.rep - kvh * a.ngrp;
     const int nh = a.group - hg * a.gh < a.gh ? a.group - hg * a.gh : a.gh, ncols = it.rows * nh;
     if (slot * 32 >= ncols) return;
-    // piece i is share w - 1 + i's: tiles from edge(i) to edge(i + 1)
+    // piece i is share w - 1 + i's: tiles from edge(i) to edge(i + 1), if any
     auto edge = [&](int i) {
         if (i == 0) return 0;
-        const u64 u = w - 1 + i < line.shares ? line.at(w - 1 + i) : line.total;
+        const u64 u = (w - 1 + i) >> line.lg ? line.total : line.at(w - 1 + i);
         return u >= end ? it.tiles : it.tile_at(u - start, at.size);
     };
-    auto piece = [&](int i) { return a.part + (size_t)((w - 1 + i) * 2 + (edge(i) == 0)) * part_floats(a.cols, HD); };
-    // the pieces that have tiles; one alone has been written
-    int pieces = 0, some = 0;
-    for (int e = 0; e < it.tiles; pieces++) {
-        const int e1 = edge(pieces + 1);
-        some += e1 > e;
-        e = e1;
+    __shared__ int list[kShares], before[4];
+    int pieces = 0;
+    {
+        const int e0 = edge(tid), e1 = edge(tid + 1);
+        // in order, so that sums are the same every time
+        const u64 have = __ballot(e0 < e1);
+        if (lane == 0) before[tid >> 6] = __popcll(have);
+        lds_sync();
+        int k = __popcll(have & (((u64)1 << lane) - 1));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i < tid >> 6) k += before[i];
+            pieces += before[i];
+        }
+        if (e0 < e1) list[k] = (w - 1 + tid) * 2 + (e0 == 0);
     }
-    if (some < 2) return;
+    lds_sync();
+    if (pieces < 2) return;     // one alone has been written
+    auto piece = [&](int i) { return a.part + (size_t)list[i] * part_floats(a.cols, HD); };
     const size_t ml = (size_t)a.cols * HD + (slot * 32 + col) * 2;
     float top = -FLT_MAX;
-    for (int i = 0; i < pieces; i++)
-        if (edge(i) < edge(i + 1)) top = fmaxf(top, piece(i)[ml]);
+#pragma unroll 4
+    for (int i = 0; i < pieces; i++) top = fmaxf(top, piece(i)[ml]);
     f4_t x[V] = {};
     float l = 0.0f;
+#pragma unroll 4
     for (int i = 0; i < pieces; i++) {
-        if (edge(i) >= edge(i + 1)) continue;
         const float* from = piece(i);
         const float2 y = *reinterpret_cast<const float2*>(from + ml);
         const float f = exp2f(y.x - top);

@@ -128,9 +128,8 @@ __device__ __forceinline__ int row_slot(int r, int c) {
 // N rows of C chunks each, from `first` on, by one wave: at(r) is row r's
 // address, box takes C chunks a row
 template <int C, int N, typename At>
-__device__ __forceinline__ void rows_to_lds(uint8_t* box, int first, At at) {
+__device__ __forceinline__ void rows_to_lds(uint8_t* box, int first, At at, int lane = threadIdx.x & 63) {
     constexpr int K = N * C / 64;
-    const int lane = threadIdx.x & 63;
     f4_t x[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
