@@ -207,8 +207,9 @@ struct Item {
     }
 };
 // floats of a partial result: 32 columns at a time in the order of a wave's
-// registers, then each column's maximum and weight sum
-__host__ __device__ inline size_t part_floats(int cols, int hd) { return (size_t)cols * (hd + 2); }
+// registers, then each column's maximum and weight sum (head_dim 512: for each
+// half of the dims, whose V rows have exponents of their own)
+__host__ __device__ inline size_t part_floats(int cols, int hd) { return (size_t)cols * (hd + 4); }
 
 // ---- types ----------------------------------------------------------------------
 // TQ: rows, TC: cache.  NQ, NK, NP: terms of q, of K (and V), of the weights.
@@ -257,7 +258,13 @@ struct Plan {
     // LDS: K and V of a tile are TB bytes each
     static constexpr int TB = 64 * HD * M::NK;
     static constexpr int NKP = DS == 2 ? 1 : 2 * KSP, NVP = DS == 2 ? 1 : KSP == 2 ? 5 : 2;
-    static constexpr int META = (NKP + NVP) * TB, XCH = META + 2 * KSP * 512;
+    // staging: a unit is a 16-token block of K or V; WPU waves have one.  BOTH: a
+    // wave has half of the dims of a block of K and of one of V instead
+    static constexpr int UNITS = 4 * KSP, WPU = NW / UNITS, KC = HD * M::ES / 64, PCS = KC / WPU;
+    static constexpr bool BOTH = M::REG && NW == 4 && KC > 1;
+    static constexpr int PH = BOTH ? KC / 2 : 1;
+    static constexpr int MB = BOTH ? 1024 : 512;                     // a tile's factors and marks
+    static constexpr int META = (NKP + NVP) * TB, TOPX = META + 2 * KSP * MB, XCH = TOPX + (BOTH ? 256 : 0);
     static constexpr int RB = HD / DS * (TQ == G4_F32 ? 4 : 2);      // bytes of a wave's part of a row
     static constexpr int END = XCH + (DS == 2 ? NW * 4096 : 0);      // DS 2: partial scores
     static constexpr int ROWS = (KSP == 1 ? NW : 0) * 32 * RB;       // the output's rows
@@ -265,19 +272,20 @@ struct Plan {
     static constexpr int TOP0 = END > ROWS ? END : ROWS, TOP = TOP0 > JOIN ? TOP0 : JOIN;
     static constexpr int RED = (TOP + 15) / 16 * 16, LDS = RED + 128;
     static_assert(LDS <= 160 * 1024 && NJ * DS * KSP == NW, "LDS");
-    // staging: a unit is a 16-token block of K or V; WPU waves have one
-    static constexpr int UNITS = 4 * KSP, WPU = NW / UNITS, KC = HD * M::ES / 64, PCS = KC / WPU;
-    static_assert(PCS * WPU == KC, "pieces");
+    static_assert(PCS * WPU == KC && (!BOTH || PH * 2 == KC), "pieces");
     static __device__ __forceinline__ int k_at(int st, int kp) { return DS == 2 ? 0 : ((st & 1) * KSP + kp) * TB; }
     static __device__ __forceinline__ int v_at(int st, int kp) {
         return (NKP + (DS == 2 ? 0 : kp == 0 ? st & 1 : 2 + st % 3)) * TB;
     }
-    static __device__ __forceinline__ int meta_at(int st, int kp) { return META + ((st & 1) * KSP + kp) * 512; }
+    static __device__ __forceinline__ int meta_at(int st, int kp) { return META + ((st & 1) * KSP + kp) * MB; }
 };
-// a tile's 512 bytes beside it: 32 factors of K (fp32: 2^e, codes: scales), 32 of V
+// What lies beside a tile: 32 factors of K (fp32: 2^e, codes: scales), 32 of V
 // (exponents, scales), fp32: 2^-e; marks of each block's keys that make a score
-// NaN; fp32: the weight sums below which lost_weight is asked for
-constexpr int kMetaV = 128, kMetaInv = 256, kMetaMarks = 384, kMetaLost = 392;
+// NaN; fp32: the weight sums below which lost_weight is asked for.  BOTH: K's, V's
+// and the inverses for each half of the dims, 32 each, marks of K and V for each
+// block and half.
+constexpr int kMetaV = 128, kMetaMarks = 384;
+constexpr int kBothV = 256, kBothInv = 512, kBothMarks = 768, kBothLost = 800;
 
 template <int TQ, int TC, int HD>
 __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW / 4)) void attn_chunk_kernel(ChunkArgs a) {
@@ -374,7 +382,6 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 return u;
             };
             uint8_t* const mine_meta = lds + kMetaMarks + ub * 4;
-            ask_page(0);
             // straight to LDS (K or V, as this wave has it)
             auto copy = [&](int st) {
                 const int pg = take_page();
@@ -435,95 +442,230 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                                     make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
                         }
                     }
-                } else if constexpr (M::F) {
-                    if (!uv) {
-                        // dims 16 i + 4 g .. + 3 of token t16
-                        unsigned top = 0;
-#pragma unroll
-                        for (int i = 0; i < PCS; i++) {
-                            const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-                            for (int k = 0; k < 4; k++) top = (w[k] & 0x7fffffffu) > top ? w[k] & 0x7fffffffu : top;
-                        }
-#pragma unroll
-                        for (int d = 16; d < 64; d <<= 1) {
-                            const unsigned o = __shfl_xor(top, d, 64);
-                            top = o > top ? o : top;
-                        }
-                        int e = (int)(top >> 23) > kLowK ? (int)(top >> 23) : kLowK;
-                        const bool bad = e == 255;
-                        if (bad) e = kLowK;
-                        marks |= (unsigned)__ballot(bad && g == 0 && (use >> t16 & 1)) & 0xffffu;
-                        const float sf = row_scale(e);
-                        if (g == 0) meta[ub * 16 + t16] = row_scale_inv(e);
-#pragma unroll
-                        for (int i = 0; i < PCS; i++) {
-                            h2v_t hi[2], lo[2];
-                            split2(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y), sf, hi[0], lo[0]);
-                            split2(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w), sf, hi[1], lo[1]);
-                            uint8_t* w = to + i * 1024 + ((g >> 1) * 32 + ub * 16 + t16) * 16 + (g & 1) * 8;
-                            *reinterpret_cast<uint2*>(w) = make_uint2(h2_bits(hi[0]), h2_bits(hi[1]));
-                            *reinterpret_cast<uint2*>(w + 64 * HD) = make_uint2(h2_bits(lo[0]), h2_bits(lo[1]));
-                        }
-                    } else {
-                        // dim 16 i + t16 of tokens 4 g .. 4 g + 3
-                        unsigned top[4] = {};
-#pragma unroll
-                        for (int i = 0; i < PCS; i++) {
-                            const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-                            for (int k = 0; k < 4; k++) top[k] = (w[k] & 0x7fffffffu) > top[k] ? w[k] & 0x7fffffffu : top[k];
-                        }
-                        float sf[4];
-                        int low = 113;
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-#pragma unroll
-                            for (int d = 1; d < 16; d <<= 1) {
-                                const unsigned o = __shfl_xor(top[k], d, 64);
-                                top[k] = o > top[k] ? o : top[k];
-                            }
-                            int e = (int)(top[k] >> 23) > kLowV ? (int)(top[k] >> 23) : kLowV;
-                            const bool on = use >> (4 * g + k) & 1, bad = e == 255;
-                            if (bad || !on) e = kLowV;
-                            // rows that nobody looks at, or that are not finite: zeros
-                            if (bad || !on) {
-#pragma unroll
-                                for (int i = 0; i < PCS; i++) {
-                                    if (k == 0) raw[i].x = 0;
-                                    else if (k == 1) raw[i].y = 0;
-                                    else if (k == 2) raw[i].z = 0;
-                                    else raw[i].w = 0;
-                                }
-                            }
-                            const u64 b = __ballot(bad && on && t16 == 0);   // lanes 0, 16, 32, 48: tokens k, 4 + k, ..
-#pragma unroll
-                            for (int j = 0; j < 4; j++) marks |= (unsigned)(b >> (16 * j) & 1) << (4 * j + k);
-                            sf[k] = row_scale(e);
-                            if (on && e - 141 < low) low = e - 141;
-                            if (t16 == 0) {
-                                meta[kMetaV / 4 + ub * 16 + 4 * g + k] = (float)(e - 141);
-                                meta[kMetaInv / 4 + ub * 16 + 4 * g + k] = sf[k];
-                            }
-                        }
-                        int o = __shfl_xor(low, 16, 64);
-                        low = o < low ? o : low;
-                        o = __shfl_xor(low, 32, 64);
-                        low = o < low ? o : low;
-                        if (lane == 0) meta[kMetaLost / 4 + ub] = __builtin_ldexpf(1.0f, 48 - 126 - low);
-#pragma unroll
-                        for (int i = 0; i < PCS; i++) {
-                            h2v_t hi[2], lo[2];
-                            split2(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y), sf[0], sf[1], hi[0], lo[0]);
-                            split2(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w), sf[2], sf[3], hi[1], lo[1]);
-                            uint8_t* w = to + ((i >> 1) * 2 + ub) * 1024 + ((g & 1) * 32 + (i & 1) * 16 + t16) * 16 + (g >> 1) * 8;
-                            *reinterpret_cast<uint2*>(w) = make_uint2(h2_bits(hi[0]), h2_bits(hi[1]));
-                            *reinterpret_cast<uint2*>(w + 64 * HD) = make_uint2(h2_bits(lo[0]), h2_bits(lo[1]));
-                        }
-                    }
                 }
                 // K's and V's marks have a word each: [K or V][block]
                 if (piece0 == 0 && lane == 0) reinterpret_cast<unsigned*>(meta)[kMetaMarks / 4 + (uv ? 0 : 4) + ub] = marks;
+            };
+
+            // BOTH: half hf of the dims of block bb, K and V.  A piece is put into LDS
+            // between the products and its registers take the next tile's at once.
+            constexpr int PH = P::PH;
+            constexpr bool BOTH = P::BOTH;
+            const int bb = wave & 1, hf = wave >> 1;
+            uint4 rk[BOTH ? PH : 1], rv[BOTH ? PH : 1];
+            float ks16 = 0.0f, vs16 = 0.0f, sfk = 0.0f, sfv[4];
+            bool keepv[4];
+            int askk = 0, askv = 0, pgk = -2, pgv = -2;     // page asked for; page of what the registers hold
+            bool onk = false, onv = false;
+            __amdgpu_buffer_rsrc_t nk, nv;
+            auto ask2 = [&](int st, int& page, bool& on) {
+                const int key = (ktb + st) * 32 + bb * 16;
+                on = st < ntile && key + 15 >= it.kfirst && key <= it.klast;
+                if (on) page = a.p.table[(size_t)at.s * a.p.table_stride + (key >> a.p.lgpage)];
+            };
+            auto take2 = [&](int page, bool on) {
+                const int p = __builtin_amdgcn_readfirstlane(page);
+                return !on ? -2 : p >= 0 && p < a.p.n_pages ? p : -1;
+            };
+            auto use2 = [&](int st) {
+                const int key = (ktb + st) * 32 + bb * 16;
+                unsigned u = 0xffffu;
+                if (it.kfirst > key) u &= it.kfirst - key < 16 ? 0xffffu << (it.kfirst - key) : 0u;
+                if (it.klast < key + 15) u &= it.klast >= key ? 0xffffu >> (15 - (it.klast - key)) : 0u;
+                return u;
+            };
+            // stage st's page looked up: its loads may follow
+            auto open2 = [&](int st, bool v) {
+                const int pg = v ? take2(askv, onv) : take2(askk, onk);
+                const size_t block = a.p.block_of(pg < 0 ? 0 : pg, kvh, (ktb + st) * 32 + bb * 16);
+                const uint8_t* pool = v ? a.p.vp : a.p.kp;
+                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(pool + block * (16 * HD * ES)), 0,
+                                                                                   pg < 0 ? 0 : 16 * HD * ES, kBufWord3);
+                float sc16 = 0.0f;
+                if (M::Q8) sc16 = reinterpret_cast<const float*>(pool + a.p.scale_off)[block * 16 + t16];
+                if (v) {
+                    nv = r;
+                    pgv = pg;
+                    vs16 = sc16;
+                    ask2(st + 1, askv, onv);
+                } else {
+                    nk = r;
+                    pgk = pg;
+                    ks16 = sc16;
+                    ask2(st + 1, askk, onk);
+                }
+            };
+            auto load2 = [&](bool v, int j) {
+                const uint4 x = buf_load16(v ? nv : nk, hf * PH * 1024 + lane * 16, j * 1024);
+                if (v) rv[j] = x;
+                else rk[j] = x;
+            };
+            // before the pieces of stage st, which the registers hold: factors, marks, and
+            // the next stage's page
+            auto begin_k = [&](int st) {
+                float* meta = reinterpret_cast<float*>(lds + P::meta_at(st, 0));
+                const unsigned use = use2(st);
+                unsigned marks = pgk == -1 ? 0xffffu : 0u;
+                if constexpr (M::F) {
+                    unsigned top = 0;
+#pragma unroll
+                    for (int i = 0; i < PH; i++) {
+                        const unsigned w[4] = {rk[i].x, rk[i].y, rk[i].z, rk[i].w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) top = (w[k] & 0x7fffffffu) > top ? w[k] & 0x7fffffffu : top;
+                    }
+#pragma unroll
+                    for (int d = 16; d < 64; d <<= 1) {
+                        const unsigned o = __shfl_xor(top, d, 64);
+                        top = o > top ? o : top;
+                    }
+                    int e = (int)(top >> 23) > kLowK ? (int)(top >> 23) : kLowK;
+                    const bool bad = e == 255;
+                    if (bad) e = kLowK;
+                    marks |= (unsigned)__ballot(bad && g == 0 && (use >> t16 & 1)) & 0xffffu;
+                    sfk = row_scale(e);
+                    if (g == 0) meta[hf * 32 + bb * 16 + t16] = row_scale_inv(e);
+                } else {
+                    const bool on = use >> t16 & 1 && pgk >= 0, bad = on && !(fabsf(ks16) < INFINITY);
+                    marks |= (unsigned)__ballot(bad && g == 0) & 0xffffu;
+                    if (g == 0 && hf == 0) meta[bb * 16 + t16] = on && !bad ? ks16 : 0.0f;
+                }
+                if (lane == 0) reinterpret_cast<unsigned*>(meta)[kBothMarks / 4 + hf * 2 + bb] = marks;
+                open2(st + 1, false);
+            };
+            // V, fp32: each token's largest, of this half of the dims
+            auto tops_v = [&](unsigned (&top)[4]) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) top[k] = 0;
+#pragma unroll
+                for (int i = 0; i < PH; i++) {
+                    const unsigned w[4] = {rv[i].x, rv[i].y, rv[i].z, rv[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) top[k] = (w[k] & 0x7fffffffu) > top[k] ? w[k] & 0x7fffffffu : top[k];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int d = 1; d < 16; d <<= 1) {
+                        const unsigned o = __shfl_xor(top[k], d, 64);
+                        top[k] = o > top[k] ? o : top[k];
+                    }
+            };
+            unsigned* const topx = reinterpret_cast<unsigned*>(lds + P::TOPX);
+            auto share_tops = [&]() {
+                unsigned top[4];
+                tops_v(top);
+                if (t16 == 0) *reinterpret_cast<uint4*>(topx + hf * 32 + bb * 16 + 4 * g) = make_uint4(top[0], top[1], top[2], top[3]);
+            };
+            auto begin_v = [&](int st) {
+                float* meta = reinterpret_cast<float*>(lds + P::meta_at(st, 0));
+                const unsigned use = use2(st);
+                unsigned marks = pgv == -1 ? 0xffffu : 0u;
+                if constexpr (M::F) {
+                    unsigned top[4];
+                    if constexpr (DS == 1) {
+                        // a token's weight carries one exponent, whichever the dim
+                        const uint4 x = *reinterpret_cast<const uint4*>(topx + bb * 16 + 4 * g);
+                        const uint4 y = *reinterpret_cast<const uint4*>(topx + 32 + bb * 16 + 4 * g);
+                        top[0] = x.x > y.x ? x.x : y.x;
+                        top[1] = x.y > y.y ? x.y : y.y;
+                        top[2] = x.z > y.z ? x.z : y.z;
+                        top[3] = x.w > y.w ? x.w : y.w;
+                    } else {
+                        tops_v(top);
+                    }
+                    int low = 113;
+                    float ex[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        int e = (int)(top[k] >> 23) > kLowV ? (int)(top[k] >> 23) : kLowV;
+                        const bool on = use >> (4 * g + k) & 1, bad = e == 255;
+                        keepv[k] = on && !bad;      // others become zeros
+                        if (!keepv[k]) e = kLowV;
+                        const u64 b = __ballot(bad && on && t16 == 0);   // lanes 0, 16, 32, 48: tokens k, 4 + k, ..
+#pragma unroll
+                        for (int j = 0; j < 4; j++) marks |= (unsigned)(b >> (16 * j) & 1) << (4 * j + k);
+                        sfv[k] = row_scale(e);
+                        ex[k] = (float)(e - 141);
+                        if (on && e - 141 < low) low = e - 141;
+                    }
+                    if (t16 == 0) {
+                        const int to = hf * 32 + bb * 16 + 4 * g;
+                        *reinterpret_cast<f4_t*>(meta + kBothV / 4 + to) = f4_t{ex[0], ex[1], ex[2], ex[3]};
+                        *reinterpret_cast<f4_t*>(meta + kBothInv / 4 + to) = f4_t{sfv[0], sfv[1], sfv[2], sfv[3]};
+                    }
+                    int o = __shfl_xor(low, 16, 64);
+                    low = o < low ? o : low;
+                    o = __shfl_xor(low, 32, 64);
+                    low = o < low ? o : low;
+                    if (lane == 0) meta[kBothLost / 4 + hf * 2 + bb] = __builtin_ldexpf(1.0f, 48 - 126 - low);
+                } else {
+                    const bool on = use >> t16 & 1 && pgv >= 0, bad = on && !(fabsf(vs16) < INFINITY);
+                    marks |= (unsigned)__ballot(bad && g == 0) & 0xffffu;
+                    if (g == 0 && hf == 0) meta[kBothV / 4 + bb * 16 + t16] = on && !bad ? vs16 : 0.0f;
+                }
+                if (lane == 0) reinterpret_cast<unsigned*>(meta)[kBothMarks / 4 + 4 + hf * 2 + bb] = marks;
+                open2(st + 1, true);
+            };
+            auto codes8 = [&](const uint4& x, unsigned (&y)[8]) {
+                const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int c0 = (int8_t)(w[k >> 1] >> (k & 1 ? 16 : 0)), c1 = (int8_t)(w[k >> 1] >> (k & 1 ? 24 : 8));
+                    y[k] = hi_halves(__float_as_uint((float)c0), __float_as_uint((float)c1));
+                }
+            };
+            // piece j of stage st to LDS, and the next stage's on its way
+            auto piece_k = [&](int st, int j) {
+                const int c = hf * PH + j;
+                uint8_t* to = lds + P::k_at(st, 0);
+                if constexpr (M::F) {
+                    h2v_t hi[2], lo[2];
+                    split2(__uint_as_float(rk[j].x), __uint_as_float(rk[j].y), sfk, hi[0], lo[0]);
+                    split2(__uint_as_float(rk[j].z), __uint_as_float(rk[j].w), sfk, hi[1], lo[1]);
+                    to += c * 1024 + ((g >> 1) * 32 + bb * 16 + t16) * 16 + (g & 1) * 8;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(h2_bits(hi[0]), h2_bits(hi[1]));
+                    *reinterpret_cast<uint2*>(to + 64 * HD) = make_uint2(h2_bits(lo[0]), h2_bits(lo[1]));
+                } else {
+                    unsigned y[8];
+                    codes8(rk[j], y);
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+                        *reinterpret_cast<uint4*>(to + (4 * c + g) * 1024 + (k * 32 + bb * 16 + t16) * 16) =
+                            make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                }
+                load2(false, j);
+            };
+            auto piece_v = [&](int st, int j) {
+                const int c = hf * PH + j;
+                uint8_t* to = lds + P::v_at(st, 0);
+                if constexpr (M::F) {
+                    const unsigned w[4] = {rv[j].x, rv[j].y, rv[j].z, rv[j].w};
+                    float x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) x[k] = keepv[k] ? __uint_as_float(w[k]) : 0.0f;
+                    h2v_t hi[2], lo[2];
+                    split2(x[0], x[1], sfv[0], sfv[1], hi[0], lo[0]);
+                    split2(x[2], x[3], sfv[2], sfv[3], hi[1], lo[1]);
+                    to += ((c >> 1) * 2 + bb) * 1024 + ((g & 1) * 32 + (c & 1) * 16 + t16) * 16 + (g >> 1) * 8;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(h2_bits(hi[0]), h2_bits(hi[1]));
+                    *reinterpret_cast<uint2*>(to + 64 * HD) = make_uint2(h2_bits(lo[0]), h2_bits(lo[1]));
+                } else {
+                    unsigned y[8];
+                    codes8(rv[j], y);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        *reinterpret_cast<uint2*>(to + ((2 * c + (k >> 1)) * 2 + bb) * 1024 +
+                                                  ((g & 1) * 32 + (k & 1) * 16 + t16) * 16 + (g >> 1) * 8) =
+                            make_uint2(y[2 * k], y[2 * k + 1]);
+                }
+                load2(true, j);
+            };
+            // pieces that belong to step i of n
+            auto pieces = [&](int i, int n, auto&& piece) {
+#pragma unroll
+                for (int j = 0; j < PH; j++)
+                    if (j * n / PH == i) piece(j);
             };
 
             // ---- q: 32 columns' rows through places in LDS that the first stage leaves free ----
@@ -640,7 +782,32 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             };
 
             // ---- first stage, q ----
-            if constexpr (M::REG) {
+            if constexpr (BOTH) {
+                ask2(0, askk, onk);
+                ask2(0, askv, onv);
+                open2(0, false);
+                open2(0, true);
+#pragma unroll
+                for (int j = 0; j < PH; j++) {
+                    load2(false, j);
+                    load2(true, j);
+                }
+                load_q();
+                if constexpr (DS == 2) lds_barrier();   // the boxes have been read
+                if constexpr (DS == 1 && M::F) {
+                    share_tops();
+                    lds_barrier();
+                }
+                begin_k(0);
+#pragma unroll
+                for (int j = 0; j < PH; j++) piece_k(0, j);
+                if constexpr (DS == 1) {
+                    begin_v(0);
+#pragma unroll
+                    for (int j = 0; j < PH; j++) piece_v(0, j);
+                }
+            } else if constexpr (M::REG) {
+                ask_page(0);
                 fetch(0);
                 load_q();
                 if constexpr (DS == 2) {
@@ -654,6 +821,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     fetch(1);
                 }
             } else {
+                ask_page(0);
                 if (DS == 1 || !uv) copy(0);
                 load_q();
                 if (DS == 2) lds_barrier();
@@ -685,7 +853,8 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     v.x[0] = __builtin_bit_cast(op, make_uint4(y.x, y.y, z.x, z.y));
                 }
             };
-            auto scores = [&](int st) {
+            // feed(i): what is done beside step i's products
+            auto scores = [&](int st, auto&& feed) {
                 const uint8_t* from = lds + P::k_at(st, kp);
                 sc = f16_t{};
                 if constexpr (NQ == 1) {
@@ -697,40 +866,66 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     }
                     order_products<KS, 3, 1, 1>();
                 } else {
-                    f16_t sx = {};
+                    f16_t sx = {}, low;
                     run_products<Ops, KS, 2>([&](int i, Ops& k) { read_k(from, i, k); },
                                              [&](int i, const Ops& k) {
                                                  sc = mfma32(k.x[0], q[0][i], sc);
+                                                 feed(i);
 #pragma unroll
                                                  for (int j = 1; j < NQ; j++) sx = mfma32(k.x[0], q[j][i], sx);
                                                  if constexpr (NK == 2) sx = mfma32(k.x[1], q[0][i], sx);
+                                                 // fp32: K's scales are those of half of the dims
+                                                 if (M::F && DS == 1 && i == KS / 2 - 1) {
+                                                     low = sc + sx;
+                                                     sc = f16_t{};
+                                                     sx = f16_t{};
+                                                 }
                                              });
                     sc += sx;
+                    if constexpr (M::F) {
+                        const float* meta = reinterpret_cast<const float*>(lds + P::meta_at(st, 0));
+#pragma unroll
+                        for (int b = 0; b < 4; b++) {
+                            const f4_t x = *reinterpret_cast<const f4_t*>(meta + (DS == 1 ? 32 : part * 32) + 8 * b + 4 * h);
+                            const f4_t y = *reinterpret_cast<const f4_t*>(meta + 8 * b + 4 * h);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                sc[4 * b + i] *= x[i];
+                                if constexpr (DS == 1) sc[4 * b + i] = __builtin_fmaf(low[4 * b + i], y[i], sc[4 * b + i]);
+                            }
+                        }
+                    }
                 }
             };
             auto weights = [&](int st) {
                 const int kt = ktb + st * KSP + kp;
                 const float* meta = reinterpret_cast<const float*>(lds + P::meta_at(st, kp));
                 const unsigned* mk = reinterpret_cast<const unsigned*>(meta) + kMetaMarks / 4;
-                unsigned marks = mk[0] | mk[1] << 16;
-                if (M::REG) marks |= mk[4] | mk[5] << 16;
+                unsigned marks;
+                if constexpr (BOTH) {
+                    const unsigned* m2 = reinterpret_cast<const unsigned*>(meta) + kBothMarks / 4;
+                    // [K, V][half][block]
+                    marks = m2[0] | m2[2] | m2[4] | m2[6] | (m2[1] | m2[3] | m2[5] | m2[7]) << 16;
+                } else {
+                    marks = mk[0] | mk[1] << 16;
+                    if (M::REG) marks |= mk[4] | mk[5] << 16;
+                }
                 marks = __builtin_amdgcn_readfirstlane(marks);
                 float fv[16];       // codes: V's scales, fp32: 2^-e
+                const int vhalf = M::F && DS == 2 ? part * 32 : 0;
                 if constexpr (M::REG) {
 #pragma unroll
                     for (int b = 0; b < 4; b++) {
-                        const float4 xk = *reinterpret_cast<const float4*>(meta + 8 * b + 4 * h);
-                        const float4 xv = *reinterpret_cast<const float4*>(meta + kMetaV / 4 + 8 * b + 4 * h);
-                        const float k[4] = {xk.x, xk.y, xk.z, xk.w}, v[4] = {xv.x, xv.y, xv.z, xv.w};
+                        const f4_t v = *reinterpret_cast<const f4_t*>(meta + (BOTH ? kBothV / 4 : kMetaV / 4) + vhalf + 8 * b + 4 * h);
                         if constexpr (M::F) {
-                            const float4 xi = *reinterpret_cast<const float4*>(meta + kMetaInv / 4 + 8 * b + 4 * h);
-                            const float vi[4] = {xi.x, xi.y, xi.z, xi.w};
+                            const f4_t vi = *reinterpret_cast<const f4_t*>(meta + kBothInv / 4 + vhalf + 8 * b + 4 * h);
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                sc[4 * b + i] = __builtin_fmaf(sc[4 * b + i], fq * k[i], v[i]);
+                                sc[4 * b + i] = __builtin_fmaf(sc[4 * b + i], fq, v[i]);
                                 fv[4 * b + i] = vi[i];
                             }
                         } else {
+                            const f4_t k = *reinterpret_cast<const f4_t*>(meta + 8 * b + 4 * h);
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
                                 sc[4 * b + i] *= NQ == 3 ? k[i] : fq * k[i];
@@ -797,18 +992,18 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     }
                 }
                 if constexpr (M::F) {
-                    const float lost = __uint_as_float(__builtin_amdgcn_readfirstlane(
-                        __float_as_uint(fmaxf(meta[kMetaLost / 4], meta[kMetaLost / 4 + 1]))));
+                    const float* ml = meta + kBothLost / 4 + (DS == 2 ? part * 2 : 0);
+                    const float lost = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(ml[0], ml[1]))));
                     if (__any(l < lost)) {
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
                             const int key = 8 * (r >> 2) + 4 * h + (r & 3);
-                            l += lost_weight(sc[r] - base, meta[kMetaV / 4 + key], fv[r]);
+                            l += lost_weight(sc[r] - base, meta[kBothV / 4 + vhalf + key], fv[r]);
                         }
                     }
                 }
             };
-            auto values = [&](int st) {
+            auto values = [&](int st, auto&& feed) {
                 const uint8_t* from = lds + P::v_at(st, kp);
                 if constexpr (NP == 1) {
 #pragma unroll
@@ -823,6 +1018,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                                                  [&](int i, const Ops& v) {
                                                      f16_t& s = o[i >> 1];
                                                      s = mfma32(v.x[0], p[0][i & 1], s);
+                                                     feed(i);
                                                      s = mfma32(v.x[0], p[1][i & 1], s);
                                                      if constexpr (NK == 2) s = mfma32(v.x[1], p[0][i & 1], s);
                                                  });
@@ -861,8 +1057,40 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 return k0 < it.kfirst || k1 > it.klast;
             };
 
+            const auto nothing = [](int) {};
             for (bool careful = false;; careful = true) {
-                if constexpr (DS == 1) {
+                if constexpr (BOTH && DS == 1) {
+                    for (int st = 0; st < stages; st++) {
+                        lds_barrier();   // the stage is there, everyone done with the one before
+                        begin_k(st + 1);
+                        if (M::F) share_tops();
+                        scores(st, [&](int i) { pieces(i, KS, [&](int j) { piece_k(st + 1, j); }); });
+                        if (M::F) lds_barrier();   // the largest of V's rows are there
+                        begin_v(st + 1);
+                        weights(st);
+                        values(st, [&](int i) { pieces(i, 2 * NT, [&](int j) { piece_v(st + 1, j); }); });
+                    }
+                } else if constexpr (BOTH) {
+                    f4_t* xch = reinterpret_cast<f4_t*>(lds + P::XCH);
+                    for (int st = 0; st < stages; st++) {
+                        lds_barrier();   // K is there, V of the tile before done with
+                        begin_v(st);
+                        scores(st, [&](int i) { pieces(i, KS, [&](int j) { piece_v(st, j); }); });
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            xch[(wave * 4 + i) * 64 + lane] = f4_t{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+                        lds_barrier();   // K is done with, the partial scores and V there
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const f4_t y = xch[((wave ^ 1) * 4 + i) * 64 + lane];
+#pragma unroll
+                            for (int j = 0; j < 4; j++) sc[4 * i + j] += y[j];
+                        }
+                        begin_k(st + 1);
+                        weights(st);
+                        values(st, [&](int i) { pieces(i, 2 * NT, [&](int j) { piece_k(st + 1, j); }); });
+                    }
+                } else if constexpr (DS == 1) {
                     // this wave's copies have landed, then everyone's; and all are done
                     // with the stage before (waves 4 .. 7 but for its V, which has three
                     // places)
@@ -887,25 +1115,25 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     if (KSP == 1 || kp == 0) {
                         for (; st < stages; st++) {
                             turn(st);
-                            scores(st);
+                            scores(st, nothing);
                             weights(st);
-                            values(st);
+                            values(st, nothing);
                         }
                     } else {
                         turn(st);
                         if (kp < ntile) {
-                            scores(st);
+                            scores(st, nothing);
                             weights(st);
                         }
                         for (st++; st < stages; st++) {
                             turn(st);
-                            values(st - 1);
+                            values(st - 1, nothing);
                             if (st * KSP + kp < ntile) {
-                                scores(st);
+                                scores(st, nothing);
                                 weights(st);
                             }
                         }
-                        if ((stages - 1) * KSP + kp < ntile) values(stages - 1);
+                        if ((stages - 1) * KSP + kp < ntile) values(stages - 1, nothing);
                     }
                 } else {
                     f4_t* xch = reinterpret_cast<f4_t*>(lds + P::XCH);
@@ -921,7 +1149,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                                 copy(st);
                             }
                         }
-                        scores(st);
+                        scores(st, nothing);
 #pragma unroll
                         for (int i = 0; i < 4; i++)
                             xch[(wave * 4 + i) * 64 + lane] = f4_t{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
@@ -953,7 +1181,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                             if (uv) wait_vm<0>();
                             lds_barrier();   // V is there
                         }
-                        values(st);
+                        values(st, nothing);
                     }
                 }
                 // ---- a result that is not finite: once more, carefully ----
@@ -1049,8 +1277,8 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
 #pragma unroll
                         for (int b = 0; b < 4; b++)
                             sums[(i * 4 + b) * 64] = f4_t{o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
-                    if (part == 0 && h == 0)
-                        *reinterpret_cast<float2*>(to + (size_t)a.cols * HD + (slot * 32 + col) * 2) = make_float2(m, l);
+                    if (h == 0)
+                        *reinterpret_cast<float2*>(to + (size_t)a.cols * HD + (part * a.cols + slot * 32 + col) * 2) = make_float2(m, l);
                 }
             }
             }
@@ -1121,7 +1349,7 @@ __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
     lds_sync();
     if (pieces < 2) return;     // one alone has been written
     auto piece = [&](int i) { return a.part + (size_t)list[i] * part_floats(a.cols, HD); };
-    const size_t ml = (size_t)a.cols * HD + (slot * 32 + col) * 2;
+    const size_t ml = (size_t)a.cols * HD + ((z * D >= 256 ? a.cols : 0) + slot * 32 + col) * 2;
     float top = -FLT_MAX;
 #pragma unroll 4
     for (int i = 0; i < pieces; i++) top = fmaxf(top, piece(i)[ml]);
