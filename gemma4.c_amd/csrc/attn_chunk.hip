@@ -10,7 +10,7 @@ namespace {
 
 constexpr int kLgShares = 8, kShares = 1 << kLgShares;   // workgroups that share the work, one a CU
 constexpr int kLead = 64;      // keys that stand for what it costs to begin and to end an item
-constexpr int kLeast = 96;     // no smaller share than this
+constexpr int kLeast = 48;     // no smaller share than this
 
 struct ChunkArgs {
     KvPool p;
@@ -23,6 +23,7 @@ struct ChunkArgs {
     int group;      // q heads a kv head
     int gh, ngrp;   // of these, a workgroup's; groups of them
     int rpi;        // rows of an item
+    int lg;         // no more shares than 2^lg, by the call's sizes
     int cols;       // columns of a partial result, a multiple of 32
     float scale;
 };
@@ -83,25 +84,32 @@ struct Line {
         return (total >> lg) * w + (((unsigned)total & ((1u << lg) - 1)) * w >> lg);
     }
 };
-__device__ __forceinline__ Line line_of(u64 total) {
-    int lg = 0;
-    while (lg < kLgShares && (total >> (lg + 1)) >= kLeast) lg++;
-    return {total, lg};
+__device__ __forceinline__ Line line_of(const ChunkArgs& a, u64 total) {
+    const u64 most = total / kLeast;
+    const int lg = 63 - __builtin_clzll(most | 1);
+    return {total, lg < a.lg ? lg : a.lg};
 }
 
 constexpr u64 kNowhere = ~(u64)0;
-// of all 64 lanes of a wave
-__device__ __forceinline__ u64 wave_scan(u64 v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
-    return v;
+// inclusive prefix sums over a wave: within rows of 16 by lane moves (lane -
+// 1, 2, 4, 8, nothing from before the row), then the totals of the rows before
+template <int CTRL>
+__device__ __forceinline__ u64 row_shr(u64 v) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, 0xf, 0xf, true);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, 0xf, 0xf, true);
+    return (u64)hi << 32 | lo;
 }
 __device__ __forceinline__ u64 lane_u64(u64 v, int l) {
     return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)v, l);
+}
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+    v += row_shr<0x111>(v);
+    v += row_shr<0x112>(v);
+    v += row_shr<0x114>(v);
+    v += row_shr<0x118>(v);
+    const u64 a = lane_u64(v, 15), b = a + lane_u64(v, 31), c = b + lane_u64(v, 47);
+    const unsigned row = (threadIdx.x & 63) >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
 }
 
 // The line, and the place at(line) on it, by all NT threads of a workgroup
@@ -116,7 +124,7 @@ __device__ __forceinline__ bool find_place(const ChunkArgs& a, At at, Line& line
         const int i = lane < a.n_seqs ? lane : a.n_seqs - 1;
         const Seq q = seq_of(a, a.cu[i], a.cu[i + 1], a.lens[i]);
         const u64 mine = lane < a.n_seqs && q.n ? items_measure(a, q, seq_items(a, q)) : 0, x = wave_scan(mine);
-        line = line_of(lane_u64(x, 63) * rep);
+        line = line_of(a, lane_u64(x, 63) * rep);
         u = at(line);
         const u64 past = __ballot(x * rep > u);
         if (!past) return false;
@@ -145,7 +153,7 @@ __device__ __forceinline__ bool find_place(const ChunkArgs& a, At at, Line& line
             if (w < wave) b += red[w];
             all += red[w];
         }
-        line = line_of(all * rep);
+        line = line_of(a, all * rep);
         u = at(line);
         if (u >= b * rep && u < (b + sum) * rep) {
             int s = s0;
@@ -252,12 +260,13 @@ template <int TQ, int TC, int HD>
 struct Plan {
     typedef Mode<TQ, TC> M;
     static constexpr int DS = HD == 512 ? 2 : 1;
-    static constexpr int NW = M::NQ == 1 ? 8 : 4;                    // waves; 8: two a SIMD
+    static constexpr int NW = M::NQ == 1 && !M::REG ? 8 : 4;         // waves; 8: two a SIMD
     static constexpr int KSP = NW == 8 && DS == 1 ? 2 : 1;           // tiles at a time
     static constexpr int NJ = NW / DS / KSP, COLS = 32 * NJ;
     // LDS: K and V of a tile are TB bytes each
     static constexpr int TB = 64 * HD * M::NK;
-    static constexpr int NKP = DS == 2 ? 1 : 2 * KSP, NVP = DS == 2 ? 1 : KSP == 2 ? 5 : 2;
+    static constexpr bool ONE = DS == 2 && M::REG;                   // one place each for K and V
+    static constexpr int NKP = ONE ? 1 : 2 * KSP, NVP = ONE ? 1 : KSP == 2 ? 5 : 2;
     // staging: a unit is a 16-token block of K or V; WPU waves have one.  BOTH: a
     // wave has half of the dims of a block of K and of one of V instead
     static constexpr int UNITS = 4 * KSP, WPU = NW / UNITS, KC = HD * M::ES / 64, PCS = KC / WPU;
@@ -266,16 +275,16 @@ struct Plan {
     static constexpr int MB = BOTH ? 1024 : 512;                     // a tile's factors and marks
     static constexpr int META = (NKP + NVP) * TB, TOPX = META + 2 * KSP * MB, XCH = TOPX + (BOTH ? 256 : 0);
     static constexpr int RB = HD / DS * (TQ == G4_F32 ? 4 : 2);      // bytes of a wave's part of a row
-    static constexpr int END = XCH + (DS == 2 ? NW * 4096 : 0);      // DS 2: partial scores
+    static constexpr int END = XCH + (DS == 2 ? 16384 : 0);          // DS 2: partial scores
     static constexpr int ROWS = (KSP == 1 ? NW : 0) * 32 * RB;       // the output's rows
     static constexpr int JOIN = KSP == 2 ? NJ * (HD * 128 + 256) : 0;   // sums of waves 4 .. 7
     static constexpr int TOP0 = END > ROWS ? END : ROWS, TOP = TOP0 > JOIN ? TOP0 : JOIN;
     static constexpr int RED = (TOP + 15) / 16 * 16, LDS = RED + 128;
     static_assert(LDS <= 160 * 1024 && NJ * DS * KSP == NW, "LDS");
     static_assert(PCS * WPU == KC && (!BOTH || PH * 2 == KC), "pieces");
-    static __device__ __forceinline__ int k_at(int st, int kp) { return DS == 2 ? 0 : ((st & 1) * KSP + kp) * TB; }
+    static __device__ __forceinline__ int k_at(int st, int kp) { return ONE ? 0 : ((st & 1) * KSP + kp) * TB; }
     static __device__ __forceinline__ int v_at(int st, int kp) {
-        return (NKP + (DS == 2 ? 0 : kp == 0 ? st & 1 : 2 + st % 3)) * TB;
+        return (NKP + (ONE ? 0 : kp == 0 ? st & 1 : 2 + st % 3)) * TB;
     }
     static __device__ __forceinline__ int meta_at(int st, int kp) { return META + ((st & 1) * KSP + kp) * MB; }
 };
@@ -329,7 +338,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 asm volatile("" : "+v"(x));
                 return x;
             };
-            const int lane = own_lane(), col = lane & 31, h = lane >> 5, t16 = lane & 15, g = lane >> 4;
+            const int lane = own_lane(), t16 = lane & 15, g = lane >> 4;
             const int kvh = at.rep / a.ngrp, hg = at.rep - kvh * a.ngrp;
             const int nh = a.group - hg * a.gh < a.gh ? a.group - hg * a.gh : a.gh;    // heads there are
             const int head0 = kvh * a.group + hg * a.gh;
@@ -344,7 +353,6 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 return it.row0 + r;
             };
             int unused;
-            const int pos = at.q.hist + col_row(slot * 32 + col, unused), kf = first_key(a, pos);
             // tiles that every column of the job sees whole: full0 .. full1
             const int jfirst = at.q.hist + col_row(slot * 32, unused), jlast = at.q.hist + col_row(slot * 32 + 31, unused);
             const int full0 = (first_key(a, jlast) + 31) >> 5, full1 = ((jfirst + 1) >> 5) - 1;
@@ -676,7 +684,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             static_assert(kBox == 32 * kChunks * 16 && kSteps * kPasses == KS, "q");
             uint8_t* box = lds + (KSP == 2 ? (slot < 2 ? 2 + slot : slot == 2 ? 5 : 7) * TB
                                   : DS == 1 ? (wave < 2 ? TB : 2 * TB) + wave * (TB / 2)
-                                  : wave < 4 ? TB + wave * (TB / 4) : P::XCH + (wave - 4) * (TB / 4));
+                                  : (wave < 4 ? TB : 3 * TB) + (wave & 3) * (TB / 4));
             auto q_row = [&](int pass) {
                 return [=](int r) {
                     int hh;
@@ -822,9 +830,8 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 }
             } else {
                 ask_page(0);
-                if (DS == 1 || !uv) copy(0);
+                copy(0);
                 load_q();
-                if (DS == 2) lds_barrier();
             }
             f16_t o[NT] = {};
             float m = -FLT_MAX, l = 0.0f;
@@ -833,31 +840,37 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             struct Ops {
                 op x[NK];
             };
-            // lane's place in a tile
-            const int kbase = M::REG ? lane * 16 : (col >> 4) * KC * 1024 + h * 256 + (col & 15) * 16;
-            const int vbase = M::REG ? lane * 16 : (h * 16 + (col & 15)) * 16 + (col >> 4) * 8;
+            // a lane's place in a tile
+            auto k_place = [&]() {
+                const int lane = own_lane(), c = lane & 31;
+                return M::REG ? lane * 16 : (c >> 4) * KC * 1024 + (lane >> 5) * 256 + (c & 15) * 16;
+            };
+            auto v_place = [&]() {
+                const int lane = own_lane(), c = lane & 31;
+                return M::REG ? lane * 16 : ((lane >> 5) * 16 + (c & 15)) * 16 + (c >> 4) * 8;
+            };
             auto read_k = [&](const uint8_t* from, int i, Ops& k) {
                 const int s = part * KS + i;
 #pragma unroll
                 for (int j = 0; j < NK; j++)
-                    k.x[j] = *reinterpret_cast<const op*>(from + kbase + (M::REG ? j * 64 * HD + s * 1024 : (s >> 1) * 1024 + (s & 1) * 512));
+                    k.x[j] = *reinterpret_cast<const op*>(from + (M::REG ? j * 64 * HD + s * 1024 : (s >> 1) * 1024 + (s & 1) * 512));
             };
             auto read_v = [&](const uint8_t* from, int i, Ops& v) {
                 const int s = part * NT * 2 + i;
                 if constexpr (M::REG) {
 #pragma unroll
-                    for (int j = 0; j < NK; j++) v.x[j] = *reinterpret_cast<const op*>(from + vbase + j * 64 * HD + s * 1024);
+                    for (int j = 0; j < NK; j++) v.x[j] = *reinterpret_cast<const op*>(from + j * 64 * HD + s * 1024);
                 } else {
-                    const uint8_t* x = from + vbase + (s & 1) * KC * 1024 + (s >> 1) * 1024;
+                    const uint8_t* x = from + (s & 1) * KC * 1024 + (s >> 1) * 1024;
                     const uint2 y = *reinterpret_cast<const uint2*>(x), z = *reinterpret_cast<const uint2*>(x + 512);
                     v.x[0] = __builtin_bit_cast(op, make_uint4(y.x, y.y, z.x, z.y));
                 }
             };
             // feed(i): what is done beside step i's products
             auto scores = [&](int st, auto&& feed) {
-                const uint8_t* from = lds + P::k_at(st, kp);
+                const uint8_t* from = lds + P::k_at(st, kp) + k_place();
                 sc = f16_t{};
-                if constexpr (NQ == 1) {
+                if constexpr (NQ == 1 && !BOTH) {
 #pragma unroll
                     for (int i = 0; i < KS; i++) {
                         Ops k;
@@ -881,9 +894,10 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                                                      sx = f16_t{};
                                                  }
                                              });
-                    sc += sx;
+                    if (NQ > 1) sc += sx;
                     if constexpr (M::F) {
                         const float* meta = reinterpret_cast<const float*>(lds + P::meta_at(st, 0));
+                        const int h = own_lane() >> 5;
 #pragma unroll
                         for (int b = 0; b < 4; b++) {
                             const f4_t x = *reinterpret_cast<const f4_t*>(meta + (DS == 1 ? 32 : part * 32) + 8 * b + 4 * h);
@@ -898,6 +912,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 }
             };
             auto weights = [&](int st) {
+                const int lane = own_lane(), h = lane >> 5;
                 const int kt = ktb + st * KSP + kp;
                 const float* meta = reinterpret_cast<const float*>(lds + P::meta_at(st, kp));
                 const unsigned* mk = reinterpret_cast<const unsigned*>(meta) + kMetaMarks / 4;
@@ -940,7 +955,8 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                         if (marks >> (8 * (r >> 2) + 4 * h + (r & 3)) & 1) sc[r] = __uint_as_float(0x7fc00000u);
                 }
                 if (kt < full0 || kt > full1) {
-                    const int hi = pos - kt * 32 - 4 * h, lo = kf - kt * 32 - 4 * h;
+                    const int pos = at.q.hist + col_row(slot * 32 + (lane & 31), unused);
+                    const int hi = pos - kt * 32 - 4 * h, lo = first_key(a, pos) - kt * 32 - 4 * h;
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
                         const int key = 8 * (r >> 2) + (r & 3);
@@ -1004,8 +1020,8 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 }
             };
             auto values = [&](int st, auto&& feed) {
-                const uint8_t* from = lds + P::v_at(st, kp);
-                if constexpr (NP == 1) {
+                const uint8_t* from = lds + P::v_at(st, kp) + v_place();
+                if constexpr (NP == 1 && !BOTH) {
 #pragma unroll
                     for (int i = 0; i < 2 * NT; i++) {
                         Ops v;
@@ -1019,7 +1035,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                                                      f16_t& s = o[i >> 1];
                                                      s = mfma32(v.x[0], p[0][i & 1], s);
                                                      feed(i);
-                                                     s = mfma32(v.x[0], p[1][i & 1], s);
+                                                     if constexpr (NP == 2) s = mfma32(v.x[0], p[NP - 1][i & 1], s);
                                                      if constexpr (NK == 2) s = mfma32(v.x[1], p[0][i & 1], s);
                                                  });
                 }
@@ -1032,24 +1048,38 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             auto clean = [&](int st, bool careful) {
                 if (M::REG || !uv || piece0 != 0) return;
                 const unsigned use = block_use(st);
-                uint8_t* v = lds + P::v_at(st, ut) + ub * KC * 1024;
-                unsigned seen = 0;
-                for (int i = lane; i < KC * 64; i += 64) {
-                    uint4 x = *reinterpret_cast<const uint4*>(v + i * 16);
-                    const int t0 = (i >> 4 & 3) * 4;
-                    unsigned w[4] = {x.x, x.y, x.z, x.w};
-                    constexpr unsigned kInf = TC == G4_F16 ? 0x7c00u : 0x7f80u;
+                const int lane = own_lane(), g = lane >> 4;
+                uint8_t* v = lds + P::v_at(st, ut) + ub * KC * 1024 + lane * 16;
+                // this lane's 16 bytes of every piece are two dims of tokens 4 g .. 4 g + 3
+                unsigned keep[2], seen = 0;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const int t = t0 + (k & 3);
-                        const unsigned sh = 16 * (k & 1), e = w[k >> 1] >> sh & kInf;
-                        const bool bad = careful && e == kInf;
-                        if (bad || !(use >> t & 1)) w[k >> 1] &= ~(0xffffu << sh);
-                        if (bad && use >> t & 1) seen |= 1u << t;
+                for (int k = 0; k < 2; k++)
+                    keep[k] = (use >> (4 * g + 2 * k) & 1 ? 0xffffu : 0u) | (use >> (4 * g + 2 * k + 1) & 1 ? 0xffff0000u : 0u);
+                if (careful) {
+#pragma nounroll
+                    for (int i = 0; i < KC; i++) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(v + i * 1024);
+                        unsigned w[4] = {x.x, x.y, x.z, x.w};
+                        constexpr unsigned kInf = TC == G4_F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const unsigned sh = 16 * (k & 1);
+                            if ((w[k >> 1] >> sh & kInf) == kInf) {
+                                w[k >> 1] &= ~(0xffffu << sh);
+                                seen |= 1u << (4 * g + (k & 3));
+                            }
+                        }
+                        *reinterpret_cast<uint4*>(v + i * 1024) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    seen &= use;
+                    if (seen) atomicOr(reinterpret_cast<unsigned*>(mine_meta + P::meta_at(st, ut)), seen);
                 }
-                if (careful && seen) atomicOr(reinterpret_cast<unsigned*>(mine_meta + P::meta_at(st, ut)), seen);
+#pragma nounroll
+                for (int i = 0; i < KC; i++) {
+                    uint4 x = *reinterpret_cast<const uint4*>(v + i * 1024);
+                    x.x &= keep[0]; x.y &= keep[1]; x.z &= keep[0]; x.w &= keep[1];
+                    *reinterpret_cast<uint4*>(v + i * 1024) = x;
+                }
             };
             // whether a stage has tokens that nobody looks at
             auto ragged = [&](int st) {
@@ -1058,6 +1088,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             };
 
             const auto nothing = [](int) {};
+            bool met = false;   // whether all waves have met since their last tile
             for (bool careful = false;; careful = true) {
                 if constexpr (BOTH && DS == 1) {
                     for (int st = 0; st < stages; st++) {
@@ -1090,7 +1121,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                         weights(st);
                         values(st, [&](int i) { pieces(i, 2 * NT, [&](int j) { piece_k(st + 1, j); }); });
                     }
-                } else if constexpr (DS == 1) {
+                } else {
                     // this wave's copies have landed, then everyone's; and all are done
                     // with the stage before (waves 4 .. 7 but for its V, which has three
                     // places)
@@ -1112,7 +1143,54 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                         }
                     };
                     int st = 0;
-                    if (KSP == 1 || kp == 0) {
+                    if constexpr (DS == 2) {
+                        for (; st < stages; st++) {
+                            turn(st);
+                            scores(st, nothing);
+                            // a job's two waves give each other their partial scores
+                            const int lane = own_lane();
+                            f4_t* xch = reinterpret_cast<f4_t*>(lds + P::XCH) + lane;
+                            auto give = [&](int box) {
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    xch[(box * 4 + i) * 64] = f4_t{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+                            };
+                            f4_t y[4];
+                            auto take = [&](int box) {
+#pragma unroll
+                                for (int i = 0; i < 4; i++) y[i] = xch[(box * 4 + i) * 64];
+                            };
+                            auto add = [&]() {
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+#pragma unroll
+                                    for (int j = 0; j < 4; j++) sc[4 * i + j] += y[i][j];
+                            };
+                            if constexpr (NW == 4) {
+                                give(wave);
+                                lds_barrier();
+                                take(wave ^ 1);
+                                add();
+                            } else {
+                                // one place a job, for one and then for the other: two would not fit
+                                if (part == 0) give(slot);
+                                lds_barrier();
+                                if (part == 1) {
+                                    take(slot);
+                                    wave_lds_order();
+                                    give(slot);
+                                    add();
+                                }
+                                lds_barrier();
+                                if (part == 0) {
+                                    take(slot);
+                                    add();
+                                }
+                            }
+                            weights(st);
+                            values(st, nothing);
+                        }
+                    } else if (KSP == 1 || kp == 0) {
                         for (; st < stages; st++) {
                             turn(st);
                             scores(st, nothing);
@@ -1135,54 +1213,6 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                         }
                         if ((stages - 1) * KSP + kp < ntile) values(stages - 1, nothing);
                     }
-                } else {
-                    f4_t* xch = reinterpret_cast<f4_t*>(lds + P::XCH);
-                    for (int st = 0; st < stages; st++) {
-                        // K is there, V of the tile before done with
-                        if (!M::REG && !uv) wait_vm<0>();
-                        lds_barrier();
-                        if (uv) {
-                            if constexpr (M::REG) {
-                                put(st);
-                                fetch(st + 1);
-                            } else {
-                                copy(st);
-                            }
-                        }
-                        scores(st, nothing);
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            xch[(wave * 4 + i) * 64 + lane] = f4_t{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
-                        lds_barrier();   // K is done with, the partial scores (and V out of registers) there
-                        if (!uv && st + 1 < stages) {
-                            if constexpr (M::REG) {
-                                put(st + 1);
-                                fetch(st + 2);
-                            } else {
-                                copy(st + 1);
-                            }
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const f4_t y = xch[((wave ^ 1) * 4 + i) * 64 + lane];
-#pragma unroll
-                            for (int j = 0; j < 4; j++) sc[4 * i + j] += y[j];
-                        }
-                        // marks have to be there before the weights
-                        const bool special = !M::REG && (careful || ragged(st));
-                        if (special) {
-                            if (uv) wait_vm<0>();
-                            lds_barrier();
-                            clean(st, careful);
-                            lds_barrier();
-                        }
-                        weights(st);
-                        if (!M::REG && !special) {
-                            if (uv) wait_vm<0>();
-                            lds_barrier();   // V is there
-                        }
-                        values(st, nothing);
-                    }
                 }
                 // ---- a result that is not finite: once more, carefully ----
                 if (M::REG || careful) break;
@@ -1199,21 +1229,24 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 unsigned any = 0;
 #pragma unroll
                 for (int w = 0; w < NW; w++) any |= votes[w];
-                if (!__builtin_amdgcn_readfirstlane(any)) break;
+                met = !__builtin_amdgcn_readfirstlane(any);
+                if (met) break;
 #pragma unroll
                 for (int i = 0; i < NT; i++) o[i] = f16_t{};
                 m = -FLT_MAX;
                 l = 0.0f;
                 ask_page(0);
-                if (DS == 1 || !uv) copy(0);
+                copy(0);
             }
 
             {
             const int lane = own_lane(), col = lane & 31, h = lane >> 5;
             const bool whole = tile0 == 0 && tile1 == it.tiles;
             l += shfl_xor(l, 32);
-            wait_vm<0>();
-            lds_barrier();
+            if (!met) {
+                wait_vm<0>();
+                lds_barrier();
+            }
             if constexpr (KSP == 2) {
                 // waves 4 .. 7 hand their sums to waves 0 .. 3
                 float* ml = reinterpret_cast<float*>(lds + NJ * HD * 128) + slot * 64 + col * 2;
@@ -1385,6 +1418,12 @@ void set_columns(ChunkArgs& a, int cols) {
     a.rpi = cols / a.gh;
     const long used = (long)a.m * a.gh;
     a.cols = used < cols ? (int)((used + 31) / 32 * 32) : cols;
+    // the most that the line can measure: fewer shares, fewer workgroups
+    double keys = (double)(a.p.table_stride * (1l << a.p.lgpage));
+    if (a.window > 0 && a.window < keys) keys = a.window;
+    const double most = ((double)a.m / a.rpi + a.n_seqs) * (keys + a.rpi + kLead) * a.p.n_kv * a.ngrp / kLeast;
+    a.lg = 0;
+    while (a.lg < kLgShares && (2 << a.lg) <= most) a.lg++;
 }
 
 template <int TQ, int TC, int HD>
@@ -1400,8 +1439,9 @@ int launch_chunk(ChunkArgs a) {
         G4_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS));
         if (dev < 64) asked |= 1ull << dev;
     }
-    hipLaunchKernelGGL(kernel, dim3(kShares), dim3(64 * P::NW), P::LDS, g4_stream(), a);
-    hipLaunchKernelGGL((attn_chunk_join_kernel<TQ, HD>), dim3(kShares - 1, a.cols / 32, HD < 128 ? 1 : HD / 128), dim3(256), 0,
+    hipLaunchKernelGGL(kernel, dim3(1 << a.lg), dim3(64 * P::NW), P::LDS, g4_stream(), a);
+    if (a.lg == 0) return g4_check_launch("attn_chunk_kernel");   // nothing to join
+    hipLaunchKernelGGL((attn_chunk_join_kernel<TQ, HD>), dim3((1 << a.lg) - 1, a.cols / 32, HD < 128 ? 1 : HD / 128), dim3(256), 0,
                        g4_stream(), a);
     return g4_check_launch("attn_chunk_kernel");
 }
