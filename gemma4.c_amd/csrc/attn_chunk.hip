@@ -259,8 +259,8 @@ struct OpOf<true> { typedef h8_t t; };
 template <int TQ, int TC, int HD>
 struct Plan {
     typedef Mode<TQ, TC> M;
-    static constexpr int DS = HD == 512 ? 2 : 1;
-    static constexpr int NW = M::NQ == 1 && !M::REG ? 8 : 4;         // waves; 8: two a SIMD
+    static constexpr int DS = HD == 512 && M::NQ > 1 ? 2 : 1;
+    static constexpr int NW = M::NQ == 1 && !M::REG && HD < 512 ? 8 : 4;   // waves; 8: two a SIMD
     static constexpr int KSP = NW == 8 && DS == 1 ? 2 : 1;           // tiles at a time
     static constexpr int NJ = NW / DS / KSP, COLS = 32 * NJ;
     // LDS: K and V of a tile are TB bytes each
@@ -391,15 +391,23 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             };
             uint8_t* const mine_meta = lds + kMetaMarks + ub * 4;
             // straight to LDS (K or V, as this wave has it)
-            auto copy = [&](int st) {
+            __amdgpu_buffer_rsrc_t copy_rsrc;
+            uint8_t* copy_to = lds;
+            auto copy_piece = [&](int i) { buf_load_lds16(copy_rsrc, copy_to + i * 1024, piece0 * 1024 + (tid & 63) * 16, i * 1024); };
+            auto begin_copy = [&](int st) {
                 const int pg = take_page();
-                const __amdgpu_buffer_rsrc_t r = block_rsrc(block_at(st, pg), pg);
-                uint8_t* to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut)) + (ub * KC + piece0) * 1024;
-#pragma unroll
-                for (int i = 0; i < PCS; i++) buf_load_lds16(r, to + i * 1024, piece0 * 1024 + lane * 16, i * 1024);
+                copy_rsrc = block_rsrc(block_at(st, pg), pg);
+                copy_to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut)) + (ub * KC + piece0) * 1024;
                 if (uv && piece0 == 0 && lane == 0) *reinterpret_cast<unsigned*>(mine_meta + P::meta_at(st, ut)) = pg == -1 ? 0xffffu : 0u;
                 ask_page(st + 1);
             };
+            auto copy = [&](int st) {
+                begin_copy(st);
+#pragma unroll
+                for (int i = 0; i < PCS; i++) copy_piece(i);
+            };
+            // one wave a SIMD: copies are issued between the products
+            constexpr bool kFeed = !M::REG && NW == 4;
             // through registers
             uint4 raw[M::REG ? PCS : 1];
             float raw_scale = 0.0f;
@@ -833,6 +841,17 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 copy(0);
                 load_q();
             }
+            // one wave a SIMD: q (two terms of it) and, but for 16 bits of 512, o stay in
+            // the accumulation registers, from which products take them as well (left
+            // to itself the compiler moves q there and back for every tile)
+            if constexpr (NW == 4 && NQ > 1 && HD >= 256) {
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int i = 0; i < KS; i++) {
+                        asm("" : "+a"(q[k][i]));
+                    }
+            }
             f16_t o[NT] = {};
             float m = -FLT_MAX, l = 0.0f;
             f16_t sc;
@@ -870,7 +889,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             auto scores = [&](int st, auto&& feed) {
                 const uint8_t* from = lds + P::k_at(st, kp) + k_place();
                 sc = f16_t{};
-                if constexpr (NQ == 1 && !BOTH) {
+                if constexpr (NW == 8) {
 #pragma unroll
                     for (int i = 0; i < KS; i++) {
                         Ops k;
@@ -974,8 +993,10 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     if constexpr (M::F) l = move_sum(l, m - top);
                     else l *= f;
                     m = top;
+                    if (__any(l != 0.0f)) {
 #pragma unroll
-                    for (int i = 0; i < NT; i++) o[i] *= f;
+                        for (int i = 0; i < NT; i++) o[i] *= f;
+                    }
                 }
                 const float base = m - M::kLift;
 #pragma unroll
@@ -1021,7 +1042,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             };
             auto values = [&](int st, auto&& feed) {
                 const uint8_t* from = lds + P::v_at(st, kp) + v_place();
-                if constexpr (NP == 1 && !BOTH) {
+                if constexpr (NW == 8) {
 #pragma unroll
                     for (int i = 0; i < 2 * NT; i++) {
                         Ops v;
@@ -1139,14 +1160,22 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                                 clean(st, careful);
                                 lds_barrier();
                             }
-                            if (st + 1 < stages) copy(st + 1);
+                            if (kFeed) begin_copy(st + 1);      // past the last tile: no bytes
+                            else if (st + 1 < stages) copy(st + 1);
+                        }
+                    };
+                    auto feed = [&](int i) {
+                        if constexpr (kFeed) {
+#pragma unroll
+                            for (int j = 0; j < PCS; j++)
+                                if (j * KS / PCS == i) copy_piece(j);
                         }
                     };
                     int st = 0;
                     if constexpr (DS == 2) {
                         for (; st < stages; st++) {
                             turn(st);
-                            scores(st, nothing);
+                            scores(st, feed);
                             // a job's two waves give each other their partial scores
                             const int lane = own_lane();
                             f4_t* xch = reinterpret_cast<f4_t*>(lds + P::XCH) + lane;
@@ -1166,48 +1195,31 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
 #pragma unroll
                                     for (int j = 0; j < 4; j++) sc[4 * i + j] += y[i][j];
                             };
-                            if constexpr (NW == 4) {
-                                give(wave);
-                                lds_barrier();
-                                take(wave ^ 1);
-                                add();
-                            } else {
-                                // one place a job, for one and then for the other: two would not fit
-                                if (part == 0) give(slot);
-                                lds_barrier();
-                                if (part == 1) {
-                                    take(slot);
-                                    wave_lds_order();
-                                    give(slot);
-                                    add();
-                                }
-                                lds_barrier();
-                                if (part == 0) {
-                                    take(slot);
-                                    add();
-                                }
-                            }
+                            give(wave);
+                            lds_barrier();
+                            take(wave ^ 1);
+                            add();
                             weights(st);
                             values(st, nothing);
                         }
                     } else if (KSP == 1 || kp == 0) {
                         for (; st < stages; st++) {
                             turn(st);
-                            scores(st, nothing);
+                            scores(st, feed);
                             weights(st);
                             values(st, nothing);
                         }
                     } else {
                         turn(st);
                         if (kp < ntile) {
-                            scores(st, nothing);
+                            scores(st, feed);
                             weights(st);
                         }
                         for (st++; st < stages; st++) {
                             turn(st);
                             values(st - 1, nothing);
                             if (st * KSP + kp < ntile) {
-                                scores(st, nothing);
+                                scores(st, feed);
                                 weights(st);
                             }
                         }
@@ -1310,8 +1322,11 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
 #pragma unroll
                         for (int b = 0; b < 4; b++)
                             sums[(i * 4 + b) * 64] = f4_t{o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
-                    if (h == 0)
-                        *reinterpret_cast<float2*>(to + (size_t)a.cols * HD + (part * a.cols + slot * 32 + col) * 2) = make_float2(m, l);
+                    if (h == 0) {
+                        float2* ml = reinterpret_cast<float2*>(to + (size_t)a.cols * HD) + slot * 32 + col;
+                        ml[part * a.cols] = make_float2(m, l);
+                        if (HD == 512 && DS == 1) ml[a.cols] = make_float2(m, l);
+                    }
                 }
             }
             }
