@@ -24,6 +24,7 @@ struct ChunkArgs {
     int gh, ngrp;   // of these, a workgroup's; groups of them
     int rpi;        // rows of an item
     int lg;         // no more shares than 2^lg, by the call's sizes
+    bool pairs;     // Mode::kPairs
     int cols;       // columns of a partial result, a multiple of 32
     float scale;
 };
@@ -231,6 +232,8 @@ struct Mode {
     static constexpr int NQ = TQ != G4_F32 ? 1 : kHalf ? 2 : 3, NK = F ? 2 : 1, NP = TQ != G4_F32 ? 1 : 2;
     // a score is the sum of products as it stands, times log2(e) scale
     static constexpr bool kRaw = !F && !Q8 && NQ < 3;
+    // rows of O^T are its dims, in 16 bits pairs of dims 16 apart
+    static constexpr bool kPairs = !REG;
     // how far a score may pass the maximum before it moves, and how far above the
     // largest score it is put.  bf16, whose V goes as far as fp32: weights are at
     // most 1; fp16's smallest numbers ask for large weights, and its V cannot overflow
@@ -866,7 +869,9 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             };
             auto v_place = [&]() {
                 const int lane = own_lane(), c = lane & 31;
-                return M::REG ? lane * 16 : ((lane >> 5) * 16 + (c & 15)) * 16 + (c >> 4) * 8;
+                // row r of a product is dim 16 (r & 1) + r / 2 of its 32: neighbours read
+                // neighbours (in the order of the dims, 16 bytes apart, twice the cycles)
+                return M::REG ? lane * 16 : (lane >> 5) * 256 + c * 8;
             };
             auto read_k = [&](const uint8_t* from, int i, Ops& k) {
                 const int s = part * KS + i;
@@ -899,7 +904,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     order_products<KS, 3, 1, 1>();
                 } else {
                     f16_t sx = {}, low;
-                    run_products<Ops, KS, 2>([&](int i, Ops& k) { read_k(from, i, k); },
+                    run_products<Ops, KS, (NQ == 1 ? 6 : NK == 2 ? 2 : 3)>([&](int i, Ops& k) { read_k(from, i, k); },
                                              [&](int i, const Ops& k) {
                                                  sc = mfma32(k.x[0], q[0][i], sc);
                                                  feed(i);
@@ -1051,7 +1056,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     }
                     order_products<2 * NT, 3, 1, 1>();
                 } else {
-                    run_products<Ops, 2 * NT, 2>([&](int i, Ops& v) { read_v(from, i, v); },
+                    run_products<Ops, 2 * NT, (NP == 1 ? 6 : NK == 2 ? 2 : 3)>([&](int i, Ops& v) { read_v(from, i, v); },
                                                  [&](int i, const Ops& v) {
                                                      f16_t& s = o[i >> 1];
                                                      s = mfma32(v.x[0], p[0][i & 1], s);
@@ -1303,10 +1308,16 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                         for (int b = 0; b < 4; b++) {
                             E y[4];
 #pragma unroll
-                            for (int j = 0; j < 4; j++) y[j] = (E)(o[i][4 * b + j] * f);
-                            uint8_t* to = rows + (TQ == G4_F32 ? row_slot<kRow>(col, i * 8 + 2 * b + h)
-                                                               : row_slot<kRow>(col, i * 4 + b) + h * 8);
-                            __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(E)), y, 4 * sizeof(E));
+                            for (int j = 0; j < 4; j++) y[j] = (E)(o[i][4 * b + (M::kPairs ? (j & 1) * 2 + (j >> 1) : j)] * f);
+                            // dims d .. d + 3, or d, d + 1 and 16 more of them
+                            constexpr int kTwo = M::kPairs ? 2 : 1;
+#pragma unroll
+                            for (int k = 0; k < kTwo; k++) {
+                                const int d = 32 * i + (M::kPairs ? 16 * k + 4 * b + 2 * h : 8 * b + 4 * h);
+                                constexpr int kPer = 16 / sizeof(E), kN = 4 / kTwo * sizeof(E);
+                                uint8_t* to = rows + row_slot<kRow>(col, d / kPer) + d % kPer * sizeof(E);
+                                __builtin_memcpy(__builtin_assume_aligned(to, kN), y + 4 / kTwo * k, kN);
+                            }
                         }
                     rows_from_lds<kRow>(rows, ncols - slot * 32, [&](int r) {
                         int hh;
@@ -1419,10 +1430,18 @@ __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
     const float f = 1.0f / l;
 #pragma unroll
     for (int k = 0; k < V; k++) {
-        // registers 4 b .. + 3 of 32-dim tile k: dims 8 b + 4 h .. + 3
-        const int d = k * 32 + (tid >> 6) * 8 + 4 * h;
+        // registers 4 b .. + 3 of 32-dim tile k: dims 8 b + 4 h .. + 3, or 4 b + 2 h, 16
+        // more, and one more of each
+        const int b = tid >> 6;
         const E y[4] = {(E)(x[k][0] * f), (E)(x[k][1] * f), (E)(x[k][2] * f), (E)(x[k][3] * f)};
-        __builtin_memcpy(__builtin_assume_aligned(out + d, 4 * sizeof(E)), y, 4 * sizeof(E));
+        if (a.pairs) {
+            const E z[4] = {y[0], y[2], y[1], y[3]};
+            E* to = out + k * 32 + 4 * b + 2 * h;
+            __builtin_memcpy(__builtin_assume_aligned(to, 2 * sizeof(E)), z, 2 * sizeof(E));
+            __builtin_memcpy(__builtin_assume_aligned(to + 16, 2 * sizeof(E)), z + 2, 2 * sizeof(E));
+        } else {
+            __builtin_memcpy(__builtin_assume_aligned(out + k * 32 + 8 * b + 4 * h, 4 * sizeof(E)), y, 4 * sizeof(E));
+        }
     }
 }
 
@@ -1445,6 +1464,7 @@ template <int TQ, int TC, int HD>
 int launch_chunk(ChunkArgs a) {
     typedef Plan<TQ, TC, HD> P;
     set_columns(a, P::COLS);
+    a.pairs = P::M::kPairs;
     auto kernel = attn_chunk_kernel<TQ, TC, HD>;
     // more than 64 KB of LDS has to be asked for, once on each device
     static std::atomic<unsigned long long> asked{0};
