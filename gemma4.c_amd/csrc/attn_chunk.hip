@@ -215,6 +215,21 @@ struct Item {
         return t < tiles ? t : tiles;
     }
 };
+// What the second launch has to know of a share, at the head of part; the place
+// in out is that of the item which the share has from the one before it.
+enum : unsigned {
+    kGoesIn = 1,      // the share's first item began before it
+    kTilesIn = 2,     // and has tiles in it,
+    kFromTile0 = 4,   // its first among them;
+    kGoesThrough = 8, // and goes on behind it
+    kGoesOut = 16,    // an item that begins in the share goes on behind it
+    kTilesOut = 32,   // and has tiles in it
+};
+struct alignas(32) ShareNote {
+    int row, cols, nh, head;   // first row of out, columns, heads, first head
+    unsigned flags;
+};
+constexpr size_t kNoteBytes = sizeof(ShareNote) * kShares;
 // floats of a partial result: 32 columns at a time in the order of a wave's
 // registers, then each column's maximum and weight sum (head_dim 512: for each
 // half of the dims, whose V rows have exponents of their own)
@@ -318,6 +333,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
     Line line;
     Place at;
     unsigned share = 0;
+    ShareNote* const notes = reinterpret_cast<ShareNote*>(a.part);
     if (!find_place<64 * NW>(
             a,
             [&](const Line& l) {
@@ -325,14 +341,29 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 share = l.lg == kLgShares ? (blockIdx.x & 7) * (kShares / 8) + (blockIdx.x >> 3) : blockIdx.x;
                 return share >> l.lg ? kNowhere : l.at(share);
             },
-            line, at, red))
+            line, at, red)) {
+        if (tid == 0) notes[share].flags = 0;
         return;
+    }
     u64 left = line.at(share + 1) - line.at(share);
+    unsigned note = at.x > 0 ? kGoesIn : 0;
+    int noted[4] = {};
 
     while (left > 0) {
         const u64 take = left < at.size - at.x ? left : at.size - at.x;
         const Item it(a, at);
         const int tile0 = it.tile_at(at.x, at.size), tile1 = it.tile_at(at.x + take, at.size);
+        const bool goes_on = at.x + take < at.size;
+        if (at.x > 0) {
+            const int kvh = at.rep / a.ngrp, hg = at.rep - kvh * a.ngrp;
+            note |= (tile0 < tile1 ? kTilesIn : 0) | (tile0 == 0 ? kFromTile0 : 0) | (goes_on ? kGoesThrough : 0);
+            noted[0] = at.q.r0 + it.row0;
+            noted[2] = a.group - hg * a.gh < a.gh ? a.group - hg * a.gh : a.gh;
+            noted[1] = it.rows * noted[2];
+            noted[3] = kvh * a.group + hg * a.gh;
+        } else if (goes_on) {
+            note |= kGoesOut | (tile0 < tile1 ? kTilesOut : 0);
+        }
         if (tile0 < tile1) {
             // every part of an item's work has a lane number of its own, so that no
             // address derived from it is kept in a register over the others
@@ -1326,17 +1357,19 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                                           part * (HD / DS));
                     });
                 } else {
-                    float* to = a.part + (size_t)(share * 2 + (tile0 == 0)) * part_floats(a.cols, HD);
+                    float* to = a.part + kNoteBytes / 4 + (size_t)(share * 2 + (tile0 == 0)) * part_floats(a.cols, HD);
                     f4_t* sums = reinterpret_cast<f4_t*>(to) + (size_t)(slot * DS + part) * NT * 256 + lane;
+                    if (slot * 32 + col < ncols) {
 #pragma unroll
-                    for (int i = 0; i < NT; i++)
+                        for (int i = 0; i < NT; i++)
 #pragma unroll
-                        for (int b = 0; b < 4; b++)
-                            sums[(i * 4 + b) * 64] = f4_t{o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
-                    if (h == 0) {
-                        float2* ml = reinterpret_cast<float2*>(to + (size_t)a.cols * HD) + slot * 32 + col;
-                        ml[part * a.cols] = make_float2(m, l);
-                        if (HD == 512 && DS == 1) ml[a.cols] = make_float2(m, l);
+                            for (int b = 0; b < 4; b++)
+                                sums[(i * 4 + b) * 64] = f4_t{o[i][4 * b], o[i][4 * b + 1], o[i][4 * b + 2], o[i][4 * b + 3]};
+                        if (h == 0) {
+                            float2* ml = reinterpret_cast<float2*>(to + (size_t)a.cols * HD) + slot * 32 + col;
+                            ml[part * a.cols] = make_float2(m, l);
+                            if (HD == 512 && DS == 1) ml[a.cols] = make_float2(m, l);
+                        }
                     }
                 }
             }
@@ -1344,7 +1377,13 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             lds_barrier();   // LDS is the next item's
         }
         left -= take;
-        if (!left) break;
+        if (!left) {
+            if (tid == 0) {
+                notes[share].flags = note;
+                *reinterpret_cast<int4*>(&notes[share].row) = make_int4(noted[0], noted[1], noted[2], noted[3]);
+            }
+            break;
+        }
         // ---- the next item ----
         at.x = 0;
         if (++at.item >= seq_items(a, at.q)) {
@@ -1352,7 +1391,10 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             if (++at.rep == a.p.n_kv * a.ngrp) {
                 at.rep = 0;
                 do {
-                    if (++at.s >= a.n_seqs) return;
+                    if (++at.s >= a.n_seqs) {   // lengths that changed meanwhile
+                        if (tid == 0) notes[share].flags = 0;
+                        return;
+                    }
                     at.q = seq_of(a, a.cu[at.s], a.cu[at.s + 1], a.lens[at.s]);
                 } while (at.q.n == 0);
             }
@@ -1364,50 +1406,47 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
 // ---- second launch: items of more than one share ---------------------------------
 // blockIdx: border between two shares, 32 columns, 128 dims (64 where there are
 // no more).  The first border inside an item joins its pieces, with the weights
-// 2^(m_i - max m).
+// 2^(m_i - max m), by what the first launch has noted of the shares.
 template <int TQ, int HD>
 __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
     typedef typename RowElem<TQ>::t E;
     constexpr int D = HD < 128 ? HD : 128, V = D / 32;     // dims, 16-byte values of a thread
-    __shared__ u64 red[8];
-    Line line;
-    Place at;
-    const unsigned w = blockIdx.x + 1;
+    __shared__ int list[kShares + 1];
+    __shared__ unsigned ends[4];
+    const int w = blockIdx.x + 1;
     const int slot = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
-    if (!find_place<256>(a, [&](const Line& l) { return w >> l.lg ? kNowhere : l.at(w); },
-                         line, at, red))
-        return;
-    const u64 start = line.at(w) - at.x, end = start + at.size;      // the item's place on the line
-    if (at.x == 0 || line.at(w - 1) > start) return;                 // an item's start, or not the first border in it
-    const Item it(a, at);
-    const int kvh = at.rep / a.ngrp, hg = at.rep - kvh * a.ngrp;
-    const int nh = a.group - hg * a.gh < a.gh ? a.group - hg * a.gh : a.gh, ncols = it.rows * nh;
-    if (slot * 32 >= ncols) return;
-    // piece i is share w - 1 + i's: tiles from edge(i) to edge(i + 1), if any
-    auto edge = [&](int i) {
-        if (i == 0) return 0;
-        const u64 u = (w - 1 + i) >> line.lg ? line.total : line.at(w - 1 + i);
-        return u >= end ? it.tiles : it.tile_at(u - start, at.size);
-    };
-    __shared__ int list[kShares], before[4];
-    int pieces = 0;
-    {
-        const int e0 = edge(tid), e1 = edge(tid + 1);
-        // in order, so that sums are the same every time
-        const u64 have = __ballot(e0 < e1);
-        if (lane == 0) before[tid >> 6] = __popcll(have);
-        lds_sync();
-        int k = __popcll(have & (((u64)1 << lane) - 1));
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (i < tid >> 6) k += before[i];
-            pieces += before[i];
-        }
-        if (e0 < e1) list[k] = (w - 1 + tid) * 2 + (e0 == 0);
+    const ShareNote* notes = reinterpret_cast<const ShareNote*>(a.part);
+    const int shares = 1 << a.lg;
+    const unsigned before = notes[w - 1].flags, mine = w + tid < shares ? notes[w + tid].flags : 0;
+    const ShareNote to = notes[w];
+    if (!(before & kGoesOut) || slot * 32 >= to.cols) return;
+    // the shares that the item goes through, up to the one that it ends in, and which
+    // of them have tiles; in order, so that sums are the same every time
+    const u64 stop = __ballot(!(mine & kGoesThrough));
+    if (lane == 0) ends[tid >> 6] = stop ? __builtin_ctzll(stop) : 64;
+    lds_sync();
+    int last = 0;
+    for (int i = 0; i < 4; i++) {
+        last += (int)ends[i];
+        if (ends[i] < 64) break;
     }
     lds_sync();
-    if (pieces < 2) return;     // one alone has been written
-    auto piece = [&](int i) { return a.part + (size_t)list[i] * part_floats(a.cols, HD); };
+    const bool in = tid <= last && mine & kTilesIn;
+    const u64 have = __ballot(in);
+    if (lane == 0) ends[tid >> 6] = __popcll(have);
+    lds_sync();
+    const int first = before & kTilesOut ? 1 : 0;
+    int k = first + __popcll(have & (((u64)1 << lane) - 1)), pieces = first;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (i < tid >> 6) k += ends[i];
+        pieces += ends[i];
+    }
+    if (in) list[k] = (w + tid) * 2 + (mine & kFromTile0 ? 1 : 0);
+    if (first && tid == 0) list[0] = (w - 1) * 2 + 1;
+    lds_sync();
+    if (pieces < 2 || slot * 32 + col >= to.cols) return;     // one alone has been written
+    auto piece = [&](int i) { return a.part + kNoteBytes / 4 + (size_t)list[i] * part_floats(a.cols, HD); };
     const size_t ml = (size_t)a.cols * HD + ((z * D >= 256 ? a.cols : 0) + slot * 32 + col) * 2;
     float top = -FLT_MAX;
 #pragma unroll 4
@@ -1424,9 +1463,8 @@ __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
 #pragma unroll
         for (int k = 0; k < V; k++) x[k] += sums[k * 256] * f;
     }
-    if (slot * 32 + col >= ncols) return;
-    const int r = (int)((unsigned)(slot * 32 + col) / (unsigned)nh), hh = slot * 32 + col - r * nh;
-    E* out = (E*)a.out + (size_t)(at.q.r0 + it.row0 + r) * a.out_stride + (size_t)(kvh * a.group + hg * a.gh + hh) * HD + z * D;
+    const int r = (int)((unsigned)(slot * 32 + col) * ((65535u + to.nh) / (unsigned)to.nh) >> 16), hh = slot * 32 + col - r * to.nh;
+    E* out = (E*)a.out + (size_t)(to.row + r) * a.out_stride + (size_t)(to.head + hh) * HD + z * D;
     const float f = 1.0f / l;
 #pragma unroll
     for (int k = 0; k < V; k++) {
@@ -1436,9 +1474,9 @@ __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
         const E y[4] = {(E)(x[k][0] * f), (E)(x[k][1] * f), (E)(x[k][2] * f), (E)(x[k][3] * f)};
         if (a.pairs) {
             const E z[4] = {y[0], y[2], y[1], y[3]};
-            E* to = out + k * 32 + 4 * b + 2 * h;
-            __builtin_memcpy(__builtin_assume_aligned(to, 2 * sizeof(E)), z, 2 * sizeof(E));
-            __builtin_memcpy(__builtin_assume_aligned(to + 16, 2 * sizeof(E)), z + 2, 2 * sizeof(E));
+            E* at = out + k * 32 + 4 * b + 2 * h;
+            __builtin_memcpy(__builtin_assume_aligned(at, 2 * sizeof(E)), z, 2 * sizeof(E));
+            __builtin_memcpy(__builtin_assume_aligned(at + 16, 2 * sizeof(E)), z + 2, 2 * sizeof(E));
         } else {
             __builtin_memcpy(__builtin_assume_aligned(out + k * 32 + 8 * b + 4 * h, 4 * sizeof(E)), y, 4 * sizeof(E));
         }
@@ -1499,7 +1537,7 @@ extern "C" size_t g4_attn_chunk_paged_part_bytes(int m, int n_heads, int n_kv, i
     // two partial results of each share
     const int group = n_heads / n_kv, cols = 128, gh = group < cols ? group : cols;
     const long used = (long)m * gh;
-    return (size_t)kShares * 2 * part_floats(used < cols ? (int)((used + 31) / 32 * 32) : cols, hd) * 4;
+    return kNoteBytes + (size_t)kShares * 2 * part_floats(used < cols ? (int)((used + 31) / 32 * 32) : cols, hd) * 4;
 }
 
 extern "C" int g4_attn_chunk_paged(const void* q, int q_stride, int q_type, const void* kp, const void* vp, int type,
