@@ -224,12 +224,15 @@ enum : unsigned {
     kGoesThrough = 8, // and goes on behind it
     kGoesOut = 16,    // an item that begins in the share goes on behind it
     kTilesOut = 32,   // and has tiles in it
+    kColsShift = 8,   // columns of the first item, at most 128
 };
-struct alignas(32) ShareNote {
-    int row, cols, nh, head;   // first row of out, columns, heads, first head
-    unsigned flags;
+struct ShareNote {
+    int row, nh, head;   // first row of out, heads, first head
 };
-constexpr size_t kNoteBytes = sizeof(ShareNote) * kShares;
+struct Notes {
+    unsigned flags[kShares];
+    ShareNote item[kShares];
+};
 // floats of a partial result: 32 columns at a time in the order of a wave's
 // registers, then each column's maximum and weight sum (head_dim 512: for each
 // half of the dims, whose V rows have exponents of their own)
@@ -333,7 +336,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
     Line line;
     Place at;
     unsigned share = 0;
-    ShareNote* const notes = reinterpret_cast<ShareNote*>(a.part);
+    Notes* const notes = reinterpret_cast<Notes*>(a.part);
     if (!find_place<64 * NW>(
             a,
             [&](const Line& l) {
@@ -342,12 +345,12 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 return share >> l.lg ? kNowhere : l.at(share);
             },
             line, at, red)) {
-        if (tid == 0) notes[share].flags = 0;
+        if (tid == 0) notes->flags[share] = 0;
         return;
     }
     u64 left = line.at(share + 1) - line.at(share);
     unsigned note = at.x > 0 ? kGoesIn : 0;
-    int noted[4] = {};
+    ShareNote noted = {};
 
     while (left > 0) {
         const u64 take = left < at.size - at.x ? left : at.size - at.x;
@@ -357,10 +360,10 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
         if (at.x > 0) {
             const int kvh = at.rep / a.ngrp, hg = at.rep - kvh * a.ngrp;
             note |= (tile0 < tile1 ? kTilesIn : 0) | (tile0 == 0 ? kFromTile0 : 0) | (goes_on ? kGoesThrough : 0);
-            noted[0] = at.q.r0 + it.row0;
-            noted[2] = a.group - hg * a.gh < a.gh ? a.group - hg * a.gh : a.gh;
-            noted[1] = it.rows * noted[2];
-            noted[3] = kvh * a.group + hg * a.gh;
+            noted.row = at.q.r0 + it.row0;
+            noted.nh = a.group - hg * a.gh < a.gh ? a.group - hg * a.gh : a.gh;
+            noted.head = kvh * a.group + hg * a.gh;
+            note |= (unsigned)(it.rows * noted.nh) << kColsShift;
         } else if (goes_on) {
             note |= kGoesOut | (tile0 < tile1 ? kTilesOut : 0);
         }
@@ -1357,7 +1360,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                                           part * (HD / DS));
                     });
                 } else {
-                    float* to = a.part + kNoteBytes / 4 + (size_t)(share * 2 + (tile0 == 0)) * part_floats(a.cols, HD);
+                    float* to = a.part + sizeof(Notes) / 4 + (size_t)(share * 2 + (tile0 == 0)) * part_floats(a.cols, HD);
                     f4_t* sums = reinterpret_cast<f4_t*>(to) + (size_t)(slot * DS + part) * NT * 256 + lane;
                     if (slot * 32 + col < ncols) {
 #pragma unroll
@@ -1379,8 +1382,8 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
         left -= take;
         if (!left) {
             if (tid == 0) {
-                notes[share].flags = note;
-                *reinterpret_cast<int4*>(&notes[share].row) = make_int4(noted[0], noted[1], noted[2], noted[3]);
+                notes->flags[share] = note;
+                notes->item[share] = noted;
             }
             break;
         }
@@ -1392,7 +1395,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 at.rep = 0;
                 do {
                     if (++at.s >= a.n_seqs) {   // lengths that changed meanwhile
-                        if (tid == 0) notes[share].flags = 0;
+                        if (tid == 0) notes->flags[share] = 0;
                         return;
                     }
                     at.q = seq_of(a, a.cu[at.s], a.cu[at.s + 1], a.lens[at.s]);
@@ -1404,82 +1407,126 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
 }
 
 // ---- second launch: items of more than one share ---------------------------------
-// blockIdx: border between two shares, 32 columns, 128 dims (64 where there are
-// no more).  The first border inside an item joins its pieces, with the weights
-// 2^(m_i - max m), by what the first launch has noted of the shares.
+// The first border inside an item stands for the item.  A workgroup takes every
+// gridDim.x-th of all such borders' units, 32 columns and 128 dims (64 where there
+// are no more), and joins the pieces with the weights 2^(m_i - max m), four at a
+// time.  (A workgroup for every border and unit, of which most have nothing to do:
+// 19 us where this takes 9, 40 sequences of a row and one of 471.)
+constexpr int kJoinWG = 1024;
 template <int TQ, int HD>
 __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
     typedef typename RowElem<TQ>::t E;
-    constexpr int D = HD < 128 ? HD : 128, V = D / 32;     // dims, 16-byte values of a thread
-    __shared__ int list[kShares + 1];
-    __shared__ unsigned ends[4];
-    const int w = blockIdx.x + 1;
-    const int slot = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, lane = tid & 63, col = lane & 31, h = lane >> 5;
-    const ShareNote* notes = reinterpret_cast<const ShareNote*>(a.part);
+    constexpr int D = HD < 128 ? HD : 128, V = D / 32, B = 4;     // dims, 16-byte values of a thread, pieces at a time
+    __shared__ unsigned flags[kShares];
+    __shared__ int list[kShares + 1], cnt[4], ends[4], found[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h = lane >> 5;
+    const Notes* notes = reinterpret_cast<const Notes*>(a.part);
     const int shares = 1 << a.lg;
-    const unsigned before = notes[w - 1].flags, mine = w + tid < shares ? notes[w + tid].flags : 0;
-    const ShareNote to = notes[w];
-    if (!(before & kGoesOut) || slot * 32 >= to.cols) return;
-    // the shares that the item goes through, up to the one that it ends in, and which
-    // of them have tiles; in order, so that sums are the same every time
-    const u64 stop = __ballot(!(mine & kGoesThrough));
-    if (lane == 0) ends[tid >> 6] = stop ? __builtin_ctzll(stop) : 64;
-    lds_sync();
-    int last = 0;
-    for (int i = 0; i < 4; i++) {
-        last += (int)ends[i];
-        if (ends[i] < 64) break;
-    }
-    lds_sync();
-    const bool in = tid <= last && mine & kTilesIn;
-    const u64 have = __ballot(in);
-    if (lane == 0) ends[tid >> 6] = __popcll(have);
-    lds_sync();
-    const int first = before & kTilesOut ? 1 : 0;
-    int k = first + __popcll(have & (((u64)1 << lane) - 1)), pieces = first;
+    // what the threads before this one have, and all of them
+    auto before = [&](int v, int& all) {
+        const int x = (int)wave_scan((u64)v);
+        lds_sync();
+        if (lane == 63) cnt[wave] = x;
+        lds_sync();
+        int k = x - v;
+        all = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (i < tid >> 6) k += ends[i];
-        pieces += ends[i];
-    }
-    if (in) list[k] = (w + tid) * 2 + (mine & kFromTile0 ? 1 : 0);
-    if (first && tid == 0) list[0] = (w - 1) * 2 + 1;
-    lds_sync();
-    if (pieces < 2 || slot * 32 + col >= to.cols) return;     // one alone has been written
-    auto piece = [&](int i) { return a.part + kNoteBytes / 4 + (size_t)list[i] * part_floats(a.cols, HD); };
-    const size_t ml = (size_t)a.cols * HD + ((z * D >= 256 ? a.cols : 0) + slot * 32 + col) * 2;
-    float top = -FLT_MAX;
-#pragma unroll 4
-    for (int i = 0; i < pieces; i++) top = fmaxf(top, piece(i)[ml]);
-    f4_t x[V] = {};
-    float l = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < pieces; i++) {
-        const float* from = piece(i);
-        const float2 y = *reinterpret_cast<const float2*>(from + ml);
-        const float f = exp2f(y.x - top);
-        l += f * y.y;
-        const f4_t* sums = reinterpret_cast<const f4_t*>(from) + (size_t)slot * HD * 8 + z * D * 8 + tid;
-#pragma unroll
-        for (int k = 0; k < V; k++) x[k] += sums[k * 256] * f;
-    }
-    const int r = (int)((unsigned)(slot * 32 + col) * ((65535u + to.nh) / (unsigned)to.nh) >> 16), hh = slot * 32 + col - r * to.nh;
-    E* out = (E*)a.out + (size_t)(to.row + r) * a.out_stride + (size_t)(to.head + hh) * HD + z * D;
-    const float f = 1.0f / l;
-#pragma unroll
-    for (int k = 0; k < V; k++) {
-        // registers 4 b .. + 3 of 32-dim tile k: dims 8 b + 4 h .. + 3, or 4 b + 2 h, 16
-        // more, and one more of each
-        const int b = tid >> 6;
-        const E y[4] = {(E)(x[k][0] * f), (E)(x[k][1] * f), (E)(x[k][2] * f), (E)(x[k][3] * f)};
-        if (a.pairs) {
-            const E z[4] = {y[0], y[2], y[1], y[3]};
-            E* at = out + k * 32 + 4 * b + 2 * h;
-            __builtin_memcpy(__builtin_assume_aligned(at, 2 * sizeof(E)), z, 2 * sizeof(E));
-            __builtin_memcpy(__builtin_assume_aligned(at + 16, 2 * sizeof(E)), z + 2, 2 * sizeof(E));
-        } else {
-            __builtin_memcpy(__builtin_assume_aligned(out + k * 32 + 8 * b + 4 * h, 4 * sizeof(E)), y, 4 * sizeof(E));
+        for (int i = 0; i < 4; i++) {
+            if (i < wave) k += cnt[i];
+            all += cnt[i];
         }
+        return k;
+    };
+    const unsigned mine = tid < shares ? notes->flags[tid] : 0;
+    flags[tid] = mine;
+    lds_sync();
+    // thread t: units of the item that goes out of share t
+    const int cols_out = mine & kGoesOut ? (int)(flags[tid + 1] >> kColsShift) : 0, units = (cols_out + 31) / 32 * (HD / D);
+    int n;
+    const int unit0 = before(units, n);
+    for (int unit = blockIdx.x; unit < n; unit += gridDim.x) {
+        if (unit >= unit0 && unit < unit0 + units) {
+            found[0] = tid + 1;
+            found[1] = unit - unit0;
+        }
+        lds_sync();
+        const int w = found[0], slot = found[1] / (HD / D), z = found[1] % (HD / D), ncols = (int)(flags[w] >> kColsShift);
+        const ShareNote to = notes->item[w];
+        // the shares that the item goes through, up to the one that it ends in, and which
+        // of them have tiles; in order, so that sums are the same every time
+        const unsigned f = w + tid < shares ? flags[w + tid] : 0;
+        const u64 stop = __ballot(!(f & kGoesThrough));
+        if (lane == 0) ends[wave] = stop ? __builtin_ctzll(stop) : 64;
+        lds_sync();
+        int last = 0;
+        for (int i = 0; i < 4; i++) {
+            last += ends[i];
+            if (ends[i] < 64) break;
+        }
+        const bool in = tid <= last && f & kTilesIn;
+        const int first = flags[w - 1] & kTilesOut ? 1 : 0;
+        int pieces;
+        const int k = before(in ? 1 : 0, pieces) + first;
+        pieces += first;
+        if (in) list[k] = (w + tid) * 2 + (f & kFromTile0 ? 1 : 0);
+        if (first && tid == 0) list[0] = (w - 1) * 2 + 1;
+        lds_sync();
+        // one piece alone has been written
+        if (pieces > 1 && slot * 32 + col < ncols) {
+            const size_t at = (size_t)slot * HD * 32 + (size_t)z * D * 32 + tid * 4;
+            const size_t ml = (size_t)a.cols * HD + ((z * D >= 256 ? a.cols : 0) + slot * 32 + col) * 2;
+            f4_t x[V] = {};
+            float m = -FLT_MAX, l = 0.0f;
+            for (int i = 0; i < pieces; i += B) {
+                float2 y[B];
+                f4_t v[B][V];
+#pragma unroll
+                for (int j = 0; j < B; j++) {
+                    const int p = list[i + j < pieces ? i + j : i];
+                    const float* from = a.part + sizeof(Notes) / 4 + (size_t)p * part_floats(a.cols, HD);
+                    y[j] = *reinterpret_cast<const float2*>(from + ml);
+#pragma unroll
+                    for (int k = 0; k < V; k++) v[j][k] = *reinterpret_cast<const f4_t*>(from + at + k * 1024);
+                }
+                float top = m;
+#pragma unroll
+                for (int j = 0; j < B; j++) top = fmaxf(top, y[j].x);
+                const float f = exp2f(m - top);
+                m = top;
+                l *= f;
+#pragma unroll
+                for (int k = 0; k < V; k++) x[k] *= f;
+#pragma unroll
+                for (int j = 0; j < B; j++) {
+                    if (i + j >= pieces) break;
+                    const float f = exp2f(y[j].x - top);
+                    l = __builtin_fmaf(f, y[j].y, l);
+#pragma unroll
+                    for (int k = 0; k < V; k++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) x[k][c] = __builtin_fmaf(f, v[j][k][c], x[k][c]);
+                }
+            }
+            const int c = slot * 32 + col, r = (int)((unsigned)c * ((65535u + to.nh) / (unsigned)to.nh) >> 16), hh = c - r * to.nh;
+            E* out = (E*)a.out + (size_t)(to.row + r) * a.out_stride + (size_t)(to.head + hh) * HD + z * D;
+            const float s = 1.0f / l;
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                // registers 4 b .. + 3 of 32-dim tile k: dims 8 b + 4 h .. + 3, or 4 b + 2 h, 16
+                // more, and one more of each
+                const int b = wave;
+                const E y[4] = {(E)(x[k][0] * s), (E)(x[k][1] * s), (E)(x[k][2] * s), (E)(x[k][3] * s)};
+                if (a.pairs) {
+                    const E y2[4] = {y[0], y[2], y[1], y[3]};
+                    E* at = out + k * 32 + 4 * b + 2 * h;
+                    __builtin_memcpy(__builtin_assume_aligned(at, 2 * sizeof(E)), y2, 2 * sizeof(E));
+                    __builtin_memcpy(__builtin_assume_aligned(at + 16, 2 * sizeof(E)), y2 + 2, 2 * sizeof(E));
+                } else {
+                    __builtin_memcpy(__builtin_assume_aligned(out + k * 32 + 8 * b + 4 * h, 4 * sizeof(E)), y, 4 * sizeof(E));
+                }
+            }
+        }
+        lds_sync();   // the list is the next unit's
     }
 }
 
@@ -1514,8 +1561,8 @@ int launch_chunk(ChunkArgs a) {
     }
     hipLaunchKernelGGL(kernel, dim3(1 << a.lg), dim3(64 * P::NW), P::LDS, g4_stream(), a);
     if (a.lg == 0) return g4_check_launch("attn_chunk_kernel");   // nothing to join
-    hipLaunchKernelGGL((attn_chunk_join_kernel<TQ, HD>), dim3((1 << a.lg) - 1, a.cols / 32, HD < 128 ? 1 : HD / 128), dim3(256), 0,
-                       g4_stream(), a);
+    const int units = ((1 << a.lg) - 1) * (a.cols / 32) * (HD < 128 ? 1 : HD / 128);
+    hipLaunchKernelGGL((attn_chunk_join_kernel<TQ, HD>), dim3(units < kJoinWG ? units : kJoinWG), dim3(256), 0, g4_stream(), a);
     return g4_check_launch("attn_chunk_kernel");
 }
 template <int TQ, int TC>
@@ -1537,7 +1584,7 @@ extern "C" size_t g4_attn_chunk_paged_part_bytes(int m, int n_heads, int n_kv, i
     // two partial results of each share
     const int group = n_heads / n_kv, cols = 128, gh = group < cols ? group : cols;
     const long used = (long)m * gh;
-    return kNoteBytes + (size_t)kShares * 2 * part_floats(used < cols ? (int)((used + 31) / 32 * 32) : cols, hd) * 4;
+    return sizeof(Notes) + (size_t)kShares * 2 * part_floats(used < cols ? (int)((used + 31) / 32 * 32) : cols, hd) * 4;
 }
 
 extern "C" int g4_attn_chunk_paged(const void* q, int q_stride, int q_type, const void* kp, const void* vp, int type,
