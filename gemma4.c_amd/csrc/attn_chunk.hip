@@ -311,11 +311,10 @@ struct Plan {
 };
 // What lies beside a tile: 32 factors of K (fp32: 2^e, codes: scales), 32 of V
 // (exponents, scales), fp32: 2^-e; marks of each block's keys that make a score
-// NaN; fp32: the weight sums below which lost_weight is asked for.  BOTH: K's, V's
-// and the inverses for each half of the dims, 32 each, marks of K and V for each
-// block and half.
+// NaN.  BOTH: K's, V's and the inverses for each half of the dims, 32 each, marks
+// of K and V for each block and half.
 constexpr int kMetaV = 128, kMetaMarks = 384;
-constexpr int kBothV = 256, kBothInv = 512, kBothMarks = 768, kBothLost = 800;
+constexpr int kBothV = 256, kBothInv = 512, kBothMarks = 768;
 
 template <int TQ, int TC, int HD>
 __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW / 4)) void attn_chunk_kernel(ChunkArgs a) {
@@ -597,12 +596,13 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     for (int k = 0; k < 4; k++) top[k] = (w[k] & 0x7fffffffu) > top[k] ? w[k] & 0x7fffffffu : top[k];
                 }
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-#pragma unroll
-                    for (int d = 1; d < 16; d <<= 1) {
-                        const unsigned o = __shfl_xor(top[k], d, 64);
-                        top[k] = o > top[k] ? o : top[k];
-                    }
+                for (int k = 0; k < 4; k++) {
+                    auto larger = [&](int o) { top[k] = (unsigned)o > top[k] ? (unsigned)o : top[k]; };
+                    larger(dpp_i<kDppXor1>((int)top[k]));
+                    larger(dpp_i<kDppXor2>((int)top[k]));
+                    larger(dpp_i<kDppHalfMirror>((int)top[k]));
+                    larger(dpp_i<kDppMirror>((int)top[k]));
+                }
             };
             unsigned* const topx = reinterpret_cast<unsigned*>(lds + P::TOPX);
             auto share_tops = [&]() {
@@ -627,31 +627,31 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     } else {
                         tops_v(top);
                     }
-                    int low = 113;
                     float ex[4];
+                    bool odd = false;
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         int e = (int)(top[k] >> 23) > kLowV ? (int)(top[k] >> 23) : kLowV;
                         const bool on = use >> (4 * g + k) & 1, bad = e == 255;
                         keepv[k] = on && !bad;      // others become zeros
+                        odd = odd || (on && bad);
                         if (!keepv[k]) e = kLowV;
-                        const u64 b = __ballot(bad && on && t16 == 0);   // lanes 0, 16, 32, 48: tokens k, 4 + k, ..
-#pragma unroll
-                        for (int j = 0; j < 4; j++) marks |= (unsigned)(b >> (16 * j) & 1) << (4 * j + k);
                         sfv[k] = row_scale(e);
-                        ex[k] = (float)(e - 141);
-                        if (on && e - 141 < low) low = e - 141;
+                        ex[k] = on ? (float)(e - 141) : 113.0f;     // of no weight: not the smallest
+                    }
+                    if (__any(odd)) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const u64 b = __ballot((use >> (4 * g + k) & 1) && !keepv[k] && t16 == 0);   // lanes 0, 16, 32, 48
+#pragma unroll
+                            for (int j = 0; j < 4; j++) marks |= (unsigned)(b >> (16 * j) & 1) << (4 * j + k);
+                        }
                     }
                     if (t16 == 0) {
                         const int to = hf * 32 + bb * 16 + 4 * g;
                         *reinterpret_cast<f4_t*>(meta + kBothV / 4 + to) = f4_t{ex[0], ex[1], ex[2], ex[3]};
                         *reinterpret_cast<f4_t*>(meta + kBothInv / 4 + to) = f4_t{sfv[0], sfv[1], sfv[2], sfv[3]};
                     }
-                    int o = __shfl_xor(low, 16, 64);
-                    low = o < low ? o : low;
-                    o = __shfl_xor(low, 32, 64);
-                    low = o < low ? o : low;
-                    if (lane == 0) meta[kBothLost / 4 + hf * 2 + bb] = __builtin_ldexpf(1.0f, 48 - 126 - low);
                 } else {
                     const bool on = use >> t16 & 1 && pgv >= 0, bad = on && !(fabsf(vs16) < INFINITY);
                     marks |= (unsigned)__ballot(bad && g == 0) & 0xffffu;
@@ -985,6 +985,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 }
                 marks = __builtin_amdgcn_readfirstlane(marks);
                 float fv[16];       // codes: V's scales, fp32: 2^-e
+                float low = 113.0f;
                 const int vhalf = M::F && DS == 2 ? part * 32 : 0;
                 if constexpr (M::REG) {
 #pragma unroll
@@ -996,6 +997,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                             for (int i = 0; i < 4; i++) {
                                 sc[4 * b + i] = __builtin_fmaf(sc[4 * b + i], fq, v[i]);
                                 fv[4 * b + i] = vi[i];
+                                low = fminf(low, v[i]);
                             }
                         } else {
                             const f4_t k = *reinterpret_cast<const f4_t*>(meta + 8 * b + 4 * h);
@@ -1068,8 +1070,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     }
                 }
                 if constexpr (M::F) {
-                    const float* ml = meta + kBothLost / 4 + (DS == 2 ? part * 2 : 0);
-                    const float lost = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(ml[0], ml[1]))));
+                    const float lost = __builtin_ldexpf(1.0f, 48 - 126 - (int)low);   // of this lane's keys
                     if (__any(l < lost)) {
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
