@@ -506,7 +506,6 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             const int bb = wave & 1, hf = wave >> 1;
             uint4 rk[BOTH ? PH : 1], rv[BOTH ? PH : 1];
             float ks16 = 0.0f, vs16 = 0.0f, sfk = 0.0f, sfv[4];
-            bool keepv[4];
             int askk = 0, askv = 0, pgk = -2, pgv = -2;     // page asked for; page of what the registers hold
             bool onk = false, onv = false;
             __amdgpu_buffer_rsrc_t nk, nv;
@@ -552,6 +551,10 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 if (v) rv[j] = x;
                 else rk[j] = x;
             };
+            // largest of two numbers and one that is positive or NaN, which it stays
+            auto larger = [](uint32_t x, uint32_t y, float top) {
+                return __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(__uint_as_float(x)), fabsf(__uint_as_float(y))), top);
+            };
             // before the pieces of stage st, which the registers hold: factors, marks, and
             // the next stage's page
             auto begin_k = [&](int st) {
@@ -559,21 +562,17 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 const unsigned use = use2(st);
                 unsigned marks = pgk == -1 ? 0xffffu : 0u;
                 if constexpr (M::F) {
-                    unsigned top = 0;
+                    float top = 0.0f;
 #pragma unroll
                     for (int i = 0; i < PH; i++) {
-                        const unsigned w[4] = {rk[i].x, rk[i].y, rk[i].z, rk[i].w};
-#pragma unroll
-                        for (int k = 0; k < 4; k++) top = (w[k] & 0x7fffffffu) > top ? w[k] & 0x7fffffffu : top;
+                        top = larger(rk[i].x, rk[i].y, top);
+                        top = larger(rk[i].z, rk[i].w, top);
                     }
 #pragma unroll
-                    for (int d = 16; d < 64; d <<= 1) {
-                        const unsigned o = __shfl_xor(top, d, 64);
-                        top = o > top ? o : top;
-                    }
-                    int e = (int)(top >> 23) > kLowK ? (int)(top >> 23) : kLowK;
-                    const bool bad = e == 255;
-                    if (bad) e = kLowK;
+                    for (int d = 16; d < 64; d <<= 1) top = __builtin_elementwise_maximum(top, shfl_xor(top, d));
+                    const bool bad = !(top < INFINITY);
+                    int e = (int)(__float_as_uint(top) >> 23);
+                    if (bad || e < kLowK) e = kLowK;
                     marks |= (unsigned)__ballot(bad && g == 0 && (use >> t16 & 1)) & 0xffffu;
                     sfk = row_scale(e);
                     if (g == 0) meta[hf * 32 + bb * 16 + t16] = row_scale_inv(e);
@@ -586,44 +585,42 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 open2(st + 1, false);
             };
             // V, fp32: each token's largest, of this half of the dims
-            auto tops_v = [&](unsigned (&top)[4]) {
+            auto tops_v = [&](float (&top)[4]) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) top[k] = 0;
+                for (int k = 0; k < 4; k++) top[k] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < PH; i++) {
-                    const unsigned w[4] = {rv[i].x, rv[i].y, rv[i].z, rv[i].w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) top[k] = (w[k] & 0x7fffffffu) > top[k] ? w[k] & 0x7fffffffu : top[k];
+                for (int i = 0; i < PH; i += 2) {
+                    top[0] = larger(rv[i].x, rv[i + 1].x, top[0]);
+                    top[1] = larger(rv[i].y, rv[i + 1].y, top[1]);
+                    top[2] = larger(rv[i].z, rv[i + 1].z, top[2]);
+                    top[3] = larger(rv[i].w, rv[i + 1].w, top[3]);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    auto larger = [&](int o) { top[k] = (unsigned)o > top[k] ? (unsigned)o : top[k]; };
-                    larger(dpp_i<kDppXor1>((int)top[k]));
-                    larger(dpp_i<kDppXor2>((int)top[k]));
-                    larger(dpp_i<kDppHalfMirror>((int)top[k]));
-                    larger(dpp_i<kDppMirror>((int)top[k]));
+                    top[k] = __builtin_elementwise_maximum(top[k], dpp_f<kDppXor1>(top[k]));
+                    top[k] = __builtin_elementwise_maximum(top[k], dpp_f<kDppXor2>(top[k]));
+                    top[k] = __builtin_elementwise_maximum(top[k], dpp_f<kDppHalfMirror>(top[k]));
+                    top[k] = __builtin_elementwise_maximum(top[k], dpp_f<kDppMirror>(top[k]));
                 }
             };
-            unsigned* const topx = reinterpret_cast<unsigned*>(lds + P::TOPX);
+            float* const topx = reinterpret_cast<float*>(lds + P::TOPX);
             auto share_tops = [&]() {
-                unsigned top[4];
+                float top[4];
                 tops_v(top);
-                if (t16 == 0) *reinterpret_cast<uint4*>(topx + hf * 32 + bb * 16 + 4 * g) = make_uint4(top[0], top[1], top[2], top[3]);
+                if (t16 == 0) *reinterpret_cast<f4_t*>(topx + hf * 32 + bb * 16 + 4 * g) = f4_t{top[0], top[1], top[2], top[3]};
             };
             auto begin_v = [&](int st) {
                 float* meta = reinterpret_cast<float*>(lds + P::meta_at(st, 0));
                 const unsigned use = use2(st);
                 unsigned marks = pgv == -1 ? 0xffffu : 0u;
                 if constexpr (M::F) {
-                    unsigned top[4];
+                    float top[4];
                     if constexpr (DS == 1) {
                         // a token's weight carries one exponent, whichever the dim
-                        const uint4 x = *reinterpret_cast<const uint4*>(topx + bb * 16 + 4 * g);
-                        const uint4 y = *reinterpret_cast<const uint4*>(topx + 32 + bb * 16 + 4 * g);
-                        top[0] = x.x > y.x ? x.x : y.x;
-                        top[1] = x.y > y.y ? x.y : y.y;
-                        top[2] = x.z > y.z ? x.z : y.z;
-                        top[3] = x.w > y.w ? x.w : y.w;
+                        const f4_t x = *reinterpret_cast<const f4_t*>(topx + bb * 16 + 4 * g);
+                        const f4_t y = *reinterpret_cast<const f4_t*>(topx + 32 + bb * 16 + 4 * g);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) top[k] = __builtin_elementwise_maximum(x[k], y[k]);
                     } else {
                         tops_v(top);
                     }
@@ -631,20 +628,30 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     bool odd = false;
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        int e = (int)(top[k] >> 23) > kLowV ? (int)(top[k] >> 23) : kLowV;
-                        const bool on = use >> (4 * g + k) & 1, bad = e == 255;
-                        keepv[k] = on && !bad;      // others become zeros
-                        odd = odd || (on && bad);
-                        if (!keepv[k]) e = kLowV;
+                        const bool on = use >> (4 * g + k) & 1, bad = !(top[k] < INFINITY);
+                        int e = (int)(__float_as_uint(top[k]) >> 23);
+                        if (bad || !on || e < kLowV) e = kLowV;
+                        odd = odd || bad || !on;
                         sfv[k] = row_scale(e);
                         ex[k] = on ? (float)(e - 141) : 113.0f;     // of no weight: not the smallest
                     }
                     if (__any(odd)) {
+                        // rows that are not finite, or that nobody looks at, become zeros
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            const u64 b = __ballot((use >> (4 * g + k) & 1) && !keepv[k] && t16 == 0);   // lanes 0, 16, 32, 48
+                            const bool on = use >> (4 * g + k) & 1, bad = !(top[k] < INFINITY);
+                            const u64 b = __ballot(on && bad && t16 == 0);   // lanes 0, 16, 32, 48: tokens k, 4 + k, ..
 #pragma unroll
                             for (int j = 0; j < 4; j++) marks |= (unsigned)(b >> (16 * j) & 1) << (4 * j + k);
+                            if (bad || !on) {
+#pragma unroll
+                                for (int i = 0; i < PH; i++) {
+                                    if (k == 0) rv[i].x = 0;
+                                    else if (k == 1) rv[i].y = 0;
+                                    else if (k == 2) rv[i].z = 0;
+                                    else rv[i].w = 0;
+                                }
+                            }
                         }
                     }
                     if (t16 == 0) {
@@ -693,13 +700,9 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 const int c = hf * PH + j;
                 uint8_t* to = lds + P::v_at(st, 0);
                 if constexpr (M::F) {
-                    const unsigned w[4] = {rv[j].x, rv[j].y, rv[j].z, rv[j].w};
-                    float x[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) x[k] = keepv[k] ? __uint_as_float(w[k]) : 0.0f;
                     h2v_t hi[2], lo[2];
-                    split2(x[0], x[1], sfv[0], sfv[1], hi[0], lo[0]);
-                    split2(x[2], x[3], sfv[2], sfv[3], hi[1], lo[1]);
+                    split2(__uint_as_float(rv[j].x), __uint_as_float(rv[j].y), sfv[0], sfv[1], hi[0], lo[0]);
+                    split2(__uint_as_float(rv[j].z), __uint_as_float(rv[j].w), sfv[2], sfv[3], hi[1], lo[1]);
                     to += ((c >> 1) * 2 + bb) * 1024 + ((g & 1) * 32 + (c & 1) * 16 + t16) * 16 + (g >> 1) * 8;
                     *reinterpret_cast<uint2*>(to) = make_uint2(h2_bits(hi[0]), h2_bits(hi[1]));
                     *reinterpret_cast<uint2*>(to + 64 * HD) = make_uint2(h2_bits(lo[0]), h2_bits(lo[1]));
