@@ -11,6 +11,7 @@ namespace {
 constexpr int kLgShares = 8, kShares = 1 << kLgShares;   // workgroups that share the work, one a CU
 constexpr int kLead = 64;      // keys that stand for what it costs to begin and to end an item
 constexpr int kLeast = 48;     // no smaller share than this
+constexpr double kFewKeys = 256, kFewPairs = 1 << 17;
 
 struct ChunkArgs {
     KvPool p;
@@ -1410,6 +1411,140 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
     }
 }
 
+template <int T>
+struct Cached { static constexpr int ES = T == G4_F32 ? 4 : T == G4_KV_Q8 ? 1 : 2; };
+
+// element i of a register's worth of cached elements (16-bit and fp32 values, codes)
+template <int T>
+__device__ __forceinline__ float cached(const uint32_t* w, int i) {
+    if constexpr (T == G4_F32) return __uint_as_float(w[i]);
+    else if constexpr (T == G4_F16) return hbits_to_f32(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
+    else if constexpr (T == G4_BF16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    else return (float)(int8_t)(w[i >> 2] >> (8 * (i & 3)));
+}
+// N elements that lie next to each other
+template <int T, int N>
+__device__ __forceinline__ void load_cached(const uint8_t* at, float (&x)[N]) {
+    constexpr int B = N * Cached<T>::ES;
+    uint32_t w[(B + 3) / 4];
+    if constexpr (B >= 16) {
+#pragma unroll
+        for (int i = 0; i < B / 16; i++) {
+            // 16 bytes are next to each other in a block, the next 16 are a token's next lane's
+            const uint4 y = *reinterpret_cast<const uint4*>(at + i * 256);
+            w[4 * i] = y.x; w[4 * i + 1] = y.y; w[4 * i + 2] = y.z; w[4 * i + 3] = y.w;
+        }
+    } else if constexpr (B == 8) {
+        const uint2 y = *reinterpret_cast<const uint2*>(at);
+        w[0] = y.x; w[1] = y.y;
+    } else if constexpr (B == 4) {
+        w[0] = *reinterpret_cast<const uint32_t*>(at);
+    } else if constexpr (B == 2) {
+        w[0] = *reinterpret_cast<const uint16_t*>(at);
+    } else {
+        w[0] = *at;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = cached<T>(w, i);
+}
+
+// One wave: one q row's head (dims lane * N .. + N - 1, times scale log2(e))
+// over positions first .. last of sequence s, `step` times four at a time
+// from the four that hold position at on; adds to the running maximum m, sum
+// l and o.  fp32 throughout; only the positions asked for have a part, so
+// that infinities and NaN elsewhere do not matter; where a page is none: NaN.
+template <int TC, int HD>
+__device__ void row_keys(const KvPool& p, int s, int kvh, int first, int last, int at, int step, const float (&q)[HD / 64],
+                         float& m, float& l, float (&o)[HD / 64]) {
+    constexpr int ES = Cached<TC>::ES, N = HD / 64;
+    const int lane = threadIdx.x & 63;
+    for (int t0 = at & ~3; t0 <= last; t0 += 4 * step) {
+        const int page = p.page_of(s, t0);
+        const size_t block = p.block_of(page < 0 ? 0 : page, kvh, t0), off = block * (16 * HD * ES);
+        const uint8_t* kb = p.kp + off;
+        const uint8_t* vb = p.vp + off;
+        const float* ks = reinterpret_cast<const float*>(p.kp + p.scale_off) + block * 16 + (t0 & 15);
+        const float* vs = reinterpret_cast<const float*>(p.vp + p.scale_off) + block * 16 + (t0 & 15);
+        float x[4], v[N][4], mn = m;
+#pragma unroll
+        for (int i = 0; i < N; i++) load_cached<TC, 4>(vb + kv_v_byte<ES>(t0 & 15, lane * N + i), v[i]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float k[N];
+            load_cached<TC, N>(kb + kv_k_byte<ES>((t0 & 15) + j, lane * N), k);
+            x[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; i++) x[j] = __builtin_fmaf(q[i], k[i], x[j]);
+            x[j] = wave_sum(x[j]);
+            if (TC == G4_KV_Q8) x[j] *= ks[j];
+            if (page < 0) x[j] = __uint_as_float(0x7fc00000u);
+            if (t0 + j < first || t0 + j > last) x[j] = -INFINITY;
+            mn = fmaxf(mn, x[j]);
+        }
+        const float f = exp2f(m - mn);
+        l *= f;
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] *= f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (t0 + j < first || t0 + j > last) continue;
+            const float w = exp2f(x[j] - mn);
+            l += w;
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = __builtin_fmaf(w, TC == G4_KV_Q8 ? v[i][j] * vs[j] : v[i][j], o[i]);
+        }
+    }
+}
+
+// ---- few keys: one launch, fp32 throughout, a workgroup a row and head ------------
+// Taken by what a call can ask for at most, its rows and the keys that the
+// window or the table allows, in units of 512 bytes of a key's row (fewer take
+// as long): up to 256 keys a row and 2^17 of all rows and heads.  8 heads, this
+// against the tiles and the join: bf16 of 256, 8 rows of 64 / 128 / 256 / 512 keys
+// 5.8 / 8.2 / 13.7 / 24.5 and 18.4 / 18.4 / 20.0 / 21.4 us, 64 rows of 128 / 256 keys
+// 11.6 / 20.4 and 19.2 / 20.6, 512 rows of 64 keys 28.2 and 19.2; fp32 of 512, 8 rows
+// of 64 / 128 keys 13.3 / 23.8 and 25.7 / 24.7, 64 rows of 64 keys 24.6 and 25.9; codes
+// of 128, 128 rows of 64 / 128 / 256 keys 8.8 / 14.9 / 27.2 and 14.6 / 15.7 / 17.6.
+template <int TQ, int TC, int HD>
+__global__ __launch_bounds__(256) void attn_chunk_row_kernel(ChunkArgs a) {
+    typedef typename RowElem<TQ>::t E;
+    constexpr int N = HD / 64;
+    const int row = blockIdx.x, h = blockIdx.y, kvh = h / a.group;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float red[4][HD + 2];
+    const SeqAt sq = find_seq(a.cu, a.lens, a.n_seqs, 1, 0, 0, (unsigned)row);
+    if (sq.r0 < 0 || sq.r1 > a.m || row < sq.r0 || row >= sq.r1 || sq.r1 - sq.r0 > sq.len || !a.p.fits(sq.len)) return;
+    const int last = sq.len - sq.r1 + row, first = a.window > 0 && last >= a.window ? last + 1 - a.window : 0;
+    const E* qr = (const E*)a.q + (size_t)row * a.q_stride + (size_t)h * HD + lane * N;
+    float q[N], o[N] = {}, m = -FLT_MAX, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) q[i] = (float)qr[i] * (a.scale * kLog2e);
+    row_keys<TC, HD>(a.p, sq.s, kvh, first, last, (first & ~3) + 4 * wave, 4, q, m, l, o);
+#pragma unroll
+    for (int i = 0; i < N; i++) red[wave][lane * N + i] = o[i];
+    if (lane == 0) {
+        red[wave][HD] = m;
+        red[wave][HD + 1] = l;
+    }
+    lds_sync();
+    float top = red[0][HD], f[4], den = 0.0f;
+#pragma unroll
+    for (int w = 1; w < 4; w++) top = fmaxf(top, red[w][HD]);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        f[w] = exp2f(red[w][HD] - top);
+        den += f[w] * red[w][HD + 1];
+    }
+    E* out = (E*)a.out + (size_t)row * a.out_stride + (size_t)h * HD;
+    for (int d = threadIdx.x; d < HD; d += 256) {
+        float num = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) num += f[w] * red[w][d];
+        out[d] = (E)(num / den);
+    }
+}
+
 // ---- second launch: items of more than one share ---------------------------------
 // The first border inside an item stands for the item.  A workgroup takes every
 // gridDim.x-th of all such borders' units, 32 columns and 128 dims (64 where there
@@ -1552,6 +1687,13 @@ void set_columns(ChunkArgs& a, int cols) {
 template <int TQ, int TC, int HD>
 int launch_chunk(ChunkArgs a) {
     typedef Plan<TQ, TC, HD> P;
+    double keys = (double)a.p.table_stride * (1 << a.p.lgpage);
+    if (a.window > 0 && a.window < keys) keys = a.window;
+    constexpr int kUnit = HD * P::M::ES > 512 ? HD * P::M::ES / 512 : 1;
+    if (keys * kUnit <= kFewKeys && keys * kUnit * a.m * a.n_heads <= kFewPairs) {
+        hipLaunchKernelGGL((attn_chunk_row_kernel<TQ, TC, HD>), dim3(a.m, a.n_heads), dim3(256), 0, g4_stream(), a);
+        return g4_check_launch("attn_chunk_row_kernel");
+    }
     set_columns(a, P::COLS);
     a.pairs = P::M::kPairs;
     auto kernel = attn_chunk_kernel<TQ, TC, HD>;

@@ -24,6 +24,17 @@ def lib():
     return L
 
 
+EXTRA = 2
+
+
+@pytest.fixture(params=[2, 3000], ids=["table", "wide"], autouse=True)
+def width(request):
+    """entries of the page tables past the longest sequence's: a call goes by what its table allows, so that with many of
+    them even short sequences are cut into tiles and shares"""
+    global EXTRA
+    EXTRA = request.param
+
+
 def run_chunk(lib, c, q, qk, n, lens, window, n_heads, scale, m=None, out_stride=None):
     """rows of the type's bits -> (out bits, out as float32); out starts as 0x3F3F..."""
     m = m or len(q)
@@ -56,13 +67,12 @@ def bound_of(bound, want, q, k, v, qk, ck, scale):
     return bound + each * (2 * (2.0 ** -22 * mags + 2 * low) + 2.0 ** -22 + 2.0 ** -39) * big
 
 
-def check(lib, seed, combo, hd, n_heads, n_kv, page, n, hist, window=0, scale=None, gain=2.0, pad=0, extra=0, some=None,
-          entries=2):
+def check(lib, seed, combo, hd, n_heads, n_kv, page, n, hist, window=0, scale=None, gain=2.0, pad=0, extra=0, some=None):
     qk, ck = combo
     rng = np.random.default_rng(seed)
     scale = hd ** -0.5 if scale is None else scale
     lens = [a + b for a, b in zip(n, hist)]
-    c = Cache(lib, rng, ck, hd, n_kv, page, lens, extra=entries)
+    c = Cache(lib, rng, ck, hd, n_kv, page, lens, extra=EXTRA)
     k, v = rows(rng, sum(lens), n_kv, hd), rows(rng, sum(lens), n_kv, hd)
     c.store(k, v, lens, lens)
     q, qf = cast(rows(rng, sum(n) + pad, 1, n_heads * hd + extra) * np.float32(gain), qk)
@@ -167,7 +177,7 @@ def test_window_pages_gone(lib):
     rng = np.random.default_rng(390)
     hd, n_kv, page, t, w, new = 128, 1, 16, 200, 50, 20
     for combo in COMBOS:
-        c = Cache(lib, rng, combo[1], hd, n_kv, page, [t])
+        c = Cache(lib, rng, combo[1], hd, n_kv, page, [t], extra=EXTRA)
         k, v = rows(rng, t, n_kv, hd), rows(rng, t, n_kv, hd)
         c.store(k, v, [t], [t])
         q = cast(rows(rng, new, 2, hd), combo[0])[0]
@@ -184,7 +194,7 @@ def test_pages_outside(lib, combo, hd):
     """a page outside the pool: NaN in the rows that see it and nowhere else"""
     rng = np.random.default_rng(391)
     n, lens, w = [40, 40, 3], [90, 90, 90], 30
-    c = Cache(lib, rng, combo[1], hd, 1, 16, lens)
+    c = Cache(lib, rng, combo[1], hd, 1, 16, lens, extra=EXTRA)
     x = rows(rng, 270, 1, hd)
     c.store(x, x, lens, lens)
     q = cast(rows(rng, 83, 2, hd), combo[0])[0]
@@ -214,7 +224,7 @@ def test_not_finite(lib, combo, hd):
     rng = np.random.default_rng(392)
     n_kv, n_heads, n, hist, w = 2, 4, [70, 50], [60, 20], 40
     lens = [130, 70]
-    c = Cache(lib, rng, combo[1], hd, n_kv, 16, lens)
+    c = Cache(lib, rng, combo[1], hd, n_kv, 16, lens, extra=EXTRA)
     k, v = rows(rng, 200, n_kv, hd), rows(rng, 200, n_kv, hd)
     c.store(k, v, lens, lens)
     q = cast(rows(rng, 120, n_heads, hd), combo[0])[0]
@@ -274,7 +284,7 @@ def test_captured(lib, combo, hd):
     plans = [([100, 1, 30], [20, 900, 0]), ([1, 1, 1], [120, 901, 30]), ([0, 150, 3], [121, 0, 1000]), ([53, 53, 54], [300, 40, 0])]
     total = [max(p[0][s] + p[1][s] for p in plans) for s in range(3)]
     with Stream(lib):
-        c = Cache(lib, rng, ck, hd, kv, page, total)
+        c = Cache(lib, rng, ck, hd, kv, page, total, extra=EXTRA)
         x = rows(rng, sum(total), kv, hd)
         c.store(x, x[::-1].copy(), total, total)
         q = [cast(rows(rng, m, heads, hd), qk)[0] for _ in plans]
@@ -325,7 +335,7 @@ def test_offsets_past_32_bits(lib, combo):
     c.store(k, v, lens, lens)
     q = cast(rows(rng, 43, 4, hd), combo[0])[0]
     big, _ = run_chunk(lib, c, q, combo[0], n, lens, 0, 4, 0.05)
-    small = Cache(lib, rng, combo[1], hd, n_kv, page, lens)
+    small = Cache(lib, rng, combo[1], hd, n_kv, page, lens, extra=EXTRA)
     small.store(k, v, lens, lens)
     assert sum(need) <= small.pages
     assert same_bits(big, run_chunk(lib, small, q, combo[0], n, lens, 0, 4, 0.05)[0])
@@ -365,7 +375,7 @@ def test_serving(lib, combo, hd, window):
     steps = [[37, 0, 1], [60, 5, 1], [1, 30, 1], [1, 1, 1], [0, 8, 40]]
     total = np.sum(steps, 0)
     from test_gpu_qkv_seqs import Rows
-    c = Cache(lib, rng, ck, hd, kv, page, [int(t) for t in total])
+    c = Cache(lib, rng, ck, hd, kv, page, [int(t) for t in total], extra=EXTRA)
     outs, qs = [[[] for _ in range(3)] for _ in range(2)]
     had = np.zeros(3, int)
     kw = None
