@@ -9,7 +9,7 @@ namespace g4 {
 namespace {
 
 constexpr int kLgShares = 8, kShares = 1 << kLgShares;   // workgroups that share the work, one a CU
-constexpr int kLead = 64;      // keys that stand for what it costs to begin and to end an item
+constexpr int kLead = 160;     // keys that stand for what it costs to begin and to end an item
 constexpr int kLeast = 48;     // no smaller share than this
 constexpr double kFewKeys = 256, kFewPairs = 1 << 17;
 
