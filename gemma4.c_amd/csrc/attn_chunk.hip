@@ -9,8 +9,14 @@ namespace g4 {
 namespace {
 
 constexpr int kLgShares = 8, kShares = 1 << kLgShares;   // workgroups that share the work, one a CU
-constexpr int kLead = 160;     // keys that stand for what it costs to begin and to end an item
-constexpr int kLeast = 48;     // no smaller share than this
+// Keys that stand for what it costs to begin and to end an item.  us with 32, 64, 96,
+// 160, 224 and 320 (8 q heads on 2 kv heads): 40 sequences of a row and one of 471, bf16
+// of 512: 93, 92, 84, 81, 80, 84; nine of 3416 rows, fp32 of 256 under a window of 512:
+// 106, 97, 96, 94, 104, 105; 32 of 4 to 8 rows, fp32 over codes of 512: 66, 59, 59, 59, 61, 60.
+constexpr int kLead = 160;
+// No smaller share than this.  Against 96: 204 rows of 4 sequences, fp32 of 256, 29 us
+// against 35, 571 rows of 31, bf16 of 512, 23 against 36 (one call 21 against 19).
+constexpr int kLeast = 48;
 constexpr double kFewKeys = 256, kFewPairs = 1 << 17;
 
 struct ChunkArgs {
@@ -275,9 +281,23 @@ struct OpOf<true> { typedef h8_t t; };
 // A wave's job is 32 columns (row, q head) of an item; a workgroup's jobs share
 // its tiles of 32 keys in LDS.  S^T = K Q^T (rows keys, columns q rows): a lane
 // holds 16 of a column's 32 scores, which are, as they stand, its operand of
-// O^T += V^T P^T.  DS 2 (head_dim 512): a job's dims are halved over two waves,
-// whose partial scores meet in LDS; KSP 2: the two waves of a SIMD have the same
-// job and every other tile, waves 4 .. 7 their second product a tile later.
+// O^T += V^T P^T.  The cache's blocks have their operands' order, so that 16-bit
+// tiles go from the pages to LDS as they are.  The running maximum moves only
+// when a score passes it by kSlack.
+//   16 bits, head_dim up to 256: eight waves, KSP 2: the two waves of a SIMD have the
+// same job and every other tile, waves 4 .. 7 their second product a tile later.
+//   16 bits, 512: four waves, q (128) and o (256) in one wave's 512 registers.  (Dims
+// halved over two of eight waves, whose partial scores met in LDS: 512 rows over
+// 32488 positions 393 us against 366.)
+//   q of several terms, and codes: four waves; 512, terms: DS 2, the dims halved over
+// two waves, whose partial scores meet in LDS.
+// 8 heads on 2 kv heads, the whole call: 512 rows over 32488 positions, bf16 of 512,
+// 315 us, 870 TFLOP/s where an 8192^3 library product reaches 1204; there LDS is read
+// for 45 % of the cycles, the matrix cores are busy for 44 %.  fp32 over fp16 of 256 (two
+// products each), 1470 rows over 4700 positions 142 us, 430 of them (865 with the
+// second terms).  fp32 of 512, 250 rows over 16001, 331 us, 200 (600): a wave's
+// instructions bound it, 1100 a tile for splitting K and V into halves (640) and
+// for the weights, against 96 products of 32 cycles.
 template <int TQ, int TC, int HD>
 struct Plan {
     typedef Mode<TQ, TC> M;
@@ -289,9 +309,9 @@ struct Plan {
     static constexpr int TB = 64 * HD * M::NK;
     static constexpr bool ONE = DS == 2 && M::REG;                   // one place each for K and V
     static constexpr int NKP = ONE ? 1 : 2 * KSP, NVP = ONE ? 1 : KSP == 2 ? 5 : 2;
-    // staging: a unit is a 16-token block of K or V; WPU waves have one.  BOTH: a
-    // wave has half of the dims of a block of K and of one of V instead
-    static constexpr int UNITS = 4 * KSP, WPU = NW / UNITS, KC = HD * M::ES / 64, PCS = KC / WPU;
+    // staging: a wave has a 16-token block of K or V, KC kilobytes.  BOTH: half of the
+    // dims of a block of K and of one of V instead
+    static constexpr int KC = HD * M::ES / 64;
     static constexpr bool BOTH = M::REG && NW == 4 && KC > 1;
     static constexpr int PH = BOTH ? KC / 2 : 1;
     static constexpr int MB = BOTH ? 1024 : 512;                     // a tile's factors and marks
@@ -303,7 +323,7 @@ struct Plan {
     static constexpr int TOP0 = END > ROWS ? END : ROWS, TOP = TOP0 > JOIN ? TOP0 : JOIN;
     static constexpr int RED = (TOP + 15) / 16 * 16, LDS = RED + 128;
     static_assert(LDS <= 160 * 1024 && NJ * DS * KSP == NW, "LDS");
-    static_assert(PCS * WPU == KC && (!BOTH || PH * 2 == KC), "pieces");
+    static_assert((BOTH || NW == 4 * KSP) && (!BOTH || PH * 2 == KC), "pieces");
     static __device__ __forceinline__ int k_at(int st, int kp) { return ONE ? 0 : ((st & 1) * KSP + kp) * TB; }
     static __device__ __forceinline__ int v_at(int st, int kp) {
         return (NKP + (ONE ? 0 : kp == 0 ? st & 1 : 2 + st % 3)) * TB;
@@ -323,15 +343,15 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
     typedef Mode<TQ, TC> M;
     typedef typename RowElem<TQ>::t E;
     typedef typename OpOf<M::kHalf>::t op;
-    constexpr int NW = P::NW, DS = P::DS, NJ = P::NJ, KSP = P::KSP, TB = P::TB, KC = P::KC, PCS = P::PCS;
+    constexpr int NW = P::NW, DS = P::DS, NJ = P::NJ, KSP = P::KSP, TB = P::TB, KC = P::KC;
     constexpr int NQ = M::NQ, NK = M::NK, NP = M::NP, ES = M::ES;
     constexpr int KS = HD / 16 / DS, NT = HD / 32 / DS;   // a wave's product steps and 32-dim tiles
     extern __shared__ __align__(16) uint8_t lds[];
     u64* red = reinterpret_cast<u64*>(lds + P::RED);
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave % DS, kp = wave / (NJ * DS), slot = wave / DS % NJ;
-    // this wave's share of the staging: tile of a stage, K or V, block of the tile, which pieces
-    const int unit = wave % P::UNITS, ut = unit >> 2, uv = unit >> 1 & 1, ub = unit & 1, piece0 = wave / P::UNITS * PCS;
+    // this wave's share of the staging: tile of a stage, K or V, block of the tile
+    const int ut = wave >> 2, uv = wave >> 1 & 1, ub = wave & 1;
 
     Line line;
     Place at;
@@ -430,23 +450,23 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             // straight to LDS (K or V, as this wave has it)
             __amdgpu_buffer_rsrc_t copy_rsrc;
             uint8_t* copy_to = lds;
-            auto copy_piece = [&](int i) { buf_load_lds16(copy_rsrc, copy_to + i * 1024, piece0 * 1024 + (tid & 63) * 16, i * 1024); };
+            auto copy_piece = [&](int i) { buf_load_lds16(copy_rsrc, copy_to + i * 1024, (tid & 63) * 16, i * 1024); };
             auto begin_copy = [&](int st) {
                 const int pg = take_page();
                 copy_rsrc = block_rsrc(block_at(st, pg), pg);
-                copy_to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut)) + (ub * KC + piece0) * 1024;
-                if (uv && piece0 == 0 && lane == 0) *reinterpret_cast<unsigned*>(mine_meta + P::meta_at(st, ut)) = pg == -1 ? 0xffffu : 0u;
+                copy_to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut)) + ub * KC * 1024;
+                if (uv && lane == 0) *reinterpret_cast<unsigned*>(mine_meta + P::meta_at(st, ut)) = pg == -1 ? 0xffffu : 0u;
                 ask_page(st + 1);
             };
             auto copy = [&](int st) {
                 begin_copy(st);
 #pragma unroll
-                for (int i = 0; i < PCS; i++) copy_piece(i);
+                for (int i = 0; i < KC; i++) copy_piece(i);
             };
             // one wave a SIMD: copies are issued between the products
             constexpr bool kFeed = !M::REG && NW == 4;
             // through registers
-            uint4 raw[M::REG ? PCS : 1];
+            uint4 raw[M::REG ? KC : 1];
             float raw_scale = 0.0f;
             int raw_pg = 0;
             auto fetch = [&](int st) {
@@ -454,7 +474,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 const size_t block = block_at(st, pg);
                 const __amdgpu_buffer_rsrc_t r = block_rsrc(block, pg);
 #pragma unroll
-                for (int i = 0; i < PCS; i++) raw[i] = buf_load16(r, piece0 * 1024 + lane * 16, i * 1024);
+                for (int i = 0; i < KC; i++) raw[i] = buf_load16(r, lane * 16, i * 1024);
                 if (M::Q8) raw_scale = reinterpret_cast<const float*>((uv ? a.p.vp : a.p.kp) + a.p.scale_off)[block * 16 + t16];
                 raw_pg = pg;
                 ask_page(st + 1);
@@ -469,10 +489,10 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     // scales that are not finite: of heads with infinities or NaN
                     const bool bad = on && !(fabsf(raw_scale) < INFINITY);
                     marks |= (unsigned)__ballot(bad && g == 0) & 0xffffu;
-                    if (g == 0 && piece0 == 0) meta[(uv ? kMetaV / 4 : 0) + ub * 16 + t16] = on && !bad ? raw_scale : 0.0f;
+                    if (g == 0) meta[(uv ? kMetaV / 4 : 0) + ub * 16 + t16] = on && !bad ? raw_scale : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < PCS; i++) {
-                        const int c = piece0 + i;
+                    for (int i = 0; i < KC; i++) {
+                        const int c = i;
                         const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                         unsigned y[8];
 #pragma unroll
@@ -497,7 +517,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     }
                 }
                 // K's and V's marks have a word each: [K or V][block]
-                if (piece0 == 0 && lane == 0) reinterpret_cast<unsigned*>(meta)[kMetaMarks / 4 + (uv ? 0 : 4) + ub] = marks;
+                if (lane == 0) reinterpret_cast<unsigned*>(meta)[kMetaMarks / 4 + (uv ? 0 : 4) + ub] = marks;
             };
 
             // BOTH: half hf of the dims of block bb, K and V.  A piece is put into LDS
@@ -867,24 +887,16 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 ask_page(0);
                 fetch(0);
                 load_q();
-                if constexpr (DS == 2) {
-                    lds_barrier();   // the boxes have been read
-                    if (!uv) {
-                        put(0);
-                        fetch(1);
-                    }
-                } else {
-                    put(0);
-                    fetch(1);
-                }
+                put(0);
+                fetch(1);
             } else {
                 ask_page(0);
                 copy(0);
                 load_q();
             }
-            // one wave a SIMD: q (two terms of it) and, but for 16 bits of 512, o stay in
-            // the accumulation registers, from which products take them as well (left
-            // to itself the compiler moves q there and back for every tile)
+            // one wave a SIMD: two terms of q stay in the accumulation registers, from which
+            // products take them as well (left to itself the compiler moves them there and
+            // back for every tile)
             if constexpr (NW == 4 && NQ > 1 && HD >= 256) {
 #pragma unroll
                 for (int k = 0; k < 2; k++)
@@ -1111,7 +1123,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             // are marked: a column that sees one gets the score NaN, the others the bits
             // they would have without it.
             auto clean = [&](int st, bool careful) {
-                if (M::REG || !uv || piece0 != 0) return;
+                if (M::REG || !uv) return;
                 const unsigned use = block_use(st);
                 const int lane = own_lane(), g = lane >> 4;
                 uint8_t* v = lds + P::v_at(st, ut) + ub * KC * 1024 + lane * 16;
@@ -1211,8 +1223,8 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     auto feed = [&](int i) {
                         if constexpr (kFeed) {
 #pragma unroll
-                            for (int j = 0; j < PCS; j++)
-                                if (j * KS / PCS == i) copy_piece(j);
+                            for (int j = 0; j < KC; j++)
+                                if (j * KS / KC == i) copy_piece(j);
                         }
                     };
                     int st = 0;
@@ -1549,14 +1561,15 @@ __global__ __launch_bounds__(256) void attn_chunk_row_kernel(ChunkArgs a) {
 // The first border inside an item stands for the item.  A workgroup takes every
 // gridDim.x-th of all such borders' units, 32 columns and 128 dims (64 where there
 // are no more), and joins the pieces with the weights 2^(m_i - max m), four at a
-// time.  (A workgroup for every border and unit, of which most have nothing to do:
-// 19 us where this takes 9, 40 sequences of a row and one of 471.)
+// time.  What bounds it: the chain flags - list - pieces (7 us for 23 rows of one
+// sequence, 2 of it the launch).  A workgroup for every border and unit, of which most
+// have nothing to do: 19 us where this takes 15, 40 sequences of a row and one of 471.
 constexpr int kJoinWG = 1024;
 template <int TQ, int HD>
 __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
     typedef typename RowElem<TQ>::t E;
     constexpr int D = HD < 128 ? HD : 128, V = D / 32, B = 4;     // dims, 16-byte values of a thread, pieces at a time
-    __shared__ unsigned flags[kShares];
+    __shared__ unsigned flags[kShares + 1];
     __shared__ int list[kShares + 1], cnt[4], ends[4], found[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h = lane >> 5;
     const Notes* notes = reinterpret_cast<const Notes*>(a.part);
@@ -1578,6 +1591,7 @@ __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
     };
     const unsigned mine = tid < shares ? notes->flags[tid] : 0;
     flags[tid] = mine;
+    if (tid == 0) flags[kShares] = 0;
     lds_sync();
     // thread t: units of the item that goes out of share t
     const int cols_out = mine & kGoesOut ? (int)(flags[tid + 1] >> kColsShift) : 0, units = (cols_out + 31) / 32 * (HD / D);
@@ -1630,16 +1644,17 @@ __global__ __launch_bounds__(256) void attn_chunk_join_kernel(ChunkArgs a) {
                 float top = m;
 #pragma unroll
                 for (int j = 0; j < B; j++) top = fmaxf(top, y[j].x);
+                // (fp32 V: l may be as far above its piece's products as 2^203)
                 const float f = exp2f(m - top);
+                l = move_sum(l, m - top);
                 m = top;
-                l *= f;
 #pragma unroll
                 for (int k = 0; k < V; k++) x[k] *= f;
 #pragma unroll
                 for (int j = 0; j < B; j++) {
                     if (i + j >= pieces) break;
                     const float f = exp2f(y[j].x - top);
-                    l = __builtin_fmaf(f, y[j].y, l);
+                    l += move_sum(y[j].y, y[j].x - top);
 #pragma unroll
                     for (int k = 0; k < V; k++)
 #pragma unroll

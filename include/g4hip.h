@@ -518,13 +518,18 @@ int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void
  * already (g4_kv_page_append): row i of the n of sequence s is position
  * p = lens[s] - n + i and sees max(0, p + 1 - window) .. p (window 0: 0 .. p).
  * q and out: rows of q_type, strides in elements (16-byte aligned rows):
- *   G4_F32 over a cache of any type: operands of the products as in
- * g4_attn_prompt_packed's F32 over a cache of that type, three terms of q over
- * BF16 and codes (exact) and weights within 2^-17, F16: q within 2^-22 of itself
- * or 2^-39 of its row's largest, weights 2^-22; fp32 sums.
+ *   G4_F32 over F32: as g4_attn_prompt_packed's F32.
+ *   G4_F32 over F16: q met within 2^-22 of itself or 2^-39 of its row's
+ * largest, weights within 2^-22 of themselves or 2^-36 of the row's largest, K and
+ * V as they are; fp32 sums.
+ *   G4_F32 over BF16 or G4_KV_Q8: q, K and V as they are (codes times their
+ * scale), weights (times the scale of V's codes) within 2^-17 of themselves; fp32 sums.
  *   G4_F16 over F16, G4_BF16 over BF16 or G4_KV_Q8: exact products of q, fp32
  * sums, weights (times the scale of a token's codes) rounded to the type before
- * they multiply V.
+ * they multiply V; the result is rounded to the type.
+ *   Few keys (the window's or all that a row of table allows, in units of 512
+ * bytes of a head's K, up to 256, and 2^17 of them over all rows and heads):
+ * fp32 throughout, so that the same rows with a wider table are rounded as above.
  * Rows of out past cu[n_seqs] and those of sequences whose cu or lens do not
  * fit (n > lens, rows past m, positions past the table) are left as they are.
  * A row that sees a page outside the pool becomes NaN.  Pages, and within a page

@@ -1,6 +1,9 @@
 """Attention of chunks of new rows over the paged cache (main.c:1909-1950 of the
 reference, which has one sequence and one row), against the formula in 64 bits."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -404,3 +407,120 @@ def test_serving(lib, combo, hd, window):
         first = [max(0, i + 1 - window) if window else 0 for i in range(t)]
         want, bound = pn.attention(q, k, v, first, scale)
         within(np.abs(o - want), bound_of(bound, want, q, k, v, qk, ck, scale), s)
+
+
+def check_far(lib, hd, k, v, gain, window=0, seed=380):
+    """fp32 rows over fp32 keys whose sizes differ much from key to key: the last 70 positions of one sequence"""
+    rng = np.random.default_rng(seed)
+    t, n, n_heads, n_kv, scale = len(v), 70, 8, 2, hd ** -0.5
+    c = Cache(lib, rng, pn.F32, hd, n_kv, 16, [t], extra=EXTRA)
+    c.store(k, v, [t], [t])
+    q = rows(rng, n, n_heads, hd) * np.float32(gain)
+    _, got = run_chunk(lib, c, q, pn.F32, [n], [t], window, n_heads, scale)
+    first = [max(0, t - n + i + 1 - window) if window else 0 for i in range(n)]
+    q, k, v = (x.reshape(len(x), -1, hd) for x in (q, k, v))
+    want, bound = pn.attention(q, k, v, first, scale)
+    big = np.abs(v).max(-1).repeat(n_heads // n_kv, 1).astype(np.float64)
+    for i in range(n):
+        seen = slice(first[i], t - n + i + 1)
+        for h in range(n_heads):
+            kh, vh = k[seen, h // (n_heads // n_kv)].astype(np.float64), np.abs(v[seen, h // (n_heads // n_kv)])
+            p = scale * (kh @ q[i, h])
+            p = np.exp(p - p.max())
+            pb = p * big[seen, h]
+            # An element of V is met within 2^-39 of its row's largest; a weight times its V row's power of two is held
+            # as two fp16, the largest of them at 2^11 or more and each within 2^-25: times V's scaled elements, below
+            # 2^15, that is 2^-10 a key where the largest stands for 2^11 * 2^14 at least, 2^-35 of it.
+            bound[i, h] += (2.0 ** -38 * pb.sum() + 2.0 ** -35 * len(p) * pb.max()) / p.sum()
+            # Rows of V below 2^-76 have the scale of 2^-76, 2^90: halves within 2^-25 of the scaled row are 2^-115 of V.
+            bound[i, h] += 2.0 ** -115
+            # A score has the row's exponent (-90 to 113) added and the maximum taken off: two roundings of numbers
+            # below 256, 2^-17 each and times ln 2 in a weight, met in the numerator and in the denominator.
+            bound[i, h] += 4 * np.log(2) * 2.0 ** -17 * (p @ vh) / p.sum()
+    within(np.abs(got.reshape(n, n_heads, hd) - want), bound, hd)
+
+
+@pytest.mark.parametrize("hd", [64, 256, 512])
+@pytest.mark.parametrize("top", [61, 62, 100, 117])
+@pytest.mark.parametrize("big_first", [False, True])
+def test_values_far_apart(lib, hd, top, big_first):
+    """V rows of zeros beside one of 2^61 and more, in front of it and behind it, with equal scores and with scores far
+    apart: a row of zeros takes its share of the weights whatever the others hold"""
+    rng = np.random.default_rng(381)
+    t = 150
+    k, v = rows(rng, t, 2, hd), np.zeros((t, 2 * hd), np.float32)
+    v[3 if big_first else 77] = np.float32(1.5 * 2.0 ** top)
+    check_far(lib, hd, k, v, 0.0)
+    check_far(lib, hd, k, v, 6.0)
+    # tiny rows, in tiles of their own and beside large ones, and a window
+    v = rows(rng, t, 2, hd) * np.exp2(np.where(np.arange(t) // 40 % 2 == big_first, top - 3, -103)).astype(np.float32)[:, None]
+    v[rng.integers(0, t, 9)] = 0
+    check_far(lib, hd, k, v, 3.0)
+    for window in (70, 270):
+        check_far(lib, hd, np.concatenate([k] * 3), np.concatenate([v] * 3), 3.0, window=window)
+
+
+@pytest.mark.parametrize("hd,window", [(64, 40), (64, 260), (256, 0), (256, 130), (512, 0), (512, 70)])
+def test_magnitudes(lib, hd, window):
+    """fp32 rows whose sizes differ by 2^60 from key to key and by 2^20 within a row: what a row does not see, and what
+    has next to no weight, costs it no precision, and a key of large scores moves the maximum far at once"""
+    rng = np.random.default_rng(390 + hd)
+    t = 430
+    k, v = rows(rng, t, 2, hd), rows(rng, t, 2, hd)
+    v *= np.exp2(rng.integers(-30, 31, (t, 2 * hd // 64))).repeat(64, 1).astype(np.float32)
+    v *= np.exp2(rng.integers(-10, 11, v.shape)).astype(np.float32)
+    k *= np.exp2(rng.integers(-6, 3, (t, 1))).astype(np.float32)
+    k[rng.integers(0, t, 12)] *= np.float32(20)
+    v[7] = v[200] = k[31] = 0
+    check_far(lib, hd, k, v, 1.0, window=window)
+
+
+FIRST = """
+import ctypes as C, sys
+import numpy as np
+sys.path[:0] = {paths!r}
+import g4, paged_np as pn, test_gpu_paged as base
+lib = g4.Lib.get()
+lib.init(0)
+with base.Stream(lib):
+    rng = np.random.default_rng(395)
+    kind, hd, n_heads, n_kv, n, lens = {kind}, {hd}, 8, 2, [200, 100], [500, 100]
+    c = base.Cache(lib, rng, kind, hd, n_kv, 16, lens, extra=2000)
+    k, v = base.rows(rng, 600, n_kv, hd), base.rows(rng, 600, n_kv, hd)
+    c.store(k, v, lens, lens)
+    q = base.cast(base.rows(rng, 300, n_heads, hd), kind)[0]
+    dq, cu, dl = base.dbuf(lib, q), base.dbuf(lib, pn.starts(n)), base.dbuf(lib, np.asarray(lens, np.int32))
+    out = base.filled(lib, q.nbytes)
+    part = base.filled(lib, lib.L.g4_attn_chunk_paged_part_bytes(300, n_heads, n_kv, hd))
+    call = lambda: lib.g4_attn_chunk_paged(dq.ptr, n_heads * hd, kind, *c.args(), cu.ptr, dl.ptr, 2, 300, 0, n_heads,
+                                           C.c_float(0.1), part.ptr, out.ptr, n_heads * hd)
+    lib.g4_graph_begin()
+    call()
+    g = C.c_void_p()
+    lib.g4_graph_end(C.byref(g))
+    got = []
+    for i in range(4):
+        lib.g4_memset(out.ptr, 0x3F, out.nbytes)
+        if i == 2:
+            call()
+        else:
+            lib.g4_graph_launch(g.value)
+        lib.g4_sync()
+        got.append(out.to_array(np.uint8))
+    lib.g4_graph_destroy(g.value)
+    assert all(np.array_equal(a, got[2]) for a in got)
+    assert (got[0].reshape(300, -1) != 0x3F).any(1).all()
+print("FIRST OK")
+"""
+
+
+def test_first_call_captured():
+    """a process whose first call of the operator is a captured one (kernels with more than 64 KB of LDS)"""
+    if EXTRA != 2:
+        return
+    here = os.path.dirname(os.path.abspath(__file__))
+    paths = [here, os.path.join(os.path.dirname(here), "gemma4.c_amd")]
+    for kind, hd in ((pn.F32, 512), (pn.BF16, 256)):
+        r = subprocess.run([sys.executable, "-c", FIRST.format(paths=paths, kind=kind, hd=hd)], capture_output=True, text=True,
+                           timeout=100)
+        assert r.returncode == 0 and "FIRST OK" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
