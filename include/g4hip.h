@@ -522,8 +522,8 @@ int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void
  *   G4_F32 over F16: q met within 2^-22 of itself or 2^-39 of its row's
  * largest, weights within 2^-22 of themselves or 2^-36 of the row's largest, K and
  * V as they are; fp32 sums.
- *   G4_F32 over BF16 or G4_KV_Q8: q, K and V as they are (codes times their
- * scale), weights (times the scale of V's codes) within 2^-17 of themselves; fp32 sums.
+ *   G4_F32 over BF16 or G4_KV_Q8: exact products of q and of the weights (times
+ * the scale of V's codes) with what the cache holds, fp32 sums.
  *   G4_F16 over F16, G4_BF16 over BF16 or G4_KV_Q8: exact products of q, fp32
  * sums, weights (times the scale of a token's codes) rounded to the type before
  * they multiply V; the result is rounded to the type.

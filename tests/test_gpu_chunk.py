@@ -60,7 +60,7 @@ def bound_of(bound, want, q, k, v, qk, ck, scale):
         # smallest subnormal's half at a maximum of 1) and the result rounded to it
         return bound + pn.HALF[qk] * (np.abs(want) + 1.01 * big) + 2.0 ** -25 * len(k) * big
     if ck in (pn.BF16, pn.Q8):
-        return bound + 2.0 ** -17 * big         # weights as two bf16 terms
+        return bound + 2.0 ** -23 * big         # weights as three bf16 terms, themselves; times a scale of codes: 2^-24
     # operands within 2^-22 of themselves or 2^-39 of their row's largest (F32: q and K, and the smaller terms' product
     # left out): a score is off by that of sum |q| |k|, its weight by twice it; weights and V 2^-22 each
     kv = np.repeat(np.abs(k), q.shape[1] // k.shape[1], 1)
@@ -173,6 +173,16 @@ def test_extremes(lib, combo):
         check(lib, 384, combo, 128, 4, 2, 16, n, hist, scale=0.0)
         if combo[0] != pn.F16:
             check(lib, 385, combo, 128, 4, 2, 16, n, hist, gain=1e-18, scale=1e17)
+
+
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+def test_next_to_no_scores(lib, combo):
+    """rows of zeros and a scale so small that their product is below fp32's smallest number"""
+    for n, hist in (([90], [60]), ([5], [900])):
+        for gain in (0.0, 1e-30):
+            for scale in (1e-9, 1e-38):
+                check(lib, 386, combo, 128, 4, 2, 16, n, hist, gain=gain, scale=scale)
+                check(lib, 387, combo, 512, 4, 2, 16, n, hist, gain=gain, scale=-scale)
 
 
 def test_window_pages_gone(lib):
@@ -473,6 +483,30 @@ def test_magnitudes(lib, hd, window):
     k[rng.integers(0, t, 12)] *= np.float32(20)
     v[7] = v[200] = k[31] = 0
     check_far(lib, hd, k, v, 1.0, window=window)
+
+
+@pytest.mark.parametrize("hd", [64, 256, 512])
+@pytest.mark.parametrize("combo", [COMBOS[2], COMBOS[3], COMBOS[5], COMBOS[6]], ids=str)
+def test_values_at_the_limit(lib, combo, hd):
+    """V so large that the keys together stay just below fp32's largest number, under scores that rise by 2^7.9 from one
+    pair of tiles to the next"""
+    qk, ck = combo
+    t, n, n_heads, n_kv, top = 400, 70, 8, 2, 119
+    assert t * 2.0 ** top < float(np.finfo(np.float32).max) < t * 2.0 ** (top + 1)
+    rng = np.random.default_rng(394)
+    k = np.zeros((t, n_kv, hd), np.float32)
+    for i in range(t):
+        k[i, :, :i // 64] = 1
+    v = np.full((t, n_kv * hd), 2.0 ** top, np.float32)
+    v *= rng.choice(np.array([1, -1], np.float32), n_kv * hd)
+    q = np.zeros((n, n_heads, hd), np.float32)
+    q[:, :, :16] = 5.46875
+    c = Cache(lib, rng, ck, hd, n_kv, 16, [t], extra=EXTRA)
+    c.store(k.reshape(t, -1), v, [t], [t])
+    _, got = run_chunk(lib, c, cast(q.reshape(n, -1), qk)[0], qk, [n], [t], 0, n_heads, 1.0)
+    hk, hv = (pn.held(x.reshape(t, -1), ck, hd).reshape(t, n_kv, hd) for x in (k, v))
+    want, bound = pn.attention(q, hk, hv, [0] * n, 1.0)
+    within(np.abs(got.reshape(n, n_heads, hd) - want), bound_of(bound, want, q, hk, hv, qk, ck, 1.0), hd)
 
 
 FIRST = """
