@@ -20,9 +20,8 @@ struct Unit {
 
 // fits(len): whether that many positions have a place
 template <typename Fits>
-__device__ __forceinline__ bool find_unit(const int* __restrict__ cu, const int* __restrict__ lens, int n_seqs, int m, Fits fits,
-                                          Unit& u) {
-    const unsigned id = blockIdx.x;
+__device__ __forceinline__ bool find_unit(const int* __restrict__ cu, const int* __restrict__ lens, int n_seqs, int m, unsigned id,
+                                          Fits fits, Unit& u) {
     const SeqAt q = find_seq(cu, lens, n_seqs, 1, 4, 2, id);
     if (q.r0 < 0 || q.r1 <= q.r0 || q.r1 > m || q.r1 - q.r0 > q.len || !fits(q.len)) return false;
     const int pos0 = q.len - (q.r1 - q.r0);

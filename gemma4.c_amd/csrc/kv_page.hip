@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void kv_store_kernel(RowArgs a) {
     typedef RowMap<HD> M;
     __shared__ __align__(16) uint8_t img[16 * HD * ES];
     Unit u;
-    if (!find_unit(a.cu, a.lens, a.n_seqs, a.m, [&](int len) { return a.p.fits(len); }, u)) return;
+    if (!find_unit(a.cu, a.lens, a.n_seqs, a.m, blockIdx.x, [&](int len) { return a.p.fits(len); }, u)) return;
     const int page = a.p.page_of(u.s, u.at);   // on its way beside the rows
     const bool is_v = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void kv_load_kernel(RowArgs a) {
     typedef RowMap<HD> M;
     __shared__ __align__(16) uint8_t img[16 * HD * ES];
     Unit u;
-    if (!find_unit(a.cu, a.lens, a.n_seqs, a.m, [&](int len) { return a.p.fits(len); }, u)) return;
+    if (!find_unit(a.cu, a.lens, a.n_seqs, a.m, blockIdx.x, [&](int len) { return a.p.fits(len); }, u)) return;
     const bool is_v = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     float* __restrict__ dst = (is_v ? a.v : a.k) + (size_t)blockIdx.y * HD;

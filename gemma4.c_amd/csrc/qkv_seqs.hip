@@ -8,6 +8,8 @@
 namespace g4 {
 namespace {
 
+constexpr int kRun = 16;   // blocks whose workgroups are neighbours, a multiple of 8
+
 struct PostArgs {
     KvPool p;            // pages (kp null: rows)
     const float* q;
@@ -43,13 +45,17 @@ __device__ __forceinline__ void store4(void* row, int c, const float4& x) {
 // lane's other four dims.  The operations and their order are those of
 // g4_qkv_post_rows, so that for HD 256 and 512 the bits are.
 // What bounds it: bytes, each read and written once, where there are thousands of
-// rows: 8 q heads on 2 kv heads, 8191 rows of 256 into fp32 pages 46 us, 4.6 TB/s read
-// and written where a large copy reaches 5.2; 3193 rows of 256 as bf16 13.2 us, 4.7;
-// 1539 rows of 512 into pages of bf16 14.5 us, 4.1.  Up to a few dozen rows the chain
-// cu and lens - (page,) row and angles - sum - store, 6 to 7 us with the launch.  One
-// head a workgroup: with six heads a workgroup, which share the search and the
-// angles, the 8191 rows took 38 us, but 12000 rows of bf16 71 where this takes 64,
-// and the 3193 rows 21.
+// rows: 8 q heads on 2 kv heads, 8191 rows of 256 into fp32 pages 34 us in a row, 3193 rows
+// of 256 as bf16 14.2 us, 4.4 TB/s; 1539 rows of 512 into pages of bf16 13.8 us, 4.3.
+// Up to a few dozen rows the chain cu and lens - (page,) row and angles - sum -
+// store, 6 to 7 us with the launch.
+// The workgroups' order: all heads of 16 blocks, then the next 16.  Workgroups go to
+// the eight XCDs in turn, so an XCD has all heads of a block, one behind the other:
+// it reads whole rows and finds their angles in its L2.  All blocks of a head, then
+// the next head's, and this: 8191 rows into fp32 pages 46 and 34 us, 16384 96 and 85;
+// bf16 of 512, 4096 rows 43 and 27, 16384 161 and 126; rows of bf16, 8191 39 and 27,
+// 12000 43 and 38; but the 3193 rows 13.4 and 14.2, 1539 8.7 and 9.1.  (8, 32 and 64
+// blocks: within 3 %.  Six heads a workgroup: 8191 rows 38, the 3193 21.)
 // PT: type of the pages, -1: K and V as rows.  RT: type of the rows.
 template <int PT, int RT, int HD>
 __global__ __launch_bounds__(256) void qkv_seqs_kernel(PostArgs a) {
@@ -57,10 +63,12 @@ __global__ __launch_bounds__(256) void qkv_seqs_kernel(PostArgs a) {
     constexpr int ES = PT < 0 ? 1 : (int)sizeof(typename Elem<PT < 0 ? G4_F32 : PT>::t);
     __shared__ __align__(16) uint8_t img[PT < 0 ? 16 : 16 * HD * ES];
     Unit u;
-    if (!find_unit(a.cu, a.lens, a.n_seqs, a.m,
+    const unsigned heads = a.n_heads + 2 * a.n_kv, run = blockIdx.x / (kRun * heads), nth = blockIdx.x - run * kRun * heads;
+    const unsigned unit = run * kRun + nth % kRun;
+    const int b = nth / kRun;
+    if (!find_unit(a.cu, a.lens, a.n_seqs, a.m, unit,
                    [&](int len) { return len <= a.tab_rows && (PT < 0 || a.p.fits(len)); }, u))
         return;
-    const int b = blockIdx.y;
     const int kind = b < a.n_heads ? 0 : b < a.n_heads + a.n_kv ? 1 : 2;
     const int head = b - (kind == 0 ? 0 : kind == 1 ? a.n_heads : a.n_heads + a.n_kv);
     int page = 0;
@@ -156,7 +164,7 @@ __global__ __launch_bounds__(256) void qkv_seqs_kernel(PostArgs a) {
 
 template <int PT, int RT>
 void launch_post(const PostArgs& a, int hd) {
-    const dim3 grid((unsigned)(a.m / 16 + 2 * a.n_seqs), a.n_heads + 2 * a.n_kv);
+    const dim3 grid((unsigned)(a.m / 16 + 2 * a.n_seqs + kRun - 1) / kRun * kRun * (a.n_heads + 2 * a.n_kv));
     if (hd == 64) hipLaunchKernelGGL((qkv_seqs_kernel<PT, RT, 64>), grid, dim3(256), 0, g4_stream(), a);
     else if (hd == 128) hipLaunchKernelGGL((qkv_seqs_kernel<PT, RT, 128>), grid, dim3(256), 0, g4_stream(), a);
     else if (hd == 256) hipLaunchKernelGGL((qkv_seqs_kernel<PT, RT, 256>), grid, dim3(256), 0, g4_stream(), a);
@@ -185,7 +193,7 @@ int post_check(const char* who, const PostArgs& a, int hd, int n_rot, int row_ty
                  "%s: bad RoPE table (%d rows of %d, even and %d at most)", who, a.tab_rows, n_rot, hd);
     G4_CHECK_ARG(a.cu && a.lens && a.n_seqs > 0 && a.n_seqs <= kKvMaxSeqs && a.m > 0, "%s: %d rows of %d sequences (1 to %d)",
                  who, a.m, a.n_seqs, kKvMaxSeqs);
-    G4_CHECK_ARG(kv_grid_fits((size_t)a.m / 16 + 2 * a.n_seqs, 256) && (a.q ? a.n_heads : 0) + 2 * a.n_kv <= 65535,
+    G4_CHECK_ARG(kv_grid_fits(((size_t)a.m / 16 + 2 * a.n_seqs + kRun) * ((size_t)a.n_heads + 2 * a.n_kv), 256),
                  "%s: %d rows of %d heads: more than one launch takes", who, a.m, a.n_heads + 2 * a.n_kv);
     return G4_OK;
 }

@@ -67,3 +67,10 @@ def test_append_refused(bad):
 def test_append_type():
     assert append(type=g4.Q4_K) == g4.G4_ERR_TYPE and "cache type" in msg()
     assert append(q_type=g4.KV_Q8) == g4.G4_ERR_TYPE and "q rows" in msg()
+
+
+def test_more_than_a_launch_takes():
+    """blocks of rows times heads are workgroups of one launch of at most 2^32 threads"""
+    for m in (1 << 25, 1 << 30):
+        assert post(m=m) == g4.G4_ERR_ARG and "one launch" in msg()
+        assert append(m=m) == g4.G4_ERR_ARG and "one launch" in msg()
