@@ -18,7 +18,7 @@ struct Unit {
     int row;           // row of token 0 of the block (may lie before the first row)
 };
 
-// fits(len): whether that many positions have a place
+// unit id of a launch.  fits(len): whether that many positions have a place
 template <typename Fits>
 __device__ __forceinline__ bool find_unit(const int* __restrict__ cu, const int* __restrict__ lens, int n_seqs, int m, unsigned id,
                                           Fits fits, Unit& u) {
