@@ -909,6 +909,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             }
             f16_t o[NT] = {};
             float m = -FLT_MAX, l = 0.0f;
+            bool fresh = true;   // no tile has been weighted: o is 0
             f16_t sc;
             op p[NP][2];
             struct Ops {
@@ -1052,11 +1053,13 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     if constexpr (M::F) l = move_sum(l, m - top);
                     else l *= f;
                     m = top;
-                    if (__any(l != 0.0f)) {
+                    // (also where l is 0 by now: the factor may have taken all of it)
+                    if (!fresh) {
 #pragma unroll
                         for (int i = 0; i < NT; i++) o[i] *= f;
                     }
                 }
+                fresh = false;
                 const float base = m - M::kLift;
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
@@ -1308,6 +1311,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 for (int i = 0; i < NT; i++) o[i] = f16_t{};
                 m = -FLT_MAX;
                 l = 0.0f;
+                fresh = true;
                 ask_page(0);
                 copy(0);
             }

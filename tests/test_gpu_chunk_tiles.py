@@ -1,0 +1,92 @@
+"""Attention of chunks of new rows over the paged cache where the call is cut
+into tiles and shares of them (g4_attn_chunk_paged), against the formula in 64
+bits.  A call of few keys takes another kernel, by the keys that its window or
+its table allows and by its rows: here each case says which of the two it is for
+and is checked to be one that goes there."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import paged_np as pn
+import test_gpu_chunk as tc
+from test_gpu_chunk import COMBOS, bound_of, run_chunk
+from test_gpu_paged import NAN, NPT, Cache, cast, dbuf, filled, rows, same_bits, within
+
+pytestmark = pytest.mark.gpu
+
+F = C.c_float
+SIZE = {pn.F32: 4, pn.F16: 2, pn.BF16: 2, pn.Q8: 1}
+WIDE = 3000     # entries of a table past the longest sequence's
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from g4 import Lib
+    L = Lib.get()
+    L.init(0)
+    L.L.g4_set_stream(None)
+    return L
+
+
+def tiles(c, window, m, n_heads):
+    """whether a call of m rows over cache c goes to the tiles: more than 256 keys a row, as its window or table allows, in
+    units of 512 bytes of a key's row, or 2^17 of them over all rows and heads"""
+    keys = c.table.shape[1] * c.page
+    keys = min(keys, window) if window else keys
+    keys *= max(1, c.hd * SIZE[c.kind] // 512)
+    return keys > 256 or keys * m * n_heads > 1 << 17
+
+
+def rows_for_tiles(c, window, n_heads):
+    """a number of rows (used or not) with which a call goes to the tiles whatever its window"""
+    return ((1 << 17) // (min(window, c.table.shape[1] * c.page) * n_heads) + 1) if window else 1
+
+
+def padded(q, m):
+    """q with rows that belong to no sequence behind it, m in all: ones, and NaN in a few of them"""
+    x = np.ones((max(m, len(q)), q.shape[1]), np.float32).astype(q.dtype) if q.dtype != np.uint16 else np.full(
+        (max(m, len(q)), q.shape[1]), 0x3F80, np.uint16)
+    x[:len(q)] = q
+    if len(x) > len(q):
+        x[-1] = np.full(1, NAN).astype(q.dtype)[0] if q.dtype != np.uint16 else 0x7FC0
+    return x
+
+
+def back(bits, kind):
+    return pn.bf16_back(bits) if kind == pn.BF16 else bits.astype(np.float32)
+
+
+def store_prefix(c, k, v):
+    """rows into the pages of the table's first sequence"""
+    c.store(k, v, [len(k)] + [0] * (len(c.table) - 1), [len(k)] * len(c.table))
+
+
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("gain", [[1.0], [1.0, 0.9, 0.8, 0.75], [1.0, 0.5, 0.25, -1.0]], ids=["one", "alike", "apart"])
+def test_scores_rise_far(lib, combo, hd, gain):
+    """One row each of many sequences that share their pages, under scores that rise by 150 (216 in the exponent of 2) from
+    64 keys to the next, in many places of many shares: what was summed before is of no weight, all of it, and is gone."""
+    qk, ck = combo
+    n_heads = len(gain)
+    rng = np.random.default_rng(500 + hd)
+    seqs, page, long = 120, 64, 640
+    table = np.tile(np.concatenate([np.arange(long // page), np.full(WIDE, -1)]).astype(np.int32), (seqs, 1))
+    c = Cache(lib, rng, ck, hd, 1, page, None, table=table, pages=long // page)
+    assert tiles(c, 0, seqs, n_heads)
+    step = 150.0 / hd
+    k = np.repeat((np.arange(long) // 64 - 4) * step, hd).reshape(long, hd).astype(np.float32)
+    v = rows(rng, long, 1, hd) + np.float32(1)
+    store_prefix(c, k, v)
+    hk, hv = (pn.held(x, ck, hd).reshape(long, 1, hd) for x in (k, v))
+    lens = [int(x) for x in rng.integers(300, long + 1, seqs)]
+    # a third of the sequences under smaller steps
+    q = np.repeat(np.array(gain)[None] * np.where(np.arange(seqs) % 3, 1.0, 0.75)[:, None], hd, 1).astype(np.float32)
+    q, qf = cast(q, qk)
+    _, got = run_chunk(lib, c, q, qk, [1] * seqs, lens, 0, n_heads, 1.0)
+    for s in range(seqs):
+        qq = qf[s:s + 1].reshape(1, n_heads, hd)
+        want, bound = pn.attention(qq, hk[:lens[s]], hv[:lens[s]], [0], 1.0)
+        bound = bound_of(bound, want, qq, hk[:lens[s]], hv[:lens[s]], qk, ck, 1.0)
+        within(np.abs(got[s].reshape(1, n_heads, hd) - want), bound, (s, lens[s]))
