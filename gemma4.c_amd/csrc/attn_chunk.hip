@@ -975,14 +975,18 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                     if constexpr (M::F) {
                         const float* meta = reinterpret_cast<const float*>(lds + P::meta_at(st, 0));
                         const int h = own_lane() >> 5;
+                        // The key's 2^e and the row's fq may be far above 1, one of them where scores
+                        // are ordinary: fq comes first if it is below 1, and last (weights) if not,
+                        // so that nothing on the way is above both the sum and the score.
+                        const float fa = fminf(fq, 1.0f);
 #pragma unroll
                         for (int b = 0; b < 4; b++) {
                             const f4_t x = *reinterpret_cast<const f4_t*>(meta + (DS == 1 ? 32 : part * 32) + 8 * b + 4 * h);
                             const f4_t y = *reinterpret_cast<const f4_t*>(meta + 8 * b + 4 * h);
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                sc[4 * b + i] *= x[i];
-                                if constexpr (DS == 1) sc[4 * b + i] = __builtin_fmaf(low[4 * b + i], y[i], sc[4 * b + i]);
+                                sc[4 * b + i] = sc[4 * b + i] * fa * x[i];
+                                if constexpr (DS == 1) sc[4 * b + i] = __builtin_fmaf(low[4 * b + i] * fa, y[i], sc[4 * b + i]);
                             }
                         }
                     }
@@ -1014,7 +1018,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                             const f4_t vi = *reinterpret_cast<const f4_t*>(meta + kBothInv / 4 + vhalf + 8 * b + 4 * h);
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                sc[4 * b + i] = __builtin_fmaf(sc[4 * b + i], fq, v[i]);
+                                sc[4 * b + i] = __builtin_fmaf(sc[4 * b + i], fq < 1.0f ? 1.0f : fq, v[i]);
                                 fv[4 * b + i] = vi[i];
                                 low = fminf(low, v[i]);
                             }

@@ -90,3 +90,50 @@ def test_scores_rise_far(lib, combo, hd, gain):
         want, bound = pn.attention(qq, hk[:lens[s]], hv[:lens[s]], [0], 1.0)
         bound = bound_of(bound, want, qq, hk[:lens[s]], hv[:lens[s]], qk, ck, 1.0)
         within(np.abs(got[s].reshape(1, n_heads, hd) - want), bound, (s, lens[s]))
+
+
+@pytest.mark.parametrize("hd", [64, 256, 512])
+@pytest.mark.parametrize("k_top,q_top", [(112, -110), (104, -100), (120, -120), (-110, 112), (-120, 120)])
+@pytest.mark.parametrize("sign", [False, True])
+def test_large_beside_small(lib, hd, k_top, q_top, sign):
+    """fp32 rows over fp32: keys as large as fp32 has them beside rows so small that the scores are ordinary, and the other
+    way round; keys of either sign, and of one"""
+    rng = np.random.default_rng(510 + hd)
+    n, lens, n_heads, n_kv = [70, 1], [300, 90], 4, 2
+    c = Cache(lib, rng, pn.F32, hd, n_kv, 16, lens, extra=WIDE)
+    assert tiles(c, 0, sum(n), n_heads)
+    k, v = rows(rng, sum(lens), n_kv, hd), rows(rng, sum(lens), n_kv, hd)
+    q = rows(rng, sum(n), n_heads, hd)
+    if sign:
+        k, q = np.abs(k), np.abs(q) * rng.choice(np.array([1, -1], np.float32), q.shape[1] // hd).repeat(hd)
+    # scores stay ordinary: up to 4 hd a product of ones
+    k, q = k * np.float32(2.0 ** k_top), (q * np.float32(2.0 ** q_top)).astype(np.float32)
+    scale = (0.25 if not sign else 4 / hd) * 2.0 ** -(k_top + q_top)
+    c.store(k, v, lens, lens)
+    _, got = run_chunk(lib, c, q, pn.F32, n, lens, 0, n_heads, scale)
+    at, key = pn.starts(n), pn.starts(lens)
+    for s in range(2):
+        kk = slice(key[s], key[s + 1])
+        qq = q[at[s]:at[s + 1]].reshape(n[s], n_heads, hd).astype(np.float64)
+        kf, vf = (x[kk].reshape(-1, n_kv, hd).astype(np.float64) for x in (k, v))
+        want, bound = pn.attention(qq, kf, vf, [0] * n[s], scale)
+        bound = bound_of(bound, want, qq, kf, vf, pn.F32, pn.F32, scale)
+        within(np.abs(got[at[s]:at[s + 1]].reshape(n[s], n_heads, hd) - want), bound, s)
+
+
+@pytest.mark.parametrize("hd", [64, 256, 512])
+@pytest.mark.parametrize("k_top,q_top", [(125, 125), (125, -100), (-100, 125)])
+def test_rows_and_keys_that_do_not_meet(lib, hd, k_top, q_top):
+    """fp32 rows over fp32 whose dims are zeros wherever the keys' are not: scores of 0, however large both are"""
+    rng = np.random.default_rng(520 + hd)
+    n, t, n_heads = 50, 200, 2
+    c = Cache(lib, rng, pn.F32, hd, 1, 16, [t], extra=WIDE)
+    assert tiles(c, 0, n, n_heads)
+    k, v, q = rows(rng, t, 1, hd), rows(rng, t, 1, hd), rows(rng, n, n_heads, hd).reshape(n, n_heads, hd)
+    on = rng.random(hd) < 0.5
+    k, q = np.where(on, k, 0) * np.float32(2.0 ** k_top), np.where(on, 0, q) * np.float32(2.0 ** q_top)
+    c.store(k.astype(np.float32), v, [t], [t])
+    _, got = run_chunk(lib, c, q.reshape(n, -1).astype(np.float32), pn.F32, [n], [t], 0, n_heads, 1.0)
+    zq, kf, vf = np.zeros((n, n_heads, hd)), np.zeros((t, 1, hd)), v.reshape(t, 1, hd).astype(np.float64)
+    want, bound = pn.attention(zq, kf, vf, [0] * n, 1.0)
+    within(np.abs(got.reshape(n, n_heads, hd) - want), bound_of(bound, want, zq, kf, vf, pn.F32, pn.F32, 1.0), hd)
