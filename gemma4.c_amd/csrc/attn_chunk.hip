@@ -34,6 +34,7 @@ struct ChunkArgs {
     bool pairs;     // Mode::kPairs
     int cols;       // columns of a partial result, a multiple of 32
     float scale;
+    float fq, by;   // rows of 16 bits: what a sum of products is multiplied by; SMALL: the rows before
 };
 
 // ---- shares of the work ------------------------------------------------------
@@ -337,7 +338,13 @@ struct Plan {
 constexpr int kMetaV = 128, kMetaMarks = 384;
 constexpr int kBothV = 256, kBothInv = 512, kBothMarks = 768;
 
-template <int TQ, int TC, int HD>
+// SMALL: bf16 rows under a scale below 1.  They go as far as fp32, and their products
+// with the keys may pass it where the scale makes ordinary scores of them: the rows take
+// the scale's power of two with them (exact but for what becomes subnormal, 2^-134).  8
+// heads, this and a.fq alone: 512 rows over 32488 positions, bf16 of 512, 313 us and 300,
+// 48 single rows 75 and 71; 23 rows of 256 24.3 and 23.7.  A kernel of its own: as a
+// branch of one kernel it cost the other scales up to 4 % (512 rows 317 -> 329).
+template <int TQ, int TC, int HD, bool SMALL>
 __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW / 4)) void attn_chunk_kernel(ChunkArgs a) {
     typedef Plan<TQ, TC, HD> P;
     typedef Mode<TQ, TC> M;
@@ -747,7 +754,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
 
             // ---- q: 32 columns' rows through places in LDS that the first stage leaves free ----
             op q[NQ][KS];
-            float fq = fabsf(a.scale) * kLog2e;
+            float fq = NQ == 1 ? a.fq : fabsf(a.scale) * kLog2e;
             constexpr int kBox = KSP == 2 ? TB : DS == 1 ? TB / 2 : TB / 4, kPasses = 32 * P::RB / kBox;
             constexpr int kChunks = P::RB / 16 / kPasses, kSteps = KS / kPasses;
             static_assert(kBox == 32 * kChunks * 16 && kSteps * kPasses == KS, "q");
@@ -767,14 +774,23 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 auto chunk = [&](int c) { return box + row_slot<kChunks>(col, c); };
                 if constexpr (TQ != G4_F32) {
                     const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;
+                    auto shrink = [&](const f4_t& x) {
+                        E e[8];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const unsigned w = __float_as_uint(x[k]);
+                            e[2 * k] = (E)(__uint_as_float(w << 16) * a.by);
+                            e[2 * k + 1] = (E)(__uint_as_float(w & 0xffff0000u) * a.by);
+                        }
+                        f4_t y;
+                        __builtin_memcpy(&y, e, 16);
+                        return y;
+                    };
 #pragma unroll
                     for (int pass = 0; pass < kPasses; pass++) {
-                        if constexpr (KSP == 2) {
-                            rows_to_lds<kChunks, 16>(box, kp * 16, q_row(pass), lane);
-                            lds_barrier();
-                        } else {
-                            rows_to_lds<kChunks, 32>(box, 0, q_row(pass), lane);
-                        }
+                        if constexpr (SMALL) rows_to_lds<kChunks, 32 / KSP>(box, kp * 16, q_row(pass), lane, shrink);
+                        else rows_to_lds<kChunks, 32 / KSP>(box, kp * 16, q_row(pass), lane);
+                        if constexpr (KSP == 2) lds_barrier();
 #pragma unroll
                         for (int i = 0; i < kSteps; i++) {
                             uint4 x = *reinterpret_cast<const uint4*>(chunk(i * 2 + h));
@@ -783,7 +799,6 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                             q[0][pass * kSteps + i] = __builtin_bit_cast(op, x);
                         }
                     }
-                    if (a.scale == 0.0f) fq = 1.0f;
                 } else if constexpr (NQ == 3) {
                     // times scale log2(e), as three terms: the float itself
                     const float qs = a.scale * kLog2e;
@@ -1712,19 +1727,19 @@ void set_columns(ChunkArgs& a, int cols) {
     while (a.lg < kLgShares && (2 << a.lg) <= most) a.lg++;
 }
 
-template <int TQ, int TC, int HD>
-int launch_chunk(ChunkArgs a) {
+template <int TQ, int TC, int HD, bool SMALL>
+int launch_tiles(ChunkArgs a) {
     typedef Plan<TQ, TC, HD> P;
-    double keys = (double)a.p.table_stride * (1 << a.p.lgpage);
-    if (a.window > 0 && a.window < keys) keys = a.window;
-    constexpr int kUnit = HD * P::M::ES > 512 ? HD * P::M::ES / 512 : 1;
-    if (keys * kUnit <= kFewKeys && keys * kUnit * a.m * a.n_heads <= kFewPairs) {
-        hipLaunchKernelGGL((attn_chunk_row_kernel<TQ, TC, HD>), dim3(a.m, a.n_heads), dim3(256), 0, g4_stream(), a);
-        return g4_check_launch("attn_chunk_row_kernel");
-    }
     set_columns(a, P::COLS);
     a.pairs = P::M::kPairs;
-    auto kernel = attn_chunk_kernel<TQ, TC, HD>;
+    // (a scale of 0: rows of zeros, and a score of -infinity times fq has to stay one)
+    a.fq = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
+    if (SMALL) {
+        int e;
+        a.fq = frexpf(fabsf(a.scale), &e) * kLog2e;
+        a.by = ldexpf(1.0f, e);
+    }
+    auto kernel = attn_chunk_kernel<TQ, TC, HD, SMALL>;
     // more than 64 KB of LDS has to be asked for, once on each device
     static std::atomic<unsigned long long> asked{0};
     int dev = 0;
@@ -1738,6 +1753,20 @@ int launch_chunk(ChunkArgs a) {
     const int units = ((1 << a.lg) - 1) * (a.cols / 32) * (HD < 128 ? 1 : HD / 128);
     hipLaunchKernelGGL((attn_chunk_join_kernel<TQ, HD>), dim3(units < kJoinWG ? units : kJoinWG), dim3(256), 0, g4_stream(), a);
     return g4_check_launch("attn_chunk_kernel");
+}
+template <int TQ, int TC, int HD>
+int launch_chunk(const ChunkArgs& a) {
+    double keys = (double)a.p.table_stride * (1 << a.p.lgpage);
+    if (a.window > 0 && a.window < keys) keys = a.window;
+    constexpr int ES = Mode<TQ, TC>::ES, kUnit = HD * ES > 512 ? HD * ES / 512 : 1;
+    if (keys * kUnit <= kFewKeys && keys * kUnit * a.m * a.n_heads <= kFewPairs) {
+        hipLaunchKernelGGL((attn_chunk_row_kernel<TQ, TC, HD>), dim3(a.m, a.n_heads), dim3(256), 0, g4_stream(), a);
+        return g4_check_launch("attn_chunk_row_kernel");
+    }
+    if constexpr (TQ == G4_BF16) {
+        if (a.scale != 0.0f && fabsf(a.scale) < 1.0f) return launch_tiles<TQ, TC, HD, true>(a);
+    }
+    return launch_tiles<TQ, TC, HD, false>(a);
 }
 template <int TQ, int TC>
 int launch_chunk(const ChunkArgs& a, int hd) {

@@ -125,10 +125,13 @@ template <int C>
 __device__ __forceinline__ int row_slot(int r, int c) {
     return (r * C + (c ^ (r & (C < 32 ? C - 1 : 31)))) * 16;
 }
+struct AsTheyAre {
+    __device__ __forceinline__ f4_t operator()(const f4_t& x) const { return x; }
+};
 // N rows of C chunks each, from `first` on, by one wave: at(r) is row r's
-// address, box takes C chunks a row
-template <int C, int N, typename At>
-__device__ __forceinline__ void rows_to_lds(uint8_t* box, int first, At at, int lane = threadIdx.x & 63) {
+// address, box takes C chunks a row; edit: of 16 bytes, on the way
+template <int C, int N, typename At, typename Edit = AsTheyAre>
+__device__ __forceinline__ void rows_to_lds(uint8_t* box, int first, At at, int lane = threadIdx.x & 63, Edit edit = {}) {
     constexpr int K = N * C / 64;
     f4_t x[K];
 #pragma unroll
@@ -140,7 +143,7 @@ __device__ __forceinline__ void rows_to_lds(uint8_t* box, int first, At at, int 
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const int p = k * 64 + lane;
-        *reinterpret_cast<f4_t*>(box + row_slot<C>(first + p / C, p % C)) = x[k];
+        *reinterpret_cast<f4_t*>(box + row_slot<C>(first + p / C, p % C)) = edit(x[k]);
     }
     wave_lds_order();
 }

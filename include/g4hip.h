@@ -524,7 +524,8 @@ int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void
  * V as they are; fp32 sums.
  *   G4_F32 over BF16 or G4_KV_Q8: exact products of q and of the weights (times
  * the scale of V's codes) with what the cache holds, fp32 sums.
- *   G4_F16 over F16, G4_BF16 over BF16 or G4_KV_Q8: exact products of q, fp32
+ *   G4_F16 over F16, G4_BF16 over BF16 or G4_KV_Q8: exact products of q (BF16
+ * under an attn_scale below 1: q times its power of two, within 2^-134), fp32
  * sums, weights (times the scale of a token's codes) rounded to the type before
  * they multiply V; the result is rounded to the type.
  *   Few keys (the window's or all that a row of table allows, in units of 512
@@ -536,11 +537,11 @@ int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void
  * tokens, that no row of the sequence sees do not matter, whatever they hold;
  * what a row does not see does not change it, infinities and NaN included.
  * |V| times the keys a row sees has to stay below fp32's largest number, scores
- * (and q times attn_scale) as well.  Where what a row's head sees holds
- * infinities or NaN, its output is what the formula gives or NaN.  out may not
- * overlap q.  part: g4_attn_chunk_paged_part_bytes() bytes (m: this call's or
- * more) that no call running at the same time uses (its contents need not be
- * kept). */
+ * (and q times attn_scale, over G4_KV_Q8 127 hd times that) as well.  Where what a
+ * row's head sees holds infinities or NaN, its output is what the formula gives or
+ * NaN.  out may not overlap q.  part: g4_attn_chunk_paged_part_bytes() bytes (m:
+ * this call's or more) that no call running at the same time uses (its contents
+ * need not be kept). */
 size_t g4_attn_chunk_paged_part_bytes(int m, int n_heads, int n_kv, int hd);
 int g4_attn_chunk_paged(const void *q, int q_stride, int q_type, const void *kp, const void *vp, int type, int n_pages,
                         int page, int n_kv, int hd, const int *table, int table_stride, const int *cu, const int *lens,

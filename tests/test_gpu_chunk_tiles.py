@@ -137,3 +137,43 @@ def test_rows_and_keys_that_do_not_meet(lib, hd, k_top, q_top):
     zq, kf, vf = np.zeros((n, n_heads, hd)), np.zeros((t, 1, hd)), v.reshape(t, 1, hd).astype(np.float64)
     want, bound = pn.attention(zq, kf, vf, [0] * n, 1.0)
     within(np.abs(got.reshape(n, n_heads, hd) - want), bound_of(bound, want, zq, kf, vf, pn.F32, pn.F32, 1.0), hd)
+
+
+# (log2 of q, of K, of the scale): q k leaves fp32's range, or comes near it, where scores do not
+FAR = {pn.BF16: [(75, 50, -122), (5, 120, -122), (122, 3, -122), (122, 0, -120), (30, 90, -118), (-8, 122, -114), (-60, 120, -60),
+                 (10, 10, -20)],
+       pn.Q8: [(121, -2, -119), (117, 2, -119), (121, -20, -101), (60, 60, -120), (-30, 115, -85), (-100, 40, 60), (10, 10, -20)]}
+
+
+@pytest.mark.parametrize("ck,case", [(ck, case) for ck in FAR for case in FAR[ck]], ids=str)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("extra", [0, WIDE], ids=["table", "wide"])
+def test_large_rows_under_a_small_scale(lib, ck, case, hd, extra):
+    """bf16 rows whose products with the keys are far larger than the scores, which the scale makes ordinary; scales of
+    either sign that are no power of two; some rows of zeros and far smaller rows among them.  The call of few keys and
+    that of tiles agree with the formula."""
+    rng = np.random.default_rng(530 + hd)
+    n, lens, n_heads, n_kv = [70, 1, 9], [124, 90, 100], 4, 2
+    c = Cache(lib, rng, ck, hd, n_kv, 16, lens, extra=extra)
+    if extra:
+        assert tiles(c, 0, sum(n), n_heads)
+    k, v = rows(rng, sum(lens), n_kv, hd), rows(rng, sum(lens), n_kv, hd)
+    q = rows(rng, sum(n), n_heads, hd)
+    q[3], q[5], q[7] = 0, q[5] * 2.0 ** -4, q[7] * 2.0 ** -60
+    k = (k * 2.0 ** case[1]).astype(np.float32)
+    q, qf = cast((q * 2.0 ** case[0]).astype(np.float32), pn.BF16)
+    c.store(k, v, lens, lens)
+    hk, hv = (pn.held(x, ck, hd).reshape(-1, n_kv, hd).astype(np.float64) for x in (k, v))
+    at, key = pn.starts(n), pn.starts(lens)
+    for sign in (0.17, -0.23):
+        scale = float(np.float32(sign * 2.0 ** case[2]))
+        _, got = run_chunk(lib, c, q, pn.BF16, n, lens, 0, n_heads, scale)
+        for s in range(len(n)):
+            kk = slice(key[s], key[s + 1])
+            qq = qf[at[s]:at[s + 1]].reshape(n[s], n_heads, hd).astype(np.float64)
+            want, bound = pn.attention(qq, hk[kk], hv[kk], [0] * n[s], scale)
+            bound = bound_of(bound, want, qq, hk[kk], hv[kk], pn.BF16, ck, scale)
+            # q times the scale's power of two as bf16: half a step of its smallest, 2^-134, below its normal range; the rest
+            # of the scale is below 2; a score's error twice, in the numerator and in the denominator
+            bound = bound + 2 * 2 * 2.0 ** -134 * np.abs(hk[kk]).sum(-1).max() * np.abs(hv[kk]).max()
+            within(np.abs(got[at[s]:at[s + 1]].reshape(n[s], n_heads, hd) - want), bound, (s, sign))
