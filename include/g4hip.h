@@ -535,7 +535,8 @@ int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void
  * fit (n > lens, rows past m, positions past the table) are left as they are.
  * A row that sees a page outside the pool becomes NaN.  Pages, and within a page
  * tokens, that no row of the sequence sees do not matter, whatever they hold;
- * what a row does not see does not change it, infinities and NaN included.
+ * what only other rows see does not change a row beyond rounding, infinities and
+ * NaN included.
  * |V| times the keys a row sees has to stay below fp32's largest number, scores
  * (and q times attn_scale, over G4_KV_Q8 127 hd times that) as well.  Where what a
  * row's head sees holds infinities or NaN, its output is what the formula gives or

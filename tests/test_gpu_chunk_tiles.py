@@ -177,3 +177,72 @@ def test_large_rows_under_a_small_scale(lib, ck, case, hd, extra):
             # of the scale is below 2; a score's error twice, in the numerator and in the denominator
             bound = bound + 2 * 2 * 2.0 ** -134 * np.abs(hk[kk]).sum(-1).max() * np.abs(hv[kk]).max()
             within(np.abs(got[at[s]:at[s + 1]].reshape(n[s], n_heads, hd) - want), bound, (s, sign))
+
+
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+@pytest.mark.parametrize("hd", [64, 256, 512])
+@pytest.mark.parametrize("window", [0, 300])
+def test_what_other_rows_see(lib, combo, hd, window):
+    """keys behind a row and before its window, and the other rows and heads of its sequence: whatever they are, finite and
+    large, tiny, infinite or NaN, the row is the formula's of what it sees, within the bound that it has without them"""
+    qk, ck = combo
+    rng = np.random.default_rng(540 + hd)
+    n, t, n_heads, n_kv = 90, 420, 4, 2
+    c = Cache(lib, rng, ck, hd, n_kv, 16, [t], extra=WIDE)
+    assert tiles(c, window, n, n_heads)
+    k, v = rows(rng, t, n_kv, hd), rows(rng, t, n_kv, hd)
+    x = rows(rng, n, n_heads, hd)
+    q, qf = cast(x, qk)
+    scale = 2 * hd ** -0.5
+    pos = np.arange(t - n, t)
+    late, early = t - 30, 60                  # changed: late and behind it; with a window, up to early
+    keep = pos < late
+    if window:
+        keep &= pos - window + 1 > early
+    assert 20 < keep.sum() < n
+    cut = np.arange(t) >= late
+    if window:
+        cut |= np.arange(t) <= early
+    hk, hv = (pn.held(y, ck, hd).reshape(t, n_kv, hd) for y in (k, v))
+    first = np.maximum(pos + 1 - window, 0) if window else pos * 0
+    at = np.flatnonzero(keep)
+    one, last = first[at[0]], pos[at[-1]] + 1
+    qq = qf.reshape(n, n_heads, hd)[keep]
+    want, bound = pn.attention(qq, hk[one:last], hv[one:last], first[keep] - one, scale)
+    bound = bound_of(bound, want, qq, hk[one:last], hv[one:last], qk, ck, scale)
+
+    def run(q):
+        got = run_chunk(lib, c, q, qk, [n], [t], window, n_heads, scale)[1]
+        return np.abs(got.reshape(n, n_heads, hd)[keep] - want)
+
+    for what in ("nothing", "large", "rising", "tiny", "infinite", "minus infinite", "mixed"):
+        k2, v2 = k.copy(), v.copy()
+        if what == "large":
+            k2[cut] *= 40
+            v2[cut] *= 1000
+        elif what == "rising":
+            k2[cut] *= np.linspace(1, 5, cut.sum(), dtype=np.float32)[:, None]
+        elif what == "tiny":
+            k2[cut] = 0
+            v2[cut] *= np.float32(2.0 ** -100) if ck != pn.F16 else np.float32(0)
+        elif what == "infinite":
+            k2[cut] = np.inf
+            v2[cut] = -np.inf
+        elif what == "minus infinite":
+            k2[cut] = -np.inf
+        elif what == "mixed":
+            k2[late], k2[late + 3, 1], v2[late + 7, hd + 1], v2[late + 9] = NAN, np.inf, np.inf, NAN
+            if window:
+                k2[3, 5], v2[early, hd + 9], v2[20] = -np.inf, np.inf, np.inf
+        c.store(k2, v2, [t], [t])
+        within(run(q), bound, what)
+    c.store(k, v, [t], [t])
+    # another row's or head's q
+    stay = np.arange(n)[keep] % 3 != 1
+    for what in (8.0, 0.0, np.inf, NAN):
+        y = x.reshape(n, n_heads, hd).copy()
+        with np.errstate(all="ignore"):
+            y[1::3] *= np.float32(what)
+            y[:, 2] *= np.float32(what)
+            err = run(cast(y.reshape(n, -1), qk)[0])
+        within(err[stay][:, [0, 1, 3]], bound[stay][:, [0, 1, 3]], what)
