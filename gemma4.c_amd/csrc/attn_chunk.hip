@@ -264,7 +264,10 @@ struct Mode {
     // largest score it is put.  bf16, whose V goes as far as fp32: weights are at
     // most 1; fp16's smallest numbers ask for large weights, and its V cannot overflow
     static constexpr float kSlack = !kHalf ? 0.0f : NQ == 1 ? 8.0f : 4.0f, kRaise = kHalf ? 0.0f : 8.0f;
-    static constexpr float kLift = kHalf && NQ > 1 ? 11.0f : 0.0f;   // fp16 terms: 2^11 above their fp32 size
+    // fp16 weights and terms: 2^7 and 2^11 above their fp32 size, with kSlack 2^15 at most.
+    // Half of fp16's smallest step is then 2^-32 (2^-36) of the largest weight: a long tail
+    // of small ones keeps its share
+    static constexpr float kLift = !kHalf ? 0.0f : NQ == 1 ? 7.0f : 11.0f;
 };
 template <int T>
 struct RowElem;

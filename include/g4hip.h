@@ -527,7 +527,8 @@ int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void
  *   G4_F16 over F16, G4_BF16 over BF16 or G4_KV_Q8: exact products of q (BF16
  * under an attn_scale below 1: q times its power of two, within 2^-134), fp32
  * sums, weights (times the scale of a token's codes) rounded to the type before
- * they multiply V; the result is rounded to the type.
+ * they multiply V (F16: also within 2^-32 of the row's largest); the result is
+ * rounded to the type.
  *   Few keys (the window's or all that a row of table allows, in units of 512
  * bytes of a head's K, up to 256, and 2^17 of them over all rows and heads):
  * fp32 throughout, so that the same rows with a wider table are rounded as above.

@@ -246,3 +246,36 @@ def test_what_other_rows_see(lib, combo, hd, window):
             y[:, 2] *= np.float32(what)
             err = run(cast(y.reshape(n, -1), qk)[0])
         within(err[stay][:, [0, 1, 3]], bound[stay][:, [0, 1, 3]], what)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("below", [20, 24, 26, 28])
+def test_long_flat_tail(lib, hd, below):
+    """fp16 rows: one key far above hundreds whose weights lie below fp16's own range beside it, and whose V is all there
+    is.  A weight is within 2^-11 of itself or 2^-32 of the largest."""
+    rng = np.random.default_rng(560 + hd)
+    seqs, page, long = 300, 64, 1024
+    table = np.tile(np.concatenate([np.arange(long // page), np.full(WIDE, -1)]).astype(np.int32), (seqs, 1))
+    c = Cache(lib, rng, pn.F16, hd, 1, page, None, table=table, pages=long // page)
+    assert tiles(c, 0, seqs, 1)
+    k, v = np.zeros((long, hd), np.float32), 1000 + 100 * rows(rng, long, 1, hd)
+    q = np.zeros((seqs, hd), np.float32)
+    q[:, 0] = 1
+    # the key that is above the others, at places all over the tiles
+    tops = np.arange(5, long, 64)
+    k[tops, 0] = np.round(below * np.log(2) * 16) / 16
+    v[tops] = 0
+    store_prefix(c, k, v)
+    hk, hv = (pn.held(x, pn.F16, hd).reshape(long, 1, hd) for x in (k, v))
+    lens = [int(x) for x in rng.integers(600, long + 1, seqs)]
+    q, qf = cast(q, pn.F16)
+    _, got = run_chunk(lib, c, q, pn.F16, [1] * seqs, lens, 0, 1, 1.0)
+    for s in range(seqs):
+        t = lens[s]
+        want, bound = pn.attention(qf[s:s + 1].reshape(1, 1, hd), hk[:t], hv[:t], [0], 1.0)
+        # the weights' rounding and the result's, each 2^-11 of the sum (V is positive); below fp16's normal range a weight
+        # is off by half a step of 2^-24 where the largest is 2^7 at least, 2^-32 of it, and all of them are divided by a
+        # sum of `above` such largest ones; the result's own smallest step, halved
+        above = (tops < t).sum()
+        bound = bound + 2.002 * 2.0 ** -11 * np.abs(want) + 2.0 ** -32 * t * np.abs(hv).max() / above + 2.0 ** -25
+        within(np.abs(got[s].reshape(1, 1, hd) - want), bound, (s, t))
