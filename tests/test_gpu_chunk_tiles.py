@@ -248,6 +248,41 @@ def test_what_other_rows_see(lib, combo, hd, window):
         within(err[stay][:, [0, 1, 3]], bound[stay][:, [0, 1, 3]], what)
 
 
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+@pytest.mark.parametrize("hd,window", [(64, 1), (64, 20), (128, 40), (256, 64), (64, 700), (256, 300), (512, 20), (512, 600)])
+def test_last_positions_there_are(lib, combo, hd, window):
+    """sequences that end at position 2^30 - 1, the last that a table allows: the same bits as at the end of a short sequence,
+    by the tiles and by the call of few keys"""
+    qk, ck = combo
+    rng = np.random.default_rng(550 + hd)
+    page, n, n_heads, n_kv = 4096, 50, 2, 1
+    top, short = 1 << 30, 2 * page
+    new = min(short, window + n + 3)
+    k, v = rows(rng, new, n_kv, hd), rows(rng, new, n_kv, hd)
+    q = cast(rows(rng, n, n_heads, hd), qk)[0]
+    got = []
+    for length in (short, top):
+        width = (length + page - 1) // page
+        table = np.full((1, width), -1, np.int32)
+        table[0, -2:] = [1, 0]
+        c = Cache(lib, rng, ck, hd, n_kv, page, None, table=table, pages=2)
+        c.store(k, v, [new], [length])
+        for m in (n, max(n, rows_for_tiles(c, window, n_heads))):
+            if m > n:
+                assert tiles(c, window, m, n_heads)
+            bits, f = run_chunk(lib, c, padded(q, m), qk, [n], [length], window, n_heads, 0.1)
+            assert np.isfinite(f[:n]).all()
+            got.append(bits[:n])
+    assert same_bits(got[0], got[2]) and same_bits(got[1], got[3])
+    hk, hv = (pn.held(x, ck, hd).reshape(-1, n_kv, hd) for x in (k, v))
+    qf = back(q, qk).reshape(n, n_heads, hd)
+    first = [new - n + i + 1 - window for i in range(n)]
+    want, bound = pn.attention(qf, hk, hv, first, 0.1)
+    bound = bound_of(bound, want, qf, hk, hv, qk, ck, 0.1)
+    for g in got[2:]:
+        within(np.abs(back(g, qk).reshape(n, n_heads, hd) - want), bound, window)
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256, 512])
 @pytest.mark.parametrize("below", [20, 24, 26, 28])
 def test_long_flat_tail(lib, hd, below):
@@ -279,3 +314,188 @@ def test_long_flat_tail(lib, hd, below):
         above = (tops < t).sum()
         bound = bound + 2.002 * 2.0 ** -11 * np.abs(want) + 2.0 ** -32 * t * np.abs(hv).max() / above + 2.0 ** -25
         within(np.abs(got[s].reshape(1, 1, hd) - want), bound, (s, t))
+
+
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+@pytest.mark.parametrize("hd,n_heads,window", [(64, 4, 1), (128, 2, 5), (256, 4, 32), (64, 8, 50), (512, 4, 31), (512, 2, 100)])
+def test_small_windows(lib, combo, hd, n_heads, window):
+    """windows of a few keys with rows enough in the call that it goes to the tiles; most of the rows are padding"""
+    qk, ck = combo
+    rng = np.random.default_rng(570 + window)
+    n, hist, n_kv = [3, 96, 150, 1, 33, 0], [0, 40, 700, 600, 31, 9], 2
+    lens = [a + b for a, b in zip(n, hist)]
+    c = Cache(lib, rng, ck, hd, n_kv, 16, lens, extra=WIDE)
+    k, v = rows(rng, sum(lens), n_kv, hd), rows(rng, sum(lens), n_kv, hd)
+    c.store(k, v, lens, lens)
+    m = rows_for_tiles(c, window, n_heads)
+    assert m > sum(n) and tiles(c, window, m, n_heads)
+    q, qf = cast(rows(rng, sum(n), n_heads, hd), qk)
+    bits, got = run_chunk(lib, c, padded(q, m), qk, n, lens, window, n_heads, 0.1)
+    assert (bits[sum(n):].view(np.uint8) == 0x3F).all()
+    hk, hv = (pn.held(x, ck, hd).reshape(-1, n_kv, hd) for x in (k, v))
+    at, key = pn.starts(n), pn.starts(lens)
+    for s, (t, h) in enumerate(zip(n, hist)):
+        for lo in range(0, t, 64):
+            hi = min(t, lo + 64)
+            first = [max(0, h + i + 1 - window) for i in range(lo, hi)]
+            kk = slice(key[s] + first[0], key[s] + h + hi)
+            qq = qf[at[s] + lo:at[s] + hi].reshape(hi - lo, n_heads, hd)
+            want, bound = pn.attention(qq, hk[kk], hv[kk], np.array(first) - first[0], 0.1)
+            bound = bound_of(bound, want, qq, hk[kk], hv[kk], qk, ck, 0.1)
+            within(np.abs(got[at[s] + lo:at[s] + hi].reshape(hi - lo, n_heads, hd) - want), bound, (s, lo))
+
+
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+@pytest.mark.parametrize("hd,window", [(64, 50), (128, 300), (256, 50), (512, 300), (512, 20)])
+def test_pages_before_a_window(lib, combo, hd, window):
+    """pages that no row sees any more: entries that are no page, that lie outside the pool, or another sequence's with
+    infinities and NaN in them"""
+    qk, ck = combo
+    rng = np.random.default_rng(580 + window)
+    page, t, new, n_heads = 16, 420, 20, 2
+    c = Cache(lib, rng, ck, hd, 1, page, [t, t], extra=WIDE)
+    k, v = rows(rng, 2 * t, 1, hd), rows(rng, 2 * t, 1, hd)
+    c.store(k, v, [t, t], [t, t])
+    q = cast(rows(rng, 2 * new, n_heads, hd), qk)[0]
+    m = max(2 * new, rows_for_tiles(c, window, n_heads))
+    assert tiles(c, window, m, n_heads)
+    q = padded(q, m)
+    a, af = run_chunk(lib, c, q, qk, [new, new], [t, t], window, n_heads, 0.1)
+    assert np.isfinite(af[:2 * new]).all()
+    gone = (t - new + 1 - window) // page
+    good = c.table.copy()
+    spare = np.setdiff1d(np.arange(c.pages), good)       # a page of no sequence: NaN, as Cache fills its pools
+    for entry in (-1, c.pages, (1 << 31) - 1, -(1 << 31), int(spare[0])):
+        c.table = good.copy()
+        c.table[0, :gone] = entry
+        c.dtable.write(c.table)
+        b, _ = run_chunk(lib, c, q, qk, [new, new], [t, t], window, n_heads, 0.1)
+        assert same_bits(a, b), entry
+    c.table = good
+    c.dtable.write(good)
+
+
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+@pytest.mark.parametrize("hd,window", [(64, 30), (256, 260), (256, 30), (512, 30), (512, 130)])
+def test_bad_pages_and_windows(lib, combo, hd, window):
+    """a page outside the pool under a window: NaN in the rows that see it, no bit of the others"""
+    qk, ck = combo
+    rng = np.random.default_rng(590 + window)
+    n, hist, n_heads = [40, 200, 3], [50, 150, 300], 2
+    lens = [a + b for a, b in zip(n, hist)]
+    c = Cache(lib, rng, ck, hd, 1, 16, lens, extra=WIDE)
+    x = rows(rng, sum(lens), 1, hd)
+    c.store(x, x, lens, lens)
+    m = max(sum(n), rows_for_tiles(c, window, n_heads))
+    assert tiles(c, window, m, n_heads)
+    q = padded(cast(rows(rng, sum(n), n_heads, hd), qk)[0], m)
+    a, _ = run_chunk(lib, c, q, qk, n, lens, window, n_heads, 0.1)
+    old = c.table.copy()
+    c.table[1, 11], c.table[2, 0], c.table[2, 18] = c.pages, -5, c.pages + 7    # positions 176 .. 191; 0 .. 15, 288 .. 303
+    c.dtable.write(c.table)
+    b, bf = run_chunk(lib, c, q, qk, n, lens, window, n_heads, 0.1)
+    c.table = old
+    c.dtable.write(old)
+    at = pn.starts(n)
+    assert same_bits(a[:at[1]], b[:at[1]]) and same_bits(a[at[3]:], b[at[3]:])
+    for s, bad in ((1, [(176, 191)]), (2, [(0, 15), (288, 303)])):
+        p = np.arange(hist[s], lens[s])
+        sees = np.zeros(len(p), bool)
+        for lo, hi in bad:
+            sees |= (p >= lo) & (p - window + 1 <= hi)
+        one = slice(at[s], at[s + 1])
+        assert np.isnan(bf[one][sees]).all() and same_bits(a[one][~sees], b[one][~sees])
+
+
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+@pytest.mark.parametrize("hd", [64, 512])
+def test_misfits(lib, combo, hd):
+    """more rows than positions, past the table, past the rows, starts that do not ascend or lie anywhere: those rows stay
+    as they are, the others are done; up to 64 sequences and more"""
+    qk, ck = combo
+    rng = np.random.default_rng(600 + hd)
+    width = WIDE
+    for seqs in (4, 100):
+        c = Cache(lib, rng, ck, hd, 1, 16, [40] * seqs, extra=width)
+        x = rows(rng, 40 * seqs, 1, hd)
+        c.store(x, x, [40] * seqs, [40] * seqs)
+        n = [6] * seqs
+        q, qf = cast(rows(rng, 6 * seqs, 2, hd), qk)
+        assert tiles(c, 0, len(q), 2)
+        lens = [40, 5, c.table.shape[1] * 16 + 1, 40] + [40] * (seqs - 4)
+        lens[-1] = 40 if seqs == 4 else -7
+        bits, got = run_chunk(lib, c, q, qk, n, lens, 0, 2, 0.1)
+        hx = pn.held(x, ck, hd).reshape(-1, 1, hd)
+        for s in range(seqs):
+            one = slice(6 * s, 6 * s + 6)
+            if lens[s] != 40:
+                assert (bits[one].view(np.uint8) == 0x3F).all()
+                continue
+            f, qq = hx[40 * s:40 * s + 40], qf[one].reshape(6, 2, hd)
+            want, bound = pn.attention(qq, f, f, [0] * 6, 0.1)
+            within(np.abs(got[one].reshape(6, 2, hd) - want), bound_of(bound, want, qq, f, f, qk, ck, 0.1), s)
+        if seqs > 4:
+            continue
+        out = filled(lib, q.nbytes, 0x3F)
+        dq, dl = dbuf(lib, q), dbuf(lib, np.array([40] * 4, np.int32))
+        part = filled(lib, lib.L.g4_attn_chunk_paged_part_bytes(24, 2, 1, hd))
+        for cu in ([0, 6, 5, -3, 200], [0, 6, 12, 30, 24], [-7, -1, 3, 2, 1 << 30], [0, 6, 6, 6, 24]):
+            dcu = dbuf(lib, np.array(cu, np.int32))
+            lib.g4_memset(out.ptr, 0x3F, out.nbytes)
+            lib.g4_attn_chunk_paged(dq.ptr, 2 * hd, qk, *c.args(), dcu.ptr, dl.ptr, 4, 24, 0, 2, F(0.1), part.ptr, out.ptr, 2 * hd)
+            lib.g4_sync()
+            o = out.to_array(NPT[qk]).reshape(24, -1)
+            may = np.zeros(24, bool)
+            for s in range(4):
+                if 0 <= cu[s] < cu[s + 1] <= 24:
+                    may[cu[s]:cu[s + 1]] = True
+            assert (o[~may].view(np.uint8) == 0x3F).all() and np.isfinite(back(o[may], qk)).all()
+
+
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+@pytest.mark.parametrize("hd", [64, 256, 512])
+def test_common_prefix(lib, combo, hd):
+    """sequences with the same first pages and rows of their own, cut into tiles: each what it would be alone"""
+    qk, ck = combo
+    rng = np.random.default_rng(610 + hd)
+    page, n_heads = 16, 2
+    table = np.full((2, 5 + WIDE), -1, np.int32)
+    table[:, :5] = [[0, 1, 2, 3, 4], [0, 1, 2, 5, 6]]
+    c = Cache(lib, rng, ck, hd, 1, page, None, table=table, pages=7)
+    x = rows(rng, 48 + 20 + 27, 1, hd)
+    c.store(x[:48], x[:48], [48, 0], [48, 48])
+    c.store(x[48:], x[48:], [20, 27], [68, 75])
+    q, qf = cast(rows(rng, 47, n_heads, hd), qk)
+    assert tiles(c, 0, 47, n_heads)
+    _, got = run_chunk(lib, c, q, qk, [20, 27], [68, 75], 0, n_heads, 0.1)
+    for r0, r1 in ((0, 20), (20, 47)):
+        f = pn.held(np.concatenate([x[:48], x[48 + r0:48 + r1]]), ck, hd).reshape(-1, 1, hd)
+        qq = qf[r0:r1].reshape(-1, n_heads, hd)
+        want, bound = pn.attention(qq, f, f, [0] * (r1 - r0), 0.1)
+        within(np.abs(got[r0:r1].reshape(-1, n_heads, hd) - want), bound_of(bound, want, qq, f, f, qk, ck, 0.1), r0)
+
+
+@pytest.mark.parametrize("combo", COMBOS, ids=str)
+def test_ended_sequences(lib, combo):
+    """many sequences without rows, at the front, at the end and between the others, whatever their lengths are"""
+    qk, ck = combo
+    rng = np.random.default_rng(620)
+    hd, n_heads = 128, 2
+    for seqs in (60, 900):
+        n, lens = [0] * seqs, [int(x) for x in rng.choice([0, 0, 50, 70, -1, 1 << 30], seqs)]
+        used = [seqs // 4, seqs // 2, seqs - 3]
+        for s, (a, b) in zip(used, ((30, 60), (1, 64), (2, 2))):
+            n[s], lens[s] = a, b
+        c = Cache(lib, rng, ck, hd, 1, 16, [lens[s] if s in used else 0 for s in range(seqs)], extra=WIDE)
+        k, v = rows(rng, 126, 1, hd), rows(rng, 126, 1, hd)
+        ns = [lens[s] if s in used else 0 for s in range(seqs)]
+        c.store(k, v, ns, ns)
+        q, qf = cast(rows(rng, 33, n_heads, hd), qk)
+        assert tiles(c, 0, 33, n_heads)
+        _, got = run_chunk(lib, c, q, qk, n, lens, 0, n_heads, 0.1)
+        hk, hv = (pn.held(x, ck, hd).reshape(-1, 1, hd) for x in (k, v))
+        for (r0, r1), (k0, k1) in zip(((0, 30), (30, 31), (31, 33)), ((0, 60), (60, 124), (124, 126))):
+            qq = qf[r0:r1].reshape(-1, n_heads, hd)
+            want, bound = pn.attention(qq, hk[k0:k1], hv[k0:k1], [0] * (r1 - r0), 0.1)
+            bound = bound_of(bound, want, qq, hk[k0:k1], hv[k0:k1], qk, ck, 0.1)
+            within(np.abs(got[r0:r1].reshape(-1, n_heads, hd) - want), bound, (seqs, r0))
