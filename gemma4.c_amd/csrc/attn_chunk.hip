@@ -430,16 +430,16 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             // The page of this wave's block of a stage, -1: not a page, -2: nobody looks
             // at it.  It is asked for a stage ahead: waiting for it would mean waiting
             // for every load before it.
+            auto page_in_pool = [&](int asked_page, bool asked) {
+                const int p = __builtin_amdgcn_readfirstlane(asked_page);
+                return !asked ? -2 : p >= 0 && p < a.p.n_pages ? p : -1;
+            };
             int asked_page = 0;
             bool asked = false;
             auto ask_page = [&](int st) {
                 const int t = st * KSP + ut, key = (ktb + t) * 32 + ub * 16;
                 asked = t < ntile && key + 15 >= it.kfirst && key <= it.klast;
                 if (asked) asked_page = a.p.table[(size_t)at.s * a.p.table_stride + (key >> a.p.lgpage)];
-            };
-            auto take_page = [&]() {
-                const int p = __builtin_amdgcn_readfirstlane(asked_page);
-                return !asked ? -2 : p >= 0 && p < a.p.n_pages ? p : -1;
             };
             auto block_at = [&](int st, int pg) {
                 return a.p.block_of(pg < 0 ? 0 : pg, kvh, (ktb + st * KSP + ut) * 32 + ub * 16);
@@ -448,21 +448,21 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 return __builtin_amdgcn_make_buffer_rsrc((void*)((uv ? a.p.vp : a.p.kp) + block * (16 * HD * ES)), 0,
                                                          pg < 0 ? 0 : 16 * HD * ES, kBufWord3);
             };
-            // tokens of this wave's block that somebody looks at, as bits
-            auto block_use = [&](int st) {
-                const int key = (ktb + st * KSP + ut) * 32 + ub * 16;
+            // tokens of the block from key on that somebody looks at, as bits
+            auto tokens_seen = [&](int key) {
                 unsigned u = 0xffffu;
                 if (it.kfirst > key) u &= it.kfirst - key < 16 ? 0xffffu << (it.kfirst - key) : 0u;
                 if (it.klast < key + 15) u &= it.klast >= key ? 0xffffu >> (15 - (it.klast - key)) : 0u;
                 return u;
             };
+            auto block_use = [&](int st) { return tokens_seen((ktb + st * KSP + ut) * 32 + ub * 16); };
             uint8_t* const mine_meta = lds + kMetaMarks + ub * 4;
             // straight to LDS (K or V, as this wave has it)
             __amdgpu_buffer_rsrc_t copy_rsrc;
             uint8_t* copy_to = lds;
             auto copy_piece = [&](int i) { buf_load_lds16(copy_rsrc, copy_to + i * 1024, (tid & 63) * 16, i * 1024); };
             auto begin_copy = [&](int st) {
-                const int pg = take_page();
+                const int pg = page_in_pool(asked_page, asked);
                 copy_rsrc = block_rsrc(block_at(st, pg), pg);
                 copy_to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut)) + ub * KC * 1024;
                 if (uv && lane == 0) *reinterpret_cast<unsigned*>(mine_meta + P::meta_at(st, ut)) = pg == -1 ? 0xffffu : 0u;
@@ -480,7 +480,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             float raw_scale = 0.0f;
             int raw_pg = 0;
             auto fetch = [&](int st) {
-                const int pg = take_page();
+                const int pg = page_in_pool(asked_page, asked);
                 const size_t block = block_at(st, pg);
                 const __amdgpu_buffer_rsrc_t r = block_rsrc(block, pg);
 #pragma unroll
@@ -488,6 +488,15 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 if (M::Q8) raw_scale = reinterpret_cast<const float*>((uv ? a.p.vp : a.p.kp) + a.p.scale_off)[block * 16 + t16];
                 raw_pg = pg;
                 ask_page(st + 1);
+            };
+            // 16 codes as bf16
+            auto codes8 = [&](const uint4& x, unsigned (&y)[8]) {
+                const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int c0 = (int8_t)(w[k >> 1] >> (k & 1 ? 16 : 0)), c1 = (int8_t)(w[k >> 1] >> (k & 1 ? 24 : 8));
+                    y[k] = hi_halves(__float_as_uint((float)c0), __float_as_uint((float)c1));
+                }
             };
             auto put = [&](int st) {
                 uint8_t* to = lds + (uv ? P::v_at(st, ut) : P::k_at(st, ut));
@@ -503,13 +512,8 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
 #pragma unroll
                     for (int i = 0; i < KC; i++) {
                         const int c = i;
-                        const unsigned w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                         unsigned y[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const int c0 = (int8_t)(w[k >> 1] >> (k & 1 ? 16 : 0)), c1 = (int8_t)(w[k >> 1] >> (k & 1 ? 24 : 8));
-                            y[k] = hi_halves(__float_as_uint((float)c0), __float_as_uint((float)c1));
-                        }
+                        codes8(raw[i], y);
                         if (uv) {
                             // dims 64 c + 16 k + t16 of tokens 4 g .. 4 g + 3
 #pragma unroll
@@ -545,20 +549,10 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 on = st < ntile && key + 15 >= it.kfirst && key <= it.klast;
                 if (on) page = a.p.table[(size_t)at.s * a.p.table_stride + (key >> a.p.lgpage)];
             };
-            auto take2 = [&](int page, bool on) {
-                const int p = __builtin_amdgcn_readfirstlane(page);
-                return !on ? -2 : p >= 0 && p < a.p.n_pages ? p : -1;
-            };
-            auto use2 = [&](int st) {
-                const int key = (ktb + st) * 32 + bb * 16;
-                unsigned u = 0xffffu;
-                if (it.kfirst > key) u &= it.kfirst - key < 16 ? 0xffffu << (it.kfirst - key) : 0u;
-                if (it.klast < key + 15) u &= it.klast >= key ? 0xffffu >> (15 - (it.klast - key)) : 0u;
-                return u;
-            };
+            auto use2 = [&](int st) { return tokens_seen((ktb + st) * 32 + bb * 16); };
             // stage st's page looked up: its loads may follow
             auto open2 = [&](int st, bool v) {
-                const int pg = v ? take2(askv, onv) : take2(askk, onk);
+                const int pg = v ? page_in_pool(askv, onv) : page_in_pool(askk, onk);
                 const size_t block = a.p.block_of(pg < 0 ? 0 : pg, kvh, (ktb + st) * 32 + bb * 16);
                 const uint8_t* pool = v ? a.p.vp : a.p.kp;
                 const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(pool + block * (16 * HD * ES)), 0,
@@ -698,14 +692,6 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                 if (lane == 0) reinterpret_cast<unsigned*>(meta)[kBothMarks / 4 + 4 + hf * 2 + bb] = marks;
                 open2(st + 1, true);
             };
-            auto codes8 = [&](const uint4& x, unsigned (&y)[8]) {
-                const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const int c0 = (int8_t)(w[k >> 1] >> (k & 1 ? 16 : 0)), c1 = (int8_t)(w[k >> 1] >> (k & 1 ? 24 : 8));
-                    y[k] = hi_halves(__float_as_uint((float)c0), __float_as_uint((float)c1));
-                }
-            };
             // piece j of stage st to LDS, and the next stage's on its way
             auto piece_k = [&](int st, int j) {
                 const int c = hf * PH + j;
@@ -763,7 +749,7 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
             static_assert(kBox == 32 * kChunks * 16 && kSteps * kPasses == KS, "q");
             uint8_t* box = lds + (KSP == 2 ? (slot < 2 ? 2 + slot : slot == 2 ? 5 : 7) * TB
                                   : DS == 1 ? (wave < 2 ? TB : 2 * TB) + wave * (TB / 2)
-                                  : (wave < 4 ? TB : 3 * TB) + (wave & 3) * (TB / 4));
+                                  : TB + wave * (TB / 4));
             auto q_row = [&](int pass) {
                 return [=](int r) {
                     int hh;
