@@ -12,7 +12,8 @@ constexpr int kLgShares = 8, kShares = 1 << kLgShares;   // workgroups that shar
 // Keys that stand for what it costs to begin and to end an item.  us with 32, 64, 96,
 // 160, 224 and 320 (8 q heads on 2 kv heads): 40 sequences of a row and one of 471, bf16
 // of 512: 93, 92, 84, 81, 80, 84; nine of 3416 rows, fp32 of 256 under a window of 512:
-// 106, 97, 96, 94, 104, 105; 32 of 4 to 8 rows, fp32 over codes of 512: 66, 59, 59, 59, 61, 60.
+// 106, 97, 96, 94, 104, 105; 32 of 4 to 8 rows, fp32 over codes of 512: 66, 59, 59, 59, 61, 60:
+// anything from 96 to 224 would do.
 constexpr int kLead = 160;
 // No smaller share than this.  Against 96: 204 rows of 4 sequences, fp32 of 256, 29 us
 // against 35, 571 rows of 31, bf16 of 512, 23 against 36 (one call 21 against 19).
@@ -295,13 +296,14 @@ struct OpOf<true> { typedef h8_t t; };
 // 32488 positions 393 us against 366.)
 //   q of several terms, and codes: four waves; 512, terms: DS 2, the dims halved over
 // two waves, whose partial scores meet in LDS.
-// 8 heads on 2 kv heads, the whole call: 512 rows over 32488 positions, bf16 of 512,
-// 315 us, 870 TFLOP/s where an 8192^3 library product reaches 1204; there LDS is read
-// for 45 % of the cycles, the matrix cores are busy for 44 %.  fp32 over fp16 of 256 (two
-// products each), 1470 rows over 4700 positions 142 us, 430 of them (865 with the
-// second terms).  fp32 of 512, 250 rows over 16001, 331 us, 200 (600): a wave's
-// instructions bound it, 1100 a tile for splitting K and V into halves (640) and
-// for the weights, against 96 products of 32 cycles.
+// 8 heads on 2 kv heads, the whole call, in a row over the same buffers (behind it with
+// others each time): 512 rows over 32488 positions, bf16 of 512, 316 us (335), 870 TFLOP/s
+// where an 8192^3 library product reaches 1204; there LDS is read for 45 % of the cycles,
+// the matrix cores are busy for 44 %.  fp32 over fp16 of 256 (two products each), 1470
+// rows over 4700 positions 142 us (143), 430 of them (865 with the second terms).  fp32 of
+// 512, 250 rows over 16001, 328 us (337), 200 (600): a wave's instructions bound it, 1100
+// a tile for splitting K and V into halves (640) and for the weights, against 96 products
+// of 32 cycles.
 template <int TQ, int TC, int HD>
 struct Plan {
     typedef Mode<TQ, TC> M;
@@ -1086,6 +1088,14 @@ __global__ __launch_bounds__((64 * Plan<TQ, TC, HD>::NW), (Plan<TQ, TC, HD>::NW 
                         if constexpr (M::Q8) w[j] *= fv[8 * t + j];
                     }
                     if constexpr (NP == 1) {
+                        // Rounded to the type, the operand's, while l keeps fp32: 512 rows over
+                        // 32488 positions, bf16 of 512, 313 us with an error of 0.00191 of the
+                        // norm, where the output's own rounding alone makes 0.00166; two terms
+                        // reach that in 404.  A chunk of 471 rows beside 40 single ones 82 us
+                        // (0.00204) and 90, over codes, whose scale is rounded with the weight, 512
+                        // rows of 512 over 16000 224 (0.00236) and 253, 1470 of 256 137 (0.00231)
+                        // and 153.  fp16 of 512 and of 256: 0.000242 and 0.000247 where its own
+                        // rounding makes 0.000208.
 #pragma unroll
                         for (int j = 0; j < 8; j++) p[0][t][j] = (E)w[j];
                     } else if constexpr (M::kHalf) {

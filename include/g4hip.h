@@ -502,7 +502,7 @@ int g4_attn_decode_paged(const float *q, int q_stride, const void *kp, const voi
  * that grows past it is rounded as above from there on.
  *   BF16 and few rows: |V| times the keys a row sees has to stay below fp32's
  * largest number; with every type scores and q times attn_scale as well (F32: a q
- * row's largest times a K row's largest times attn_scale).
+ * row's largest times a K row's largest times attn_scale; BF16: q times k too).
  * Where what a row's head sees holds infinities or NaN, its output is what the
  * formula gives or NaN; what it does not see does not matter beyond rounding.  work:
  * g4_attn_prompt_packed_work_bytes() bytes that no call running at the same
@@ -527,8 +527,9 @@ int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void
  *   G4_F16 over F16, G4_BF16 over BF16 or G4_KV_Q8: exact products of q (BF16
  * under an attn_scale below 1: q times its power of two, within 2^-134), fp32
  * sums, weights (times the scale of a token's codes) rounded to the type before
- * they multiply V (F16: also within 2^-32 of the row's largest); the result is
- * rounded to the type.
+ * they multiply V (F16: also within 2^-32 of the row's largest): against 64 bits
+ * the result is off by about 1.2 times (over codes 1.4 times) what its own rounding
+ * to the type costs.
  *   Few keys (the window's or all that a row of table allows, in units of 512
  * bytes of a head's K, up to 256, and 2^17 of them over all rows and heads):
  * fp32 throughout, so that the same rows with a wider table are rounded as above.
