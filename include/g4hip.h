@@ -528,7 +528,7 @@ int g4_attn_prompt_packed(const void *q, int q_stride, const void *k, const void
  * under an attn_scale below 1: q times its power of two, within 2^-134), fp32
  * sums, weights (times the scale of a token's codes) rounded to the type before
  * they multiply V (F16: also within 2^-32 of the row's largest): against 64 bits
- * the result is off by about 1.2 times (over codes 1.4 times) what its own rounding
+ * the result is off by about 1.2 times (over codes 1.5 times) what its own rounding
  * to the type costs.
  *   Few keys (the window's or all that a row of table allows, in units of 512
  * bytes of a head's K, up to 256, and 2^17 of them over all rows and heads):
